@@ -240,7 +240,6 @@ def prepare(case, seed):
         state.update(q=q, k=k, positions=start + torch.arange(n, device=DEVICE))
         if case["direction"] == "train":
             state.update(gq=_randn(q.shape, g, dtype), gk=_randn(k.shape, g, dtype))
-            state["q"], state["k"] = q.detach().requires_grad_(), k.detach().requires_grad_()
         if own:
             from fireprot_amd import rotary
 
@@ -306,13 +305,12 @@ def _run_rotary(state):
                                   state["frequencies"], layout=case["layout"])
         if case["direction"] == "forward":
             return out
-        grads = torch.autograd.grad(out, (state["q"], state["k"]), (state["gq"], state["gk"]))
-        return out[0].detach(), out[1].detach(), *grads
+        return *out, *rotary.rotary_backward(state["gq"], state["gk"], state["positions"],
+                                             state["frequencies"], layout=case["layout"])
     frequencies, factor = state["frequencies"]
     angle = (state["positions"].double()[..., None] * frequencies)[:, :, None]
     cos, sin = (torch.cos(angle) * factor).float(), (torch.sin(angle) * factor).float()
-    q, k = state["q"].detach(), state["k"].detach()
-    out = _rotate(q, cos, sin, case), _rotate(k, cos, sin, case)
+    out = (_rotate(state["q"], cos, sin, case), _rotate(state["k"], cos, sin, case))
     if case["direction"] == "forward":
         return out
     return *out, _rotate(state["gq"], cos, -sin, case), _rotate(state["gk"], cos, -sin, case)
@@ -431,7 +429,7 @@ def exact(case, seed):
         r = case["rotary_dim"]
 
         def turned(x, by):
-            x = x.detach().double()
+            x = x.double()
             if case["layout"] == "half":
                 z = torch.complex(x[..., :r // 2].contiguous(), x[..., r // 2:r].contiguous()) * by
                 head = torch.cat([z.real, z.imag], -1)
