@@ -25,6 +25,9 @@ FPX_ERR_POINTER = 3
 FPX_ERR_WORKSPACE = 4
 FPX_F32 = 0
 FPX_BF16 = 1
+FPX_F16 = 2
+FPX_F8E4M3 = 3
+FPX_I8 = 4
 
 _p = ctypes.c_void_p
 _i = ctypes.c_int
@@ -110,6 +113,16 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "fpx_qkv_projection": (_i, [_p, _i64, _p, _p, _p, _p, _p]),
     "fpx_sigmoid_mul_out": (_i, [_p, _p, _p, _i64, _p]),
     "fpx_split_planes": (_i, [_p, _i64, _p, _p]),
+    "fpx_rotary": (_i, [
+        _i, _i,                      # dtype, layout
+        _p, _i64, _i64, _i64,        # q, strides (batch, token, head)
+        _p, _i64, _i64, _i64, _i,    # q_out, strides, q_heads
+        _p, _i64, _i64, _i64,        # k
+        _p, _i64, _i64, _i64, _i,    # k_out, strides, k_heads (0: none)
+        _p, _i, _i64, _i64,          # positions, 64-bit, strides (batch, token)
+        _p, _f, _i,                  # inv_freq (double), scale, inverse
+        _i64, _i64, _i, _i, _p,      # batch, tokens, head_dim, rotary_dim, stream
+    ]),
 }
 
 _lock = threading.RLock()
@@ -164,3 +177,30 @@ def check(code: int, what: str) -> None:
                  FPX_ERR_POINTER: "null or misaligned pointer",
                  FPX_ERR_WORKSPACE: "workspace too small"}
         raise RuntimeError(f"{what} failed with status {code} ({names.get(code, 'HIP error')})")
+
+
+class on_device:
+    """``with on_device(d) as stream``: device ``d`` current inside, and the
+    handle of its current stream.  Where ``d`` is current already, which is
+    the ordinary call, nothing is switched (a call of a few microseconds
+    otherwise pays as much for the switch as for its launch)."""
+
+    __slots__ = ("index", "previous")
+
+    def __init__(self, device: Any) -> None:
+        self.index = device.index
+
+    def __enter__(self) -> int:
+        import torch
+
+        self.previous = torch.cuda.current_device()
+        if self.index != self.previous:
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *exc_info: Any) -> bool:
+        if self.index != self.previous:
+            import torch
+
+            torch.cuda.set_device(self.previous)
+        return False

@@ -807,4 +807,57 @@ int fpx_split_planes(const float* x, int64_t count, uint16_t* planes, void* stre
   return status(fpx::launch_split_planes(x, planes, count / 8, static_cast<hipStream_t>(stream)));
 }
 
+int fpx_rotary(int dtype, int layout, const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh,
+               void* q_out, int64_t qo_sb, int64_t qo_sn, int64_t qo_sh, int q_heads,
+               const void* k, int64_t k_sb, int64_t k_sn, int64_t k_sh, void* k_out,
+               int64_t ko_sb, int64_t ko_sn, int64_t ko_sh, int k_heads, const void* positions,
+               int positions_64, int64_t p_sb, int64_t p_sn, const double* inv_freq, float scale,
+               int inverse, int64_t batch, int64_t tokens, int head_dim, int rotary_dim,
+               void* stream) {
+  if (dtype != FPX_F32 && dtype != FPX_BF16 && dtype != FPX_F16) return FPX_ERR_DIMS;
+  if (layout != FPX_ROTARY_HALF && layout != FPX_ROTARY_INTERLEAVED) return FPX_ERR_DIMS;
+  if (positions_64 != 0 && positions_64 != 1) return FPX_ERR_DIMS;
+  if (inverse != 0 && inverse != 1) return FPX_ERR_DIMS;
+  if (head_dim < 2 || head_dim > fpx::kRotaryMaxDim || rotary_dim < 2 || rotary_dim > head_dim ||
+      rotary_dim % 2)
+    return FPX_ERR_DIMS;
+  if (q_heads < 1 || k_heads < 0 || q_heads > 8192 || k_heads > 8192 - q_heads)
+    return FPX_ERR_DIMS;
+  if (batch < 0 || tokens < 0 || batch > 0x7fffffff || tokens > 0x7fffffff ||
+      batch * tokens > 0x7fffffff)
+    return FPX_ERR_DIMS;
+  if (q_sb < 0 || q_sn < 0 || q_sh < 0 || qo_sb < 0 || qo_sn < 0 || qo_sh < 0 || p_sb < 0 ||
+      p_sn < 0)
+    return FPX_ERR_DIMS;
+  if (q == q_out && (q_sb != qo_sb || q_sn != qo_sn || q_sh != qo_sh)) return FPX_ERR_DIMS;
+  if (k_heads > 0) {
+    if (k_sb < 0 || k_sn < 0 || k_sh < 0 || ko_sb < 0 || ko_sn < 0 || ko_sh < 0)
+      return FPX_ERR_DIMS;
+    if (k == k_out && (k_sb != ko_sb || k_sn != ko_sn || k_sh != ko_sh)) return FPX_ERR_DIMS;
+  }
+  if (batch == 0 || tokens == 0) return FPX_OK;
+  const uintptr_t elem = elem_bytes(dtype == FPX_F16 ? FPX_BF16 : dtype);
+  if (!aligned(q, elem) || !aligned(q_out, elem) || !aligned(positions, positions_64 ? 8 : 4) ||
+      !aligned(inv_freq, 8))
+    return FPX_ERR_POINTER;
+  if (k_heads > 0 && (!aligned(k, elem) || !aligned(k_out, elem))) return FPX_ERR_POINTER;
+  fpx::RotaryArgs a{};
+  a.x[0] = {q, q_out, q_sb, q_sn, q_sh, qo_sb, qo_sn, qo_sh, q_heads};
+  if (k_heads > 0) a.x[1] = {k, k_out, k_sb, k_sn, k_sh, ko_sb, ko_sn, ko_sh, k_heads};
+  a.pos = positions;
+  a.pos_b = p_sb;
+  a.pos_n = p_sn;
+  a.pos64 = positions_64;
+  a.freq = inv_freq;
+  a.scale = scale;
+  a.inverse = inverse;
+  a.dtype = dtype;
+  a.interleaved = layout == FPX_ROTARY_INTERLEAVED;
+  a.tokens = (int)tokens;
+  a.total = (int)(batch * tokens);
+  a.head_dim = head_dim;
+  a.rot = rotary_dim;
+  return status(fpx::launch_rotary(a, static_cast<hipStream_t>(stream)));
+}
+
 }  // extern "C"

@@ -377,6 +377,40 @@ struct TransitionArgs {
 
 hipError_t launch_transition(const TransitionArgs& args, hipStream_t stream);
 
+// ------------------------------------------------------------------ rotary
+// Rows of head_dim channels at in + b*in_b + n*in_n + h*in_h (channel stride
+// 1), written likewise; heads == 0: no such tensor.  out may be in itself with
+// the same strides.
+constexpr int kRotaryMaxDim = 512;
+
+struct RotaryTensor {
+  const void* in;
+  void* out;
+  int64_t in_b, in_n, in_h;
+  int64_t out_b, out_n, out_h;
+  int heads;
+};
+
+struct RotaryArgs {
+  RotaryTensor x[2];   // queries and keys, turned by the same positions
+  const void* pos;     // int32 or int64 at b*pos_b + n*pos_n
+  int64_t pos_b, pos_n;
+  int pos64;
+  const double* freq;  // [rot / 2] radians a position
+  float scale;         // of the rotated channels
+  int inverse;         // negated angles: the gradient
+  int dtype;           // FPX_F32, FPX_BF16 or FPX_F16
+  int interleaved;
+  int tokens, total;   // per batch entry, of the whole call
+  int head_dim, rot;
+  // launch shape, set by launch_rotary: vectors of a row, log2 of the threads
+  // a row takes, tokens of a work-group, 2^32 / heads rounded up
+  int units, unit_shift, tt;
+  unsigned heads_magic;
+};
+
+hipError_t launch_rotary(const RotaryArgs& args, hipStream_t stream);
+
 int device_cu_count();
 
 }  // namespace fpx

@@ -37,6 +37,15 @@ extern "C" {
 
 #define FPX_F32 0
 #define FPX_BF16 1
+/* Types of the decoding operators (fpx_rotary, fpx_cache_*, fpx_paged_attention)
+ * only: */
+#define FPX_F16 2
+#define FPX_F8E4M3 3 /* OCP 8-bit float, 4 exponent and 3 mantissa bits */
+#define FPX_I8 4
+
+/* Layouts of the pairs that fpx_rotary turns. */
+#define FPX_ROTARY_HALF 0        /* channels i and i + rotary_dim / 2 */
+#define FPX_ROTARY_INTERLEAVED 1 /* channels 2i and 2i + 1 */
 
 /* ABI version of the loaded library (FPX_ABI_VERSION).
  * Replaces the reference bridge's ABI_VERSION probe
@@ -321,6 +330,34 @@ int fpx_sigmoid_mul_out(const float* gate, const float* value, float* out, int64
  * reference (its kernels compute in FP32 or round once); used by this
  * library's own parity tests. */
 int fpx_split_planes(const float* x, int64_t count, uint16_t* planes, void* stream);
+
+/* Rotary positions of queries and keys in one launch: of each row x of
+ * head_dim channels the first rotary_dim are turned in pairs (x1, x2),
+ *   y1 = scale * (x1 cos a - x2 sin a),  y2 = scale * (x2 cos a + x1 sin a),
+ *   a = positions[b][n] * inv_freq[i],
+ * and the rest copied.  inverse = 1 negates the angles: the gradient of the
+ * outputs turned back to that of the inputs.  Stands in for the reference's
+ * protein-language-model rotary kernel (kernels/amd/fireprot_esmc_rope.hip).
+ *   dtype     FPX_F32, FPX_BF16 or FPX_F16 of q, k and their outputs;
+ *             arithmetic in FP32, the angles in FP64
+ *   q         row (b, n, h) at q + b*q_sb + n*q_sn + h*q_sh, channel stride 1;
+ *             any alignment of the type (16-byte rows are fastest)
+ *   q_out     likewise; may be q itself with the same strides (in place); any
+ *             other overlap is unsupported (status 2 when q_out == q with
+ *             different strides)
+ *   k, k_out  the same; k_heads = 0: no keys, pointers and strides ignored
+ *   positions int32 (positions_64 = 0) or int64 (1) at b*p_sb + n*p_sn, any sign
+ *   inv_freq  [rotary_dim / 2] doubles, radians a position
+ * Supported: even rotary_dim, 2 <= rotary_dim <= head_dim <= 512,
+ * batch * tokens < 2^31, q_heads >= 1, q_heads + k_heads <= 8192; nothing is
+ * launched when batch or tokens is 0. */
+int fpx_rotary(int dtype, int layout, const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh,
+               void* q_out, int64_t qo_sb, int64_t qo_sn, int64_t qo_sh, int q_heads,
+               const void* k, int64_t k_sb, int64_t k_sn, int64_t k_sh, void* k_out,
+               int64_t ko_sb, int64_t ko_sn, int64_t ko_sh, int k_heads, const void* positions,
+               int positions_64, int64_t p_sb, int64_t p_sn, const double* inv_freq, float scale,
+               int inverse, int64_t batch, int64_t tokens, int head_dim, int rotary_dim,
+               void* stream);
 
 #ifdef __cplusplus
 }
