@@ -123,6 +123,22 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         _p, _f, _i,                  # inv_freq (double), scale, inverse
         _i64, _i64, _i, _i, _p,      # batch, tokens, head_dim, rotary_dim, stream
     ]),
+    "fpx_cache_write": (_i, [
+        _i, _i,                      # row_dtype, cache_dtype
+        _p, _i64, _i64,              # k, strides (token, head)
+        _p, _i64, _i64,              # v, strides
+        _p, _i64,                    # slots, tokens
+        _p, _p, _p, _p,              # cache_k, cache_v, k_scale, v_scale
+        _i64, _i, _i, _i, _p,        # pages, heads, page_size, head_dim, stream
+    ]),
+    "fpx_cache_read": (_i, [
+        _i, _i,                      # row_dtype, cache_dtype
+        _p, _i64, _i64,              # k (written), strides (token, head)
+        _p, _i64, _i64,              # v (written), strides
+        _p, _i64,                    # slots, tokens
+        _p, _p, _p, _p,              # cache_k, cache_v, k_scale, v_scale
+        _i64, _i, _i, _i, _p,        # pages, heads, page_size, head_dim, stream
+    ]),
 }
 
 _lock = threading.RLock()

@@ -20,7 +20,8 @@ INCLUDE = ROOT / "include"
 LIB_DIR = PACKAGE / "_lib"
 LIB_PATH = LIB_DIR / "libfireprot_amd.so"
 SOURCES = ("attention.hip", "attention_split.hip", "projection.hip", "bf16.hip",
-           "elementwise.hip", "trimul.hip", "transition.hip", "rotary.hip", "capi.hip")
+           "elementwise.hip", "trimul.hip", "transition.hip", "rotary.hip",
+           "kv_cache.hip", "capi.hip")
 ARCH = "gfx950"
 
 HIPCC_FLAGS = (

@@ -358,6 +358,71 @@ void* device_scratch(hipError_t* err) {
   return scratch_ptr[device];
 }
 
+// ---- paged key-value cache: what its entries share
+
+bool is_coded(int dtype) { return dtype == FPX_F8E4M3 || dtype == FPX_I8; }
+
+uintptr_t type_bytes(int dtype) {
+  return dtype == FPX_F32 ? 4 : dtype == FPX_BF16 || dtype == FPX_F16 ? 2 : 1;
+}
+
+bool row_type_ok(int dtype) {
+  return dtype == FPX_F32 || dtype == FPX_BF16 || dtype == FPX_F16;
+}
+
+// Status of a cache's sizes, and its page shift.
+int cache_dims(int cache_dtype, int64_t pages, int heads, int page_size, int head_dim,
+               int* page_shift) {
+  if (!row_type_ok(cache_dtype) && !is_coded(cache_dtype)) return FPX_ERR_DIMS;
+  if (head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256) return FPX_ERR_DIMS;
+  if (page_size < 16 || page_size > 4096 || (page_size & (page_size - 1))) return FPX_ERR_DIMS;
+  if (heads < 1 || heads > 65535 || pages < 1 || pages > 0x7fffffff) return FPX_ERR_DIMS;
+  *page_shift = __builtin_ctz((unsigned)page_size);
+  return FPX_OK;
+}
+
+bool cache_pointers_ok(int cache_dtype, const void* k, const void* v, const float* k_scale,
+                       const float* v_scale) {
+  if (!aligned(k, 16) || !aligned(v, 16)) return false;
+  return !is_coded(cache_dtype) || (aligned(k_scale, 16) && aligned(v_scale, 16));
+}
+
+int cache_impl(bool read, int row_dtype, int cache_dtype, const void* k, int64_t k_st,
+               int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const int64_t* slots,
+               int64_t tokens, const void* cache_k, const void* cache_v, const float* k_scale,
+               const float* v_scale, int64_t pages, int heads, int page_size, int head_dim,
+               void* stream) {
+  fpx::CacheArgs a{};
+  const int rc = cache_dims(cache_dtype, pages, heads, page_size, head_dim, &a.page_shift);
+  if (rc != FPX_OK) return rc;
+  if (!row_type_ok(row_dtype)) return FPX_ERR_DIMS;
+  if (k_st < 0 || k_sh < 0 || v_st < 0 || v_sh < 0) return FPX_ERR_DIMS;
+  if (tokens < 0 || tokens > 0x7fffffff || tokens * heads > 0x7fffffff) return FPX_ERR_DIMS;
+  if (tokens == 0) return FPX_OK;
+  const uintptr_t elem = type_bytes(row_dtype);
+  if (!aligned(k, elem) || !aligned(v, elem) || !aligned(slots, 8) ||
+      !cache_pointers_ok(cache_dtype, cache_k, cache_v, k_scale, v_scale))
+    return FPX_ERR_POINTER;
+  a.rows[0] = k;
+  a.rows[1] = v;
+  a.stride_t[0] = k_st;
+  a.stride_t[1] = v_st;
+  a.stride_h[0] = k_sh;
+  a.stride_h[1] = v_sh;
+  a.slots = slots;
+  a.cache[0] = const_cast<void*>(cache_k);
+  a.cache[1] = const_cast<void*>(cache_v);
+  a.scale[0] = const_cast<float*>(k_scale);
+  a.scale[1] = const_cast<float*>(v_scale);
+  a.tokens = tokens;
+  a.pages = pages;
+  a.heads = heads;
+  a.head_dim = head_dim;
+  a.row_dtype = row_dtype;
+  a.cache_dtype = cache_dtype;
+  return status(fpx::launch_cache(a, read, static_cast<hipStream_t>(stream)));
+}
+
 }  // namespace
 
 extern "C" {
@@ -836,7 +901,7 @@ int fpx_rotary(int dtype, int layout, const void* q, int64_t q_sb, int64_t q_sn,
     if (k == k_out && (k_sb != ko_sb || k_sn != ko_sn || k_sh != ko_sh)) return FPX_ERR_DIMS;
   }
   if (batch == 0 || tokens == 0) return FPX_OK;
-  const uintptr_t elem = elem_bytes(dtype == FPX_F16 ? FPX_BF16 : dtype);
+  const uintptr_t elem = type_bytes(dtype);
   if (!aligned(q, elem) || !aligned(q_out, elem) || !aligned(positions, positions_64 ? 8 : 4) ||
       !aligned(inv_freq, 8))
     return FPX_ERR_POINTER;
@@ -858,6 +923,23 @@ int fpx_rotary(int dtype, int layout, const void* q, int64_t q_sb, int64_t q_sn,
   a.head_dim = head_dim;
   a.rot = rotary_dim;
   return status(fpx::launch_rotary(a, static_cast<hipStream_t>(stream)));
+}
+
+int fpx_cache_write(int row_dtype, int cache_dtype, const void* k, int64_t k_st, int64_t k_sh,
+                    const void* v, int64_t v_st, int64_t v_sh, const int64_t* slots,
+                    int64_t tokens, void* cache_k, void* cache_v, float* k_scale, float* v_scale,
+                    int64_t pages, int heads, int page_size, int head_dim, void* stream) {
+  return cache_impl(false, row_dtype, cache_dtype, k, k_st, k_sh, v, v_st, v_sh, slots, tokens,
+                    cache_k, cache_v, k_scale, v_scale, pages, heads, page_size, head_dim, stream);
+}
+
+int fpx_cache_read(int row_dtype, int cache_dtype, void* k, int64_t k_st, int64_t k_sh, void* v,
+                   int64_t v_st, int64_t v_sh, const int64_t* slots, int64_t tokens,
+                   const void* cache_k, const void* cache_v, const float* k_scale,
+                   const float* v_scale, int64_t pages, int heads, int page_size, int head_dim,
+                   void* stream) {
+  return cache_impl(true, row_dtype, cache_dtype, k, k_st, k_sh, v, v_st, v_sh, slots, tokens,
+                    cache_k, cache_v, k_scale, v_scale, pages, heads, page_size, head_dim, stream);
 }
 
 }  // extern "C"

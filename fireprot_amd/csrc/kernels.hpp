@@ -411,6 +411,22 @@ struct RotaryArgs {
 
 hipError_t launch_rotary(const RotaryArgs& args, hipStream_t stream);
 
+// ------------------------------------------------------ paged key-value cache
+// Rows of keys [0] and values [1] at rows + t*stride_t + h*stride_h (channel
+// stride 1) and their places in the cache (paged_layout.hpp).
+struct CacheArgs {
+  const void* rows[2];  // sources of a write; written by a read
+  int64_t stride_t[2], stride_h[2];
+  const int64_t* slots;  // [tokens]
+  void* cache[2];
+  float* scale[2];       // 8-bit caches only
+  int64_t tokens, pages;
+  int heads, head_dim, page_shift;
+  int row_dtype, cache_dtype;  // FPX_*
+};
+
+hipError_t launch_cache(const CacheArgs& args, bool read, hipStream_t stream);
+
 int device_cu_count();
 
 }  // namespace fpx

@@ -1,0 +1,79 @@
+// Index rules of the paged key-value cache, shared by its kernels and by the
+// host: plain C++ with no device types, so they are tested on the CPU as they
+// stand.
+//
+// A cache holds `pages` pages of 2^page_shift slots.  k and v each are
+// [pages][heads][slots of a page][head_dim], the scales of an 8-bit cache
+// [pages][heads][slots of a page]: one head's keys of a page are contiguous,
+// which is what an attention work-group reads.
+#pragma once
+
+#include <cstdint>
+
+#ifdef __HIPCC__
+#define FPX_HD __host__ __device__ __forceinline__
+#else
+#define FPX_HD inline
+#endif
+
+namespace fpx {
+
+constexpr int64_t kSlotNone = -1;     // a negative slot: no token
+constexpr int64_t kSlotOutside = -2;  // a slot past the cache's end
+
+// Row (of head_dim channels, and of the scales) of a slot and head, or
+// kSlotNone / kSlotOutside.
+FPX_HD int64_t cache_row(int64_t slot, int head, int64_t pages, int heads, int page_shift) {
+  if (slot < 0) return kSlotNone;
+  const int64_t page = slot >> page_shift;
+  if (page >= pages) return kSlotOutside;
+  return ((page * heads + head) << page_shift) + (slot & ((int64_t(1) << page_shift) - 1));
+}
+
+// Keys [first, end) that a sequence of `length` tokens attends to, or invalid
+// where the length does not fit the call (negative, or above max_length).
+struct KeyRange {
+  int first, end;
+  bool valid;
+};
+
+FPX_HD KeyRange key_range(int length, int max_length, int window) {
+  if (length < 0 || length > max_length) return {0, 0, false};
+  return {window > 0 && length > window ? length - window : 0, length, true};
+}
+
+// The work on a range is cut into chunks that start at a tile's first key.
+constexpr int kKeyTile = 32;
+
+FPX_HD int chunk_count(const KeyRange& r, int chunk) {
+  const int start = r.first & ~(kKeyTile - 1);
+  return r.end <= r.first ? 0 : (r.end - start - 1) / chunk + 1;
+}
+
+// Most chunks a row of this call can have: the longest range, begun at the
+// last key of a tile.
+FPX_HD int chunk_limit(int max_length, int window, int chunk) {
+  if (max_length <= 0) return 0;
+  if (window <= 0 || window >= max_length) return (max_length - 1) / chunk + 1;
+  // a window of w keys begins anywhere in a tile; it never spans more than
+  // max_length keys
+  const int64_t span = (int64_t)window + kKeyTile - 1 < max_length
+                           ? (int64_t)window + kKeyTile - 1
+                           : max_length;
+  return (int)((span - 1) / chunk + 1);
+}
+
+// Entry of the block table that serves a group of keys from `key` on: that of
+// the nearest key of the range, so that a group wholly outside it (its keys
+// are masked) names no page the sequence does not hold.
+FPX_HD int table_entry(int key, const KeyRange& r, int page_shift) {
+  const int k = key < r.first ? r.first : key >= r.end ? r.end - 1 : key;
+  return k >> page_shift;
+}
+
+// Whether a block-table entry names a page of the cache.
+FPX_HD bool page_valid(int page, int64_t pages) {
+  return page >= 0 && (int64_t)page < pages;
+}
+
+}  // namespace fpx

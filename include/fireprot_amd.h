@@ -359,6 +359,43 @@ int fpx_rotary(int dtype, int layout, const void* q, int64_t q_sb, int64_t q_sn,
                int inverse, int64_t batch, int64_t tokens, int head_dim, int rotary_dim,
                void* stream);
 
+/* A paged key-value cache: `pages` pages of page_size slots; k and v each
+ * [pages][heads][page_size][head_dim] of cache_dtype, contiguous; for the 8-bit
+ * types scales [pages][heads][page_size] float each, else null.  Slot s is slot
+ * s % page_size of page s / page_size.  No counterpart in the reference.
+ *
+ * fpx_cache_write puts token t's rows (every head) at slots[t]: converted to a
+ * plain cache_dtype, or as 8-bit codes with a scale per row, top being the
+ * row's largest magnitude:
+ *   FPX_F8E4M3  scale = 2^e, the least e with top <= 448 * 2^e; the codes are
+ *               x / scale rounded to nearest even
+ *   FPX_I8      scale = top * (1/127); codes x * (1/scale), to nearest even
+ *   both        zeros with scale 0 where top < 2^-100; zeros with scale NaN
+ *               where top is infinite or NaN (the row reads back as NaN)
+ * A token with a negative slot, or one past the cache, is not written.  The
+ * other slots of one call must be distinct, as must be its k and v tensors and
+ * the cache's.
+ *   k, v      row (t, h) at k + t*k_st + h*k_sh, channel stride 1, of row_dtype
+ *             (FPX_F32, FPX_BF16, FPX_F16); any alignment of the type (16-byte
+ *             rows are fastest)
+ *   slots     [tokens] int64
+ * Supported: head_dim 32, 64, 128 or 256; page_size a power of two from 16 to
+ * 4096; heads >= 1; pages >= 1; tokens * heads < 2^31; nothing is launched
+ * when tokens is 0.  The cache's tensors are 16-byte aligned. */
+int fpx_cache_write(int row_dtype, int cache_dtype, const void* k, int64_t k_st, int64_t k_sh,
+                    const void* v, int64_t v_st, int64_t v_sh, const int64_t* slots,
+                    int64_t tokens, void* cache_k, void* cache_v, float* k_scale, float* v_scale,
+                    int64_t pages, int heads, int page_size, int head_dim, void* stream);
+
+/* The rows of `slots` read back as row_dtype: code times scale, rounded once.
+ * A negative slot gives zeros, one past the cache NaN; slots may repeat.
+ * Arguments as fpx_cache_write's, k and v written. */
+int fpx_cache_read(int row_dtype, int cache_dtype, void* k, int64_t k_st, int64_t k_sh, void* v,
+                   int64_t v_st, int64_t v_sh, const int64_t* slots, int64_t tokens,
+                   const void* cache_k, const void* cache_v, const float* k_scale,
+                   const float* v_scale, int64_t pages, int heads, int page_size, int head_dim,
+                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif
