@@ -131,6 +131,18 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         _p, _p, _p, _p,              # cache_k, cache_v, k_scale, v_scale
         _i64, _i, _i, _i, _p,        # pages, heads, page_size, head_dim, stream
     ]),
+    "fpx_paged_attention_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i64, _i64]),
+    "fpx_paged_attention": (_i, [
+        _i, _i,                      # dtype, cache_dtype
+        _p, _i64, _i64,              # q, strides (batch, head)
+        _p, _p, _p, _p,              # cache_k, cache_v, k_scale, v_scale
+        _i64, _i, _i, _i,            # pages, heads, page_size, head_dim
+        _p, _i64, _i64,              # block_table, stride, pages a sequence
+        _p, _i64, _i,                # lengths, batch, q_heads
+        _i64, _i64, _f,              # max_length, window, scale
+        _p, _i64, _i64, _p,          # out, strides (batch, head), lse (nullable)
+        _p, _sz, _p,                 # workspace, bytes, stream
+    ]),
     "fpx_cache_read": (_i, [
         _i, _i,                      # row_dtype, cache_dtype
         _p, _i64, _i64,              # k (written), strides (token, head)

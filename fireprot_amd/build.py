@@ -21,7 +21,8 @@ LIB_DIR = PACKAGE / "_lib"
 LIB_PATH = LIB_DIR / "libfireprot_amd.so"
 SOURCES = ("attention.hip", "attention_split.hip", "projection.hip", "bf16.hip",
            "elementwise.hip", "trimul.hip", "transition.hip", "rotary.hip",
-           "kv_cache.hip", "capi.hip")
+           "kv_cache.hip", "paged_attention.hip", "paged_attention_plain.hip",
+           "paged_attention_fp8.hip", "paged_attention_int8.hip", "capi.hip")
 ARCH = "gfx950"
 
 HIPCC_FLAGS = (

@@ -423,6 +423,27 @@ int cache_impl(bool read, int row_dtype, int cache_dtype, const void* k, int64_t
   return status(fpx::launch_cache(a, read, static_cast<hipStream_t>(stream)));
 }
 
+constexpr int64_t kPagedMaxRows = 1 << 23;  // 2^31 threads of 256 a row
+
+// The cut of a call's work, blocks = 0 for unsupported sizes.
+fpx::PagedPlan paged_plan(int64_t batch, int q_heads, int heads, int head_dim, int64_t max_length,
+                          int64_t window) {
+  fpx::PagedPlan none{};
+  if (batch < 0 || batch >= kPagedMaxRows || heads < 1 || q_heads < heads || q_heads % heads ||
+      q_heads >= kPagedMaxRows || batch * q_heads >= kPagedMaxRows)
+    return none;
+  if (head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256) return none;
+  if (max_length < 0 || max_length >= (1 << 30) || window < 0) return none;
+  const int w = window < (1 << 30) ? (int)window : 0;  // wider than any sequence: all keys
+  const fpx::PagedPlan p = fpx::plan_paged(batch < 1 ? 1 : batch, heads, q_heads / heads, head_dim,
+                                           (int)max_length, w);
+  return p.blocks < kPagedMaxRows ? p : none;
+}
+
+size_t paged_part_bytes(const fpx::PagedPlan& p, int64_t batch, int q_heads, int head_dim) {
+  return (size_t)round_up((int64_t)batch * q_heads * p.splits * head_dim * 4, 256);
+}
+
 }  // namespace
 
 extern "C" {
@@ -940,6 +961,79 @@ int fpx_cache_read(int row_dtype, int cache_dtype, void* k, int64_t k_st, int64_
                    void* stream) {
   return cache_impl(true, row_dtype, cache_dtype, k, k_st, k_sh, v, v_st, v_sh, slots, tokens,
                     cache_k, cache_v, k_scale, v_scale, pages, heads, page_size, head_dim, stream);
+}
+
+size_t fpx_paged_attention_workspace_bytes(int64_t batch, int q_heads, int heads, int head_dim,
+                                           int64_t max_length, int64_t window) {
+  const fpx::PagedPlan p = paged_plan(batch, q_heads, heads, head_dim, max_length, window);
+  if (p.blocks == 0) return 0;
+  if (p.splits == 1) return 256;  // nothing is left between launches
+  return paged_part_bytes(p, batch, q_heads, head_dim) + (size_t)batch * q_heads * p.splits * 8;
+}
+
+int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb, int64_t q_sh,
+                        const void* cache_k, const void* cache_v, const float* k_scale,
+                        const float* v_scale, int64_t pages, int heads, int page_size,
+                        int head_dim, const int32_t* block_table, int64_t table_sb,
+                        int64_t table_pages, const int32_t* lengths, int64_t batch, int q_heads,
+                        int64_t max_length, int64_t window, float scale, void* out, int64_t o_sb,
+                        int64_t o_sh, float* lse, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  fpx::PagedArgs a{};
+  const int rc = cache_dims(cache_dtype, pages, heads, page_size, head_dim, &a.page_shift);
+  if (rc != FPX_OK) return rc;
+  if (!row_type_ok(dtype) || (!is_coded(cache_dtype) && cache_dtype != dtype)) return FPX_ERR_DIMS;
+  const fpx::PagedPlan p = paged_plan(batch, q_heads, heads, head_dim, max_length, window);
+  if (p.blocks == 0) return FPX_ERR_DIMS;
+  const int64_t row = 16 / (int64_t)type_bytes(dtype);
+  if (q_sb < 0 || q_sh < 0 || o_sb < 0 || o_sh < 0 || q_sb % row || q_sh % row || o_sb % row ||
+      o_sh % row)
+    return FPX_ERR_DIMS;
+  if (out == q && (o_sb != q_sb || o_sh != q_sh)) return FPX_ERR_DIMS;
+  if (table_sb < 0 || table_pages < (max_length + page_size - 1) / page_size) return FPX_ERR_DIMS;
+  if (!(scale - scale == 0.0f)) return FPX_ERR_DIMS;  // infinite or NaN
+  if (batch == 0) return FPX_OK;
+  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(lengths, 4) ||
+      !aligned_or_null(lse, 4) || (max_length > 0 && !aligned(block_table, 4)) ||
+      !cache_pointers_ok(cache_dtype, cache_k, cache_v, k_scale, v_scale))
+    return FPX_ERR_POINTER;
+  if (!aligned(workspace, 256)) return FPX_ERR_POINTER;
+  if (workspace_bytes <
+      fpx_paged_attention_workspace_bytes(batch, q_heads, heads, head_dim, max_length, window))
+    return FPX_ERR_WORKSPACE;
+  a.q = q;
+  a.q_b = q_sb;
+  a.q_h = q_sh;
+  a.k = cache_k;
+  a.v = cache_v;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  a.table = block_table;
+  a.table_b = table_sb;
+  a.lengths = lengths;
+  a.out = out;
+  a.o_b = o_sb;
+  a.o_h = o_sh;
+  a.lse = lse;
+  a.part = static_cast<float*>(workspace);
+  a.part_ml = as<float>(static_cast<char*>(workspace) +
+                        paged_part_bytes(p, batch, q_heads, head_dim));
+  a.scale_log2 = scale * fpx::kLog2e;
+  a.weight_shift = cache_dtype == FPX_F16 ? fpx::kWeightShiftF16 : 0.0f;
+  a.pages = pages;
+  a.batch = (int)batch;
+  a.heads = heads;
+  a.group = q_heads / heads;
+  a.head_dim = head_dim;
+  a.max_length = (int)max_length;
+  a.window = window < (1 << 30) ? (int)window : 0;
+  a.dtype = dtype;
+  a.cache_dtype = cache_dtype;
+  a.chunk = p.chunk;
+  a.splits = p.splits;
+  a.qtiles = p.qtiles;
+  a.query_tiles = p.query_tiles;
+  return status(fpx::launch_paged_attention(a, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -427,6 +427,51 @@ struct CacheArgs {
 
 hipError_t launch_cache(const CacheArgs& args, bool read, hipStream_t stream);
 
+// --------------------------------------- attention of new tokens over the cache
+constexpr int kMaxChunks = 256;     // of a sequence: threads of the join
+constexpr int kPagedGroups = 2048;  // work-groups aimed at
+constexpr float kWeightShiftF16 = 14.0f;  // log2 of the FP16 weights' factor
+
+struct PagedArgs {
+  const void* q;     // [batch][heads * group] rows at q + b*q_b + h*q_h
+  int64_t q_b, q_h;
+  const void* k;     // the cache (paged_layout.hpp)
+  const void* v;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* table;    // pages of a sequence at table + b*table_b
+  int64_t table_b;
+  const int32_t* lengths;  // [batch]
+  void* out;         // as q, strides o_b, o_h
+  int64_t o_b, o_h;
+  float* lse;        // nullable [batch][heads * group]
+  float* part;       // [batch][heads * group][splits][head_dim]: chunk outputs
+  float* part_ml;    // [batch][heads * group][splits][2]: max (log2), sum
+  float scale_log2;  // of the scores, times log2(e)
+  float weight_shift;  // log2 of the factor the weights carry in `part`
+  int64_t pages;
+  int batch, heads, group, head_dim, page_shift, max_length, window;
+  int dtype, cache_dtype;  // FPX_*
+  // how the work is cut: keys of a chunk (a multiple of 128), chunks of a
+  // sequence at most, tiles of query heads, 16-query tiles of one of those
+  int chunk, splits, qtiles, query_tiles;
+};
+
+struct PagedPlan {
+  int chunk, splits, qtiles, query_tiles;
+  int64_t blocks;
+};
+
+PagedPlan plan_paged(int64_t batch, int heads, int group, int head_dim, int max_length,
+                     int window);
+hipError_t launch_paged_attention(const PagedArgs& args, hipStream_t stream);
+// one cache type each (paged_attention_*.hip)
+hipError_t launch_paged_f32(const PagedArgs& args, unsigned blocks, hipStream_t stream);
+hipError_t launch_paged_bf16(const PagedArgs& args, unsigned blocks, hipStream_t stream);
+hipError_t launch_paged_f16(const PagedArgs& args, unsigned blocks, hipStream_t stream);
+hipError_t launch_paged_fp8(const PagedArgs& args, unsigned blocks, hipStream_t stream);
+hipError_t launch_paged_int8(const PagedArgs& args, unsigned blocks, hipStream_t stream);
+
 int device_cu_count();
 
 }  // namespace fpx

@@ -1,0 +1,602 @@
+// Attention of one new token per sequence over a paged key-value cache: the
+// kernel, instantiated per cache type by the paged_attention_*.hip files.
+//
+//   o[b][h] = sum_j w_j v_j,  w = softmax_j(scale q[b][h] . k_j),
+//   j over the sequence's keys [first, length), query head h reading cache
+//   head h / group.
+//
+// One work-group takes one chunk of one sequence's keys for one cache head and
+// all (up to 16 QT) query heads that share it, so every key and value is read
+// from memory once; its four waves take the chunk's tiles in turn, each with
+// an online softmax of its own, and join at the end.  Sequences of more than
+// one chunk leave (max, sum, o) per chunk to combine_chunks_kernel.
+//
+// The bound is memory: 2 D bytes-of-type per key against 4 D group flop.  So
+// all products run on the matrix cores with the queries padded to 16 (at one
+// query head a 16th of their rate, still several times what the reads need),
+// nothing goes through LDS in the loop, and no operand is transposed there:
+//   * S^T = K Q^T: a lane holds 8 channels of one key, as they lie in memory.
+//     The channels may be contracted in any order, so a lane takes 16
+//     consecutive bytes and the queries are loaded in the same order.
+//   * the scores of key 4g + r of a 16-key half come out in register r of lane
+//     group g (= lane / 16), one query per lane % 16, which is already the B
+//     operand of O^T = V^T P^T with its keys in that order: P needs no move.
+//   * a lane reads V's rows for its group's eight keys, a 16-byte piece of each
+//     row; 4 v_perm per two channels pair the keys up into A operands.
+// K of the next tile is in flight during the softmax and the second product,
+// V of the next during the first.
+//
+// Rounding: scores, softmax and accumulators are FP32.  The weights (times the
+// value's scale in an 8-bit cache) enter the second product as two 16-bit
+// terms, hi + lo, which keeps 16 (BF16) or 22 (FP16) bits of each; FP16
+// weights are scaled by 2^14 so that small ones keep their bits.  Queries of
+// another type than the operands' are split likewise into two or three terms
+// (exactly).  8-bit codes are exact in BF16.
+#pragma once
+
+#include "common.hpp"
+#include "kernels.hpp"
+#include "paged_layout.hpp"
+
+#include <type_traits>
+
+namespace fpx {
+
+struct Fp8Cache {};
+struct Int8Cache {};
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kPagedThreads = 256;
+constexpr int kPagedWaves = kPagedThreads / kWave;
+constexpr float kLn2 = 0.69314718055994531f;
+
+// Sum and maximum over the four lane groups l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float groups_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v),
+                                                  __builtin_bit_cast(unsigned, v), false, false);
+  v = __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+  const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v),
+                                                  __builtin_bit_cast(unsigned, v), false, false);
+  return __builtin_bit_cast(float, (unsigned)s[0]) + __builtin_bit_cast(float, (unsigned)s[1]);
+}
+
+__device__ __forceinline__ float groups_max(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v),
+                                                  __builtin_bit_cast(unsigned, v), false, false);
+  v = fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+  const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v),
+                                                  __builtin_bit_cast(unsigned, v), false, false);
+  return fmaxf(__builtin_bit_cast(float, (unsigned)s[0]),
+               __builtin_bit_cast(float, (unsigned)s[1]));
+}
+
+// kBytes (2, 4, 8 or 16) bytes into 32-bit words, the first in the low bits.
+template <int kBytes>
+__device__ __forceinline__ void load_words(const char* p, uint32_t* w) {
+  if constexpr (kBytes == 2) {
+    w[0] = *reinterpret_cast<const uint16_t*>(p);
+  } else if constexpr (kBytes == 4) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (kBytes == 8) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    w[0] = x.x;
+    w[1] = x.y;
+  } else {
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    w[0] = x.x;
+    w[1] = x.y;
+    w[2] = x.z;
+    w[3] = x.w;
+  }
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const bf16x2 v = {(__bf16)lo, (__bf16)hi};
+  return __builtin_bit_cast(uint32_t, v);
+}
+
+// Two weights as hi + lo 16-bit words.  hi is cut, not rounded, so that lo is
+// never negative, and where values may be infinite (kInfinite) lo is kept above
+// zero: then a value of infinity times a weight comes out infinite, and not as
+// the NaN of a product with zero or of opposite infinities.  What that adds is
+// at most 2^-40 of a weight (FP16: 2^-38 of the largest).
+template <bool kF16, bool kInfinite>
+__device__ __forceinline__ void split_weights(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+  if constexpr (kF16) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x0, x1));
+    float e0 = x0 - (float)h[0], e1 = x1 - (float)h[1];
+    if constexpr (kInfinite) {
+      e0 = fmaxf(e0, fminf(x0, 0x1p-24f));
+      e1 = fmaxf(e1, fminf(x1, 0x1p-24f));
+    }
+    const f16x2 e = {(_Float16)e0, (_Float16)e1};
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, e);
+  } else {
+    const uint32_t b0 = __builtin_bit_cast(uint32_t, x0), b1 = __builtin_bit_cast(uint32_t, x1);
+    hi = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+    float e0 = x0 - __builtin_bit_cast(float, b0 & 0xffff0000u);
+    float e1 = x1 - __builtin_bit_cast(float, b1 & 0xffff0000u);
+    if constexpr (kInfinite) {
+      e0 = fmaxf(e0, x0 * 0x1p-40f);
+      e1 = fmaxf(e1, x1 * 0x1p-40f);
+    }
+    lo = pack_bf16(e0, e1);
+  }
+}
+
+// Two 8-bit codes (bytes 2 kHalf and 2 kHalf + 1 of w) as a word of BF16.
+template <typename C, int kHalf>
+__device__ __forceinline__ uint32_t codes_bf16(uint32_t w) {
+  if constexpr (std::is_same_v<C, Fp8Cache>)
+    return __builtin_bit_cast(uint32_t,
+                              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, kHalf != 0));
+  else
+    return pack_bf16((float)(int8_t)(w >> (16 * kHalf)), (float)(int8_t)(w >> (16 * kHalf + 8)));
+}
+
+template <typename Q, typename C, int D, int QT>
+struct PagedTraits {
+  static constexpr bool kF32 = std::is_same_v<C, float>;
+  static constexpr bool kCoded = std::is_same_v<C, Fp8Cache> || std::is_same_v<C, Int8Cache>;
+  static constexpr bool kF16 = std::is_same_v<C, _Float16>;
+  static constexpr int kElem = kF32 ? 4 : kCoded ? 1 : 2;      // bytes of a cached channel
+  static constexpr int kRow = D * kElem;                       // of a cached row
+  static constexpr int kHalves = kF32 ? 1 : 2;                 // 16-key halves of a tile
+  static constexpr int kTile = 16 * kHalves;
+  // terms a query is split into: all of its bits in BF16, 8 to a term
+  static constexpr int kTerms = !kCoded ? 1 : std::is_same_v<Q, __bf16> ? 1
+                                          : std::is_same_v<Q, _Float16> ? 2 : 3;
+  // K: pieces of kPiece bytes a lane holds of its key's row (16 where a
+  // quarter of the row has them)
+  static constexpr int kPiece = kRow / 4 < 16 ? kRow / 4 : 16;
+  static constexpr int kPieces = kRow / 4 / kPiece;
+  static constexpr int kSteps = kF32 ? D / 4 : D / 32;         // of the first product
+  // V: channels a lane holds of a row, in pieces
+  static constexpr int kChannels = D / 16;
+  static constexpr int kPart = kChannels * kElem < 16 ? kChannels * kElem : 16;  // bytes
+  static constexpr int kParts = kChannels * kElem / kPart;
+  static constexpr int kPartChannels = kPart / kElem;
+  static constexpr int kPartWords = (kPart + 3) / 4;
+  static constexpr float kShift = kF16 ? kWeightShiftF16 : 0.0f;
+};
+
+template <typename Q, typename C, int D, int QT>
+__global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(PagedArgs a) {
+  using T = PagedTraits<Q, C, D, QT>;
+  constexpr int kHalves = T::kHalves;
+  __shared__ float joined[2][QT * T::kChannels * 4][kWave];
+  __shared__ float wave_m[kPagedWaves][QT * 16], wave_l[kPagedWaves][QT * 16];
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = lane & 15, g = lane >> 4;
+  uint32_t block = blockIdx.x;
+  const int split = block % (uint32_t)a.splits;
+  block /= (uint32_t)a.splits;
+  const int qtile = block % (uint32_t)a.qtiles;
+  block /= (uint32_t)a.qtiles;
+  const int head = block % (uint32_t)a.heads;
+  const int b = block / (uint32_t)a.heads;
+
+  const KeyRange range = key_range(a.lengths[b], a.max_length, a.window);
+  const int chunks = chunk_count(range, a.chunk);
+  // a row without keys is written by its first work-group
+  if (split > 0 && split >= chunks) return;
+  const bool direct = chunks <= 1;
+  const int q0 = qtile * 16 * QT;  // the tile's first query head of the group
+
+  const int start = (range.first & ~(kKeyTile - 1)) + split * a.chunk;
+  const int stop = min(range.end, start + a.chunk);
+  const int tiles = stop > start ? (stop - start + T::kTile - 1) / T::kTile : 0;
+  const int mine = tiles > wave ? (tiles - wave + kPagedWaves - 1) / kPagedWaves : 0;
+
+  // the B operand of S^T = K Q^T: query `col`, channels in K's order
+  uint32_t qw[QT][T::kF32 ? T::kSteps : T::kSteps * T::kTerms * 4];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int qi = q0 + t * 16 + col;
+    const bool real = qi < a.group;
+    const Q* q = static_cast<const Q*>(a.q) + b * a.q_b +
+                 (int64_t)(head * a.group + (real ? qi : 0)) * a.q_h;
+    if constexpr (T::kF32) {
+#pragma unroll
+      for (int c = 0; c < T::kPieces; ++c) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(q + 16 * c + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          qw[t][4 * c + i] = real ? __builtin_bit_cast(uint32_t, (float)x[i]) : 0u;
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < T::kSteps; ++s) {
+        const int d = T::kCoded && D > 32 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
+        if constexpr (T::kTerms == 1) {
+          uint32_t w[4];
+          load_words<16>(reinterpret_cast<const char*>(q + d), w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) qw[t][4 * s + i] = real ? w[i] : 0u;
+        } else {
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = real ? (float)q[d + i] : 0.0f;
+#pragma unroll
+          for (int p = 0; p < T::kTerms; ++p) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t w = pack_bf16(x[2 * i], x[2 * i + 1]);
+              qw[t][(p * T::kSteps + s) * 4 + i] = w;
+              // what is left of an infinite value is NaN, which its product
+              // with a key would not be: the first term carries it alone
+              const float r0 = x[2 * i] - __builtin_bit_cast(float, w << 16);
+              const float r1 = x[2 * i + 1] - __builtin_bit_cast(float, w & 0xffff0000u);
+              x[2 * i] = __builtin_isinf(x[2 * i]) ? 0.0f : r0;
+              x[2 * i + 1] = __builtin_isinf(x[2 * i + 1]) ? 0.0f : r1;
+            }
+          }
+        }
+      }
+    }
+  }
+
+  float m[QT], l[QT];
+  f32x4 o[QT][T::kChannels];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    m[t] = -__builtin_inff();
+    l[t] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < T::kChannels; ++c) o[t][c] = {0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  const int page_mask = (1 << a.page_shift) - 1;
+  const char* kbase = static_cast<const char*>(a.k);
+  const char* vbase = static_cast<const char*>(a.v);
+  const int k_lane = col * T::kRow + g * T::kPiece;
+  const int v_lane = 4 * g * T::kRow + col * T::kPart;
+
+  uint32_t kw[kHalves][T::kPieces * T::kPiece / 4];
+  uint32_t vw[kHalves * 4][T::kParts * T::kPartWords];
+  f32x4 ks[kHalves], vs[kHalves];
+
+  // Pages of the wave's next 64 halves, one to a lane; a page outside the
+  // cache is never read: page 0 stands in and the row comes out NaN.
+  int pages_ahead = 0;
+  bool bad = !range.valid;
+  auto look_up = [&](int n) {
+    const int i = n + lane / kHalves;
+    const int key = start + (wave + kPagedWaves * i) * T::kTile + 16 * (lane % kHalves);
+    const int page = a.table[b * a.table_b + table_entry(key, range, a.page_shift)];
+    const bool ok = page_valid(page, a.pages);
+    bad |= !ok;
+    pages_ahead = ok ? page : 0;
+  };
+  constexpr int kAhead = kWave / kHalves;  // tiles a look-up serves
+  auto row_of = [&](int n, int u) -> int64_t {
+    const int page = __builtin_amdgcn_readlane(pages_ahead, (n % kAhead) * kHalves + u);
+    const int key = start + (wave + kPagedWaves * n) * T::kTile + 16 * u;
+    return (((int64_t)page * a.heads + head) << a.page_shift) + (key & page_mask);
+  };
+  auto load_k = [&](int n) {
+#pragma unroll
+    for (int u = 0; u < kHalves; ++u) {
+      const int64_t row = row_of(n, u);
+      const char* p = kbase + row * T::kRow + k_lane;
+#pragma unroll
+      for (int c = 0; c < T::kPieces; ++c)
+        load_words<T::kPiece>(p + c * 64, &kw[u][c * T::kPiece / 4]);
+      if constexpr (T::kCoded) ks[u] = *reinterpret_cast<const f32x4*>(a.k_scale + row + 4 * g);
+    }
+  };
+  auto load_v = [&](int n) {
+#pragma unroll
+    for (int u = 0; u < kHalves; ++u) {
+      const int64_t row = row_of(n, u);
+      const char* p = vbase + row * T::kRow + v_lane;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int c = 0; c < T::kParts; ++c)
+          load_words<T::kPart>(p + r * T::kRow + c * 256, &vw[u * 4 + r][c * T::kPartWords]);
+      if constexpr (T::kCoded) vs[u] = *reinterpret_cast<const f32x4*>(a.v_scale + row + 4 * g);
+    }
+  };
+
+  if (mine > 0) {
+    look_up(0);
+    load_k(0);
+    load_v(0);
+  }
+  for (int n = 0; n < mine; ++n) {
+    const int key0 = start + (wave + kPagedWaves * n) * T::kTile;
+    // ---- S^T = K Q^T
+    f32x4 s[QT][kHalves];
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int u = 0; u < kHalves; ++u) s[t][u] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int u = 0; u < kHalves; ++u) {
+#pragma unroll
+      for (int st = 0; st < T::kSteps; ++st) {
+        if constexpr (T::kF32) {
+          const float x = __builtin_bit_cast(float, kw[u][st]);
+#pragma unroll
+          for (int t = 0; t < QT; ++t)
+            s[t][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                x, __builtin_bit_cast(float, qw[t][st]), s[t][u], 0, 0, 0);
+        } else {
+          u32x4_t x;
+          if constexpr (T::kCoded) {
+            x[0] = codes_bf16<C, 0>(kw[u][2 * st]);
+            x[1] = codes_bf16<C, 1>(kw[u][2 * st]);
+            x[2] = codes_bf16<C, 0>(kw[u][2 * st + 1]);
+            x[3] = codes_bf16<C, 1>(kw[u][2 * st + 1]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = kw[u][4 * st + i];
+          }
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+#pragma unroll
+            for (int p = T::kTerms - 1; p >= 0; --p) {  // the smallest term first
+              const uint32_t* w = &qw[t][(p * T::kSteps + st) * 4];
+              const u32x4_t y = {w[0], w[1], w[2], w[3]};
+              if constexpr (T::kF16)
+                s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                    __builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), s[t][u], 0, 0, 0);
+              else
+                s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    __builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), s[t][u], 0, 0,
+                    0);
+            }
+          }
+        }
+      }
+    }
+    // ---- scores in log2 units, keys outside the range left out
+    const bool edge = key0 < range.first || key0 + T::kTile > range.end;
+#pragma unroll
+    for (int u = 0; u < kHalves; ++u) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int key = key0 + 16 * u + 4 * g + r;
+        const bool seen = !edge || (key >= range.first && key < range.end);
+        float f = a.scale_log2;
+        if constexpr (T::kCoded) f *= ks[u][r];
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+          s[t][u][r] = seen ? s[t][u][r] * f : -__builtin_inff();
+        // what the page holds past the range may be NaN: it must not meet a
+        // weight of zero
+        if (edge && !seen) {
+          if constexpr (T::kCoded) vs[u][r] = 0.0f;
+#pragma unroll
+          for (int i = 0; i < T::kParts * T::kPartWords; ++i) vw[u * 4 + r][i] = 0u;
+        }
+      }
+    }
+    if (n + 1 < mine) {
+      // V of this tile still needs its pages only for what is already loaded
+      if ((n + 1) % kAhead == 0) look_up(n + 1);
+      load_k(n + 1);
+    }
+    // ---- online softmax; a lane's l covers its own group's keys
+    float p[QT][kHalves * 4];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      float top = s[t][0][0];
+#pragma unroll
+      for (int u = 0; u < kHalves; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, s[t][u][r]);
+      const float next = fmaxf(m[t], groups_max(top));
+      const float ref = next == -__builtin_inff() ? 0.0f : next;
+      if (__any(next > m[t])) {
+        const float alpha = exp2_fast(m[t] - ref);
+        l[t] *= alpha;
+#pragma unroll
+        for (int c = 0; c < T::kChannels; ++c) o[t][c] *= alpha;
+      }
+      m[t] = next;
+#pragma unroll
+      for (int u = 0; u < kHalves; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float w = exp2_fast(s[t][u][r] - ref + T::kShift);
+          l[t] += w;
+          if constexpr (T::kCoded)
+            p[t][u * 4 + r] = w * vs[u][r];
+          else
+            p[t][u * 4 + r] = w;
+        }
+    }
+    // ---- O^T += V^T P^T
+    if constexpr (T::kF32) {
+#pragma unroll
+      for (int c = 0; c < T::kChannels; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int t = 0; t < QT; ++t)
+            o[t][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                __builtin_bit_cast(float, vw[r][c]), p[t][r], o[t][c], 0, 0, 0);
+    } else {
+      u32x4_t hi[QT], lo[QT];
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t h, e;
+          split_weights<T::kF16, !T::kCoded>(p[t][2 * i], p[t][2 * i + 1], h, e);
+          hi[t][i] = h;
+          lo[t][i] = e;
+        }
+      constexpr int kWords = (T::kChannels + 1) / 2;  // of 16-bit channels
+      uint32_t v16[8][T::kCoded ? kWords : 1];
+      if constexpr (T::kCoded) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int i = 0; i < kWords; ++i)
+            v16[j][i] = i % 2 == 0 ? codes_bf16<C, 0>(vw[j][i / 2]) : codes_bf16<C, 1>(vw[j][i / 2]);
+      }
+#pragma unroll
+      for (int c = 0; c < T::kChannels; ++c) {
+        u32x4_t x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t first, second;  // keys 2i and 2i + 1 of the lane's eight
+          if constexpr (T::kCoded) {
+            first = v16[2 * i][c / 2];
+            second = v16[2 * i + 1][c / 2];
+          } else {
+            first = vw[2 * i][c / 2];
+            second = vw[2 * i + 1][c / 2];
+          }
+          x[i] = __builtin_amdgcn_perm(second, first, c % 2 ? 0x07060302u : 0x05040100u);
+        }
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          if constexpr (T::kF16) {
+            o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                __builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, lo[t]), o[t][c], 0, 0, 0);
+            o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                __builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, hi[t]), o[t][c], 0, 0, 0);
+          } else {
+            o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                __builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, lo[t]), o[t][c], 0, 0,
+                0);
+            o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                __builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, hi[t]), o[t][c], 0, 0,
+                0);
+          }
+        }
+      }
+    }
+    if (n + 1 < mine) load_v(n + 1);
+  }
+
+  // ---- the four waves joined, in their order
+  if (__any(bad)) {
+#pragma unroll
+    for (int t = 0; t < QT; ++t) l[t] = __builtin_nanf("");
+  }
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    l[t] = groups_sum(l[t]);
+    if (g == 0) {
+      wave_m[wave][t * 16 + col] = m[t];
+      wave_l[wave][t * 16 + col] = l[t];
+    }
+  }
+  __syncthreads();
+  float total[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int w = 0; w < kPagedWaves; ++w) top = fmaxf(top, wave_m[w][t * 16 + col]);
+    const float ref = top == -__builtin_inff() ? 0.0f : top;
+    total[t] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kPagedWaves; ++w)
+      total[t] += wave_l[w][t * 16 + col] * exp2_fast(wave_m[w][t * 16 + col] - ref);
+    const float mine_scale = exp2_fast(m[t] - ref);
+#pragma unroll
+    for (int c = 0; c < T::kChannels; ++c) o[t][c] *= mine_scale;
+    m[t] = top;
+  }
+  // two exchanges: waves 2 and 3 into 0 and 1, then 1 into 0
+#pragma unroll
+  for (int round = 2; round >= 1; round >>= 1) {
+    if (wave >= round && wave < 2 * round) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int c = 0; c < T::kChannels; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            joined[wave - round][(t * T::kChannels + c) * 4 + r][lane] = o[t][c][r];
+    }
+    __syncthreads();
+    if (wave < round) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int c = 0; c < T::kChannels; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            o[t][c][r] += joined[wave][(t * T::kChannels + c) * 4 + r][lane];
+    }
+    __syncthreads();
+  }
+  if (wave != 0) return;
+
+  // ---- O^T: lane (query col, group g), register r of channel c of a part:
+  // channel (4g + r) * kPartChannels + c of the part's 16 * kPartChannels
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int qi = q0 + t * 16 + col;
+    if (qi >= a.group) continue;
+    const int hq = head * a.group + qi;
+    const int64_t row = (int64_t)b * a.heads * a.group + hq;
+    const bool empty = range.valid && range.end <= range.first;
+    const float scale = direct ? (empty ? 0.0f : 1.0f / total[t]) : 1.0f;
+    float* part = a.part + (row * a.splits + split) * D;
+    Q* out = static_cast<Q*>(a.out) + b * a.o_b + hq * a.o_h;
+#pragma unroll
+    for (int pt = 0; pt < T::kParts; ++pt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = pt * 16 * T::kPartChannels + (4 * g + r) * T::kPartChannels;
+#pragma unroll
+        for (int c = 0; c < T::kPartChannels; ++c) {
+          const float x = o[t][pt * T::kPartChannels + c][r] * scale;
+          if (direct)
+            out[d + c] = (Q)x;
+          else
+            part[d + c] = x;
+        }
+      }
+    if (g == 0) {
+      if (!direct) {
+        float* ml = a.part_ml + (row * a.splits + split) * 2;
+        ml[0] = m[t];
+        ml[1] = total[t];
+      } else if (a.lse) {
+        a.lse[row] = empty ? -__builtin_inff()
+                           : (m[t] + __builtin_amdgcn_logf(total[t]) - T::kShift) * kLn2;
+      }
+    }
+  }
+}
+
+template <typename Q, typename C, int D>
+hipError_t launch_paged_dim(const PagedArgs& a, unsigned blocks, hipStream_t stream) {
+  if (a.query_tiles == 1) {
+    paged_attention_kernel<Q, C, D, 1><<<blocks, kPagedThreads, 0, stream>>>(a);
+  } else {
+    if constexpr (D <= 128)
+      paged_attention_kernel<Q, C, D, 2><<<blocks, kPagedThreads, 0, stream>>>(a);
+    else
+      return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+template <typename Q, typename C>
+hipError_t launch_paged_type(const PagedArgs& a, unsigned blocks, hipStream_t stream) {
+  switch (a.head_dim) {
+    case 32: return launch_paged_dim<Q, C, 32>(a, blocks, stream);
+    case 64: return launch_paged_dim<Q, C, 64>(a, blocks, stream);
+    case 128: return launch_paged_dim<Q, C, 128>(a, blocks, stream);
+    default: return launch_paged_dim<Q, C, 256>(a, blocks, stream);
+  }
+}
+
+}  // namespace fpx

@@ -396,6 +396,42 @@ int fpx_cache_read(int row_dtype, int cache_dtype, void* k, int64_t k_st, int64_
                    const float* v_scale, int64_t pages, int heads, int page_size, int head_dim,
                    void* stream);
 
+/* Bytes of workspace fpx_paged_attention needs; 0 for unsupported sizes. */
+size_t fpx_paged_attention_workspace_bytes(int64_t batch, int q_heads, int heads, int head_dim,
+                                           int64_t max_length, int64_t window);
+
+/* Attention of one new token per sequence over a paged cache:
+ *   out[b][h] = sum_j softmax_j(scale * q[b][h] . k_j) v_j
+ * over sequence b's keys j in [max(0, length - window), length) (window = 0:
+ * all), in FP32 with one rounding at the end; query head h reads cache head
+ * h / (q_heads / heads).  No counterpart in the reference.
+ *   dtype       FPX_F32, FPX_BF16 or FPX_F16 of q and out; a plain cache has
+ *               the same type, an 8-bit cache takes any
+ *   q, out      row (b, h) at q + b*q_sb + h*q_sh, channel stride 1, rows
+ *               16-byte aligned; out may be q itself with the same strides
+ *   cache       as fpx_cache_write's
+ *   block_table int32, sequence b's pages at block_table + b*table_sb, at least
+ *               max_length / page_size (rounded up) of them; only the entries
+ *               of pages that hold the keys above are read
+ *   lengths     [batch] int32, the sequences' tokens with the new one
+ *   max_length  no length is larger; the work is cut for it, so a bound near
+ *               the true maximum is fastest
+ *   lse         nullable [batch][q_heads] float: log sum_j exp(scale q . k_j)
+ * A sequence of length 0 gives zeros (lse -inf).  One whose length is negative
+ * or above max_length, or whose block table names a page outside the cache,
+ * gives NaN (out and lse); nothing outside the cache is read.
+ * Supported: the cache's sizes; q_heads a multiple of heads; max_length < 2^30;
+ * batch * q_heads < 2^23 (and its product with the chunks a sequence is cut
+ * into); nothing is launched when batch is 0. */
+int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb, int64_t q_sh,
+                        const void* cache_k, const void* cache_v, const float* k_scale,
+                        const float* v_scale, int64_t pages, int heads, int page_size,
+                        int head_dim, const int32_t* block_table, int64_t table_sb,
+                        int64_t table_pages, const int32_t* lengths, int64_t batch, int q_heads,
+                        int64_t max_length, int64_t window, float scale, void* out, int64_t o_sb,
+                        int64_t o_sh, float* lse, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif
