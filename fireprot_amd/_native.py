@@ -207,28 +207,21 @@ def check(code: int, what: str) -> None:
         raise RuntimeError(f"{what} failed with status {code} ({names.get(code, 'HIP error')})")
 
 
-class on_device:
-    """``with on_device(d) as stream``: device ``d`` current inside, and the
-    handle of its current stream.  Where ``d`` is current already, which is
-    the ordinary call, nothing is switched (a call of a few microseconds
-    otherwise pays as much for the switch as for its launch)."""
+def launch(device: Any, entry: Any, *args: Any) -> int:
+    """``entry(*args, stream)`` with ``device`` current and the handle of its
+    current stream; returns the status.  Where the device is current already,
+    the ordinary call, nothing is switched: a call of a few microseconds would
+    otherwise pay as much for the switch as for its launch."""
+    import torch
 
-    __slots__ = ("index", "previous")
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        return entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return entry(*args, torch._C._cuda_getCurrentRawStream(index))
 
-    def __init__(self, device: Any) -> None:
-        self.index = device.index
 
-    def __enter__(self) -> int:
-        import torch
-
-        self.previous = torch.cuda.current_device()
-        if self.index != self.previous:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
-
-    def __exit__(self, *exc_info: Any) -> bool:
-        if self.index != self.previous:
-            import torch
-
-            torch.cuda.set_device(self.previous)
-        return False
+def repeats(t: Any) -> bool:
+    """Whether some of ``t``'s elements share memory through a zero stride (a
+    broadcast tensor: no output)."""
+    return 0 in t.stride() and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape))

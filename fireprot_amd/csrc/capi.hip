@@ -997,10 +997,12 @@ int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb,
       !aligned_or_null(lse, 4) || (max_length > 0 && !aligned(block_table, 4)) ||
       !cache_pointers_ok(cache_dtype, cache_k, cache_v, k_scale, v_scale))
     return FPX_ERR_POINTER;
-  if (!aligned(workspace, 256)) return FPX_ERR_POINTER;
-  if (workspace_bytes <
-      fpx_paged_attention_workspace_bytes(batch, q_heads, heads, head_dim, max_length, window))
-    return FPX_ERR_WORKSPACE;
+  if (p.splits > 1) {
+    if (!aligned(workspace, 256)) return FPX_ERR_POINTER;
+    if (workspace_bytes <
+        fpx_paged_attention_workspace_bytes(batch, q_heads, heads, head_dim, max_length, window))
+      return FPX_ERR_WORKSPACE;
+  }
   a.q = q;
   a.q_b = q_sb;
   a.q_h = q_sh;

@@ -163,6 +163,12 @@ struct PagedTraits {
   static constexpr int kParts = kChannels * kElem / kPart;
   static constexpr int kPartChannels = kPart / kElem;
   static constexpr int kPartWords = (kPart + 3) / 4;
+  // Registers of a lane: its queries, the tile of K and V in flight, the
+  // accumulators, and what codes are decoded to.  Where they would spill (256 channels, split queries of two
+  // tiles) the queries stay in LDS, which the four waves share.
+  static constexpr int kQueryWords = QT * (kF32 ? kSteps : kSteps * kTerms * 4);
+  static constexpr int kTileWords = kHalves * (kRow / 16 + 4 * kParts * kPartWords);
+  static constexpr bool kQueryLds = kQueryWords + kTileWords + QT * kChannels * 4 + (kCoded ? 16 : 0) > 160;
   static constexpr float kShift = kF16 ? kWeightShiftF16 : 0.0f;
 };
 
@@ -170,6 +176,7 @@ template <typename Q, typename C, int D, int QT>
 __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(PagedArgs a) {
   using T = PagedTraits<Q, C, D, QT>;
   constexpr int kHalves = T::kHalves;
+  __shared__ u32x4_t query_lds[T::kQueryLds ? T::kQueryWords / 4 : 1][kWave];
   __shared__ float joined[2][QT * T::kChannels * 4][kWave];
   __shared__ float wave_m[kPagedWaves][QT * 16], wave_l[kPagedWaves][QT * 16];
 
@@ -196,9 +203,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
   const int mine = tiles > wave ? (tiles - wave + kPagedWaves - 1) / kPagedWaves : 0;
 
   // the B operand of S^T = K Q^T: query `col`, channels in K's order
-  uint32_t qw[QT][T::kF32 ? T::kSteps : T::kSteps * T::kTerms * 4];
+  u32x4_t qw[T::kQueryWords / 4];
+  constexpr int kQuads = T::kQueryWords / 4 / QT;  // of one query tile
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
+    if (T::kQueryLds && wave != 0) break;
     const int qi = q0 + t * 16 + col;
     const bool real = qi < a.group;
     const Q* q = static_cast<const Q*>(a.q) + b * a.q_b +
@@ -209,7 +218,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
         const f32x4 x = *reinterpret_cast<const f32x4*>(q + 16 * c + 4 * g);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          qw[t][4 * c + i] = real ? __builtin_bit_cast(uint32_t, (float)x[i]) : 0u;
+          qw[t * kQuads + c][i] = real ? __builtin_bit_cast(uint32_t, (float)x[i]) : 0u;
       }
     } else {
 #pragma unroll
@@ -219,7 +228,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
           uint32_t w[4];
           load_words<16>(reinterpret_cast<const char*>(q + d), w);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) qw[t][4 * s + i] = real ? w[i] : 0u;
+          for (int i = 0; i < 4; ++i) qw[t * kQuads + s][i] = real ? w[i] : 0u;
         } else {
           float x[8];
 #pragma unroll
@@ -229,7 +238,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const uint32_t w = pack_bf16(x[2 * i], x[2 * i + 1]);
-              qw[t][(p * T::kSteps + s) * 4 + i] = w;
+              qw[t * kQuads + p * T::kSteps + s][i] = w;
               // what is left of an infinite value is NaN, which its product
               // with a key would not be: the first term carries it alone
               const float r0 = x[2 * i] - __builtin_bit_cast(float, w << 16);
@@ -242,6 +251,21 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
       }
     }
   }
+
+  if constexpr (T::kQueryLds) {
+    if (wave == 0) {
+#pragma unroll
+      for (int i = 0; i < T::kQueryWords / 4; ++i) query_lds[i][lane] = qw[i];
+    }
+    __syncthreads();
+  }
+  int query_lane = lane;
+  auto query = [&](int i) -> u32x4_t {
+    if constexpr (T::kQueryLds)
+      return query_lds[i][query_lane];
+    else
+      return qw[i];
+  };
 
   float m[QT], l[QT];
   f32x4 o[QT][T::kChannels];
@@ -313,23 +337,34 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
   }
   for (int n = 0; n < mine; ++n) {
     const int key0 = start + (wave + kPagedWaves * n) * T::kTile;
-    // ---- S^T = K Q^T
+    // (not known to be the same in every tile, so the reads stay in the loop)
+    if constexpr (T::kQueryLds) asm volatile("" : "+v"(query_lane));
+    // ---- S^T = K Q^T.  FP32: four sums of a quarter of the channels, which
+    // halves the rounding of one long sum
     f32x4 s[QT][kHalves];
 #pragma unroll
     for (int t = 0; t < QT; ++t)
 #pragma unroll
       for (int u = 0; u < kHalves; ++u) s[t][u] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (T::kF32) {
 #pragma unroll
-    for (int u = 0; u < kHalves; ++u) {
+      for (int t = 0; t < QT; ++t) {
+        f32x4 sum[4] = {};
 #pragma unroll
-      for (int st = 0; st < T::kSteps; ++st) {
-        if constexpr (T::kF32) {
-          const float x = __builtin_bit_cast(float, kw[u][st]);
+        for (int c = 0; c < T::kPieces; ++c) {
+          const f32x4 y = __builtin_bit_cast(f32x4, query(t * kQuads + c));
 #pragma unroll
-          for (int t = 0; t < QT; ++t)
-            s[t][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                x, __builtin_bit_cast(float, qw[t][st]), s[t][u], 0, 0, 0);
-        } else {
+          for (int i = 0; i < 4; ++i)
+            sum[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                __builtin_bit_cast(float, kw[0][4 * c + i]), y[i], sum[i], 0, 0, 0);
+        }
+        s[t][0] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kHalves; ++u) {
+#pragma unroll
+        for (int st = 0; st < T::kSteps; ++st) {
           u32x4_t x;
           if constexpr (T::kCoded) {
             x[0] = codes_bf16<C, 0>(kw[u][2 * st]);
@@ -344,8 +379,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
           for (int t = 0; t < QT; ++t) {
 #pragma unroll
             for (int p = T::kTerms - 1; p >= 0; --p) {  // the smallest term first
-              const uint32_t* w = &qw[t][(p * T::kSteps + st) * 4];
-              const u32x4_t y = {w[0], w[1], w[2], w[3]};
+              const u32x4_t y = query(t * kQuads + p * T::kSteps + st);
               if constexpr (T::kF16)
                 s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
                     __builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), s[t][u], 0, 0, 0);
@@ -358,30 +392,31 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
         }
       }
     }
-    // ---- scores in log2 units, keys outside the range left out
+    // ---- factors of the scores in log2 units; keys outside the range left out
     const bool edge = key0 < range.first || key0 + T::kTile > range.end;
+    float f[kHalves][T::kCoded ? 4 : 1];
+    uint32_t unseen = 0;  // bit 4u + r
 #pragma unroll
-    for (int u = 0; u < kHalves; ++u) {
+    for (int u = 0; u < kHalves; ++u)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int key = key0 + 16 * u + 4 * g + r;
-        const bool seen = !edge || (key >= range.first && key < range.end);
-        float f = a.scale_log2;
-        if constexpr (T::kCoded) f *= ks[u][r];
+      for (int r = 0; r < (T::kCoded ? 4 : 1); ++r)
+        f[u][r] = T::kCoded ? a.scale_log2 * ks[u][r] : a.scale_log2;
+    if (edge) {
 #pragma unroll
-        for (int t = 0; t < QT; ++t)
-          s[t][u][r] = seen ? s[t][u][r] * f : -__builtin_inff();
-        // what the page holds past the range may be NaN: it must not meet a
-        // weight of zero
-        if (edge && !seen) {
+      for (int u = 0; u < kHalves; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = key0 + 16 * u + 4 * g + r;
+          if (key >= range.first && key < range.end) continue;
+          unseen |= 1u << (4 * u + r);
+          // what the page holds there may be NaN: it must not meet a weight
+          // of zero
           if constexpr (T::kCoded) vs[u][r] = 0.0f;
 #pragma unroll
           for (int i = 0; i < T::kParts * T::kPartWords; ++i) vw[u * 4 + r][i] = 0u;
         }
-      }
     }
     if (n + 1 < mine) {
-      // V of this tile still needs its pages only for what is already loaded
       if ((n + 1) % kAhead == 0) look_up(n + 1);
       load_k(n + 1);
     }
@@ -389,11 +424,14 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
     float p[QT][kHalves * 4];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      float top = s[t][0][0];
+      float top = -__builtin_inff();
 #pragma unroll
       for (int u = 0; u < kHalves; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) top = fmaxf(top, s[t][u][r]);
+        for (int r = 0; r < 4; ++r) {
+          const float x = s[t][u][r] * f[u][T::kCoded ? r : 0];
+          top = fmaxf(top, unseen & (1u << (4 * u + r)) ? -__builtin_inff() : x);
+        }
       const float next = fmaxf(m[t], groups_max(top));
       const float ref = next == -__builtin_inff() ? 0.0f : next;
       if (__any(next > m[t])) {
@@ -407,7 +445,10 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
       for (int u = 0; u < kHalves; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float w = exp2_fast(s[t][u][r] - ref + T::kShift);
+          // one rounding from the product to the exponent
+          const float e = __builtin_fmaf(s[t][u][r], f[u][T::kCoded ? r : 0], -ref);
+          float w = exp2_fast(T::kShift == 0.0f ? e : e + T::kShift);
+          w = unseen & (1u << (4 * u + r)) ? 0.0f : w;
           l[t] += w;
           if constexpr (T::kCoded)
             p[t][u * 4 + r] = w * vs[u][r];
@@ -436,30 +477,23 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
           hi[t][i] = h;
           lo[t][i] = e;
         }
-      constexpr int kWords = (T::kChannels + 1) / 2;  // of 16-bit channels
-      uint32_t v16[8][T::kCoded ? kWords : 1];
-      if constexpr (T::kCoded) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int i = 0; i < kWords; ++i)
-            v16[j][i] = i % 2 == 0 ? codes_bf16<C, 0>(vw[j][i / 2]) : codes_bf16<C, 1>(vw[j][i / 2]);
-      }
+      uint32_t pair[8];  // two channels of the lane's eight keys
 #pragma unroll
       for (int c = 0; c < T::kChannels; ++c) {
+        if (c % 2 == 0) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if constexpr (!T::kCoded)
+              pair[j] = vw[j][c / 2];
+            else
+              pair[j] = c % 4 == 0 ? codes_bf16<C, 0>(vw[j][c / 4]) : codes_bf16<C, 1>(vw[j][c / 4]);
+          }
+        }
         u32x4_t x;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t first, second;  // keys 2i and 2i + 1 of the lane's eight
-          if constexpr (T::kCoded) {
-            first = v16[2 * i][c / 2];
-            second = v16[2 * i + 1][c / 2];
-          } else {
-            first = vw[2 * i][c / 2];
-            second = vw[2 * i + 1][c / 2];
-          }
-          x[i] = __builtin_amdgcn_perm(second, first, c % 2 ? 0x07060302u : 0x05040100u);
-        }
+        for (int i = 0; i < 4; ++i)
+          x[i] = __builtin_amdgcn_perm(pair[2 * i + 1], pair[2 * i],
+                                       c % 2 ? 0x07060302u : 0x05040100u);
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
           if constexpr (T::kF16) {

@@ -126,14 +126,13 @@ def cache_slots(block_table: torch.Tensor, positions: torch.Tensor,
     return torch.where(positions < 0, -1, inside)
 
 
-def _check_rows(t: torch.Tensor, name: str, cache: PagedCache, tokens: int) -> torch.Tensor:
-    if (t.dim() != 3 or t.shape[0] != tokens or t.shape[1] != cache.heads
-            or t.shape[2] != cache.head_dim):
-        raise ValueError(f"{name} must be [{tokens}, {cache.heads}, {cache.head_dim}], "
+def _check_rows(t: torch.Tensor, name: str, cache: PagedCache, tokens: int) -> None:
+    shape = cache.k.shape
+    if t.shape != (tokens, shape[1], shape[3]):
+        raise ValueError(f"{name} must be [{tokens}, {shape[1]}, {shape[3]}], "
                          f"got {tuple(t.shape)}")
     if t.dtype not in ROW_DTYPES or t.device != cache.k.device:
         raise ValueError(f"{name} must be float32, bfloat16 or float16 on the cache's device")
-    return t
 
 
 def _check_slots(slots: torch.Tensor, cache: PagedCache) -> torch.Tensor:
@@ -145,12 +144,11 @@ def _check_slots(slots: torch.Tensor, cache: PagedCache) -> torch.Tensor:
 
 
 def _call(entry, what, row_dtype, cache, k, v, slots):
-    shape = cache.k.shape
-    with _native.on_device(cache.k.device) as stream:
-        code = entry(ROW_DTYPES[row_dtype], CACHE_DTYPES[cache.k.dtype],
-                     k.data_ptr(), k.stride(0), k.stride(1),
-                     v.data_ptr(), v.stride(0), v.stride(1), slots.data_ptr(), slots.shape[0],
-                     *cache.pointers(), shape[0], shape[1], shape[2], shape[3], stream)
+    pages, heads, page_size, head_dim = cache.k.shape
+    code = _native.launch(
+        cache.k.device, entry, ROW_DTYPES[row_dtype], CACHE_DTYPES[cache.k.dtype],
+        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+        slots.data_ptr(), slots.shape[0], *cache.pointers(), pages, heads, page_size, head_dim)
     _native.check(code, what)
 
 
@@ -166,8 +164,8 @@ def cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor,
     """
     lib = _native.library()
     slots = _check_slots(slots, cache)
-    k = _check_rows(k, "k", cache, slots.shape[0])
-    v = _check_rows(v, "v", cache, slots.shape[0])
+    _check_rows(k, "k", cache, slots.shape[0])
+    _check_rows(v, "v", cache, slots.shape[0])
     if v.dtype != k.dtype:
         raise ValueError("k and v must have one type")
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
@@ -194,17 +192,16 @@ def cache_read(cache: PagedCache, slots: torch.Tensor, *, dtype: torch.dtype | N
                  else torch.float32 if cache.dtype in CODED_DTYPES else cache.dtype)
     if dtype not in ROW_DTYPES:
         raise ValueError("rows are read as float32, bfloat16 or float16")
-    outs = []
+    outs, shape = [], cache.k.shape
     for out, name in ((k_out, "k_out"), (v_out, "v_out")):
         if out is None:
-            out = torch.empty((slots.shape[0], cache.heads, cache.head_dim), dtype=dtype,
+            out = torch.empty((slots.shape[0], shape[1], shape[3]), dtype=dtype,
                               device=cache.k.device)
         else:
             _check_rows(out, name, cache, slots.shape[0])
-            if out.dtype != dtype or out.stride(2) != 1:
-                raise ValueError(f"{name} must be {dtype} with unit channel stride")
-            if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
-                raise ValueError(f"{name} must not repeat its elements")
+            if out.dtype != dtype or out.stride(2) != 1 or _native.repeats(out):
+                raise ValueError(f"{name} must be {dtype} with unit channel stride and no "
+                                 "repeated elements")
             if torch.is_grad_enabled() and out.requires_grad:
                 raise ValueError("a cache records no gradient: detach the outputs")
         outs.append(out)

@@ -16,9 +16,12 @@ import torch
 from . import _native
 from .kv_cache import CACHE_DTYPES, CODED_DTYPES, ROW_DTYPES, PagedCache
 
+NO_WORKSPACE = 256  # the size that stands for none
+
 
 def workspace_bytes(q: torch.Tensor, cache: PagedCache, max_length: int, window: int = 0) -> int:
-    """Device workspace of one call (any contents); 0 for unsupported sizes."""
+    """Device workspace of one call (any contents); 0 for unsupported sizes,
+    ``NO_WORKSPACE`` where none is used."""
     return int(_native.library().fpx_paged_attention_workspace_bytes(
         q.shape[0], q.shape[1], cache.k.shape[1], cache.k.shape[3], max_length, window))
 
@@ -84,36 +87,35 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
         block_table = block_table.contiguous()
     if not lengths.is_contiguous():
         lengths = lengths.contiguous()
-    with _native.on_device(q.device) as stream:
-        if out is None:
-            out = torch.empty((batch, q_heads, head_dim), dtype=q.dtype, device=q.device)
-        elif (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device
-              or not _aligned_rows(out)
-              or any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride()))):
-            raise ValueError("out must have q's shape, type and device, 16-byte aligned rows and "
-                             "no repeated elements")
-        lse = (torch.empty((batch, q_heads), dtype=torch.float32, device=q.device)
-               if return_lse else None)
-        size = lib.fpx_paged_attention_workspace_bytes(batch, q_heads, heads, head_dim, max_length,
-                                                       window)
-        if size == 0:
-            raise ValueError(f"unsupported sizes: batch {batch}, {q_heads} query heads, "
-                             f"max_length {max_length}, window {window}")
-        if workspace is None:
-            # of the current stream, and of the graph where one is captured: no
-            # two calls that may overlap share it
-            workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
-        elif (workspace.dtype != torch.uint8 or workspace.device != q.device
-              or workspace.numel() < size or not workspace.is_contiguous()):
+    if out is None:
+        out = torch.empty((batch, q_heads, head_dim), dtype=q.dtype, device=q.device)
+    elif (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device
+          or not _aligned_rows(out) or _native.repeats(out)):
+        raise ValueError("out must have q's shape, type and device, 16-byte aligned rows and "
+                         "no repeated elements")
+    lse = (torch.empty((batch, q_heads), dtype=torch.float32, device=q.device)
+           if return_lse else None)
+    size = lib.fpx_paged_attention_workspace_bytes(batch, q_heads, heads, head_dim, max_length,
+                                                   window)
+    if size == 0:
+        raise ValueError(f"unsupported sizes: batch {batch}, {q_heads} query heads, "
+                         f"max_length {max_length}, window {window}")
+    if workspace is not None:
+        if (workspace.dtype != torch.uint8 or workspace.device != q.device
+                or workspace.numel() < size or not workspace.is_contiguous()):
             raise ValueError(f"workspace must be {size} contiguous bytes on q's device")
-        code = lib.fpx_paged_attention(
-            ROW_DTYPES[q.dtype], CACHE_DTYPES[k.dtype], q.data_ptr(), q.stride(0), q.stride(1),
-            *cache.pointers(), pages, heads, page_size, head_dim,
-            block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-            lengths.data_ptr(), batch, q_heads, max_length, window,
-            head_dim ** -0.5 if scale is None else scale,
-            out.data_ptr(), out.stride(0), out.stride(1),
-            None if lse is None else lse.data_ptr(), workspace.data_ptr(), workspace.numel(),
-            stream)
+    elif size > NO_WORKSPACE:
+        # of the current stream, and of the graph where one is captured: no two
+        # calls that may overlap share it
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+    qs, os = q.stride(), out.stride()
+    code = _native.launch(
+        q.device, lib.fpx_paged_attention, ROW_DTYPES[q.dtype], CACHE_DTYPES[k.dtype],
+        q.data_ptr(), qs[0], qs[1], *cache.pointers(), pages, heads, page_size, head_dim,
+        block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+        lengths.data_ptr(), batch, q_heads, max_length, window,
+        head_dim ** -0.5 if scale is None else scale, out.data_ptr(), os[0], os[1],
+        None if lse is None else lse.data_ptr(),
+        None if workspace is None else workspace.data_ptr(), size)
     _native.check(code, "fpx_paged_attention")
     return (out, lse) if return_lse else out

@@ -27,6 +27,7 @@ MAX_HEAD_DIM = 512
 LAYOUTS = {"half": 0, "interleaved": 1}
 DTYPES = {torch.float32: _native.FPX_F32, torch.bfloat16: _native.FPX_BF16,
           torch.float16: _native.FPX_F16}
+POSITION_DTYPES = {torch.int32: 0, torch.int64: 1}
 
 
 @dataclasses.dataclass
@@ -90,68 +91,71 @@ def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
     """``t`` as [batch, tokens, heads, head_dim] with unit channel stride."""
     if t.dim() == 3:
         t = t.unsqueeze(0)
-    if t.dim() != 4:
+    elif t.dim() != 4:
         raise ValueError(f"{name} must be [batch, tokens, heads, head_dim] or "
                          f"[tokens, heads, head_dim], got {tuple(t.shape)}")
-    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+    return t if t.stride(3) == 1 else t.contiguous()
+
+
+def _output(given: torch.Tensor | None, like: torch.Tensor, rows: torch.Tensor, name: str):
+    """(the four-axis output, what the caller gets) for an input and its rows."""
+    if given is None:
+        out = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
+        return out, out if like.dim() == 4 else out[0]
+    if (given.shape != like.shape or given.dtype != like.dtype or given.device != like.device
+            or given.stride(-1) != 1 or _native.repeats(given)):
+        raise ValueError(f"{name} must have its input's shape, type and device, unit channel "
+                         "stride and no repeated elements")
+    return given if given.dim() == 4 else given.unsqueeze(0), given
 
 
 def _launch(q, k, positions, frequencies, layout, inverse, q_out, k_out):
     """Checks, then one fpx_rotary call into q_out and k_out (new where None)."""
     lib = _native.library()
-    if layout not in LAYOUTS:
+    mode = LAYOUTS.get(layout)
+    if mode is None:
         raise ValueError(f"layout must be one of {sorted(LAYOUTS)}")
-    inv_freq = frequencies.inv_freq
-    if not q.is_cuda or q.dtype not in DTYPES:
+    kind, device = DTYPES.get(q.dtype), q.device
+    if kind is None or not q.is_cuda:
         raise ValueError("q must be a float32, bfloat16 or float16 tensor on a HIP device")
-    device = q.device
-    if k is not None and (k.dtype != q.dtype or k.device != device or k.dim() != q.dim()
-                          or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]):
-        raise ValueError("k must have q's type, device, batch, tokens and head_dim")
+    x = _rows(q, "q")
+    batch, tokens, q_heads, head_dim = x.shape
+    inv_freq = frequencies.inv_freq
     if (inv_freq.dtype != torch.float64 or inv_freq.device != device or inv_freq.dim() != 1
             or not inv_freq.is_contiguous()):
         raise ValueError("inv_freq must be a contiguous float64 vector on q's device")
-    x, y = _rows(q, "q"), None if k is None else _rows(k, "k")
-    batch, tokens, q_heads, head_dim = x.shape
-    k_heads = 0 if y is None else y.shape[2]
-    rotary_dim = frequencies.rotary_dim
+    rotary_dim = 2 * inv_freq.shape[0]
     if not 2 <= rotary_dim <= head_dim <= MAX_HEAD_DIM:
         raise ValueError(f"needs 2 <= rotary_dim ({rotary_dim}) <= head_dim ({head_dim}) "
                          f"<= {MAX_HEAD_DIM}")
-    if (positions.dtype not in (torch.int32, torch.int64) or positions.device != device
-            or tuple(positions.shape) not in ((batch, tokens), (tokens,))):
+    wide = positions.dim() == 2
+    if (positions.dtype not in POSITION_DTYPES or positions.device != device
+            or positions.shape != ((batch, tokens) if wide else (tokens,))):
         raise ValueError("positions must be int32 or int64 [batch, tokens] or [tokens] "
                          "on q's device")
-    outs = []
-    for given, source, name in ((q_out, x, "q"), (k_out, y, "k")):
-        if source is None:
-            outs.append((None, None))
-            continue
-        if given is None:
-            given = torch.empty(source.shape, dtype=q.dtype, device=device)
-            outs.append((given, given if q.dim() == 4 else given[0]))
-            continue
-        if (given.shape != (q if name == "q" else k).shape or given.dtype != q.dtype
-                or given.device != device or given.stride(-1) != 1):
-            raise ValueError(f"{name}_out must have {name}'s shape, type and device and unit "
-                             "channel stride")
-        if any(n > 1 and s == 0 for n, s in zip(given.shape, given.stride())):
-            raise ValueError(f"{name}_out must not repeat its elements")
-        outs.append((given if given.dim() == 4 else given.unsqueeze(0), given))
-    (a, q_ret), (b, k_ret) = outs
-    if q.numel() == 0 and k_heads == 0:
+    a, q_ret = _output(q_out, q, x, "q_out")
+    if k is None:
+        k_heads, k_ret = 0, None
+        k_args = k_out_args = (None, 0, 0, 0)
+    else:
+        if (k.dtype != q.dtype or k.device != device or k.dim() != q.dim()
+                or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != head_dim):
+            raise ValueError("k must have q's type, device, batch, tokens and head_dim")
+        y = _rows(k, "k")
+        k_heads = y.shape[2]
+        b, k_ret = _output(k_out, k, y, "k_out")
+        s, t = y.stride(), b.stride()
+        k_args = (y.data_ptr(), s[0], s[1], s[2])
+        k_out_args = (b.data_ptr(), t[0], t[1], t[2])
+    if q_heads == 0 and k_heads == 0:
         return q_ret, k_ret
-    none = (None, 0, 0, 0)
-    with _native.on_device(device) as stream:
-        code = lib.fpx_rotary(
-            DTYPES[q.dtype], LAYOUTS[layout], x.data_ptr(), *x.stride()[:3],
-            a.data_ptr(), *a.stride()[:3], q_heads,
-            *(none if y is None else (y.data_ptr(), *y.stride()[:3])),
-            *(none if b is None else (b.data_ptr(), *b.stride()[:3])), k_heads,
-            positions.data_ptr(), int(positions.dtype == torch.int64),
-            positions.stride(0) if positions.dim() == 2 else 0, positions.stride(-1),
-            inv_freq.data_ptr(), frequencies.scale, int(inverse), batch, tokens, head_dim,
-            rotary_dim, stream)
+    s, t = x.stride(), a.stride()
+    code = _native.launch(
+        device, lib.fpx_rotary, kind, mode, x.data_ptr(), s[0], s[1], s[2],
+        a.data_ptr(), t[0], t[1], t[2], q_heads, *k_args, *k_out_args, k_heads,
+        positions.data_ptr(), POSITION_DTYPES[positions.dtype],
+        positions.stride(0) if wide else 0, positions.stride(-1),
+        inv_freq.data_ptr(), frequencies.scale, inverse, batch, tokens, head_dim, rotary_dim)
     _native.check(code, "fpx_rotary")
     return q_ret, k_ret
 

@@ -396,7 +396,9 @@ int fpx_cache_read(int row_dtype, int cache_dtype, void* k, int64_t k_st, int64_
                    const float* v_scale, int64_t pages, int heads, int page_size, int head_dim,
                    void* stream);
 
-/* Bytes of workspace fpx_paged_attention needs; 0 for unsupported sizes. */
+/* Bytes of workspace fpx_paged_attention needs; 0 for unsupported sizes, 256
+ * where it uses none (no sequence can need more than one chunk): its workspace
+ * may then be null. */
 size_t fpx_paged_attention_workspace_bytes(int64_t batch, int q_heads, int heads, int head_dim,
                                            int64_t max_length, int64_t window);
 

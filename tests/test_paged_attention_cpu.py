@@ -41,7 +41,8 @@ def test_sizes_are_refused(lib, bad):
 @pytest.mark.parametrize("bad", [
     dict(q=None), dict(q=264), dict(out=None), dict(out=2056), dict(cache_k=None),
     dict(cache_v=520), dict(block_table=None), dict(block_table=258), dict(lengths=None),
-    dict(lengths=257), dict(lse=258), dict(workspace=None), dict(workspace=128),
+    dict(lengths=257), dict(lse=258), dict(workspace=None, max_length=4096, table_pages=256),
+    dict(workspace=128, max_length=4096, table_pages=256),
     dict(cache_dtype=3), dict(cache_dtype=4, k_scale=256, v_scale=264)])
 def test_pointers_are_refused(lib, bad):
     assert lib.fpx_paged_attention(*_args(**bad)) == _native.FPX_ERR_POINTER
@@ -49,7 +50,6 @@ def test_pointers_are_refused(lib, bad):
 
 def test_workspace(lib):
     size = lib.fpx_paged_attention_workspace_bytes
-    assert lib.fpx_paged_attention(*_args(workspace_bytes=255)) == _native.FPX_ERR_WORKSPACE
     long = dict(max_length=1 << 16, table_pages=1 << 12)
     need = size(3, 8, 2, 128, 1 << 16, 0)
     assert need > 3 * 8 * 2 * (128 + 2) * 4  # at least two chunks a sequence
