@@ -423,7 +423,7 @@ int cache_impl(bool read, int row_dtype, int cache_dtype, const void* k, int64_t
   return status(fpx::launch_cache(a, read, static_cast<hipStream_t>(stream)));
 }
 
-constexpr int64_t kPagedMaxRows = 1 << 23;  // 2^31 threads of 256 a row
+constexpr int64_t kPagedMaxRows = 1 << 23;  // work-groups of 256: 2^31 threads
 
 // The cut of a call's work, blocks = 0 for unsupported sizes.
 fpx::PagedPlan paged_plan(int64_t batch, int q_heads, int heads, int head_dim, int64_t max_length,
@@ -435,8 +435,11 @@ fpx::PagedPlan paged_plan(int64_t batch, int q_heads, int heads, int head_dim, i
   if (head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256) return none;
   if (max_length < 0 || max_length >= (1 << 30) || window < 0) return none;
   const int w = window < (1 << 30) ? (int)window : 0;  // wider than any sequence: all keys
+  if (batch > 65535 || q_heads > 65535) return none;  // the grid's y and z
   const fpx::PagedPlan p = fpx::plan_paged(batch < 1 ? 1 : batch, heads, q_heads / heads, head_dim,
                                            (int)max_length, w);
+  // (the join's grid: 32 channels of a row each)
+  if (p.splits > 1 && batch * q_heads * (head_dim / 32) >= 2 * kPagedMaxRows) return none;
   return p.blocks < kPagedMaxRows ? p : none;
 }
 

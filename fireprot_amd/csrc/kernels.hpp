@@ -466,11 +466,11 @@ PagedPlan plan_paged(int64_t batch, int heads, int group, int head_dim, int max_
                      int window);
 hipError_t launch_paged_attention(const PagedArgs& args, hipStream_t stream);
 // one cache type each (paged_attention_*.hip)
-hipError_t launch_paged_f32(const PagedArgs& args, unsigned blocks, hipStream_t stream);
-hipError_t launch_paged_bf16(const PagedArgs& args, unsigned blocks, hipStream_t stream);
-hipError_t launch_paged_f16(const PagedArgs& args, unsigned blocks, hipStream_t stream);
-hipError_t launch_paged_fp8(const PagedArgs& args, unsigned blocks, hipStream_t stream);
-hipError_t launch_paged_int8(const PagedArgs& args, unsigned blocks, hipStream_t stream);
+hipError_t launch_paged_f32(const PagedArgs& args, hipStream_t stream);
+hipError_t launch_paged_bf16(const PagedArgs& args, hipStream_t stream);
+hipError_t launch_paged_f16(const PagedArgs& args, hipStream_t stream);
+hipError_t launch_paged_fp8(const PagedArgs& args, hipStream_t stream);
+hipError_t launch_paged_int8(const PagedArgs& args, hipStream_t stream);
 
 int device_cu_count();
 

@@ -8,72 +8,103 @@ namespace fpx {
 namespace {
 
 constexpr int kCombineThreads = 256;
+constexpr int kCombineAhead = 4;       // chunks of a thread
+constexpr int kCombineFewRows = 256;   // rows that take several work-groups each
 
-// One work-group per (sequence, query head) of more than one chunk: the
-// chunks' (max, sum) become weights in LDS, then 4-channel vectors of the
-// chunks' outputs are summed, 256 / (D / 4) chunks at a time and in a fixed
-// order.
-template <typename Q, int D>
+// One work-group per kChannels channels of a (sequence, query head): the
+// chunks' (max, sum) become weights in LDS, 4-channel vectors of the chunks'
+// outputs are summed kLanes chunks at a time, and those sums in a fixed order.
+// The launch is a chain of waits and little else, so the first outputs are
+// asked for before anything is known of the chunks' number (their places exist
+// in every row; those past the row's chunks are never used).
+template <typename Q, int D, int kChannels>
 __global__ __launch_bounds__(kCombineThreads) void combine_chunks_kernel(PagedArgs a) {
-  constexpr int kVecs = D / 4;
-  constexpr int kLanes = kCombineThreads / kVecs;  // chunks at a time
+  constexpr int kVecs = kChannels / 4;
+  constexpr int kLanes = kCombineThreads / kVecs;
   __shared__ float weight[kMaxChunks];
-  __shared__ float red[kCombineThreads / kWave];
+  __shared__ float red[2][kCombineThreads / kWave];
   __shared__ f32x4 sums[kLanes][kVecs];
   const int row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const int vec = tid % kVecs, first = tid / kVecs;
+  const f32x4* parts = reinterpret_cast<const f32x4*>(a.part + (int64_t)row * a.splits * D +
+                                                      blockIdx.y * kChannels) + vec;
+  const float* ml = a.part_ml + (int64_t)row * a.splits * 2;
+  f32x4 ahead[kCombineAhead];
+#pragma unroll
+  for (int i = 0; i < kCombineAhead; ++i) {
+    const int c = first + i * kLanes;
+    if (c < a.splits) ahead[i] = parts[(int64_t)c * (D / 4)];
+  }
+  float m = -__builtin_inff(), l = 0.0f;
+  if (tid < a.splits) {
+    m = ml[2 * tid];
+    l = ml[2 * tid + 1];
+  }
   const int q_heads = a.heads * a.group;
   const int b = row / q_heads, hq = row - b * q_heads;
   const int chunks = chunk_count(key_range(a.lengths[b], a.max_length, a.window), a.chunk);
   if (chunks <= 1) return;  // written by its only work-group
-
-  const float* ml = a.part_ml + (int64_t)row * a.splits * 2;
-  const int tid = threadIdx.x;
-  const bool has = tid < chunks;
-  const float m = has ? ml[2 * tid] : -__builtin_inff();
-  const float l = has ? ml[2 * tid + 1] : 0.0f;
-  // (a NaN maximum cannot be: a NaN score leaves it out and makes the sum NaN)
+  if (tid >= chunks) {
+    m = -__builtin_inff();
+    l = 0.0f;
+  }
+  // (a maximum is never NaN: a NaN score leaves it alone and makes the sum NaN)
   float top = wave_max(m);
-  if ((tid & 63) == 0) red[tid >> 6] = top;
+  if ((tid & 63) == 0) red[0][tid >> 6] = top;
   __syncthreads();
-  top = red[0];
+  top = red[0][0];
 #pragma unroll
-  for (int w = 1; w < kCombineThreads / kWave; ++w) top = fmaxf(top, red[w]);
-  const float ref = top == -__builtin_inff() ? 0.0f : top;
-  const float w = exp2_fast(m - ref);
+  for (int w = 1; w < kCombineThreads / kWave; ++w) top = fmaxf(top, red[0][w]);
+  const float w = exp2_fast(m - (top == -__builtin_inff() ? 0.0f : top));
   weight[tid] = w;
+  const float part = wave_sum(w * l);
+  if ((tid & 63) == 0) red[1][tid >> 6] = part;
   __syncthreads();
-  const float part = wave_sum(has ? w * l : 0.0f);
-  if ((tid & 63) == 0) red[tid >> 6] = part;
-  __syncthreads();
-  float total = red[0];
+  float total = red[1][0];
 #pragma unroll
-  for (int i = 1; i < kCombineThreads / kWave; ++i) total += red[i];
+  for (int i = 1; i < kCombineThreads / kWave; ++i) total += red[1][i];
 
-  const int vec = tid % kVecs, first = tid / kVecs;
-  const f32x4* parts = reinterpret_cast<const f32x4*>(a.part + (int64_t)row * a.splits * D) + vec;
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int c = first; c < chunks; c += kLanes) acc += parts[(int64_t)c * kVecs] * weight[c];
+#pragma unroll
+  for (int i = 0; i < kCombineAhead; ++i) {
+    const int c = first + i * kLanes;
+    if (c < chunks) acc += ahead[i] * weight[c];
+  }
+  for (int c = first + kCombineAhead * kLanes; c < chunks; c += kLanes)
+    acc += parts[(int64_t)c * (D / 4)] * weight[c];
   sums[first][vec] = acc;
   __syncthreads();
-  if (first == 0) {
-#pragma unroll
-    for (int i = 1; i < kLanes; ++i) acc += sums[i][vec];
-    Q* out = static_cast<Q*>(a.out) + b * a.o_b + hq * a.o_h + 4 * vec;
-    const float scale = 1.0f / total;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] = (Q)(acc[i] * scale);
+  if (tid < kChannels) {
+    const float* column = reinterpret_cast<const float*>(sums) + tid;
+    const int used = chunks < kLanes ? chunks : kLanes;
+    float x = 0.0f;
+    for (int i = 0; i < used; ++i) x += column[i * kChannels];
+    static_cast<Q*>(a.out)[b * a.o_b + hq * a.o_h + blockIdx.y * kChannels + tid] =
+        (Q)(x / total);
   }
-  if (tid == 0 && a.lse)
+  if (tid == 0 && blockIdx.y == 0 && a.lse)
     a.lse[row] = (top + __builtin_amdgcn_logf(total) - a.weight_shift) * 0.69314718055994531f;
+}
+
+// 32 channels to a work-group while there are few rows (32 rows of 256 chunks:
+// 5.5 us, 15 us with whole rows), whole rows otherwise (1024 rows of 7 chunks:
+// 4.9 us, 7.0 us in 32s).
+template <typename Q, int D>
+void launch_combine_dim(const PagedArgs& a, unsigned rows, hipStream_t stream) {
+  if (D > 32 && rows <= kCombineFewRows)
+    combine_chunks_kernel<Q, D, 32><<<dim3(rows, D / 32), kCombineThreads, 0, stream>>>(a);
+  else
+    combine_chunks_kernel<Q, D, D><<<rows, kCombineThreads, 0, stream>>>(a);
 }
 
 template <typename Q>
 void launch_combine(const PagedArgs& a, unsigned rows, hipStream_t stream) {
   switch (a.head_dim) {
-    case 32: combine_chunks_kernel<Q, 32><<<rows, kCombineThreads, 0, stream>>>(a); break;
-    case 64: combine_chunks_kernel<Q, 64><<<rows, kCombineThreads, 0, stream>>>(a); break;
-    case 128: combine_chunks_kernel<Q, 128><<<rows, kCombineThreads, 0, stream>>>(a); break;
-    default: combine_chunks_kernel<Q, 256><<<rows, kCombineThreads, 0, stream>>>(a); break;
+    case 32: launch_combine_dim<Q, 32>(a, rows, stream); break;
+    case 64: launch_combine_dim<Q, 64>(a, rows, stream); break;
+    case 128: launch_combine_dim<Q, 128>(a, rows, stream); break;
+    default: launch_combine_dim<Q, 256>(a, rows, stream); break;
   }
 }
 
@@ -103,14 +134,13 @@ PagedPlan plan_paged(int64_t batch, int heads, int group, int head_dim, int max_
 }
 
 hipError_t launch_paged_attention(const PagedArgs& a, hipStream_t stream) {
-  const unsigned blocks = (unsigned)((int64_t)a.batch * a.heads * a.qtiles * a.splits);
   hipError_t e;
   switch (a.cache_dtype) {
-    case 0: e = launch_paged_f32(a, blocks, stream); break;
-    case 1: e = launch_paged_bf16(a, blocks, stream); break;
-    case 2: e = launch_paged_f16(a, blocks, stream); break;
-    case 3: e = launch_paged_fp8(a, blocks, stream); break;
-    default: e = launch_paged_int8(a, blocks, stream); break;
+    case 0: e = launch_paged_f32(a, stream); break;
+    case 1: e = launch_paged_bf16(a, stream); break;
+    case 2: e = launch_paged_f16(a, stream); break;
+    case 3: e = launch_paged_fp8(a, stream); break;
+    default: e = launch_paged_int8(a, stream); break;
   }
   if (e != hipSuccess || a.splits == 1) return e;
   const unsigned rows = (unsigned)((int64_t)a.batch * a.heads * a.group);

@@ -3,11 +3,11 @@
 
 namespace fpx {
 
-hipError_t launch_paged_int8(const PagedArgs& a, unsigned blocks, hipStream_t stream) {
+hipError_t launch_paged_int8(const PagedArgs& a, hipStream_t stream) {
   switch (a.dtype) {
-    case 0: return launch_paged_type<float, Int8Cache>(a, blocks, stream);
-    case 1: return launch_paged_type<__bf16, Int8Cache>(a, blocks, stream);
-    default: return launch_paged_type<_Float16, Int8Cache>(a, blocks, stream);
+    case 0: return launch_paged_type<float, Int8Cache>(a, stream);
+    case 1: return launch_paged_type<__bf16, Int8Cache>(a, stream);
+    default: return launch_paged_type<_Float16, Int8Cache>(a, stream);
   }
 }
 

@@ -423,8 +423,8 @@ size_t fpx_paged_attention_workspace_bytes(int64_t batch, int q_heads, int heads
  * or above max_length, or whose block table names a page outside the cache,
  * gives NaN (out and lse); nothing outside the cache is read.
  * Supported: the cache's sizes; q_heads a multiple of heads; max_length < 2^30;
- * batch * q_heads < 2^23 (and its product with the chunks a sequence is cut
- * into); nothing is launched when batch is 0. */
+ * batch and q_heads up to 65535, their product, and its product with the chunks
+ * a sequence is cut into, below 2^23; nothing is launched when batch is 0. */
 int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb, int64_t q_sh,
                         const void* cache_k, const void* cache_v, const float* k_scale,
                         const float* v_scale, int64_t pages, int heads, int page_size,
