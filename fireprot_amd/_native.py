@@ -131,7 +131,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         _p, _p, _p, _p,              # cache_k, cache_v, k_scale, v_scale
         _i64, _i, _i, _i, _p,        # pages, heads, page_size, head_dim, stream
     ]),
-    "fpx_paged_attention_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i64, _i64]),
+    "fpx_paged_attention_workspace_bytes": (_sz, [_i, _i64, _i, _i, _i, _i64, _i64]),
     "fpx_paged_attention": (_i, [
         _i, _i,                      # dtype, cache_dtype
         _p, _i64, _i64,              # q, strides (batch, head)

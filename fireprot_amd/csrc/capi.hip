@@ -423,28 +423,34 @@ int cache_impl(bool read, int row_dtype, int cache_dtype, const void* k, int64_t
   return status(fpx::launch_cache(a, read, static_cast<hipStream_t>(stream)));
 }
 
-constexpr int64_t kPagedMaxRows = 1 << 23;  // work-groups of 256: 2^31 threads
+constexpr int64_t kPagedMaxRows = 1 << 20;  // (sequence, query head): the join's grid
 
-// The cut of a call's work, blocks = 0 for unsupported sizes.
-fpx::PagedPlan paged_plan(int64_t batch, int q_heads, int heads, int head_dim, int64_t max_length,
-                          int64_t window) {
-  fpx::PagedPlan none{};
-  if (batch < 0 || batch >= kPagedMaxRows || heads < 1 || q_heads < heads || q_heads % heads ||
-      q_heads >= kPagedMaxRows || batch * q_heads >= kPagedMaxRows)
+// The cut of a call's work, units = 0 for unsupported sizes.
+fpx::PagedPlan paged_plan(int cache_dtype, int64_t batch, int q_heads, int heads, int head_dim,
+                          int64_t max_length, int64_t window) {
+  const fpx::PagedPlan none{};
+  if (!row_type_ok(cache_dtype) && !is_coded(cache_dtype)) return none;
+  if (batch < 0 || batch > kPagedMaxRows || heads < 1 || q_heads < heads || q_heads % heads ||
+      q_heads > kPagedMaxRows || batch * q_heads > kPagedMaxRows)
     return none;
   if (head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256) return none;
   if (max_length < 0 || max_length >= (1 << 30) || window < 0) return none;
-  const int w = window < (1 << 30) ? (int)window : 0;  // wider than any sequence: all keys
-  if (batch > 65535 || q_heads > 65535) return none;  // the grid's y and z
-  const fpx::PagedPlan p = fpx::plan_paged(batch < 1 ? 1 : batch, heads, q_heads / heads, head_dim,
-                                           (int)max_length, w);
-  // (the join's grid: 32 channels of a row each)
-  if (p.splits > 1 && batch * q_heads * (head_dim / 32) >= 2 * kPagedMaxRows) return none;
-  return p.blocks < kPagedMaxRows ? p : none;
+  return fpx::plan_paged(cache_dtype, batch < 1 ? 1 : batch, heads, q_heads / heads, head_dim,
+                         max_length, window < (1 << 30) ? window : 0);
 }
 
-size_t paged_part_bytes(const fpx::PagedPlan& p, int64_t batch, int q_heads, int head_dim) {
-  return (size_t)round_up((int64_t)batch * q_heads * p.splits * head_dim * 4, 256);
+// Places of the rows' shares, their (max, sum), and the rows' places.
+struct PagedWorkspace {
+  size_t ml, info, total;
+};
+
+PagedWorkspace paged_workspace(const fpx::PagedPlan& p, int64_t batch, int heads, int head_dim) {
+  const int64_t places = (int64_t)p.groups * 2 * p.tile_queries;
+  PagedWorkspace w{};
+  w.ml = (size_t)round_up(places * head_dim * 4, 256);
+  w.info = w.ml + (size_t)round_up(places * 8, 256);
+  w.total = w.info + (size_t)(batch * heads * p.qtiles * 8);
+  return w;
 }
 
 }  // namespace
@@ -966,12 +972,12 @@ int fpx_cache_read(int row_dtype, int cache_dtype, void* k, int64_t k_st, int64_
                     cache_k, cache_v, k_scale, v_scale, pages, heads, page_size, head_dim, stream);
 }
 
-size_t fpx_paged_attention_workspace_bytes(int64_t batch, int q_heads, int heads, int head_dim,
-                                           int64_t max_length, int64_t window) {
-  const fpx::PagedPlan p = paged_plan(batch, q_heads, heads, head_dim, max_length, window);
-  if (p.blocks == 0) return 0;
-  if (p.splits == 1) return 256;  // nothing is left between launches
-  return paged_part_bytes(p, batch, q_heads, head_dim) + (size_t)batch * q_heads * p.splits * 8;
+size_t fpx_paged_attention_workspace_bytes(int cache_dtype, int64_t batch, int q_heads, int heads,
+                                           int head_dim, int64_t max_length, int64_t window) {
+  const fpx::PagedPlan p =
+      paged_plan(cache_dtype, batch, q_heads, heads, head_dim, max_length, window);
+  if (p.units == 0) return 0;
+  return p.split ? paged_workspace(p, batch, heads, head_dim).total : 256;
 }
 
 int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb, int64_t q_sh,
@@ -986,8 +992,9 @@ int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb,
   const int rc = cache_dims(cache_dtype, pages, heads, page_size, head_dim, &a.page_shift);
   if (rc != FPX_OK) return rc;
   if (!row_type_ok(dtype) || (!is_coded(cache_dtype) && cache_dtype != dtype)) return FPX_ERR_DIMS;
-  const fpx::PagedPlan p = paged_plan(batch, q_heads, heads, head_dim, max_length, window);
-  if (p.blocks == 0) return FPX_ERR_DIMS;
+  const fpx::PagedPlan p =
+      paged_plan(cache_dtype, batch, q_heads, heads, head_dim, max_length, window);
+  if (p.units == 0) return FPX_ERR_DIMS;
   const int64_t row = 16 / (int64_t)type_bytes(dtype);
   if (q_sb < 0 || q_sh < 0 || o_sb < 0 || o_sh < 0 || q_sb % row || q_sh % row || o_sb % row ||
       o_sh % row)
@@ -1000,11 +1007,14 @@ int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb,
       !aligned_or_null(lse, 4) || (max_length > 0 && !aligned(block_table, 4)) ||
       !cache_pointers_ok(cache_dtype, cache_k, cache_v, k_scale, v_scale))
     return FPX_ERR_POINTER;
-  if (p.splits > 1) {
+  const PagedWorkspace ws = paged_workspace(p, batch, heads, head_dim);
+  if (p.split) {
     if (!aligned(workspace, 256)) return FPX_ERR_POINTER;
-    if (workspace_bytes <
-        fpx_paged_attention_workspace_bytes(batch, q_heads, heads, head_dim, max_length, window))
-      return FPX_ERR_WORKSPACE;
+    if (workspace_bytes < ws.total) return FPX_ERR_WORKSPACE;
+    char* base = static_cast<char*>(workspace);
+    a.part = as<float>(base);
+    a.part_ml = as<float>(base + ws.ml);
+    a.row_info = as<int>(base + ws.info);
   }
   a.q = q;
   a.q_b = q_sb;
@@ -1020,9 +1030,6 @@ int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb,
   a.o_b = o_sb;
   a.o_h = o_sh;
   a.lse = lse;
-  a.part = static_cast<float*>(workspace);
-  a.part_ml = as<float>(static_cast<char*>(workspace) +
-                        paged_part_bytes(p, batch, q_heads, head_dim));
   a.scale_log2 = scale * fpx::kLog2e;
   a.weight_shift = cache_dtype == FPX_F16 ? fpx::kWeightShiftF16 : 0.0f;
   a.pages = pages;
@@ -1034,8 +1041,9 @@ int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb,
   a.window = window < (1 << 30) ? (int)window : 0;
   a.dtype = dtype;
   a.cache_dtype = cache_dtype;
-  a.chunk = p.chunk;
-  a.splits = p.splits;
+  a.groups = p.groups;
+  a.split = p.split;
+  a.tile_queries = p.tile_queries;
   a.qtiles = p.qtiles;
   a.query_tiles = p.query_tiles;
   return status(fpx::launch_paged_attention(a, static_cast<hipStream_t>(stream)));

@@ -428,8 +428,8 @@ struct CacheArgs {
 hipError_t launch_cache(const CacheArgs& args, bool read, hipStream_t stream);
 
 // --------------------------------------- attention of new tokens over the cache
-constexpr int kMaxChunks = 256;     // of a sequence: threads of the join
-constexpr int kPagedGroups = 2048;  // work-groups aimed at
+constexpr int kPagedMaxGroups = 1024;  // work-groups of a call
+constexpr int kPagedFlight = 128 << 10;  // bytes of K and V in flight aimed at on a CU
 constexpr float kWeightShiftF16 = 14.0f;  // log2 of the FP16 weights' factor
 
 struct PagedArgs {
@@ -445,25 +445,31 @@ struct PagedArgs {
   void* out;         // as q, strides o_b, o_h
   int64_t o_b, o_h;
   float* lse;        // nullable [batch][heads * group]
-  float* part;       // [batch][heads * group][splits][head_dim]: chunk outputs
-  float* part_ml;    // [batch][heads * group][splits][2]: max (log2), sum
+  // Rows (sequence, cache head, tile of query heads) that several work-groups
+  // share: each leaves its share in one of its two places, [groups][2][tile's
+  // queries][head_dim] and [groups][2][queries][2] (max in log2, sum); a row's
+  // first place and their number are in row_info [batch][heads][qtiles][2].
+  float* part;
+  float* part_ml;
+  int* row_info;
   float scale_log2;  // of the scores, times log2(e)
   float weight_shift;  // log2 of the factor the weights carry in `part`
   int64_t pages;
   int batch, heads, group, head_dim, page_shift, max_length, window;
   int dtype, cache_dtype;  // FPX_*
-  // how the work is cut: keys of a chunk (a multiple of 128), chunks of a
-  // sequence at most, tiles of query heads, 16-query tiles of one of those
-  int chunk, splits, qtiles, query_tiles;
+  // how the work is cut: work-groups, tiles of a cache head's query heads and
+  // 16-query tiles of one of those, queries of a tile at most, whether a
+  // sequence can have more than one unit of keys
+  int groups, qtiles, query_tiles, tile_queries, split;
 };
 
 struct PagedPlan {
-  int chunk, splits, qtiles, query_tiles;
-  int64_t blocks;
+  int64_t units;  // at most, 0 for unsupported sizes
+  int groups, qtiles, query_tiles, tile_queries, split;
 };
 
-PagedPlan plan_paged(int64_t batch, int heads, int group, int head_dim, int max_length,
-                     int window);
+PagedPlan plan_paged(int cache_dtype, int64_t batch, int heads, int group, int head_dim,
+                     int64_t max_length, int64_t window);
 hipError_t launch_paged_attention(const PagedArgs& args, hipStream_t stream);
 // one cache type each (paged_attention_*.hip)
 hipError_t launch_paged_f32(const PagedArgs& args, hipStream_t stream);

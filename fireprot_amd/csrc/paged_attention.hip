@@ -1,5 +1,5 @@
-// Attention over the paged cache: how its work is cut, the join of a row's
-// chunks, and the choice of kernel (paged_attention.hpp).
+// Attention over the paged cache: how its work is cut, the join of rows that
+// work-groups shared, and the choice of kernel (paged_attention.hpp).
 #include "common.hpp"
 #include "kernels.hpp"
 #include "paged_layout.hpp"
@@ -7,129 +7,134 @@
 namespace fpx {
 namespace {
 
-constexpr int kCombineThreads = 256;
-constexpr int kCombineAhead = 4;       // chunks of a thread
-constexpr int kCombineFewRows = 256;   // rows that take several work-groups each
+constexpr int kJoinThreads = 256;
+constexpr int kJoinFewRows = 256;   // rows that take several work-groups each
 
-// One work-group per kChannels channels of a (sequence, query head): the
-// chunks' (max, sum) become weights in LDS, 4-channel vectors of the chunks'
-// outputs are summed kLanes chunks at a time, and those sums in a fixed order.
-// The launch is a chain of waits and little else, so the first outputs are
-// asked for before anything is known of the chunks' number (their places exist
-// in every row; those past the row's chunks are never used).
+// One work-group per kChannels channels of a (sequence, query head) whose keys
+// several shares covered: their (max, sum) become weights in LDS, 4-channel
+// vectors of their outputs are summed kLanes shares at a time, and those sums in
+// a fixed order.
 template <typename Q, int D, int kChannels>
-__global__ __launch_bounds__(kCombineThreads) void combine_chunks_kernel(PagedArgs a) {
+__global__ __launch_bounds__(kJoinThreads) void join_shares_kernel(PagedArgs a) {
   constexpr int kVecs = kChannels / 4;
-  constexpr int kLanes = kCombineThreads / kVecs;
-  __shared__ float weight[kMaxChunks];
-  __shared__ float red[2][kCombineThreads / kWave];
+  constexpr int kLanes = kJoinThreads / kVecs;
+  constexpr int kEach = kPagedMaxGroups / kJoinThreads;
+  __shared__ float weight[kPagedMaxGroups];
+  __shared__ float red[2][kJoinThreads / kWave];
   __shared__ f32x4 sums[kLanes][kVecs];
-  const int row = blockIdx.x;
   const int tid = threadIdx.x;
-  const int vec = tid % kVecs, first = tid / kVecs;
-  const f32x4* parts = reinterpret_cast<const f32x4*>(a.part + (int64_t)row * a.splits * D +
-                                                      blockIdx.y * kChannels) + vec;
-  const float* ml = a.part_ml + (int64_t)row * a.splits * 2;
-  f32x4 ahead[kCombineAhead];
-#pragma unroll
-  for (int i = 0; i < kCombineAhead; ++i) {
-    const int c = first + i * kLanes;
-    if (c < a.splits) ahead[i] = parts[(int64_t)c * (D / 4)];
-  }
-  float m = -__builtin_inff(), l = 0.0f;
-  if (tid < a.splits) {
-    m = ml[2 * tid];
-    l = ml[2 * tid + 1];
-  }
   const int q_heads = a.heads * a.group;
-  const int b = row / q_heads, hq = row - b * q_heads;
-  const int chunks = chunk_count(key_range(a.lengths[b], a.max_length, a.window), a.chunk);
-  if (chunks <= 1) return;  // written by its only work-group
-  if (tid >= chunks) {
-    m = -__builtin_inff();
-    l = 0.0f;
+  const int b = blockIdx.x / (unsigned)q_heads, hq = blockIdx.x - b * q_heads;
+  const int head = hq / a.group, qi = hq - head * a.group;
+  const int tile = 16 * a.query_tiles;
+  const int qtile = qi / tile;
+  const int* info = a.row_info + ((int64_t)(b * a.heads + head) * a.qtiles + qtile) * 2;
+  const int place = info[0], count = info[1];
+  if (count <= 1) return;  // written by its only work-group
+  // the row's part from work-group place / 2 + i
+  auto part_row = [&](int i) -> int64_t {
+    const int p = i == 0 ? place : (place / 2 + i) * 2;
+    return (int64_t)p * a.tile_queries + (qi - qtile * tile);
+  };
+  const int vec = tid % kVecs, first = tid / kVecs;
+  const float* column = a.part + blockIdx.y * kChannels + 4 * vec;
+  f32x4 ahead = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (first < count) ahead = *reinterpret_cast<const f32x4*>(column + part_row(first) * D);
+
+  float m[kEach], l[kEach];
+  float top = -__builtin_inff();
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int c = tid + i * kJoinThreads;
+    m[i] = -__builtin_inff();
+    l[i] = 0.0f;
+    if (c < count) {
+      m[i] = a.part_ml[part_row(c) * 2];
+      l[i] = a.part_ml[part_row(c) * 2 + 1];
+    }
+    // (a maximum is never NaN: a NaN score leaves it alone and makes the sum NaN)
+    top = fmaxf(top, m[i]);
   }
-  // (a maximum is never NaN: a NaN score leaves it alone and makes the sum NaN)
-  float top = wave_max(m);
+  top = wave_max(top);
   if ((tid & 63) == 0) red[0][tid >> 6] = top;
   __syncthreads();
   top = red[0][0];
 #pragma unroll
-  for (int w = 1; w < kCombineThreads / kWave; ++w) top = fmaxf(top, red[0][w]);
-  const float w = exp2_fast(m - (top == -__builtin_inff() ? 0.0f : top));
-  weight[tid] = w;
-  const float part = wave_sum(w * l);
+  for (int w = 1; w < kJoinThreads / kWave; ++w) top = fmaxf(top, red[0][w]);
+  const float ref = top == -__builtin_inff() ? 0.0f : top;
+  float part = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const float w = exp2_fast(m[i] - ref);
+    weight[tid + i * kJoinThreads] = w;
+    part += w * l[i];
+  }
+  part = wave_sum(part);
   if ((tid & 63) == 0) red[1][tid >> 6] = part;
   __syncthreads();
   float total = red[1][0];
 #pragma unroll
-  for (int i = 1; i < kCombineThreads / kWave; ++i) total += red[1][i];
+  for (int i = 1; i < kJoinThreads / kWave; ++i) total += red[1][i];
 
-  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int i = 0; i < kCombineAhead; ++i) {
-    const int c = first + i * kLanes;
-    if (c < chunks) acc += ahead[i] * weight[c];
-  }
-  for (int c = first + kCombineAhead * kLanes; c < chunks; c += kLanes)
-    acc += parts[(int64_t)c * (D / 4)] * weight[c];
+  f32x4 acc = first < count ? ahead * weight[first] : ahead;
+  for (int c = first + kLanes; c < count; c += kLanes)
+    acc += *reinterpret_cast<const f32x4*>(column + part_row(c) * D) * weight[c];
   sums[first][vec] = acc;
   __syncthreads();
   if (tid < kChannels) {
-    const float* column = reinterpret_cast<const float*>(sums) + tid;
-    const int used = chunks < kLanes ? chunks : kLanes;
+    const float* sum = reinterpret_cast<const float*>(sums) + tid;
+    const int used = count < kLanes ? count : kLanes;
     float x = 0.0f;
-    for (int i = 0; i < used; ++i) x += column[i * kChannels];
+    for (int i = 0; i < used; ++i) x += sum[i * kChannels];
     static_cast<Q*>(a.out)[b * a.o_b + hq * a.o_h + blockIdx.y * kChannels + tid] =
         (Q)(x / total);
   }
   if (tid == 0 && blockIdx.y == 0 && a.lse)
-    a.lse[row] = (top + __builtin_amdgcn_logf(total) - a.weight_shift) * 0.69314718055994531f;
+    a.lse[blockIdx.x] =
+        (top + __builtin_amdgcn_logf(total) - a.weight_shift) * 0.69314718055994531f;
 }
 
-// 32 channels to a work-group while there are few rows (32 rows of 256 chunks:
-// 5.5 us, 15 us with whole rows), whole rows otherwise (1024 rows of 7 chunks:
+// 32 channels to a work-group while there are few rows (32 rows of 256 shares:
+// 5.5 us, 15 us with whole rows), whole rows otherwise (1024 rows of 7 shares:
 // 4.9 us, 7.0 us in 32s).
 template <typename Q, int D>
-void launch_combine_dim(const PagedArgs& a, unsigned rows, hipStream_t stream) {
-  if (D > 32 && rows <= kCombineFewRows)
-    combine_chunks_kernel<Q, D, 32><<<dim3(rows, D / 32), kCombineThreads, 0, stream>>>(a);
+void launch_join_dim(const PagedArgs& a, unsigned rows, hipStream_t stream) {
+  if (D > 32 && rows <= kJoinFewRows)
+    join_shares_kernel<Q, D, 32><<<dim3(rows, D / 32), kJoinThreads, 0, stream>>>(a);
   else
-    combine_chunks_kernel<Q, D, D><<<rows, kCombineThreads, 0, stream>>>(a);
+    join_shares_kernel<Q, D, D><<<rows, kJoinThreads, 0, stream>>>(a);
 }
 
 template <typename Q>
-void launch_combine(const PagedArgs& a, unsigned rows, hipStream_t stream) {
+void launch_join(const PagedArgs& a, unsigned rows, hipStream_t stream) {
   switch (a.head_dim) {
-    case 32: launch_combine_dim<Q, 32>(a, rows, stream); break;
-    case 64: launch_combine_dim<Q, 64>(a, rows, stream); break;
-    case 128: launch_combine_dim<Q, 128>(a, rows, stream); break;
-    default: launch_combine_dim<Q, 256>(a, rows, stream); break;
+    case 32: launch_join_dim<Q, 32>(a, rows, stream); break;
+    case 64: launch_join_dim<Q, 64>(a, rows, stream); break;
+    case 128: launch_join_dim<Q, 128>(a, rows, stream); break;
+    default: launch_join_dim<Q, 256>(a, rows, stream); break;
   }
 }
 
 }  // namespace
 
-PagedPlan plan_paged(int64_t batch, int heads, int group, int head_dim, int max_length,
-                     int window) {
+PagedPlan plan_paged(int cache_dtype, int64_t batch, int heads, int group, int head_dim,
+                     int64_t max_length, int64_t window) {
   PagedPlan p{};
   p.query_tiles = group > 16 && head_dim <= 128 ? 2 : 1;
   p.qtiles = (group + 16 * p.query_tiles - 1) / (16 * p.query_tiles);
+  p.tile_queries = group < 16 * p.query_tiles ? group : 16 * p.query_tiles;
+  const int unit = cache_dtype == 0 ? 64 : 128;  // PagedTraits::kUnit
+  const int64_t each = unit_limit(max_length, window, unit);
+  p.split = each > 1;
   const int64_t rows = batch * heads * p.qtiles;
-  const int64_t span = window > 0 && (int64_t)window + kKeyTile - 1 < max_length
-                           ? (int64_t)window + kKeyTile - 1
-                           : max_length;
-  const int64_t unit = kKeyTile * 4;  // every wave a tile
-  const int64_t wanted = (span * rows + kPagedGroups - 1) / kPagedGroups;
-  int64_t chunk = (wanted + unit - 1) / unit * unit;
-  const int64_t least = (span + kMaxChunks - 1) / kMaxChunks;
-  if (chunk < least) chunk = (least + unit - 1) / unit * unit;
-  if (chunk < 2 * unit) chunk = 2 * unit;
-  if (chunk > (1 << 30)) chunk = 1 << 30;
-  p.chunk = (int)chunk;
-  p.splits = chunk_limit(max_length, window, p.chunk);
-  if (p.splits < 1) p.splits = 1;
-  p.blocks = rows * p.splits;
+  if (rows < 1 || rows >= (1ll << 31) || each >= (1ll << 31) / rows) return p;
+  p.units = rows * each;
+  // As many work-groups to a CU as bring their waves' tiles in flight to
+  // kPagedFlight bytes, all resident
+  const int64_t row_bytes = head_dim * (cache_dtype == 0 ? 4 : cache_dtype <= 2 ? 2 : 1);
+  const int64_t each_cu = kPagedFlight / (2 * unit * row_bytes);
+  const int64_t wanted = 256 * (each_cu < 1 ? 1 : each_cu > 4 ? 4 : each_cu);
+  p.groups = (int)(p.units < wanted ? p.units : wanted);
   return p;
 }
 
@@ -142,12 +147,12 @@ hipError_t launch_paged_attention(const PagedArgs& a, hipStream_t stream) {
     case 3: e = launch_paged_fp8(a, stream); break;
     default: e = launch_paged_int8(a, stream); break;
   }
-  if (e != hipSuccess || a.splits == 1) return e;
+  if (e != hipSuccess || !a.split) return e;
   const unsigned rows = (unsigned)((int64_t)a.batch * a.heads * a.group);
   switch (a.dtype) {
-    case 0: launch_combine<float>(a, rows, stream); break;
-    case 1: launch_combine<__bf16>(a, rows, stream); break;
-    default: launch_combine<_Float16>(a, rows, stream); break;
+    case 0: launch_join<float>(a, rows, stream); break;
+    case 1: launch_join<__bf16>(a, rows, stream); break;
+    default: launch_join<_Float16>(a, rows, stream); break;
   }
   return hipGetLastError();
 }

@@ -5,11 +5,17 @@
 //   j over the sequence's keys [first, length), query head h reading cache
 //   head h / group.
 //
-// One work-group takes one chunk of one sequence's keys for one cache head and
-// all (up to 16 QT) query heads that share it, so every key and value is read
-// from memory once; its four waves take the chunk's tiles in turn, each with
-// an online softmax of its own, and join at the end.  Sequences of more than
-// one chunk leave (max, sum, o) per chunk to combine_chunks_kernel.
+// A row of the work is one sequence's keys for one cache head and all (up to
+// 16 QT) query heads that share it, so every key and value is read from memory
+// once.  The rows of all sequences, cut into units of 128 keys (FP32: 64), form
+// one line of units, of which each of a fixed number of resident work-groups
+// takes an equal share, whatever the sequences' lengths: cutting every sequence
+// into chunks of one size instead took 62 us at best where this takes @@ (32
+// sequences of 1 to 4097 BF16 keys, 8 heads of 128), since few large chunks
+// leave CUs idle and many small ones are mostly start and join.  In a row the
+// four waves take its tiles in turn, each with an online softmax of its own, and
+// join at its end.  Rows that two shares meet in leave (max, sum, o) of each to
+// join_shares_kernel.
 //
 // The bound is memory: 2 D bytes-of-type per key against 4 D group flop.  So
 // all products run on the matrix cores with the queries padded to 16 (at one
@@ -150,6 +156,7 @@ struct PagedTraits {
   static constexpr int kRow = D * kElem;                       // of a cached row
   static constexpr int kHalves = kF32 ? 1 : 2;                 // 16-key halves of a tile
   static constexpr int kTile = 16 * kHalves;
+  static constexpr int kUnit = kPagedWaves * kTile;            // every wave a tile
   // terms a query is split into: all of its bits in BF16, 8 to a term
   static constexpr int kTerms = !kCoded ? 1 : std::is_same_v<Q, __bf16> ? 1
                                           : std::is_same_v<Q, _Float16> ? 2 : 3;
@@ -158,6 +165,7 @@ struct PagedTraits {
   static constexpr int kPiece = kRow / 4 < 16 ? kRow / 4 : 16;
   static constexpr int kPieces = kRow / 4 / kPiece;
   static constexpr int kSteps = kF32 ? D / 4 : D / 32;         // of the first product
+  static constexpr int kQuerySteps = kF32 ? D / 16 : kSteps;   // 16 bytes of a term each
   // V: channels a lane holds of a row, in pieces
   static constexpr int kChannels = D / 16;
   static constexpr int kPart = kChannels * kElem < 16 ? kChannels * kElem : 16;  // bytes
@@ -167,94 +175,114 @@ struct PagedTraits {
   // Registers of a lane: its queries, the tile of K and V in flight, the
   // accumulators, and what codes are decoded to.  Where they would spill (256 channels, split queries of two
   // tiles) the queries stay in LDS, which the four waves share.
-  static constexpr int kQueryWords = QT * (kF32 ? kSteps : kSteps * kTerms * 4);
+  static constexpr int kQueryWords = QT * kQuerySteps * kTerms * 4;
   static constexpr int kTileWords = kHalves * (kRow / 16 + 4 * kParts * kPartWords);
   static constexpr bool kQueryLds = kQueryWords + kTileWords + QT * kChannels * 4 + (kCoded ? 16 : 0) > 160;
   static constexpr float kShift = kF16 ? kWeightShiftF16 : 0.0f;
+};
+
+// Units before sequence `seq` of one row per sequence, of the sequence that unit
+// `first` of all is in: found by the work-group together.
+struct Place {
+  int seq, base;
 };
 
 template <typename Q, typename C, int D, int QT>
 __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(PagedArgs a) {
   using T = PagedTraits<Q, C, D, QT>;
   constexpr int kHalves = T::kHalves;
+  constexpr int kUnit = T::kUnit;
   __shared__ u32x4_t query_lds[T::kQueryLds ? T::kQueryWords / 4 : 1][kWave];
   __shared__ float joined[2][QT * T::kChannels * 4][kWave];
   __shared__ float wave_m[kPagedWaves][QT * 16], wave_l[kPagedWaves][QT * 16];
+  __shared__ int wave_units[kPagedWaves];
+  __shared__ Place found;
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int col = lane & 15, g = lane >> 4;
-  // Chunks are the slowest index: work-groups go to the XCDs in turn, and with
-  // the chunks fastest those that shorter sequences lack would all be missing
-  // on the same XCDs.
-  const int split = blockIdx.z, b = blockIdx.y;
-  int head = blockIdx.x, qtile = 0;
-  if (a.qtiles > 1) {
-    head = (uint32_t)blockIdx.x / (uint32_t)a.qtiles;
-    qtile = blockIdx.x - head * a.qtiles;
-  }
+  // (scalar, so that tile counts and page rows are)
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rows = a.heads * a.qtiles;  // of a sequence
+  const int group = blockIdx.x;
 
-  const int q0 = qtile * 16 * QT;  // the tile's first query head of the group
-
-  // Everything whose place is known without the sequence's length is asked for
-  // before it: the wave's first 64 pages (without a window the chunk's start is
-  // known; the table has entries up to max_length), then the queries.
-  constexpr int kAhead = kWave / kHalves;  // tiles that 64 pages serve
-  const int lane_key = (wave + kPagedWaves * (lane / kHalves)) * T::kTile + 16 * (lane % kHalves);
-  int early = 0;
-  const int early_key = split * a.chunk + lane_key;
-  const bool has_early = a.window <= 0 && early_key < a.max_length;
-  if (has_early) early = a.table[b * a.table_b + (early_key >> a.page_shift)];
-
-  // queries as they lie in memory: the channels of query `col` in K's order
-  // (lanes past the group's last query compute its first one again; their
-  // columns are not stored)
-  constexpr int kRaw = T::kF32 ? D / 16 : T::kSteps * (int)sizeof(Q) / 2;  // 16-byte words
-  u32x4_t raw[QT][kRaw];
-  if (!T::kQueryLds || wave == 0) {
+  // ---- this work-group's share of the units
+  Place at = {0, 0};
+  int total;
+  auto units_of = [&](int seq) {
+    return unit_count(key_range(a.lengths[seq], a.max_length, a.window), kUnit);
+  };
+  int thread_first = 0, thread_sum = 0, thread_base = 0;
+  if (a.batch == 1) {
+    total = units_of(0);
+  } else {
+    const int per = (a.batch + kPagedThreads - 1) / kPagedThreads;
+    thread_first = threadIdx.x * per;
+    const int last = min(a.batch, thread_first + per);
+    for (int i = thread_first; i < last; ++i) thread_sum += units_of(i);
+    const int lane = threadIdx.x & 63;
+    int upto = thread_sum;
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      const int qi = q0 + t * 16 + col;
-      const Q* q = static_cast<const Q*>(a.q) + b * a.q_b +
-                   (int64_t)(head * a.group + (qi < a.group ? qi : 0)) * a.q_h;
+    for (int d = 1; d < kWave; d *= 2) {
+      const int below = __shfl_up(upto, d);
+      upto += lane >= d ? below : 0;
+    }
+    if (lane == kWave - 1) wave_units[wave] = upto;
+    __syncthreads();
+    total = 0;
+    thread_base = upto - thread_sum;
 #pragma unroll
-      for (int i = 0; i < kRaw; ++i) {
-        constexpr int kPer = kRaw / (T::kF32 ? kRaw : T::kSteps);  // of eight channels
-        const int st = i / kPer;
-        const int d = T::kF32 ? 16 * i + 4 * g
-                              : (T::kCoded && D > 32 ? 64 * (st >> 1) + 16 * g + 8 * (st & 1)
-                                                     : 32 * st + 8 * g) +
-                                    (i % kPer) * 4;
-        raw[t][i] = *reinterpret_cast<const u32x4_t*>(q + d);
-      }
+    for (int w = 0; w < kPagedWaves; ++w) {
+      thread_base += w < wave ? wave_units[w] : 0;
+      total += wave_units[w];
     }
   }
-
-  const KeyRange range = key_range(a.lengths[b], a.max_length, a.window);
-  const int chunks = chunk_count(range, a.chunk);
-  // a row without keys is written by its first work-group
-  if (split > 0 && split >= chunks) return;
-  const bool direct = chunks <= 1;
-
-  const int start = (range.first & ~(kKeyTile - 1)) + split * a.chunk;
-  const int stop = min(range.end, start + a.chunk);
-  const int tiles = stop > start ? (stop - start + T::kTile - 1) / T::kTile : 0;
-  const int mine = tiles > wave ? (tiles - wave + kPagedWaves - 1) / kPagedWaves : 0;
-
-  float m[QT], l[QT];
-  f32x4 o[QT][T::kChannels];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    m[t] = -__builtin_inff();
-    l[t] = 0.0f;
-#pragma unroll
-    for (int c = 0; c < T::kChannels; ++c) o[t][c] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const Shares shares = make_shares(total * rows, gridDim.x);
+  int unit = share_start(shares, group);
+  const int share_first = unit, share_end = share_start(shares, group + 1);
+  if (unit >= share_end) return;
+  if (a.batch > 1) {
+    const int target = unit / rows;  // of the units of one row per sequence
+    if (target >= thread_base && target < thread_base + thread_sum) {
+      int seq = thread_first, base = thread_base;
+      for (int n = units_of(seq); target >= base + n; n = units_of(++seq)) base += n;
+      found = {seq, base};
+    }
+    __syncthreads();
+    at.seq = __builtin_amdgcn_readfirstlane(found.seq);
+    at.base = __builtin_amdgcn_readfirstlane(found.base);
   }
+  KeyRange range = key_range(a.lengths[at.seq], a.max_length, a.window);
+  int row_units = unit_count(range, kUnit);
 
   const int page_mask = (1 << a.page_shift) - 1;
   const char* kbase = static_cast<const char*>(a.k);
   const char* vbase = static_cast<const char*>(a.v);
+  constexpr int kAhead = kWave / kHalves;  // tiles that 64 pages serve
+
+  // ---- the rows of the share, one after another
+  while (true) {
+  // (not known to be the same for every row: what is derived from the lane is
+  // formed again for each, not kept in registers through the loop on its keys)
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  const int col = lane & 15, g = lane >> 4;
   const int k_lane = col * T::kRow + g * T::kPiece;
   const int v_lane = 4 * g * T::kRow + col * T::kPart;
+  const int lane_key = (wave + kPagedWaves * (lane / kHalves)) * T::kTile + 16 * (lane % kHalves);
+  const int b = at.seq;
+  const int in_seq = unit - rows * at.base;
+  const int row = in_seq / row_units;
+  const int unit0 = in_seq - row * row_units;
+  const int unit1 = min(row_units, unit0 + share_end - unit);
+  int head = row, qtile = 0;
+  if (a.qtiles > 1) {
+    head = row / a.qtiles;
+    qtile = row - head * a.qtiles;
+  }
+  const int q0 = qtile * 16 * QT;  // the tile's first query head of the cache head's
+  const bool direct = unit0 == 0 && unit1 == row_units;
+  const int start = first_key(range) + unit0 * kUnit;
+  const int stop = min(range.end, first_key(range) + unit1 * kUnit);
+  const int tiles = stop > start ? (stop - start + T::kTile - 1) / T::kTile : 0;
+  const int mine = tiles > wave ? (tiles - wave + kPagedWaves - 1) / kPagedWaves : 0;
 
   uint32_t kw[kHalves][T::kPieces * T::kPiece / 4];
   uint32_t vw[kHalves * 4][T::kParts * T::kPartWords];
@@ -262,15 +290,17 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
 
   // Pages of the wave's next 64 halves, one to a lane; a page outside the
   // cache is never read: page 0 stands in and the row comes out NaN.
-  int pages_ahead = 0;
   bool bad = !range.valid;
-  auto look_up = [&](int n) {
+  auto look_up = [&](int n) -> int {
     const int key = start + kPagedWaves * n * T::kTile + lane_key;
-    const int page = a.table[b * a.table_b + table_entry(key, range, a.page_shift)];
+    return a.table[b * a.table_b + table_entry(key, range, a.page_shift)];
+  };
+  auto checked = [&](int page) -> int {
     const bool ok = page_valid(page, a.pages);
     bad |= !ok;
-    pages_ahead = ok ? page : 0;
+    return ok ? page : 0;
   };
+  int pages_ahead = 0;
   auto row_of = [&](int n, int u) -> int64_t {
     const int page = __builtin_amdgcn_readlane(pages_ahead, (n % kAhead) * kHalves + u);
     const int key = start + (wave + kPagedWaves * n) * T::kTile + 16 * u;
@@ -300,65 +330,97 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
       if constexpr (T::kCoded) vs[u] = *reinterpret_cast<const f32x4*>(a.v_scale + row + 4 * g);
     }
   };
+  if (mine > 0) pages_ahead = look_up(0);
 
-  if (mine > 0) {
-    if (a.window <= 0) {
-      // pages past the sequence's last key were looked up too: its first page
-      // stands in for them (it holds keys, as the wave has a tile)
-      const bool held = early_key < range.end;
-      const bool ok = page_valid(early, a.pages);
-      bad |= held && !ok;
-      const int page = held && ok ? early : 0;
-      const int lead = __builtin_amdgcn_readfirstlane(page);
-      pages_ahead = held ? page : lead;
+  // ---- the B operand of S^T = K Q^T: the channels of query `col` in K's order,
+  // a step at a time, as they lie in memory and split into terms.  (Lanes past
+  // the tile's last query compute its first one again; their columns are not
+  // stored.)
+  constexpr int kRaw = T::kF32 ? 1 : (int)sizeof(Q) / 2;  // 16-byte words of a step
+  constexpr int kQuads = T::kQuerySteps * T::kTerms;      // of a query tile, term by term
+  auto load_step = [&](int t, int st, u32x4_t* raw) {
+    const int qi = q0 + t * 16 + col;
+    const Q* q = static_cast<const Q*>(a.q) + b * a.q_b +
+                 (int64_t)(head * a.group + (qi < a.group ? qi : 0)) * a.q_h;
+    const int d = T::kF32               ? 16 * st + 4 * g
+                  : T::kCoded && D > 32 ? 64 * (st >> 1) + 16 * g + 8 * (st & 1)
+                                        : 32 * st + 8 * g;
+#pragma unroll
+    for (int i = 0; i < kRaw; ++i) raw[i] = *reinterpret_cast<const u32x4_t*>(q + d + 4 * i);
+  };
+  auto split_step = [&](const u32x4_t* raw, u32x4_t* terms) {
+    if constexpr (T::kTerms == 1) {
+      terms[0] = raw[0];
     } else {
-      look_up(0);
+      typedef Q Eight __attribute__((ext_vector_type(8)));
+      Eight v;
+      __builtin_memcpy(&v, raw, sizeof(v));
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
+#pragma unroll
+      for (int p = 0; p < T::kTerms; ++p) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t w = pack_bf16(x[2 * i], x[2 * i + 1]);
+          terms[p][i] = w;
+          // what is left of an infinite value is NaN, which its product with a
+          // key would not be: the first term carries it alone
+          const float r0 = x[2 * i] - __builtin_bit_cast(float, w << 16);
+          const float r1 = x[2 * i + 1] - __builtin_bit_cast(float, w & 0xffff0000u);
+          x[2 * i] = __builtin_isinf(x[2 * i]) ? 0.0f : r0;
+          x[2 * i + 1] = __builtin_isinf(x[2 * i + 1]) ? 0.0f : r1;
+        }
+      }
     }
+  };
+  u32x4_t raw[QT][T::kQuerySteps][kRaw];
+  if constexpr (T::kQueryLds) {
+    // the waves share the steps
+    for (int i = wave; i < QT * T::kQuerySteps; i += kPagedWaves) {
+      const int t = i / T::kQuerySteps, st = i - t * T::kQuerySteps;
+      u32x4_t step[kRaw], terms[T::kTerms];
+      load_step(t, st, step);
+      split_step(step, terms);
+#pragma unroll
+      for (int p = 0; p < T::kTerms; ++p)
+        query_lds[t * kQuads + p * T::kQuerySteps + st][lane] = terms[p];
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int st = 0; st < T::kQuerySteps; ++st) load_step(t, st, raw[t][st]);
+  }
+  if (mine > 0) {
+    pages_ahead = checked(pages_ahead);
     load_k(0);
     load_v(0);
   }
 
-  // ---- the B operand of S^T = K Q^T
-  u32x4_t qw[T::kQueryWords / 4];
-  constexpr int kQuads = T::kQueryWords / 4 / QT;  // of one query tile
-  if (!T::kQueryLds || wave == 0) {
+  float m[QT], l[QT];
+  f32x4 o[QT][T::kChannels];
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      if constexpr (T::kTerms == 1) {
+  for (int t = 0; t < QT; ++t) {
+    m[t] = -__builtin_inff();
+    l[t] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kRaw; ++i) qw[t * kQuads + i] = raw[t][i];
-      } else {
-#pragma unroll
-        for (int st = 0; st < T::kSteps; ++st) {
-          typedef Q Eight __attribute__((ext_vector_type(8)));
-          const Eight v = *reinterpret_cast<const Eight*>(&raw[t][st * (kRaw / T::kSteps)]);
-          float x[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
-#pragma unroll
-          for (int p = 0; p < T::kTerms; ++p) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t w = pack_bf16(x[2 * i], x[2 * i + 1]);
-              qw[t * kQuads + p * T::kSteps + st][i] = w;
-              // what is left of an infinite value is NaN, which its product
-              // with a key would not be: the first term carries it alone
-              const float r0 = x[2 * i] - __builtin_bit_cast(float, w << 16);
-              const float r1 = x[2 * i + 1] - __builtin_bit_cast(float, w & 0xffff0000u);
-              x[2 * i] = __builtin_isinf(x[2 * i]) ? 0.0f : r0;
-              x[2 * i + 1] = __builtin_isinf(x[2 * i + 1]) ? 0.0f : r1;
-            }
-          }
-        }
-      }
-    }
+    for (int c = 0; c < T::kChannels; ++c) o[t][c] = {0.0f, 0.0f, 0.0f, 0.0f};
   }
+
+  u32x4_t qw[QT * kQuads];
   if constexpr (T::kQueryLds) {
-    if (wave == 0) {
-#pragma unroll
-      for (int i = 0; i < T::kQueryWords / 4; ++i) query_lds[i][lane] = qw[i];
-    }
     __syncthreads();
+  } else {
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int st = 0; st < T::kQuerySteps; ++st) {
+        u32x4_t terms[T::kTerms];
+        split_step(raw[t][st], terms);
+#pragma unroll
+        for (int p = 0; p < T::kTerms; ++p) qw[t * kQuads + p * T::kQuerySteps + st] = terms[p];
+      }
   }
   int query_lane = lane;
   auto query = [&](int i) -> u32x4_t {
@@ -412,7 +474,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
           for (int t = 0; t < QT; ++t) {
 #pragma unroll
             for (int p = T::kTerms - 1; p >= 0; --p) {  // the smallest term first
-              const u32x4_t y = query(t * kQuads + p * T::kSteps + st);
+              const u32x4_t y = query(t * kQuads + p * T::kQuerySteps + st);
               if constexpr (T::kF16)
                 s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
                     __builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), s[t][u], 0, 0, 0);
@@ -450,7 +512,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
         }
     }
     if (n + 1 < mine) {
-      if ((n + 1) % kAhead == 0) look_up(n + 1);
+      if ((n + 1) % kAhead == 0) pages_ahead = checked(look_up(n + 1));
       load_k(n + 1);
     }
     // ---- online softmax; a lane's l covers its own group's keys
@@ -562,17 +624,17 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
     }
   }
   __syncthreads();
-  float total[QT];
+  float total_l[QT];
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     float top = -__builtin_inff();
 #pragma unroll
     for (int w = 0; w < kPagedWaves; ++w) top = fmaxf(top, wave_m[w][t * 16 + col]);
     const float ref = top == -__builtin_inff() ? 0.0f : top;
-    total[t] = 0.0f;
+    total_l[t] = 0.0f;
 #pragma unroll
     for (int w = 0; w < kPagedWaves; ++w)
-      total[t] += wave_l[w][t * 16 + col] * exp2_fast(wave_m[w][t * 16 + col] - ref);
+      total_l[t] += wave_l[w][t * 16 + col] * exp2_fast(wave_m[w][t * 16 + col] - ref);
     const float mine_scale = exp2_fast(m[t] - ref);
 #pragma unroll
     for (int c = 0; c < T::kChannels; ++c) o[t][c] *= mine_scale;
@@ -602,55 +664,71 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
     }
     __syncthreads();
   }
-  if (wave != 0) return;
-
   // ---- O^T: lane (query col, group g), register r of channel c of a part:
   // channel (4g + r) * kPartChannels + c of the part's 16 * kPartChannels
+  if (wave == 0) {
+    const int place = group * 2 + (unit == share_first ? 0 : 1);
+    if (unit0 == 0 && a.split && lane == 0) {
+      int* info = a.row_info + ((int64_t)(b * a.heads + head) * a.qtiles + qtile) * 2;
+      info[0] = place;
+      info[1] = share_of(shares, unit + row_units - 1) - group + 1;
+    }
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int qi = q0 + t * 16 + col;
-    if (qi >= a.group) continue;
-    const int hq = head * a.group + qi;
-    const int64_t row = (int64_t)b * a.heads * a.group + hq;
-    const bool empty = range.valid && range.end <= range.first;
-    const float scale = direct ? (empty ? 0.0f : 1.0f / total[t]) : 1.0f;
-    float* part = a.part + (row * a.splits + split) * D;
-    Q* out = static_cast<Q*>(a.out) + b * a.o_b + hq * a.o_h;
+    for (int t = 0; t < QT; ++t) {
+      const int qi = q0 + t * 16 + col;
+      if (qi >= a.group) continue;
+      const int hq = head * a.group + qi;
+      const bool empty = range.valid && range.end <= range.first;
+      const float scale = direct ? (empty ? 0.0f : 1.0f / total_l[t]) : 1.0f;
+      const int64_t part_row = (int64_t)place * a.tile_queries + t * 16 + col;
+      float* part = a.part + part_row * D;
+      Q* out = static_cast<Q*>(a.out) + b * a.o_b + hq * a.o_h;
 #pragma unroll
-    for (int pt = 0; pt < T::kParts; ++pt)
+      for (int pt = 0; pt < T::kParts; ++pt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = pt * 16 * T::kPartChannels + (4 * g + r) * T::kPartChannels;
+        for (int r = 0; r < 4; ++r) {
+          const int d = pt * 16 * T::kPartChannels + (4 * g + r) * T::kPartChannels;
 #pragma unroll
-        for (int c = 0; c < T::kPartChannels; ++c) {
-          const float x = o[t][pt * T::kPartChannels + c][r] * scale;
-          if (direct)
-            out[d + c] = (Q)x;
-          else
-            part[d + c] = x;
+          for (int c = 0; c < T::kPartChannels; ++c) {
+            const float x = o[t][pt * T::kPartChannels + c][r] * scale;
+            if (direct)
+              out[d + c] = (Q)x;
+            else
+              part[d + c] = x;
+          }
+        }
+      if (g == 0) {
+        if (!direct) {
+          a.part_ml[part_row * 2] = m[t];
+          a.part_ml[part_row * 2 + 1] = total_l[t];
+        } else if (a.lse) {
+          a.lse[(int64_t)b * a.heads * a.group + hq] =
+              empty ? -__builtin_inff()
+                    : (m[t] + __builtin_amdgcn_logf(total_l[t]) - T::kShift) * kLn2;
         }
       }
-    if (g == 0) {
-      if (!direct) {
-        float* ml = a.part_ml + (row * a.splits + split) * 2;
-        ml[0] = m[t];
-        ml[1] = total[t];
-      } else if (a.lse) {
-        a.lse[row] = empty ? -__builtin_inff()
-                           : (m[t] + __builtin_amdgcn_logf(total[t]) - T::kShift) * kLn2;
-      }
     }
+  }
+
+  // ---- the next row
+  unit += unit1 - unit0;
+  if (unit >= share_end) break;
+  if (unit1 == row_units && row + 1 == rows) {
+    at.base += row_units;
+    ++at.seq;
+    range = key_range(a.lengths[at.seq], a.max_length, a.window);
+    row_units = unit_count(range, kUnit);
+  }
   }
 }
 
 template <typename Q, typename C, int D>
 hipError_t launch_paged_dim(const PagedArgs& a, hipStream_t stream) {
-  const dim3 blocks(a.heads * a.qtiles, a.batch, a.splits);
   if (a.query_tiles == 1) {
-    paged_attention_kernel<Q, C, D, 1><<<blocks, kPagedThreads, 0, stream>>>(a);
+    paged_attention_kernel<Q, C, D, 1><<<a.groups, kPagedThreads, 0, stream>>>(a);
   } else {
     if constexpr (D <= 128)
-      paged_attention_kernel<Q, C, D, 2><<<blocks, kPagedThreads, 0, stream>>>(a);
+      paged_attention_kernel<Q, C, D, 2><<<a.groups, kPagedThreads, 0, stream>>>(a);
     else
       return hipErrorInvalidValue;
   }

@@ -42,25 +42,40 @@ FPX_HD KeyRange key_range(int length, int max_length, int window) {
   return {window > 0 && length > window ? length - window : 0, length, true};
 }
 
-// The work on a range is cut into chunks that start at a tile's first key.
-constexpr int kKeyTile = 32;
+// The work on a range is counted in units of `unit` keys, the first begun at a
+// multiple of 32; a sequence without keys is one unit (somebody writes its
+// rows).
+constexpr int kKeyAlign = 32;
 
-FPX_HD int chunk_count(const KeyRange& r, int chunk) {
-  const int start = r.first & ~(kKeyTile - 1);
-  return r.end <= r.first ? 0 : (r.end - start - 1) / chunk + 1;
+FPX_HD int first_key(const KeyRange& r) { return r.first & ~(kKeyAlign - 1); }
+
+FPX_HD int unit_count(const KeyRange& r, int unit) {
+  return r.end <= r.first ? 1 : (r.end - first_key(r) - 1) / unit + 1;
 }
 
-// Most chunks a row of this call can have: the longest range, begun at the
-// last key of a tile.
-FPX_HD int chunk_limit(int max_length, int window, int chunk) {
-  if (max_length <= 0) return 0;
-  if (window <= 0 || window >= max_length) return (max_length - 1) / chunk + 1;
-  // a window of w keys begins anywhere in a tile; it never spans more than
-  // max_length keys
-  const int64_t span = (int64_t)window + kKeyTile - 1 < max_length
-                           ? (int64_t)window + kKeyTile - 1
-                           : max_length;
-  return (int)((span - 1) / chunk + 1);
+// Most units a sequence of this call can have: the longest range, begun at the
+// last key of an aligned group (a window begins anywhere in one).
+FPX_HD int64_t unit_limit(int64_t max_length, int64_t window, int unit) {
+  int64_t span = max_length;
+  if (window > 0 && window + kKeyAlign - 1 < span) span = window + kKeyAlign - 1;
+  return span < 1 ? 1 : (span - 1) / unit + 1;
+}
+
+// `total` units in equal shares for `groups` work-groups, one more for the first
+// few: the first unit of a share, and the share that a unit is in.
+struct Shares {
+  int size, larger;  // units of a share; the first `larger` shares have one more
+};
+
+FPX_HD Shares make_shares(int total, int groups) { return {total / groups, total % groups}; }
+
+FPX_HD int share_start(const Shares& s, int group) {
+  return group * s.size + (group < s.larger ? group : s.larger);
+}
+
+FPX_HD int share_of(const Shares& s, int unit) {
+  const int wide = s.larger * (s.size + 1);
+  return unit < wide ? unit / (s.size + 1) : s.larger + (unit - wide) / s.size;
 }
 
 // Entry of the block table that serves a group of keys from `key` on: that of

@@ -5,9 +5,9 @@ attention: each sequence's query heads attend to the keys its row of the block
 table names, ``lengths[b]`` of them (the new token's own among them), where
 they lie in the ``PagedCache`` (``fpx_paged_attention``).  Query heads share
 cache heads in groups; 8-bit caches are dequantised on the way; scores, softmax
-and sums are FP32.  A long sequence is cut into chunks that different
-work-groups take and a second launch joins.  There is no counterpart in the
-reference.
+and sums are FP32.  All sequences' keys are dealt out evenly to the card's
+work-groups, and a second launch joins what several of them share.  There is no
+counterpart in the reference.
 """
 from __future__ import annotations
 
@@ -23,7 +23,8 @@ def workspace_bytes(q: torch.Tensor, cache: PagedCache, max_length: int, window:
     """Device workspace of one call (any contents); 0 for unsupported sizes,
     ``NO_WORKSPACE`` where none is used."""
     return int(_native.library().fpx_paged_attention_workspace_bytes(
-        q.shape[0], q.shape[1], cache.k.shape[1], cache.k.shape[3], max_length, window))
+        CACHE_DTYPES[cache.k.dtype], q.shape[0], q.shape[1], cache.k.shape[1], cache.k.shape[3],
+        max_length, window))
 
 
 def _aligned_rows(t: torch.Tensor) -> bool:
@@ -45,8 +46,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
     * ``block_table`` int32 ``[batch, p]``: a sequence's pages in order.
       Entries past its length, or before its window, are not read.
     * ``lengths`` int32 ``[batch]``, up to ``max_length`` (default: what the
-      table holds; a bound near the true maximum cuts the work best, and a
-      captured graph keeps the bound it was captured with).
+      table holds; a captured graph keeps the bound it was captured with).
     * ``scale`` of the scores, ``head_dim ** -0.5`` by default; ``window`` > 0
       keeps the last ``window`` keys only.
     * ``lse`` float32 ``[batch, q_heads]``: the logarithm of the softmax's sum.
@@ -95,8 +95,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
                          "no repeated elements")
     lse = (torch.empty((batch, q_heads), dtype=torch.float32, device=q.device)
            if return_lse else None)
-    size = lib.fpx_paged_attention_workspace_bytes(batch, q_heads, heads, head_dim, max_length,
-                                                   window)
+    size = lib.fpx_paged_attention_workspace_bytes(CACHE_DTYPES[k.dtype], batch, q_heads, heads,
+                                                   head_dim, max_length, window)
     if size == 0:
         raise ValueError(f"unsupported sizes: batch {batch}, {q_heads} query heads, "
                          f"max_length {max_length}, window {window}")

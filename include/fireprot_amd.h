@@ -397,10 +397,10 @@ int fpx_cache_read(int row_dtype, int cache_dtype, void* k, int64_t k_st, int64_
                    void* stream);
 
 /* Bytes of workspace fpx_paged_attention needs; 0 for unsupported sizes, 256
- * where it uses none (no sequence can need more than one chunk): its workspace
- * may then be null. */
-size_t fpx_paged_attention_workspace_bytes(int64_t batch, int q_heads, int heads, int head_dim,
-                                           int64_t max_length, int64_t window);
+ * where it uses none (sequences too short to be shared by work-groups): its
+ * workspace may then be null. */
+size_t fpx_paged_attention_workspace_bytes(int cache_dtype, int64_t batch, int q_heads, int heads,
+                                           int head_dim, int64_t max_length, int64_t window);
 
 /* Attention of one new token per sequence over a paged cache:
  *   out[b][h] = sum_j softmax_j(scale * q[b][h] . k_j) v_j
@@ -416,15 +416,14 @@ size_t fpx_paged_attention_workspace_bytes(int64_t batch, int q_heads, int heads
  *               max_length / page_size (rounded up) of them; only the entries
  *               of pages that hold the keys above are read
  *   lengths     [batch] int32, the sequences' tokens with the new one
- *   max_length  no length is larger; the work is cut for it, so a bound near
- *               the true maximum is fastest
+ *   max_length  no length is larger
  *   lse         nullable [batch][q_heads] float: log sum_j exp(scale q . k_j)
  * A sequence of length 0 gives zeros (lse -inf).  One whose length is negative
  * or above max_length, or whose block table names a page outside the cache,
  * gives NaN (out and lse); nothing outside the cache is read.
  * Supported: the cache's sizes; q_heads a multiple of heads; max_length < 2^30;
- * batch and q_heads up to 65535, their product, and its product with the chunks
- * a sequence is cut into, below 2^23; nothing is launched when batch is 0. */
+ * batch * q_heads up to 2^20, and its product with max_length / 64 (a window
+ * bounds it as well) below 2^31; nothing is launched when batch is 0. */
 int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb, int64_t q_sh,
                         const void* cache_k, const void* cache_v, const float* k_scale,
                         const float* v_scale, int64_t pages, int heads, int page_size,

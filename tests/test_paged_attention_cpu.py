@@ -51,17 +51,21 @@ def test_pointers_are_refused(lib, bad):
 def test_workspace(lib):
     size = lib.fpx_paged_attention_workspace_bytes
     long = dict(max_length=1 << 16, table_pages=1 << 12)
-    need = size(3, 8, 2, 128, 1 << 16, 0)
-    assert need > 3 * 8 * 2 * (128 + 2) * 4  # at least two chunks a sequence
+    need = size(1, 3, 8, 2, 128, 1 << 16, 0)
+    assert need > 3 * 8 * 2 * (128 + 2) * 4  # at least two shares a row
     assert lib.fpx_paged_attention(*_args(workspace_bytes=need - 1, **long)) \
         == _native.FPX_ERR_WORKSPACE
-    assert size(3, 8, 2, 128, 128, 0) == 256
+    assert size(1, 3, 8, 2, 128, 128, 0) == 256
     # a window bounds the work as a length does
-    assert size(3, 8, 2, 128, 1 << 16, 64) == 256
-    assert size(3, 8, 2, 128, 1 << 16, 1 << 40) == need
-    for bad in ((-1, 8, 2, 128, 128, 0), (3, 7, 2, 128, 128, 0), (3, 8, 2, 100, 128, 0),
-                (3, 8, 2, 128, -1, 0), (3, 8, 2, 128, 1 << 30, 0), (3, 8, 2, 128, 128, -1),
-                (1 << 22, 8, 2, 128, 128, 0), (3, 0, 0, 128, 128, 0)):
+    assert size(1, 3, 8, 2, 128, 1 << 16, 64) == 256
+    assert size(1, 3, 8, 2, 128, 1 << 16, 1 << 40) == need
+    # one place a work-group and side, whatever the length
+    assert size(1, 3, 8, 2, 128, 1 << 24, 0) == need
+    for bad in ((5, 3, 8, 2, 128, 128, 0), (1, -1, 8, 2, 128, 128, 0), (1, 3, 7, 2, 128, 128, 0),
+                (1, 3, 8, 2, 100, 128, 0), (1, 3, 8, 2, 128, -1, 0),
+                (1, 3, 8, 2, 128, 1 << 30, 0), (1, 3, 8, 2, 128, 128, -1),
+                (1, 1 << 18, 8, 2, 128, 128, 0), (1, 3, 0, 0, 128, 128, 0),
+                (1, 1 << 17, 8, 8, 128, 1 << 20, 0)):
         assert size(*bad) == 0
 
 

@@ -25,8 +25,10 @@ int t_range(int length, int max_length, int window, int* first, int* end) {
   *first = r.first; *end = r.end;
   return r.valid;
 }
-int t_chunks(int first, int end, int chunk) { return chunk_count({first, end, true}, chunk); }
-int t_limit(int max_length, int window, int chunk) { return chunk_limit(max_length, window, chunk); }
+int t_units(int first, int end, int unit) { return unit_count({first, end, true}, unit); }
+int64_t t_limit(int64_t max_length, int64_t window, int unit) { return unit_limit(max_length, window, unit); }
+int t_start(int total, int groups, int group) { return share_start(make_shares(total, groups), group); }
+int t_share(int total, int groups, int unit) { return share_of(make_shares(total, groups), unit); }
 int t_entry(int key, int first, int end, int shift) { return table_entry(key, {first, end, true}, shift); }
 int t_page(int page, int64_t pages) { return page_valid(page, pages); }
 }
@@ -46,6 +48,8 @@ def rules(tmp_path_factory):
     lib.t_row.restype = ctypes.c_int64
     lib.t_row.argtypes = [ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int]
     lib.t_page.argtypes = [ctypes.c_int, ctypes.c_int64]
+    lib.t_limit.restype = ctypes.c_int64
+    lib.t_limit.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int]
     return lib
 
 
@@ -77,26 +81,43 @@ def test_ranges(rules):
                 assert first.value == end.value == 0
 
 
-def test_chunks_cover_a_range_and_never_pass_their_limit(rules):
+def test_units_cover_a_range_and_never_pass_their_limit(rules):
     rng = random.Random(3)
     for _ in range(4000):
-        chunk = 32 * rng.choice([1, 2, 4, 7, 64])
-        max_length = rng.choice([0, 1, 31, 32, 33, rng.randrange(1, 20000), 2 ** 31 - 1])
-        window = rng.choice([0, 1, rng.randrange(1, 5000), 2 ** 31 - 1])
+        unit = rng.choice([64, 128])
+        max_length = rng.choice([0, 1, 31, 32, 33, rng.randrange(1, 20000), 2 ** 30 - 1])
+        window = rng.choice([0, 1, rng.randrange(1, 5000), 2 ** 30 - 1])
         length = rng.randint(0, min(max_length, 40000))
         if rng.random() < 0.3:
             length = max_length
         first = max(0, length - window) if window else 0
-        n = rules.t_chunks(first, length, chunk)
-        assert n <= rules.t_limit(max_length, window, chunk)
+        n = rules.t_units(first, length, unit)
+        assert 1 <= n <= rules.t_limit(max_length, window, unit)
         start = first // 32 * 32
-        if length > first:  # the last chunk holds the last key
-            assert start + (n - 1) * chunk < length <= start + n * chunk
+        if length > first:  # the last unit holds the last key
+            assert start + (n - 1) * unit < length <= start + n * unit
         else:
-            assert n == 0
+            assert n == 1
     # the limit is reached
-    assert rules.t_limit(1000, 0, 128) == 8 and rules.t_chunks(0, 1000, 128) == 8
-    assert rules.t_limit(1000, 98, 128) == 2 and rules.t_chunks(31, 129, 128) == 2
+    assert rules.t_limit(1000, 0, 128) == 8 and rules.t_units(0, 1000, 128) == 8
+    assert rules.t_limit(1000, 98, 128) == 2 and rules.t_units(31, 129, 128) == 2
+
+
+def test_shares_are_equal_and_cover_all_units(rules):
+    rng = random.Random(4)
+    for _ in range(300):
+        groups = rng.choice([1, 2, 255, 256, 512, 1024])
+        total = rng.choice([1, groups - 1, groups, groups + 1, rng.randrange(1, 5000),
+                            2 ** 31 - 1 - rng.randrange(1000)])
+        total = max(1, total)
+        starts = [rules.t_start(total, groups, i) for i in range(groups + 1)]
+        assert starts[0] == 0 and starts[-1] == total
+        sizes = [b - a for a, b in zip(starts, starts[1:])]
+        assert max(sizes) - min(sizes) <= 1
+        for i in range(groups):
+            for unit in {starts[i], starts[i + 1] - 1}:
+                if starts[i] <= unit < starts[i + 1]:
+                    assert rules.t_share(total, groups, unit) == i
 
 
 def test_table_entries_stay_in_the_range(rules):
