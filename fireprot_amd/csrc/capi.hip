@@ -425,7 +425,7 @@ int cache_impl(bool read, int row_dtype, int cache_dtype, const void* k, int64_t
 
 constexpr int64_t kPagedMaxRows = 1 << 20;  // (sequence, query head): the join's grid
 
-// The cut of a call's work, units = 0 for unsupported sizes.
+// The cut of a call's work, groups = 0 for unsupported sizes.
 fpx::PagedPlan paged_plan(int cache_dtype, int64_t batch, int q_heads, int heads, int head_dim,
                           int64_t max_length, int64_t window) {
   const fpx::PagedPlan none{};
@@ -976,7 +976,7 @@ size_t fpx_paged_attention_workspace_bytes(int cache_dtype, int64_t batch, int q
                                            int head_dim, int64_t max_length, int64_t window) {
   const fpx::PagedPlan p =
       paged_plan(cache_dtype, batch, q_heads, heads, head_dim, max_length, window);
-  if (p.units == 0) return 0;
+  if (p.groups == 0) return 0;
   return p.split ? paged_workspace(p, batch, heads, head_dim).total : 256;
 }
 
@@ -994,7 +994,7 @@ int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb,
   if (!row_type_ok(dtype) || (!is_coded(cache_dtype) && cache_dtype != dtype)) return FPX_ERR_DIMS;
   const fpx::PagedPlan p =
       paged_plan(cache_dtype, batch, q_heads, heads, head_dim, max_length, window);
-  if (p.units == 0) return FPX_ERR_DIMS;
+  if (p.groups == 0) return FPX_ERR_DIMS;
   const int64_t row = 16 / (int64_t)type_bytes(dtype);
   if (q_sb < 0 || q_sh < 0 || o_sb < 0 || o_sh < 0 || q_sb % row || q_sh % row || o_sb % row ||
       o_sh % row)
@@ -1043,6 +1043,8 @@ int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb,
   a.cache_dtype = cache_dtype;
   a.groups = p.groups;
   a.split = p.split;
+  a.unit = p.unit;
+  a.each = p.each;
   a.tile_queries = p.tile_queries;
   a.qtiles = p.qtiles;
   a.query_tiles = p.query_tiles;

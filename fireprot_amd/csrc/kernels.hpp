@@ -428,7 +428,10 @@ struct CacheArgs {
 hipError_t launch_cache(const CacheArgs& args, bool read, hipStream_t stream);
 
 // --------------------------------------- attention of new tokens over the cache
-constexpr int kPagedMaxGroups = 1024;  // work-groups of a call
+constexpr int kPagedMaxGroups = 1024;  // work-groups that share a row
+constexpr int kPagedFew = 4;           // tiles of a wave in a small call's unit
+constexpr int kPagedEnough = 128;      // work-groups, below which it takes fewer
+constexpr int kPagedFixed = 1152;      // work-groups of a small call
 constexpr int kPagedFlight = 128 << 10;  // bytes of K and V in flight aimed at on a CU
 constexpr float kWeightShiftF16 = 14.0f;  // log2 of the FP16 weights' factor
 
@@ -461,11 +464,13 @@ struct PagedArgs {
   // 16-query tiles of one of those, queries of a tile at most, whether a
   // sequence can have more than one unit of keys
   int groups, qtiles, query_tiles, tile_queries, split;
+  int unit;  // keys of a unit of the work
+  int each;  // > 0: work-groups of a row, one unit each; 0: equal shares
 };
 
 struct PagedPlan {
-  int64_t units;  // at most, 0 for unsupported sizes
-  int groups, qtiles, query_tiles, tile_queries, split;
+  int groups;  // 0 for unsupported sizes
+  int qtiles, query_tiles, tile_queries, split, unit, each;
 };
 
 PagedPlan plan_paged(int cache_dtype, int64_t batch, int heads, int group, int head_dim,

@@ -156,7 +156,6 @@ struct PagedTraits {
   static constexpr int kRow = D * kElem;                       // of a cached row
   static constexpr int kHalves = kF32 ? 1 : 2;                 // 16-key halves of a tile
   static constexpr int kTile = 16 * kHalves;
-  static constexpr int kUnit = kPagedWaves * kTile;            // every wave a tile
   // terms a query is split into: all of its bits in BF16, 8 to a term
   static constexpr int kTerms = !kCoded ? 1 : std::is_same_v<Q, __bf16> ? 1
                                           : std::is_same_v<Q, _Float16> ? 2 : 3;
@@ -181,156 +180,196 @@ struct PagedTraits {
   static constexpr float kShift = kF16 ? kWeightShiftF16 : 0.0f;
 };
 
-// Units before sequence `seq` of one row per sequence, of the sequence that unit
-// `first` of all is in: found by the work-group together.
-struct Place {
-  int seq, base;
+// Units [unit0, unit1) of the row_units of a row: one sequence's keys for one
+// cache head and one tile of its query heads.
+struct Segment {
+  int seq, head, qtile, unit0, unit1, row_units;
+  KeyRange range;
 };
 
 template <typename Q, typename C, int D, int QT>
 __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(PagedArgs a) {
   using T = PagedTraits<Q, C, D, QT>;
   constexpr int kHalves = T::kHalves;
-  constexpr int kUnit = T::kUnit;
   __shared__ u32x4_t query_lds[T::kQueryLds ? T::kQueryWords / 4 : 1][kWave];
-  __shared__ float joined[2][QT * T::kChannels * 4][kWave];
+  __shared__ f32x4 joined[2][QT * T::kChannels][kWave];
   __shared__ float wave_m[kPagedWaves][QT * 16], wave_l[kPagedWaves][QT * 16];
   __shared__ int wave_units[kPagedWaves];
-  __shared__ Place found;
+  __shared__ int found[2];
 
-  // (scalar, so that tile counts and page rows are)
+  // (scalar, so that tile counts and the pages' rows are)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rows = a.heads * a.qtiles;  // of a sequence
-  const int group = blockIdx.x;
-
-  // ---- this work-group's share of the units
-  Place at = {0, 0};
-  int total;
-  auto units_of = [&](int seq) {
-    return unit_count(key_range(a.lengths[seq], a.max_length, a.window), kUnit);
+  const int group = ((int)blockIdx.y * rows + (int)blockIdx.x) * (int)gridDim.z + (int)blockIdx.z;
+  // (scalar: the compiler cannot know that no store changes the lengths)
+  auto range_of = [&](int seq) {
+    return key_range(__builtin_amdgcn_readfirstlane(a.lengths[seq]), a.max_length, a.window);
   };
-  int thread_first = 0, thread_sum = 0, thread_base = 0;
-  if (a.batch == 1) {
-    total = units_of(0);
-  } else {
-    const int per = (a.batch + kPagedThreads - 1) / kPagedThreads;
-    thread_first = threadIdx.x * per;
-    const int last = min(a.batch, thread_first + per);
-    for (int i = thread_first; i < last; ++i) thread_sum += units_of(i);
+  auto units_of = [&](int seq) {  // each thread's own sequence
+    return unit_count(key_range(a.lengths[seq], a.max_length, a.window), a.unit);
+  };
+
+  // ---- this work-group's share of the units: one unit of one row, each row
+  // having places for a.each of them, or an equal part of them all
+  Segment cur;
+  Shares shares = {1, 0};
+  int share_first, share_end;
+  int early_pages = 0, early_key = 0;  // looked up before the length is known
+  const bool fixed = a.each > 0;
+  if (fixed) {
+    cur.seq = blockIdx.y;
+    cur.head = blockIdx.x;
+    cur.unit0 = blockIdx.z;
+    cur.unit1 = cur.unit0 + 1;
+    share_first = group;
+    share_end = group + 1;
+    // without a window the unit's keys are known, and the table has entries up
+    // to max_length
     const int lane = threadIdx.x & 63;
-    int upto = thread_sum;
+    early_key = cur.unit0 * a.unit + (wave + kPagedWaves * (lane / kHalves)) * T::kTile +
+                16 * (lane % kHalves);
+    if (a.window <= 0 && early_key < a.max_length)
+      early_pages = a.table[cur.seq * a.table_b + (early_key >> a.page_shift)];
+  } else {
+    int total, thread_first = 0, thread_sum = 0, thread_base = 0;
+    if (a.batch == 1) {
+      total = unit_count(range_of(0), a.unit);
+    } else {
+      const int per = (a.batch + kPagedThreads - 1) / kPagedThreads;
+      thread_first = threadIdx.x * per;
+      const int last = min(a.batch, thread_first + per);
+      for (int i = thread_first; i < last; ++i) thread_sum += units_of(i);
+      const int lane = threadIdx.x & 63;
+      int upto = thread_sum;
 #pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-      const int below = __shfl_up(upto, d);
-      upto += lane >= d ? below : 0;
-    }
-    if (lane == kWave - 1) wave_units[wave] = upto;
-    __syncthreads();
-    total = 0;
-    thread_base = upto - thread_sum;
+      for (int d = 1; d < kWave; d *= 2) {
+        const int below = __shfl_up(upto, d);
+        upto += lane >= d ? below : 0;
+      }
+      if (lane == kWave - 1) wave_units[wave] = upto;
+      __syncthreads();
+      total = 0;
+      thread_base = upto - thread_sum;
 #pragma unroll
-    for (int w = 0; w < kPagedWaves; ++w) {
-      thread_base += w < wave ? wave_units[w] : 0;
-      total += wave_units[w];
+      for (int w = 0; w < kPagedWaves; ++w) {
+        thread_base += w < wave ? wave_units[w] : 0;
+        total += wave_units[w];
+      }
+      total = __builtin_amdgcn_readfirstlane(total);
     }
-  }
-  const Shares shares = make_shares(total * rows, gridDim.x);
-  int unit = share_start(shares, group);
-  const int share_first = unit, share_end = share_start(shares, group + 1);
-  if (unit >= share_end) return;
-  if (a.batch > 1) {
-    const int target = unit / rows;  // of the units of one row per sequence
-    if (target >= thread_base && target < thread_base + thread_sum) {
-      int seq = thread_first, base = thread_base;
-      for (int n = units_of(seq); target >= base + n; n = units_of(++seq)) base += n;
-      found = {seq, base};
+    shares = make_shares(total * rows, a.groups);
+    share_first = share_start(shares, group);
+    share_end = share_start(shares, group + 1);
+    if (share_first >= share_end) return;
+    int base = 0;  // units before the sequence, of one row per sequence
+    cur.seq = 0;
+    if (a.batch > 1) {
+      const int target = share_first / rows;
+      if (target >= thread_base && target < thread_base + thread_sum) {
+        int seq = thread_first, before = thread_base;
+        for (int n = units_of(seq); target >= before + n; n = units_of(++seq)) before += n;
+        found[0] = seq;
+        found[1] = before;
+      }
+      __syncthreads();
+      cur.seq = __builtin_amdgcn_readfirstlane(found[0]);
+      base = __builtin_amdgcn_readfirstlane(found[1]);
     }
-    __syncthreads();
-    at.seq = __builtin_amdgcn_readfirstlane(found.seq);
-    at.base = __builtin_amdgcn_readfirstlane(found.base);
+    cur.range = range_of(cur.seq);
+    cur.row_units = unit_count(cur.range, a.unit);
+    const int in_seq = share_first - rows * base;
+    cur.head = in_seq / cur.row_units;
+    cur.unit0 = in_seq - cur.head * cur.row_units;
+    cur.unit1 = min(cur.row_units, cur.unit0 + share_end - share_first);
   }
-  KeyRange range = key_range(a.lengths[at.seq], a.max_length, a.window);
-  int row_units = unit_count(range, kUnit);
+  // (so far the row of the sequence)
+  cur.qtile = 0;
+  if (a.qtiles > 1) {
+    const int row = cur.head;
+    cur.head = row / a.qtiles;
+    cur.qtile = row - cur.head * a.qtiles;
+  }
+  int unit = share_first;  // the segment's first
 
   const int page_mask = (1 << a.page_shift) - 1;
   const char* kbase = static_cast<const char*>(a.k);
   const char* vbase = static_cast<const char*>(a.v);
   constexpr int kAhead = kWave / kHalves;  // tiles that 64 pages serve
 
-  // ---- the rows of the share, one after another
-  while (true) {
-  // (not known to be the same for every row: what is derived from the lane is
-  // formed again for each, not kept in registers through the loop on its keys)
-  int lane = threadIdx.x & 63;
-  asm volatile("" : "+v"(lane));
-  const int col = lane & 15, g = lane >> 4;
-  const int k_lane = col * T::kRow + g * T::kPiece;
-  const int v_lane = 4 * g * T::kRow + col * T::kPart;
-  const int lane_key = (wave + kPagedWaves * (lane / kHalves)) * T::kTile + 16 * (lane % kHalves);
-  const int b = at.seq;
-  const int in_seq = unit - rows * at.base;
-  const int row = in_seq / row_units;
-  const int unit0 = in_seq - row * row_units;
-  const int unit1 = min(row_units, unit0 + share_end - unit);
-  int head = row, qtile = 0;
-  if (a.qtiles > 1) {
-    head = row / a.qtiles;
-    qtile = row - head * a.qtiles;
-  }
-  const int q0 = qtile * 16 * QT;  // the tile's first query head of the cache head's
-  const bool direct = unit0 == 0 && unit1 == row_units;
-  const int start = first_key(range) + unit0 * kUnit;
-  const int stop = min(range.end, first_key(range) + unit1 * kUnit);
-  const int tiles = stop > start ? (stop - start + T::kTile - 1) / T::kTile : 0;
-  const int mine = tiles > wave ? (tiles - wave + kPagedWaves - 1) / kPagedWaves : 0;
-
   uint32_t kw[kHalves][T::kPieces * T::kPiece / 4];
   uint32_t vw[kHalves * 4][T::kParts * T::kPartWords];
   f32x4 ks[kHalves], vs[kHalves];
-
-  // Pages of the wave's next 64 halves, one to a lane; a page outside the
-  // cache is never read: page 0 stands in and the row comes out NaN.
-  bool bad = !range.valid;
-  auto look_up = [&](int n) -> int {
-    const int key = start + kPagedWaves * n * T::kTile + lane_key;
-    return a.table[b * a.table_b + table_entry(key, range, a.page_shift)];
-  };
-  auto checked = [&](int page) -> int {
-    const bool ok = page_valid(page, a.pages);
-    bad |= !ok;
-    return ok ? page : 0;
-  };
+  // The next 64 halves' pages, one to a lane; a page outside the cache is never
+  // read: page 0 stands in and the row comes out NaN.
   int pages_ahead = 0;
-  auto row_of = [&](int n, int u) -> int64_t {
-    const int page = __builtin_amdgcn_readlane(pages_ahead, (n % kAhead) * kHalves + u);
-    const int key = start + (wave + kPagedWaves * n) * T::kTile + 16 * u;
-    return (((int64_t)page * a.heads + head) << a.page_shift) + (key & page_mask);
+  bool bad = false;
+
+  int lane = threadIdx.x & 63;
+  auto start_of = [&](const Segment& x) { return first_key(x.range) + x.unit0 * a.unit; };
+  auto tiles_of = [&](const Segment& x) {
+    const int keys = min(x.range.end, first_key(x.range) + x.unit1 * a.unit) - start_of(x);
+    const int tiles = keys > 0 ? (keys + T::kTile - 1) / T::kTile : 0;
+    return tiles > wave ? (tiles - wave + kPagedWaves - 1) / kPagedWaves : 0;
   };
-  auto load_k = [&](int n) {
+  auto look_up = [&](const Segment& x, int n) -> int {
+    const int key = start_of(x) + (wave + kPagedWaves * (n + lane / kHalves)) * T::kTile +
+                    16 * (lane % kHalves);
+    return a.table[x.seq * a.table_b + table_entry(key, x.range, a.page_shift)];
+  };
+  auto take_pages = [&](int pages) {
+    const bool ok = page_valid(pages, a.pages);
+    bad |= !ok;
+    pages_ahead = ok ? pages : 0;
+  };
+  auto row_of = [&](const Segment& x, int n, int u) -> int64_t {
+    const int page = __builtin_amdgcn_readlane(pages_ahead, (n % kAhead) * kHalves + u);
+    const int key = start_of(x) + (wave + kPagedWaves * n) * T::kTile + 16 * u;
+    return (((int64_t)page * a.heads + x.head) << a.page_shift) + (key & page_mask);
+  };
+  auto load_k = [&](const Segment& x, int n) {
+    const int at = (lane & 15) * T::kRow + (lane >> 4) * T::kPiece;
 #pragma unroll
     for (int u = 0; u < kHalves; ++u) {
-      const int64_t row = row_of(n, u);
-      const char* p = kbase + row * T::kRow + k_lane;
+      const int64_t row = row_of(x, n, u);
+      const char* p = kbase + row * T::kRow + at;
 #pragma unroll
       for (int c = 0; c < T::kPieces; ++c)
         load_words<T::kPiece, false>(p + c * 64, &kw[u][c * T::kPiece / 4]);
-      if constexpr (T::kCoded) ks[u] = *reinterpret_cast<const f32x4*>(a.k_scale + row + 4 * g);
+      if constexpr (T::kCoded)
+        ks[u] = *reinterpret_cast<const f32x4*>(a.k_scale + row + 4 * (lane >> 4));
     }
   };
-  auto load_v = [&](int n) {
+  auto load_v = [&](const Segment& x, int n) {
+    const int at = 4 * (lane >> 4) * T::kRow + (lane & 15) * T::kPart;
 #pragma unroll
     for (int u = 0; u < kHalves; ++u) {
-      const int64_t row = row_of(n, u);
-      const char* p = vbase + row * T::kRow + v_lane;
+      const int64_t row = row_of(x, n, u);
+      const char* p = vbase + row * T::kRow + at;
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int c = 0; c < T::kParts; ++c)
           load_words<T::kPart, true>(p + r * T::kRow + c * 256, &vw[u * 4 + r][c * T::kPartWords]);
-      if constexpr (T::kCoded) vs[u] = *reinterpret_cast<const f32x4*>(a.v_scale + row + 4 * g);
+      if constexpr (T::kCoded)
+        vs[u] = *reinterpret_cast<const f32x4*>(a.v_scale + row + 4 * (lane >> 4));
     }
   };
-  if (mine > 0) pages_ahead = look_up(0);
+  // the segment after x, where the share goes on
+  auto after = [&](const Segment& x) {
+    Segment y = x;
+    y.unit0 = 0;
+    if (++y.qtile == a.qtiles) {
+      y.qtile = 0;
+      ++y.head;
+    }
+    if (y.head == a.heads) {
+      y.head = 0;
+      y.range = range_of(++y.seq);
+      y.row_units = unit_count(y.range, a.unit);
+    }
+    y.unit1 = min(y.row_units, share_end - (unit + x.unit1 - x.unit0));
+    return y;
+  };
 
   // ---- the B operand of S^T = K Q^T: the channels of query `col` in K's order,
   // a step at a time, as they lie in memory and split into terms.  (Lanes past
@@ -338,10 +377,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
   // stored.)
   constexpr int kRaw = T::kF32 ? 1 : (int)sizeof(Q) / 2;  // 16-byte words of a step
   constexpr int kQuads = T::kQuerySteps * T::kTerms;      // of a query tile, term by term
-  auto load_step = [&](int t, int st, u32x4_t* raw) {
-    const int qi = q0 + t * 16 + col;
-    const Q* q = static_cast<const Q*>(a.q) + b * a.q_b +
-                 (int64_t)(head * a.group + (qi < a.group ? qi : 0)) * a.q_h;
+  auto load_step = [&](const Segment& x, int t, int st, u32x4_t* raw) {
+    const int g = lane >> 4;
+    const int qi = (x.qtile * QT + t) * 16 + (lane & 15);
+    const Q* q = static_cast<const Q*>(a.q) + x.seq * a.q_b +
+                 (int64_t)(x.head * a.group + (qi < a.group ? qi : 0)) * a.q_h;
     const int d = T::kF32               ? 16 * st + 4 * g
                   : T::kCoded && D > 32 ? 64 * (st >> 1) + 16 * g + 8 * (st & 1)
                                         : 32 * st + 8 * g;
@@ -374,28 +414,58 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
       }
     }
   };
-  u32x4_t raw[QT][T::kQuerySteps][kRaw];
-  if constexpr (T::kQueryLds) {
-    // the waves share the steps
-    for (int i = wave; i < QT * T::kQuerySteps; i += kPagedWaves) {
-      const int t = i / T::kQuerySteps, st = i - t * T::kQuerySteps;
-      u32x4_t step[kRaw], terms[T::kTerms];
-      load_step(t, st, step);
-      split_step(step, terms);
+  // (with the queries in LDS the waves share the steps)
+  constexpr int kAllSteps = QT * T::kQuerySteps;
+  constexpr int kMySteps =
+      T::kQueryLds ? (kAllSteps + kPagedWaves - 1) / kPagedWaves : kAllSteps;
+  auto step_of = [&](int i) { return T::kQueryLds ? wave + kPagedWaves * i : i; };
+  u32x4_t raw[kMySteps][kRaw];
+  auto load_queries = [&](const Segment& x) {
 #pragma unroll
-      for (int p = 0; p < T::kTerms; ++p)
-        query_lds[t * kQuads + p * T::kQuerySteps + st][lane] = terms[p];
-    }
-  } else {
-#pragma unroll
-    for (int t = 0; t < QT; ++t)
-#pragma unroll
-      for (int st = 0; st < T::kQuerySteps; ++st) load_step(t, st, raw[t][st]);
+    for (int i = 0; i < kMySteps; ++i)
+      if (step_of(i) < kAllSteps)
+        load_step(x, step_of(i) / T::kQuerySteps, step_of(i) % T::kQuerySteps, raw[i]);
+  };
+
+  // ---- the rows of the share, one after another.  What the next one begins with
+  // is asked for before this one is joined: its pages at this one's start, its
+  // first tile (and queries) after this one's last.
+  load_queries(cur);
+  if (fixed) {
+    cur.range = range_of(cur.seq);
+    cur.row_units = unit_count(cur.range, a.unit);
+    if (cur.unit0 >= cur.row_units) return;
   }
+  int mine = tiles_of(cur);
   if (mine > 0) {
-    pages_ahead = checked(pages_ahead);
-    load_k(0);
-    load_v(0);
+    int pages;
+    if (fixed && a.window <= 0) {
+      // past the sequence's last key its first page here stands in, which
+      // holds keys as the wave has a tile
+      const int lead = __builtin_amdgcn_readfirstlane(early_pages);
+      pages = early_key < cur.range.end ? early_pages : lead;
+    } else {
+      pages = look_up(cur, 0);
+    }
+    take_pages(pages);
+    load_k(cur, 0);
+    load_v(cur, 0);
+  }
+  while (true) {
+  // (not known to be the same for every row: what is derived from the lane is
+  // formed again for each, not kept in registers through the loop on its keys)
+  asm volatile("" : "+v"(lane));
+  const int col = lane & 15, g = lane >> 4;
+  const KeyRange range = cur.range;
+  const int start = start_of(cur);
+  const int next_unit = unit + cur.unit1 - cur.unit0;
+  const bool more = next_unit < share_end;
+  Segment next = cur;
+  int next_pages = 0, next_mine = 0;
+  if (more) {
+    next = after(cur);
+    next_mine = tiles_of(next);
+    if (next_mine > 0) next_pages = look_up(next, 0);
   }
 
   float m[QT], l[QT];
@@ -407,21 +477,21 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
 #pragma unroll
     for (int c = 0; c < T::kChannels; ++c) o[t][c] = {0.0f, 0.0f, 0.0f, 0.0f};
   }
-
-  u32x4_t qw[QT * kQuads];
-  if constexpr (T::kQueryLds) {
-    __syncthreads();
-  } else {
+  u32x4_t qw[T::kQueryLds ? 1 : QT * kQuads];
 #pragma unroll
-    for (int t = 0; t < QT; ++t)
+  for (int i = 0; i < kMySteps; ++i) {
+    const int t = step_of(i) / T::kQuerySteps, st = step_of(i) % T::kQuerySteps;
+    u32x4_t terms[T::kTerms];
+    split_step(raw[i], terms);
 #pragma unroll
-      for (int st = 0; st < T::kQuerySteps; ++st) {
-        u32x4_t terms[T::kTerms];
-        split_step(raw[t][st], terms);
-#pragma unroll
-        for (int p = 0; p < T::kTerms; ++p) qw[t * kQuads + p * T::kQuerySteps + st] = terms[p];
-      }
+    for (int p = 0; p < T::kTerms; ++p) {
+      if constexpr (!T::kQueryLds)
+        qw[t * kQuads + p * T::kQuerySteps + st] = terms[p];
+      else if (t < QT)
+        query_lds[t * kQuads + p * T::kQuerySteps + st][lane] = terms[p];
+    }
   }
+  if constexpr (T::kQueryLds) __syncthreads();
   int query_lane = lane;
   auto query = [&](int i) -> u32x4_t {
     if constexpr (T::kQueryLds)
@@ -512,8 +582,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
         }
     }
     if (n + 1 < mine) {
-      if ((n + 1) % kAhead == 0) pages_ahead = checked(look_up(n + 1));
-      load_k(n + 1);
+      if ((n + 1) % kAhead == 0) take_pages(look_up(cur, n + 1));
+      load_k(cur, n + 1);
     }
     // ---- online softmax; a lane's l covers its own group's keys
     float p[QT][kHalves * 4];
@@ -607,11 +677,22 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
         }
       }
     }
-    if (n + 1 < mine) load_v(n + 1);
+    if (n + 1 < mine) load_v(cur, n + 1);
+  }
+
+  const bool any_bad = __any(bad) || !range.valid;
+  bad = false;
+  if (more) {
+    if constexpr (!T::kQueryLds) load_queries(next);
+    if (next_mine > 0) {
+      take_pages(next_pages);
+      load_k(next, 0);
+      load_v(next, 0);
+    }
   }
 
   // ---- the four waves joined, in their order
-  if (__any(bad)) {
+  if (any_bad) {
 #pragma unroll
     for (int t = 0; t < QT; ++t) l[t] = __builtin_nanf("");
   }
@@ -640,17 +721,16 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
     for (int c = 0; c < T::kChannels; ++c) o[t][c] *= mine_scale;
     m[t] = top;
   }
-  // two exchanges: waves 2 and 3 into 0 and 1, then 1 into 0
-#pragma unroll
+  // two exchanges: waves 2 and 3 into 0 and 1, then 1 into 0 (a loop, as this
+  // code runs once a row and its fetch is not hidden)
+#pragma unroll 1
   for (int round = 2; round >= 1; round >>= 1) {
     if (wave >= round && wave < 2 * round) {
 #pragma unroll
       for (int t = 0; t < QT; ++t)
 #pragma unroll
         for (int c = 0; c < T::kChannels; ++c)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            joined[wave - round][(t * T::kChannels + c) * 4 + r][lane] = o[t][c][r];
+          joined[wave - round][t * T::kChannels + c][lane] = o[t][c];
     }
     __syncthreads();
     if (wave < round) {
@@ -658,20 +738,22 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
       for (int t = 0; t < QT; ++t)
 #pragma unroll
         for (int c = 0; c < T::kChannels; ++c)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            o[t][c][r] += joined[wave][(t * T::kChannels + c) * 4 + r][lane];
+          o[t][c] += joined[wave][t * T::kChannels + c][lane];
     }
     __syncthreads();
   }
   // ---- O^T: lane (query col, group g), register r of channel c of a part:
   // channel (4g + r) * kPartChannels + c of the part's 16 * kPartChannels
   if (wave == 0) {
+    const int b = cur.seq, head = cur.head;
+    const int q0 = cur.qtile * 16 * QT;  // the tile's first query head of the cache head's
+    const bool direct = cur.unit0 == 0 && cur.unit1 == cur.row_units;
     const int place = group * 2 + (unit == share_first ? 0 : 1);
-    if (unit0 == 0 && a.split && lane == 0) {
-      int* info = a.row_info + ((int64_t)(b * a.heads + head) * a.qtiles + qtile) * 2;
+    if (cur.unit0 == 0 && a.split && lane == 0) {
+      int* info = a.row_info + ((int64_t)b * rows + head * a.qtiles + cur.qtile) * 2;
       info[0] = place;
-      info[1] = share_of(shares, unit + row_units - 1) - group + 1;
+      info[1] = fixed ? cur.row_units
+                           : share_of(shares, unit + cur.row_units - 1) - group + 1;
     }
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
@@ -681,21 +763,24 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
       const bool empty = range.valid && range.end <= range.first;
       const float scale = direct ? (empty ? 0.0f : 1.0f / total_l[t]) : 1.0f;
       const int64_t part_row = (int64_t)place * a.tile_queries + t * 16 + col;
-      float* part = a.part + part_row * D;
-      Q* out = static_cast<Q*>(a.out) + b * a.o_b + hq * a.o_h;
+      // (rows of out are 16-byte aligned)
+      char* to = direct ? reinterpret_cast<char*>(static_cast<Q*>(a.out) + b * a.o_b + hq * a.o_h)
+                        : reinterpret_cast<char*>(a.part + part_row * D);
+      typedef float Piece __attribute__((ext_vector_type(T::kPartChannels)));
+      typedef Q OutPiece __attribute__((ext_vector_type(T::kPartChannels)));
 #pragma unroll
       for (int pt = 0; pt < T::kParts; ++pt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int d = pt * 16 * T::kPartChannels + (4 * g + r) * T::kPartChannels;
+          const int d = (16 * pt + 4 * g + r) * T::kPartChannels;
+          Piece x;
 #pragma unroll
-          for (int c = 0; c < T::kPartChannels; ++c) {
-            const float x = o[t][pt * T::kPartChannels + c][r] * scale;
-            if (direct)
-              out[d + c] = (Q)x;
-            else
-              part[d + c] = x;
-          }
+          for (int c = 0; c < T::kPartChannels; ++c)
+            x[c] = o[t][pt * T::kPartChannels + c][r] * scale;
+          if (std::is_same_v<Q, float> || !direct)
+            *reinterpret_cast<Piece*>(to + d * 4) = x;
+          else
+            *reinterpret_cast<OutPiece*>(to + d * sizeof(Q)) = __builtin_convertvector(x, OutPiece);
         }
       if (g == 0) {
         if (!direct) {
@@ -710,25 +795,25 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
     }
   }
 
-  // ---- the next row
-  unit += unit1 - unit0;
-  if (unit >= share_end) break;
-  if (unit1 == row_units && row + 1 == rows) {
-    at.base += row_units;
-    ++at.seq;
-    range = key_range(a.lengths[at.seq], a.max_length, a.window);
-    row_units = unit_count(range, kUnit);
-  }
+  if (!more) break;
+  if constexpr (T::kQueryLds) load_queries(next);  // (no registers for them before)
+  unit = next_unit;
+  cur = next;
+  mine = next_mine;
   }
 }
 
 template <typename Q, typename C, int D>
 hipError_t launch_paged_dim(const PagedArgs& a, hipStream_t stream) {
+  // a unit of a row to a work-group, the units slowest (work-groups go to the
+  // XCDs in turn: with the units fastest those that shorter sequences lack would
+  // all be missing on the same XCDs), or equal shares
+  const dim3 groups = a.each > 0 ? dim3(a.heads * a.qtiles, a.batch, a.each) : dim3(a.groups);
   if (a.query_tiles == 1) {
-    paged_attention_kernel<Q, C, D, 1><<<a.groups, kPagedThreads, 0, stream>>>(a);
+    paged_attention_kernel<Q, C, D, 1><<<groups, kPagedThreads, 0, stream>>>(a);
   } else {
     if constexpr (D <= 128)
-      paged_attention_kernel<Q, C, D, 2><<<a.groups, kPagedThreads, 0, stream>>>(a);
+      paged_attention_kernel<Q, C, D, 2><<<groups, kPagedThreads, 0, stream>>>(a);
     else
       return hipErrorInvalidValue;
   }

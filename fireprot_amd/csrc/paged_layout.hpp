@@ -33,13 +33,12 @@ FPX_HD int64_t cache_row(int64_t slot, int head, int64_t pages, int heads, int p
 // Keys [first, end) that a sequence of `length` tokens attends to, or invalid
 // where the length does not fit the call (negative, or above max_length).
 struct KeyRange {
-  int first, end;
-  bool valid;
+  int first, end, valid;
 };
 
 FPX_HD KeyRange key_range(int length, int max_length, int window) {
-  if (length < 0 || length > max_length) return {0, 0, false};
-  return {window > 0 && length > window ? length - window : 0, length, true};
+  if (length < 0 || length > max_length) return {0, 0, 0};
+  return {window > 0 && length > window ? length - window : 0, length, 1};
 }
 
 // The work on a range is counted in units of `unit` keys, the first begun at a

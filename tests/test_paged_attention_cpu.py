@@ -59,8 +59,8 @@ def test_workspace(lib):
     # a window bounds the work as a length does
     assert size(1, 3, 8, 2, 128, 1 << 16, 64) == 256
     assert size(1, 3, 8, 2, 128, 1 << 16, 1 << 40) == need
-    # one place a work-group and side, whatever the length
-    assert size(1, 3, 8, 2, 128, 1 << 24, 0) == need
+    # two places a work-group, whatever the length
+    assert size(1, 3, 8, 2, 128, 1 << 24, 0) == size(1, 3, 8, 2, 128, 1 << 20, 0)
     for bad in ((5, 3, 8, 2, 128, 128, 0), (1, -1, 8, 2, 128, 128, 0), (1, 3, 7, 2, 128, 128, 0),
                 (1, 3, 8, 2, 100, 128, 0), (1, 3, 8, 2, 128, -1, 0),
                 (1, 3, 8, 2, 128, 1 << 30, 0), (1, 3, 8, 2, 128, 128, -1),
