@@ -207,14 +207,13 @@ def check(code: int, what: str) -> None:
         raise RuntimeError(f"{what} failed with status {code} ({names.get(code, 'HIP error')})")
 
 
-def launch(device: Any, entry: Any, *args: Any) -> int:
-    """``entry(*args, stream)`` with ``device`` current and the handle of its
-    current stream; returns the status.  Where the device is current already,
-    the ordinary call, nothing is switched: a call of a few microseconds would
-    otherwise pay as much for the switch as for its launch."""
+def launch(index: int, entry: Any, *args: Any) -> int:
+    """``entry(*args, stream)`` with HIP device ``index`` current and the handle
+    of its current stream; returns the status.  Where the device is current
+    already, the ordinary call, nothing is switched: a call of a few microseconds
+    would otherwise pay as much for the switch as for its launch."""
     import torch
 
-    index = device.index
     if torch._C._cuda_getDevice() == index:
         return entry(*args, torch._C._cuda_getCurrentRawStream(index))
     with torch.cuda.device(index):

@@ -126,30 +126,28 @@ def cache_slots(block_table: torch.Tensor, positions: torch.Tensor,
     return torch.where(positions < 0, -1, inside)
 
 
-def _check_rows(t: torch.Tensor, name: str, cache: PagedCache, tokens: int) -> None:
-    shape = cache.k.shape
-    if t.shape != (tokens, shape[1], shape[3]):
-        raise ValueError(f"{name} must be [{tokens}, {shape[1]}, {shape[3]}], "
-                         f"got {tuple(t.shape)}")
-    if t.dtype not in ROW_DTYPES or t.device != cache.k.device:
+def _check_rows(t: torch.Tensor, name: str, shape: tuple[int, int, int], device: int) -> None:
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {tuple(t.shape)}")
+    if t.dtype not in ROW_DTYPES or t.get_device() != device:
         raise ValueError(f"{name} must be float32, bfloat16 or float16 on the cache's device")
 
 
-def _check_slots(slots: torch.Tensor, cache: PagedCache) -> torch.Tensor:
-    if slots.dim() != 1 or slots.dtype != torch.int64 or slots.device != cache.k.device:
-        raise ValueError("slots must be an int64 vector on the cache's device")
-    if not cache.k.is_cuda:
+def _check_slots(slots: torch.Tensor, device: int) -> torch.Tensor:
+    if device < 0:
         raise ValueError("the cache must be on a HIP device")
+    if slots.dim() != 1 or slots.dtype != torch.int64 or slots.get_device() != device:
+        raise ValueError("slots must be an int64 vector on the cache's device")
     return slots if slots.is_contiguous() else slots.contiguous()
 
 
-def _call(entry, what, row_dtype, cache, k, v, slots):
-    pages, heads, page_size, head_dim = cache.k.shape
+def _call(entry, what, device, row_dtype, cache, k, v, slots):
     code = _native.launch(
-        cache.k.device, entry, ROW_DTYPES[row_dtype], CACHE_DTYPES[cache.k.dtype],
-        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-        slots.data_ptr(), slots.shape[0], *cache.pointers(), pages, heads, page_size, head_dim)
-    _native.check(code, what)
+        device, entry, ROW_DTYPES[row_dtype], CACHE_DTYPES[cache.k.dtype],
+        k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2],
+        slots.data_ptr(), slots.shape[0], *cache.pointers(), *cache.k.shape)
+    if code:
+        _native.check(code, what)
 
 
 def cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor,
@@ -163,9 +161,12 @@ def cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor,
     one slot it is not defined what the slot holds.
     """
     lib = _native.library()
-    slots = _check_slots(slots, cache)
-    _check_rows(k, "k", cache, slots.shape[0])
-    _check_rows(v, "v", cache, slots.shape[0])
+    _, heads, _, head_dim = cache.k.shape
+    device = cache.k.get_device()
+    slots = _check_slots(slots, device)
+    shape = (slots.shape[0], heads, head_dim)
+    _check_rows(k, "k", shape, device)
+    _check_rows(v, "v", shape, device)
     if v.dtype != k.dtype:
         raise ValueError("k and v must have one type")
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
@@ -174,7 +175,7 @@ def cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor,
         k = k.contiguous()
     if v.stride(2) != 1:
         v = v.contiguous()
-    _call(lib.fpx_cache_write, "fpx_cache_write", k.dtype, cache, k, v, slots)
+    _call(lib.fpx_cache_write, "fpx_cache_write", device, k.dtype, cache, k, v, slots)
 
 
 def cache_read(cache: PagedCache, slots: torch.Tensor, *, dtype: torch.dtype | None = None,
@@ -185,25 +186,26 @@ def cache_read(cache: PagedCache, slots: torch.Tensor, *, dtype: torch.dtype | N
     the rows at ``slots``, dequantised in 32 bits and rounded once.  A negative
     slot gives zeros, one past the cache NaN.  Slots may repeat."""
     lib = _native.library()
-    slots = _check_slots(slots, cache)
+    _, heads, _, head_dim = cache.k.shape
+    device = cache.k.get_device()
+    slots = _check_slots(slots, device)
     if dtype is None:
         given = k_out if k_out is not None else v_out
         dtype = (given.dtype if given is not None
                  else torch.float32 if cache.dtype in CODED_DTYPES else cache.dtype)
     if dtype not in ROW_DTYPES:
         raise ValueError("rows are read as float32, bfloat16 or float16")
-    outs, shape = [], cache.k.shape
+    outs, shape = [], (slots.shape[0], heads, head_dim)
     for out, name in ((k_out, "k_out"), (v_out, "v_out")):
         if out is None:
-            out = torch.empty((slots.shape[0], shape[1], shape[3]), dtype=dtype,
-                              device=cache.k.device)
+            out = slots.new_empty(shape, dtype=dtype)
         else:
-            _check_rows(out, name, cache, slots.shape[0])
+            _check_rows(out, name, shape, device)
             if out.dtype != dtype or out.stride(2) != 1 or _native.repeats(out):
                 raise ValueError(f"{name} must be {dtype} with unit channel stride and no "
                                  "repeated elements")
             if torch.is_grad_enabled() and out.requires_grad:
                 raise ValueError("a cache records no gradient: detach the outputs")
         outs.append(out)
-    _call(lib.fpx_cache_read, "fpx_cache_read", dtype, cache, outs[0], outs[1], slots)
+    _call(lib.fpx_cache_read, "fpx_cache_read", device, dtype, cache, outs[0], outs[1], slots)
     return outs[0], outs[1]

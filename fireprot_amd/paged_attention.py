@@ -58,7 +58,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
     """
     lib = _native.library()
     k = cache.k
-    if q.dim() != 3 or q.dtype not in ROW_DTYPES or q.device != k.device or not q.is_cuda:
+    device = k.get_device()
+    if q.dim() != 3 or q.dtype not in ROW_DTYPES or device < 0 or q.get_device() != device:
         raise ValueError("q must be float32, bfloat16 or float16 [batch, q_heads, head_dim] on "
                          "the cache's HIP device")
     batch, q_heads, head_dim = q.shape
@@ -69,9 +70,9 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
     if k.dtype not in CODED_DTYPES and k.dtype != q.dtype:
         raise ValueError(f"a {k.dtype} cache needs {k.dtype} queries")
     if (block_table.dim() != 2 or block_table.shape[0] != batch or block_table.dtype != torch.int32
-            or block_table.device != q.device):
+            or block_table.get_device() != device):
         raise ValueError("block_table must be int32 [batch, pages] on q's device")
-    if lengths.shape != (batch,) or lengths.dtype != torch.int32 or lengths.device != q.device:
+    if lengths.shape != (batch,) or lengths.dtype != torch.int32 or lengths.get_device() != device:
         raise ValueError("lengths must be int32 [batch] on q's device")
     held = block_table.shape[1] * page_size
     if max_length is None:
@@ -88,34 +89,33 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
     if not lengths.is_contiguous():
         lengths = lengths.contiguous()
     if out is None:
-        out = torch.empty((batch, q_heads, head_dim), dtype=q.dtype, device=q.device)
-    elif (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device
+        out = q.new_empty((batch, q_heads, head_dim))
+    elif (out.shape != q.shape or out.dtype != q.dtype or out.get_device() != device
           or not _aligned_rows(out) or _native.repeats(out)):
         raise ValueError("out must have q's shape, type and device, 16-byte aligned rows and "
                          "no repeated elements")
-    lse = (torch.empty((batch, q_heads), dtype=torch.float32, device=q.device)
-           if return_lse else None)
+    lse = q.new_empty((batch, q_heads), dtype=torch.float32) if return_lse else None
     size = lib.fpx_paged_attention_workspace_bytes(CACHE_DTYPES[k.dtype], batch, q_heads, heads,
                                                    head_dim, max_length, window)
     if size == 0:
         raise ValueError(f"unsupported sizes: batch {batch}, {q_heads} query heads, "
                          f"max_length {max_length}, window {window}")
     if workspace is not None:
-        if (workspace.dtype != torch.uint8 or workspace.device != q.device
+        if (workspace.dtype != torch.uint8 or workspace.get_device() != device
                 or workspace.numel() < size or not workspace.is_contiguous()):
             raise ValueError(f"workspace must be {size} contiguous bytes on q's device")
     elif size > NO_WORKSPACE:
         # of the current stream, and of the graph where one is captured: no two
         # calls that may overlap share it
-        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
-    qs, os = q.stride(), out.stride()
+        workspace = q.new_empty(size, dtype=torch.uint8)
     code = _native.launch(
-        q.device, lib.fpx_paged_attention, ROW_DTYPES[q.dtype], CACHE_DTYPES[k.dtype],
-        q.data_ptr(), qs[0], qs[1], *cache.pointers(), pages, heads, page_size, head_dim,
+        device, lib.fpx_paged_attention, ROW_DTYPES[q.dtype], CACHE_DTYPES[k.dtype],
+        q.data_ptr(), *q.stride()[:2], *cache.pointers(), pages, heads, page_size, head_dim,
         block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
         lengths.data_ptr(), batch, q_heads, max_length, window,
-        head_dim ** -0.5 if scale is None else scale, out.data_ptr(), os[0], os[1],
+        head_dim ** -0.5 if scale is None else scale, out.data_ptr(), *out.stride()[:2],
         None if lse is None else lse.data_ptr(),
         None if workspace is None else workspace.data_ptr(), size)
-    _native.check(code, "fpx_paged_attention")
+    if code:
+        _native.check(code, "fpx_paged_attention")
     return (out, lse) if return_lse else out

@@ -30,13 +30,18 @@ DTYPES = {torch.float32: _native.FPX_F32, torch.bfloat16: _native.FPX_BF16,
 POSITION_DTYPES = {torch.int32: 0, torch.int64: 1}
 
 
-@dataclasses.dataclass
+@dataclasses.dataclass(frozen=True, eq=False)
 class RotaryFrequencies:
-    """``inv_freq``: float64 ``[rotary_dim / 2]``, radians a position of each
-    pair; ``scale``: factor of the rotated channels."""
+    """``inv_freq``: contiguous float64 ``[rotary_dim / 2]``, radians a position
+    of each pair; ``scale``: factor of the rotated channels."""
 
     inv_freq: torch.Tensor
     scale: float = 1.0
+
+    def __post_init__(self) -> None:
+        f = self.inv_freq
+        if f.dtype != torch.float64 or f.dim() != 1 or f.numel() < 1 or not f.is_contiguous():
+            raise ValueError("inv_freq must be a contiguous float64 vector, not empty")
 
     @property
     def rotary_dim(self) -> int:
@@ -100,7 +105,7 @@ def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
 def _output(given: torch.Tensor | None, like: torch.Tensor, rows: torch.Tensor, name: str):
     """(the four-axis output, what the caller gets) for an input and its rows."""
     if given is None:
-        out = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
+        out = rows.new_empty(rows.shape)
         return out, out if like.dim() == 4 else out[0]
     if (given.shape != like.shape or given.dtype != like.dtype or given.device != like.device
             or given.stride(-1) != 1 or _native.repeats(given)):
@@ -115,48 +120,44 @@ def _launch(q, k, positions, frequencies, layout, inverse, q_out, k_out):
     mode = LAYOUTS.get(layout)
     if mode is None:
         raise ValueError(f"layout must be one of {sorted(LAYOUTS)}")
-    kind, device = DTYPES.get(q.dtype), q.device
-    if kind is None or not q.is_cuda:
+    kind, device = DTYPES.get(q.dtype), q.get_device()
+    if kind is None or device < 0:
         raise ValueError("q must be a float32, bfloat16 or float16 tensor on a HIP device")
-    x = _rows(q, "q")
+    x = q if q.dim() == 4 and q.stride(3) == 1 else _rows(q, "q")
     batch, tokens, q_heads, head_dim = x.shape
     inv_freq = frequencies.inv_freq
-    if (inv_freq.dtype != torch.float64 or inv_freq.device != device or inv_freq.dim() != 1
-            or not inv_freq.is_contiguous()):
-        raise ValueError("inv_freq must be a contiguous float64 vector on q's device")
     rotary_dim = 2 * inv_freq.shape[0]
-    if not 2 <= rotary_dim <= head_dim <= MAX_HEAD_DIM:
-        raise ValueError(f"needs 2 <= rotary_dim ({rotary_dim}) <= head_dim ({head_dim}) "
+    if rotary_dim > head_dim or head_dim > MAX_HEAD_DIM:
+        raise ValueError(f"needs rotary_dim ({rotary_dim}) <= head_dim ({head_dim}) "
                          f"<= {MAX_HEAD_DIM}")
     wide = positions.dim() == 2
-    if (positions.dtype not in POSITION_DTYPES or positions.device != device
+    place = POSITION_DTYPES.get(positions.dtype)
+    if (place is None or positions.get_device() != device or inv_freq.get_device() != device
             or positions.shape != ((batch, tokens) if wide else (tokens,))):
-        raise ValueError("positions must be int32 or int64 [batch, tokens] or [tokens] "
-                         "on q's device")
+        raise ValueError("positions must be int32 or int64 [batch, tokens] or [tokens], and they "
+                         "and inv_freq on q's device")
     a, q_ret = _output(q_out, q, x, "q_out")
     if k is None:
         k_heads, k_ret = 0, None
         k_args = k_out_args = (None, 0, 0, 0)
     else:
-        if (k.dtype != q.dtype or k.device != device or k.dim() != q.dim()
+        if (k.dtype != q.dtype or k.get_device() != device or k.dim() != q.dim()
                 or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != head_dim):
             raise ValueError("k must have q's type, device, batch, tokens and head_dim")
-        y = _rows(k, "k")
+        y = k if k.dim() == 4 and k.stride(3) == 1 else _rows(k, "k")
         k_heads = y.shape[2]
         b, k_ret = _output(k_out, k, y, "k_out")
-        s, t = y.stride(), b.stride()
-        k_args = (y.data_ptr(), s[0], s[1], s[2])
-        k_out_args = (b.data_ptr(), t[0], t[1], t[2])
+        k_args = (y.data_ptr(), *y.stride()[:3])
+        k_out_args = (b.data_ptr(), *b.stride()[:3])
     if q_heads == 0 and k_heads == 0:
         return q_ret, k_ret
-    s, t = x.stride(), a.stride()
     code = _native.launch(
-        device, lib.fpx_rotary, kind, mode, x.data_ptr(), s[0], s[1], s[2],
-        a.data_ptr(), t[0], t[1], t[2], q_heads, *k_args, *k_out_args, k_heads,
-        positions.data_ptr(), POSITION_DTYPES[positions.dtype],
-        positions.stride(0) if wide else 0, positions.stride(-1),
+        device, lib.fpx_rotary, kind, mode, x.data_ptr(), *x.stride()[:3],
+        a.data_ptr(), *a.stride()[:3], q_heads, *k_args, *k_out_args, k_heads,
+        positions.data_ptr(), place, positions.stride(0) if wide else 0, positions.stride(-1),
         inv_freq.data_ptr(), frequencies.scale, inverse, batch, tokens, head_dim, rotary_dim)
-    _native.check(code, "fpx_rotary")
+    if code:
+        _native.check(code, "fpx_rotary")
     return q_ret, k_ret
 
 

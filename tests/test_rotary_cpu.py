@@ -97,6 +97,14 @@ def test_frequencies_refuse(bad):
         rotary.rotary_frequencies(**bad)
 
 
+@pytest.mark.parametrize("inv_freq", [
+    torch.ones(4), torch.ones(2, 2, dtype=torch.float64), torch.ones(0, dtype=torch.float64),
+    torch.ones(8, dtype=torch.float64)[::2]])
+def test_given_frequencies_are_checked(inv_freq):
+    with pytest.raises(ValueError, match="inv_freq"):
+        rotary.RotaryFrequencies(inv_freq)
+
+
 def test_cpu_tensors_are_refused(lib):
     q = torch.zeros(1, 2, 4, 32)
     with pytest.raises(ValueError, match="HIP device"):
