@@ -38,7 +38,11 @@ template <typename T>
 struct Eight {
   typedef T Vec __attribute__((ext_vector_type(8)));
   Vec x;
-  __device__ __forceinline__ void load(const T* p) { x = *reinterpret_cast<const Vec*>(p); }
+  template <bool kStream>
+  __device__ __forceinline__ void load(const T* p) {
+    const Vec* v = reinterpret_cast<const Vec*>(p);
+    x = kStream ? __builtin_nontemporal_load(v) : *v;
+  }
   // rows of any alignment of T
   __device__ __forceinline__ void load_each(const T* p) {
 #pragma unroll
@@ -56,8 +60,10 @@ struct Eight {
 // Eight codes of a row.
 struct Codes {
   u32x2 x;
+  template <bool kStream>
   __device__ __forceinline__ void load(const uint8_t* p) {
-    x = *reinterpret_cast<const u32x2*>(p);
+    const u32x2* v = reinterpret_cast<const u32x2*>(p);
+    x = kStream ? __builtin_nontemporal_load(v) : *v;
   }
   __device__ __forceinline__ void store(uint8_t* p) const { *reinterpret_cast<u32x2*>(p) = x; }
 };
@@ -149,7 +155,7 @@ __device__ __forceinline__ void decode(u32x2 codes, float scale, float* x) {
 
 // tokens x heads rows of S into a cache of C.  kVec: the source rows are
 // 16-byte aligned.
-template <typename S, typename C, int kDim, bool kVec>
+template <typename S, typename C, int kDim, bool kVec, bool kStream>
 __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(CacheArgs a) {
   constexpr int kGroup = kDim / 8;                  // threads of a row
   constexpr int kPass = kCacheThreads / kGroup;     // rows of a pass
@@ -171,7 +177,7 @@ __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(CacheArgs a)
       for (int w = 0; w < 2; ++w) {
         const S* src = static_cast<const S*>(a.rows[w]) + t * a.stride_t[w] + h * a.stride_h[w] + c;
         if constexpr (kVec)
-          x[r][w].load(src);
+          x[r][w].template load<kStream>(src);
         else
           x[r][w].load_each(src);
       }
@@ -214,7 +220,7 @@ __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(CacheArgs a)
 
 // The rows of `slots` back as S: zeros where there is no slot, NaN for a slot
 // past the cache's end.
-template <typename S, typename C, int kDim, bool kVec>
+template <typename S, typename C, int kDim, bool kVec, bool kStream>
 __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(CacheArgs a) {
   constexpr int kGroup = kDim / 8;
   constexpr int kPass = kCacheThreads / kGroup;
@@ -242,7 +248,8 @@ __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(CacheArgs a) 
       if (at[r] < 0) continue;
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        held[r][w].load(static_cast<const Elem<C>*>(a.cache[w]) + at[r] * kDim + c);
+        held[r][w].template load<kStream>(static_cast<const Elem<C>*>(a.cache[w]) + at[r] * kDim +
+                                          c);
         if constexpr (kCoded<C>) scale[r][w] = a.scale[w][at[r]];
       }
     }
@@ -290,16 +297,23 @@ hipError_t launch_dim(const CacheArgs& a, bool read, hipStream_t stream) {
     bytes |= reinterpret_cast<uintptr_t>(a.rows[w]) |
              (uint64_t)(a.stride_t[w] | a.stride_h[w]) * sizeof(S);
   const bool vec = bytes % 16 == 0;
+  // what is read and no cache holds anyway is streamed past them
+  const int64_t row = kDim * (read ? (int64_t)sizeof(Elem<C>) : (int64_t)sizeof(S));
+  const bool once = 2 * a.tokens * a.heads * row >= kStreamBytes;
   if (read) {
-    if (vec)
-      cache_read_kernel<S, C, kDim, true><<<grid, kCacheThreads, 0, stream>>>(a);
+    if (!vec)
+      cache_read_kernel<S, C, kDim, false, false><<<grid, kCacheThreads, 0, stream>>>(a);
+    else if (once)
+      cache_read_kernel<S, C, kDim, true, true><<<grid, kCacheThreads, 0, stream>>>(a);
     else
-      cache_read_kernel<S, C, kDim, false><<<grid, kCacheThreads, 0, stream>>>(a);
+      cache_read_kernel<S, C, kDim, true, false><<<grid, kCacheThreads, 0, stream>>>(a);
   } else {
-    if (vec)
-      cache_write_kernel<S, C, kDim, true><<<grid, kCacheThreads, 0, stream>>>(a);
+    if (!vec)
+      cache_write_kernel<S, C, kDim, false, false><<<grid, kCacheThreads, 0, stream>>>(a);
+    else if (once)
+      cache_write_kernel<S, C, kDim, true, true><<<grid, kCacheThreads, 0, stream>>>(a);
     else
-      cache_write_kernel<S, C, kDim, false><<<grid, kCacheThreads, 0, stream>>>(a);
+      cache_write_kernel<S, C, kDim, true, false><<<grid, kCacheThreads, 0, stream>>>(a);
   }
   return hipGetLastError();
 }

@@ -51,13 +51,18 @@ __device__ __forceinline__ float2 turn(double pos, double freq) {
   return {(q == 1 || q == 2) ? -cs : cs, (q >= 2) ? -sn : sn};
 }
 
+// x / n by n's magic number 2^32 / n + 1, for x * n < 2^32.
+__device__ __forceinline__ int divide(int x, int n, unsigned magic) {
+  return n == 1 ? x : (int)__umulhi((unsigned)x, magic);
+}
+
 // Work-group: `tt` tokens of all heads of both tensors.  The factors of each
-// (token, pair) are computed once, into LDS, and serve every head.  Then each
-// row (token, head) is taken by 2^unit_shift consecutive threads, one W-byte
-// vector of each half (or one vector of pairs) each, kRotaryBatch rows at a
-// time with their loads issued before the first use.  In place is safe: a
-// thread's stores go to exactly the channels it has read.
-template <typename T, int W, bool kInterleaved>
+// (token, pair) are computed once, into LDS, and serve every head.  Then the
+// threads take the units of all rows (token, head) in turn, one W-byte vector of
+// each half (or one vector of pairs) to a unit, kRotaryBatch at a time with their
+// loads issued before the first use.  In place is safe: a thread's stores go to
+// exactly the channels it has read.
+template <typename T, int W, bool kInterleaved, bool kStream>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
   constexpr int kElems = W / (int)sizeof(T);                // of one vector
   constexpr bool kPairVector = kInterleaved && kElems >= 2; // a vector holds whole pairs
@@ -88,69 +93,69 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
   }
   __syncthreads();
 
-  const int width = 1 << a.unit_shift;  // threads of a row
-  const int step = kRotaryThreads >> a.unit_shift;
   const int q_heads = a.x[0].heads, heads = q_heads + a.x[1].heads;
-  const int rows = tokens * heads;
+  const int items = tokens * heads * a.units;
   const int rot_units = half / kPairs;
-  for (int unit = threadIdx.x & (width - 1); unit < a.units; unit += width) {
-    // a unit's first and second channel; a unit past the rotated part copies
-    // one vector
-    const bool turned = unit < rot_units;
-    const int c0 = !turned        ? a.rot + (unit - rot_units) * kElems
-                   : kInterleaved ? 2 * unit * kPairs
-                                  : unit * kPairs;
-    const int c1 = kInterleaved ? c0 + 1 : c0 + half;
-    const bool second = turned && !kPairVector;
-    for (int base = threadIdx.x >> a.unit_shift; base < rows; base += step * kRotaryBatch) {
-      Vec u[kRotaryBatch], v[kRotaryBatch];
-      T* dst[kRotaryBatch];
-      int local[kRotaryBatch];
+  for (int base = threadIdx.x; base < items; base += kRotaryThreads * kRotaryBatch) {
+    Vec u[kRotaryBatch], v[kRotaryBatch];
+    T* dst[kRotaryBatch];   // the unit's first channel
+    int local[kRotaryBatch];  // its first factor; negative: a copy
 #pragma unroll
-      for (int r = 0; r < kRotaryBatch; ++r) {
-        const int row = base + r * step;
-        if (row >= rows) continue;
-        const int tl = heads == 1 ? row : (int)__umulhi((unsigned)row, a.heads_magic);
-        int h = row - tl * heads;
-        const int w = h >= q_heads;
-        h -= w ? q_heads : 0;
-        const T* src = row_in[tl][w] + h * (w ? a.x[1].in_h : a.x[0].in_h);
-        dst[r] = row_out[tl][w] + h * (w ? a.x[1].out_h : a.x[0].out_h);
-        local[r] = tl * half + unit * kPairs;
-        u[r] = *reinterpret_cast<const Vec*>(src + c0);
-        if (second) v[r] = *reinterpret_cast<const Vec*>(src + c1);
+    for (int r = 0; r < kRotaryBatch; ++r) {
+      const int item = base + r * kRotaryThreads;
+      if (item >= items) continue;
+      const int row = divide(item, a.units, a.units_magic);
+      const int unit = item - row * a.units;
+      const int tl = divide(row, heads, a.heads_magic);
+      int h = row - tl * heads;
+      const int w = h >= q_heads;
+      h -= w ? q_heads : 0;
+      // a unit past the rotated part copies one vector
+      const bool turned = unit < rot_units;
+      const int c0 = !turned        ? a.rot + (unit - rot_units) * kElems
+                     : kInterleaved ? 2 * unit * kPairs
+                                    : unit * kPairs;
+      const T* src = row_in[tl][w] + h * (w ? a.x[1].in_h : a.x[0].in_h) + c0;
+      dst[r] = row_out[tl][w] + h * (w ? a.x[1].out_h : a.x[0].out_h) + c0;
+      local[r] = turned ? tl * half + unit * kPairs : -1;
+      const Vec* p0 = reinterpret_cast<const Vec*>(src);
+      u[r] = kStream ? __builtin_nontemporal_load(p0) : *p0;
+      if (turned && !kPairVector) {
+        const Vec* p1 = reinterpret_cast<const Vec*>(src + (kInterleaved ? 1 : half));
+        v[r] = kStream ? __builtin_nontemporal_load(p1) : *p1;
       }
+    }
 #pragma unroll
-      for (int r = 0; r < kRotaryBatch; ++r) {
-        if (base + r * step >= rows) continue;
-        if (turned) {
+    for (int r = 0; r < kRotaryBatch; ++r) {
+      if (base + r * kRotaryThreads >= items) continue;
+      if (local[r] >= 0) {
 #pragma unroll
-          for (int p = 0; p < kPairs; ++p) {
-            const float2 f = factor[local[r] + p];
-            if constexpr (kPairVector) {
-              const float x1 = (float)u[r][2 * p], x2 = (float)u[r][2 * p + 1];
-              u[r][2 * p] = (T)__builtin_fmaf(x1, f.x, -(x2 * f.y));
-              u[r][2 * p + 1] = (T)__builtin_fmaf(x2, f.x, x1 * f.y);
-            } else {
-              const float x1 = (float)u[r][p], x2 = (float)v[r][p];
-              u[r][p] = (T)__builtin_fmaf(x1, f.x, -(x2 * f.y));
-              v[r][p] = (T)__builtin_fmaf(x2, f.x, x1 * f.y);
-            }
+        for (int p = 0; p < kPairs; ++p) {
+          const float2 f = factor[local[r] + p];
+          if constexpr (kPairVector) {
+            const float x1 = (float)u[r][2 * p], x2 = (float)u[r][2 * p + 1];
+            u[r][2 * p] = (T)__builtin_fmaf(x1, f.x, -(x2 * f.y));
+            u[r][2 * p + 1] = (T)__builtin_fmaf(x2, f.x, x1 * f.y);
+          } else {
+            const float x1 = (float)u[r][p], x2 = (float)v[r][p];
+            u[r][p] = (T)__builtin_fmaf(x1, f.x, -(x2 * f.y));
+            v[r][p] = (T)__builtin_fmaf(x2, f.x, x1 * f.y);
           }
         }
-        *reinterpret_cast<Vec*>(dst[r] + c0) = u[r];
-        if (second) *reinterpret_cast<Vec*>(dst[r] + c1) = v[r];
+        if constexpr (!kPairVector)
+          *reinterpret_cast<Vec*>(dst[r] + (kInterleaved ? 1 : half)) = v[r];
       }
+      *reinterpret_cast<Vec*>(dst[r]) = u[r];
     }
   }
 }
 
-template <typename T, int W>
+template <typename T, int W, bool kStream>
 hipError_t launch_width(const RotaryArgs& a, unsigned blocks, hipStream_t stream) {
   if (a.interleaved)
-    rotary_kernel<T, W, true><<<blocks, kRotaryThreads, 0, stream>>>(a);
+    rotary_kernel<T, W, true, kStream><<<blocks, kRotaryThreads, 0, stream>>>(a);
   else
-    rotary_kernel<T, W, false><<<blocks, kRotaryThreads, 0, stream>>>(a);
+    rotary_kernel<T, W, false, kStream><<<blocks, kRotaryThreads, 0, stream>>>(a);
   return hipGetLastError();
 }
 
@@ -181,23 +186,29 @@ hipError_t launch_type(RotaryArgs& a, hipStream_t stream) {
   if (copies && a.x[0].in == a.x[0].out && (a.x[1].heads == 0 || a.x[1].in == a.x[1].out))
     copies = false;
   a.units = half / pairs + (copies ? (a.head_dim - a.rot) / elems : 0);
-  a.unit_shift = 0;
-  while ((1 << a.unit_shift) < a.units && (1 << a.unit_shift) < kRotaryThreads) ++a.unit_shift;
-  // Tokens per work-group: enough rows to fill the threads' batches, as long
-  // as the grid still covers the 256 CUs several times over.
+  // Tokens of a work-group: a unit for every thread, as long as the grid still
+  // covers the 256 CUs several times over (16384 tokens of 40 heads of 128 take
+  // 56 us with one token, 62 with four; 32768 tokens of 4 heads of 64 take 11 us
+  // with sixteen, 40 with one).
   a.tt = 1;
   const int heads = a.x[0].heads + a.x[1].heads;
-  a.heads_magic = 0xffffffffu / (unsigned)heads + 1;  // row / heads for row * heads < 2^32
+  a.units_magic = 0xffffffffu / (unsigned)a.units + 1;
+  a.heads_magic = 0xffffffffu / (unsigned)heads + 1;
   while (a.tt < kRotaryTokens && a.total / (2 * a.tt) >= 2048 && 2 * a.tt * half <= kRotaryAngles &&
-         a.tt * heads * (1 << a.unit_shift) < kRotaryThreads * kRotaryBatch)
+         a.tt * heads * a.units < kRotaryThreads)
     a.tt *= 2;
   const unsigned blocks = ((unsigned)a.total + a.tt - 1) / a.tt;
+  // Rows of whole 16-byte vectors that no cache holds anyway are streamed past
+  // them (see kStreamBytes); narrower vectors read a line several times over.
+  const bool stream_rows = (int64_t)a.total * heads * a.head_dim * (int64_t)sizeof(T) >= kStreamBytes;
   switch (w) {
-    case 16: return launch_width<T, 16>(a, blocks, stream);
-    case 8: return launch_width<T, 8>(a, blocks, stream);
-    case 4: return launch_width<T, 4>(a, blocks, stream);
+    case 16:
+      return stream_rows ? launch_width<T, 16, true>(a, blocks, stream)
+                         : launch_width<T, 16, false>(a, blocks, stream);
+    case 8: return launch_width<T, 8, false>(a, blocks, stream);
+    case 4: return launch_width<T, 4, false>(a, blocks, stream);
     default:
-      if constexpr (sizeof(T) == 2) return launch_width<T, 2>(a, blocks, stream);
+      if constexpr (sizeof(T) == 2) return launch_width<T, 2, false>(a, blocks, stream);
       return hipErrorInvalidValue;
   }
 }

@@ -270,3 +270,34 @@ def test_other_stream_and_graph():
         wback = rotary.rotary_backward(*want, positions, f)
         assert torch.equal(qo, want[0]) and torch.equal(ko, want[1])
         assert torch.equal(back[0], wback[0]) and torch.equal(back[1], wback[1])
+
+
+@pytest.mark.parametrize("dtype,layout", [(torch.bfloat16, "half"), (torch.float32, "interleaved")])
+def test_large_calls_equal_small_ones(dtype, layout):
+    """Rows of 64 MB and more are loaded past the caches, several tokens to a
+    work-group: the same bits as call by call."""
+    tokens, heads, dim = (64 << 20) // (20 * 128 * dtype.itemsize) + 7, 16, 128
+    f = rotary.rotary_frequencies(96, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(8)
+    q = torch.randn(tokens, heads, dim, device="cuda", generator=g).to(dtype)
+    k = torch.randn(tokens, 4, dim, device="cuda", generator=g).to(dtype)
+    positions = torch.arange(tokens, device="cuda") * 3
+    whole = rotary.apply_rotary(q, k, positions, f, layout=layout)
+    for lo in (0, 1000, tokens - 300):
+        part = slice(lo, lo + 300)
+        small = rotary.apply_rotary(q[part], k[part], positions[part], f, layout=layout)
+        assert torch.equal(whole[0][part], small[0]) and torch.equal(whole[1][part], small[1])
+    check(whole[0][-5:], q[-5:], positions[-5:], f, layout)
+
+
+def test_many_heads_and_units():
+    """The most heads, and rows of more vectors than a work-group has threads."""
+    f = rotary.rotary_frequencies(2, device="cuda")
+    q, k = randn((1, 2, 8191, 6), torch.bfloat16), randn((1, 2, 1, 6), torch.bfloat16, 2)
+    positions = torch.tensor([1, 77]).cuda()
+    out = rotary.apply_rotary(q, k, positions, f)
+    check(out[0], q, positions, f, "half")
+    check(out[1], k, positions, f, "half")
+    wide = randn((1, 3, 8, 513), torch.float16)[..., 1:]  # 512 channels, one element a vector
+    out = rotary.apply_rotary(wide, None, positions.new_tensor([0, 5, 9]), f)
+    check(out, wide, positions.new_tensor([0, 5, 9]), f, "half")
