@@ -83,8 +83,9 @@ class Setup:
         return paged_attention(kw.pop("q", self.q), self.cache, kw.pop("table", self.table),
                                kw.pop("lengths", self.lengths), **kw)
 
-    def reference(self, scale=None):
-        """(o, lse, tolerance of o, tolerance of lse), float64 on the CPU."""
+    def reference(self, scale=None, only=None):
+        """(o, lse, tolerance of o, tolerance of lse), float64 on the CPU, of the
+        sequences ``only`` (all)."""
         scale = self.scale if scale is None else scale
         b, hq, d = self.q.shape
         heads, page = self.cache.heads, self.cache.page_size
@@ -98,7 +99,7 @@ class Setup:
             data.append((t, None if s is None else s.cpu()))
         for i, slots in enumerate(self.slots):
             n = len(slots)
-            if n == 0:
+            if n == 0 or (only is not None and i not in only):
                 continue
             kv = []
             for t, s in data:
@@ -125,9 +126,12 @@ class Setup:
             ltol[i] = (2 * relative + 2.0 ** -22 * total.abs()).reshape(hq)
         return out, lse, tol, ltol
 
-    def check(self, got, scale=None):
+    def check(self, got, scale=None, only=None):
         out, lse = got
-        want, want_lse, tol, ltol = self.reference(scale)
+        want, want_lse, tol, ltol = self.reference(scale, only)
+        if only is not None:
+            out, lse, want, want_lse, tol, ltol = (
+                t[sorted(only)] for t in (out, lse, want, want_lse, tol, ltol))
         gap = (out.cpu().double() - want).abs()
         assert not torch.isnan(gap).any()
         assert (gap <= tol).all(), f"out {(gap / tol.clamp(min=1e-300)).max().item()} of the bound"
@@ -178,6 +182,45 @@ def test_many_chunks(q_type, cache_type):
     wide = Setup(q_type, cache_type, 64, 64, 32, 32, [900] * 40, seed=8)
     assert workspace_bytes(wide.q, wide.cache, wide.max_length) >= 256
     wide.check(wide.call())
+
+
+@pytest.mark.parametrize("q_type,cache_type", PAIRS)
+@pytest.mark.parametrize("batch,q_heads,heads,dim,longest,window", [
+    (700, 4, 2, 32, 600, 0), (300, 24, 1, 64, 1500, 0), (257, 40, 1, 128, 700, 300),
+    (1025, 3, 1, 256, 300, 0), (5000, 2, 2, 32, 130, 50)])
+def test_shares_of_many_sequences(q_type, cache_type, batch, q_heads, heads, dim, longest, window):
+    """More rows than work-groups: shares begin and end inside rows, span several
+    and start anywhere in the batch (empty sequences among them)."""
+    print(f"paged {q_type} {cache_type} {batch, q_heads, heads, dim, longest, window}", flush=True)
+    g = torch.Generator().manual_seed(batch)
+    lengths = torch.randint(0, longest + 1, (batch,), generator=g)
+    lengths[torch.rand(batch, generator=g) < 0.2] = 0
+    lengths[-1] = longest
+    s = Setup(q_type, cache_type, q_heads, heads, dim, 16, lengths.tolist(), window=window, seed=6)
+    got = s.call()
+    only = set(torch.randint(0, batch, (60,), generator=g).tolist()) | {0, batch - 1}
+    s.check(got, only=only)
+    assert (got[0][lengths == 0] == 0).all() and torch.isfinite(got[0]).all()
+    # bad pages and lengths of some leave the others alone
+    table, n = s.table.clone(), s.lengths.clone()
+    bad = [i for i in range(batch) if i % 7 == 3 and lengths[i] > 0]
+    for i in bad[::2]:
+        table[i, (int(lengths[i]) - 1) // 16] = s.cache.pages
+    n[bad[1::2]] = -5
+    again = s.call(table=table, lengths=n)
+    rest = torch.ones(batch, dtype=torch.bool)
+    rest[bad] = False
+    assert torch.isnan(again[0][bad]).all() and torch.isnan(again[1][bad]).all()
+    # (a length left out moves the shares, and with them the sums' order)
+    s.check(again, only={i for i in only if rest[i]})
+
+
+@pytest.mark.parametrize("q_type,cache_type", [(BF16, BF16), (BF16, FP8), (F32, F32)])
+def test_long_shares(q_type, cache_type):
+    """Shares of more keys than one look-up of pages serves."""
+    lengths = [9000 - 101 * i for i in range(40)]
+    s = Setup(q_type, cache_type, 32, 32, 32, 16, lengths, seed=16)
+    s.check(s.call(), only={0, 1, 17, 38, 39})
 
 
 @pytest.mark.parametrize("q_type,cache_type", PAIRS)
