@@ -435,7 +435,7 @@ hipError_t launch_cache(const CacheArgs& args, bool read, hipStream_t stream);
 
 // --------------------------------------- attention of new tokens over the cache
 constexpr int kPagedMaxGroups = 1024;  // work-groups that share a row
-constexpr int kPagedFew = 4;           // tiles of a wave in a small call's unit
+constexpr int kPagedUnit = 512;        // keys of a small call's unit
 constexpr int kPagedEnough = 128;      // work-groups, below which it takes fewer
 constexpr int kPagedFixed = 1152;      // work-groups of a small call
 constexpr int kPagedFlight = 128 << 10;  // bytes of K and V in flight aimed at on a CU

@@ -123,18 +123,19 @@ PagedPlan plan_paged(int cache_dtype, int64_t batch, int heads, int group, int h
   p.query_tiles = group > 16 && head_dim <= 128 ? 2 : 1;
   p.qtiles = (group + 16 * p.query_tiles - 1) / (16 * p.query_tiles);
   p.tile_queries = group < 16 * p.query_tiles ? group : 16 * p.query_tiles;
-  const int tile = cache_dtype == 0 ? 64 : 128;  // keys: a tile for each wave
+  const int row_bytes = head_dim * (cache_dtype == 0 ? 4 : cache_dtype <= 2 ? 2 : 1);
+  const int tile = cache_dtype == 0 ? 64 : 128;  // keys: one of PagedTraits::kTile a wave
   const int64_t rows = batch * heads * p.qtiles;
   const int64_t span = unit_limit(max_length, window, 1);
   if (rows < 1 || rows >= (1ll << 31) || (span + tile - 1) / tile >= (1ll << 31) / rows) return p;
-  // Small calls: a unit of a row to a work-group, of kPagedFew tiles a wave, or
-  // fewer where that leaves CUs without work
-  int64_t few = kPagedFew;
-  while (few > 1 && rows * ((span + few * tile - 1) / (few * tile)) < kPagedEnough && span > kPagedFew * tile)
-    few /= 2;
-  const int64_t each = (span + few * tile - 1) / (few * tile);
+  // Small calls: a unit of a row to a work-group, of kPagedUnit keys, or fewer
+  // where that leaves CUs without work and a sequence is longer
+  int64_t unit = kPagedUnit;
+  while (unit > tile && span > kPagedUnit && rows * ((span + unit - 1) / unit) < kPagedEnough)
+    unit /= 2;
+  const int64_t each = (span + unit - 1) / unit;
   if ((rows * each <= kPagedFixed || each == 1) && batch <= 65535) {
-    p.unit = (int)(few * tile);
+    p.unit = (int)unit;
     p.each = (int)each;
     p.split = each > 1;
     p.groups = (int)(rows * each);
@@ -144,7 +145,6 @@ PagedPlan plan_paged(int cache_dtype, int64_t batch, int heads, int group, int h
   // tiles in flight to kPagedFlight bytes, all resident
   p.unit = tile;
   p.split = 1;
-  const int64_t row_bytes = head_dim * (cache_dtype == 0 ? 4 : cache_dtype <= 2 ? 2 : 1);
   const int64_t each_cu = kPagedFlight / (2 * tile * row_bytes);
   const int64_t most = head_dim > 128 || p.query_tiles > 1 ? 2 : 3;  // what the registers allow
   const int64_t wanted = 256 * (each_cu < 1 ? 1 : each_cu > most ? most : each_cu);
