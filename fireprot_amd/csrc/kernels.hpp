@@ -409,9 +409,9 @@ struct RotaryArgs {
   int interleaved;
   int tokens, total;   // per batch entry, of the whole call
   int head_dim, rot;
-  // launch shape, set by launch_rotary: vectors (or pairs of them) of a row,
-  // tokens of a work-group, magic numbers of units and heads
-  int units, tt;
+  // launch shape, set by launch_rotary: first token, vectors (or pairs of them)
+  // of a row, tokens of a work-group, magic numbers of units and heads
+  int first, units, tt;
   unsigned units_magic, heads_magic;
 };
 

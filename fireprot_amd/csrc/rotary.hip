@@ -17,6 +17,7 @@ namespace {
 constexpr int kRotaryThreads = 256;
 constexpr int kRotaryBatch = 4;       // rows in flight per thread
 constexpr int kRotaryTokens = 16;      // at most, per work-group
+constexpr int kRotaryMaxGroups = 1 << 22;  // work-groups of a launch
 constexpr int kRotaryAngles = 2048;   // (token, pair) factors held in LDS: 16 KB
 
 // cos and sin of pos * freq, in FP32 to a few units of 2^-24.  The product is
@@ -73,7 +74,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
   __shared__ T* row_out[kRotaryTokens][2];
 
   const int half = a.rot >> 1;
-  const int first = blockIdx.x * a.tt;
+  const int first = a.first + blockIdx.x * a.tt;
   const int tokens = min(a.total - first, a.tt);
   for (int i = threadIdx.x; i < tokens * half; i += kRotaryThreads) {
     const int tl = i / half, p = i - tl * half;
@@ -197,20 +198,28 @@ hipError_t launch_type(RotaryArgs& a, hipStream_t stream) {
   while (a.tt < kRotaryTokens && a.total / (2 * a.tt) >= 2048 && 2 * a.tt * half <= kRotaryAngles &&
          a.tt * heads * a.units < kRotaryThreads)
     a.tt *= 2;
-  const unsigned blocks = ((unsigned)a.total + a.tt - 1) / a.tt;
   // Rows of whole 16-byte vectors that no cache holds anyway are streamed past
   // them (see kStreamBytes); narrower vectors read a line several times over.
   const bool stream_rows = (int64_t)a.total * heads * a.head_dim * (int64_t)sizeof(T) >= kStreamBytes;
-  switch (w) {
-    case 16:
-      return stream_rows ? launch_width<T, 16, true>(a, blocks, stream)
-                         : launch_width<T, 16, false>(a, blocks, stream);
-    case 8: return launch_width<T, 8, false>(a, blocks, stream);
-    case 4: return launch_width<T, 4, false>(a, blocks, stream);
-    default:
-      if constexpr (sizeof(T) == 2) return launch_width<T, 2, false>(a, blocks, stream);
-      return hipErrorInvalidValue;
+  hipError_t e = hipSuccess;
+  for (int64_t first = 0; first < a.total && e == hipSuccess;
+       first += (int64_t)kRotaryMaxGroups * a.tt) {
+    a.first = (int)first;
+    const int64_t left = (a.total - first + a.tt - 1) / a.tt;
+    const unsigned blocks = (unsigned)(left < kRotaryMaxGroups ? left : kRotaryMaxGroups);
+    switch (w) {
+      case 16:
+        e = stream_rows ? launch_width<T, 16, true>(a, blocks, stream)
+                        : launch_width<T, 16, false>(a, blocks, stream);
+        break;
+      case 8: e = launch_width<T, 8, false>(a, blocks, stream); break;
+      case 4: e = launch_width<T, 4, false>(a, blocks, stream); break;
+      default:
+        e = hipErrorInvalidValue;
+        if constexpr (sizeof(T) == 2) e = launch_width<T, 2, false>(a, blocks, stream);
+    }
   }
+  return e;
 }
 
 }  // namespace

@@ -301,3 +301,15 @@ def test_many_heads_and_units():
     wide = randn((1, 3, 8, 513), torch.float16)[..., 1:]  # 512 channels, one element a vector
     out = rotary.apply_rotary(wide, None, positions.new_tensor([0, 5, 9]), f)
     check(out, wide, positions.new_tensor([0, 5, 9]), f, "half")
+
+
+def test_more_tokens_than_one_launch():
+    """2^22 groups of 16 tokens and more: a second launch."""
+    tokens = 2 ** 26 + 35
+    f = rotary.rotary_frequencies(2, device="cuda")
+    q = torch.ones(tokens, 1, 2, device="cuda", dtype=torch.bfloat16)
+    positions = torch.arange(tokens, device="cuda", dtype=torch.int32) % 1000
+    out = rotary.apply_rotary(q, None, positions, f)
+    for part in (slice(0, 2000), slice(2 ** 26 - 1000, tokens)):
+        assert torch.equal(out[part], rotary.apply_rotary(q[part], None, positions[part], f))
+    check(out[-300:], q[-300:], positions[-300:], f, "half")
