@@ -47,6 +47,8 @@ class PagedCache:
                              f"{[str(t) for t in CACHE_DTYPES]}")
         if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
             raise ValueError("v must have k's shape, type and device")
+        if v is k or (v.data_ptr() == k.data_ptr() and k.numel()):
+            raise ValueError("k and v must not share memory")
         pages, heads, page_size, head_dim = k.shape
         if head_dim not in HEAD_DIMS or page_size not in PAGE_SIZES or pages < 1 or heads < 1:
             raise ValueError(f"needs head_dim in {HEAD_DIMS}, page_size in {PAGE_SIZES}, and at "
