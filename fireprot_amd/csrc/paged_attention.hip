@@ -31,6 +31,9 @@ __global__ __launch_bounds__(kJoinThreads) void join_shares_kernel(PagedArgs a) 
   const int* info = a.row_info + ((int64_t)(b * a.heads + head) * a.qtiles + qtile) * 2;
   const int place = info[0], count = info[1];
   if (count <= 1) return;  // written by its only work-group
+  // (lengths that another stream changes during the call could leave anything
+  // here: nothing outside the places is read for it)
+  if (place < 0 || place >= 2 * a.groups || count > a.groups - place / 2) return;
   // the row's part from work-group place / 2 + i
   auto part_row = [&](int i) -> int64_t {
     const int p = i == 0 ? place : (place / 2 + i) * 2;
@@ -134,7 +137,7 @@ PagedPlan plan_paged(int cache_dtype, int64_t batch, int heads, int group, int h
   while (unit > tile && span > kPagedUnit && rows * ((span + unit - 1) / unit) < kPagedEnough)
     unit /= 2;
   const int64_t each = (span + unit - 1) / unit;
-  if ((rows * each <= kPagedFixed || each == 1) && batch <= 65535) {
+  if ((each == 1 || (rows * each <= kPagedFixed && each <= kPagedMaxGroups)) && batch <= 65535) {
     p.unit = (int)unit;
     p.each = (int)each;
     p.split = each > 1;

@@ -231,13 +231,13 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
     if (a.window <= 0 && early_key < a.max_length)
       early_pages = a.table[cur.seq * a.table_b + (early_key >> a.page_shift)];
   } else {
-    int total, thread_first = 0, thread_sum = 0, thread_base = 0;
+    int total, thread_first = 0, last = 0, thread_sum = 0, thread_base = 0;
     if (a.batch == 1) {
       total = unit_count(range_of(0), a.unit);
     } else {
       const int per = (a.batch + kPagedThreads - 1) / kPagedThreads;
       thread_first = threadIdx.x * per;
-      const int last = min(a.batch, thread_first + per);
+      last = min(a.batch, thread_first + per);
       for (int i = thread_first; i < last; ++i) thread_sum += units_of(i);
       const int lane = threadIdx.x & 63;
       int upto = thread_sum;
@@ -267,7 +267,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
       const int target = share_first / rows;
       if (target >= thread_base && target < thread_base + thread_sum) {
         int seq = thread_first, before = thread_base;
-        for (int n = units_of(seq); target >= before + n; n = units_of(++seq)) before += n;
+        for (int n = units_of(seq); target >= before + n && seq + 1 < last; n = units_of(++seq))
+          before += n;
         found[0] = seq;
         found[1] = before;
       }
@@ -364,7 +365,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
     }
     if (y.head == a.heads) {
       y.head = 0;
-      y.range = range_of(++y.seq);
+      y.seq = min(y.seq + 1, a.batch - 1);
+      y.range = range_of(y.seq);
       y.row_units = unit_count(y.range, a.unit);
     }
     y.unit1 = min(y.row_units, share_end - (unit + x.unit1 - x.unit0));
@@ -402,7 +404,10 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
       for (int p = 0; p < T::kTerms; ++p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t w = pack_bf16(x[2 * i], x[2 * i + 1]);
+          // cut, not rounded: a value near the largest would round to infinity
+          const uint32_t w = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, x[2 * i + 1]),
+                                                   __builtin_bit_cast(uint32_t, x[2 * i]),
+                                                   0x07060302u);
           terms[p][i] = w;
           // what is left of an infinite value is NaN, which its product with a
           // key would not be: the first term carries it alone

@@ -41,8 +41,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
 
     * ``q`` ``[batch, q_heads, head_dim]``, any strides; ``q_heads`` a multiple
       of the cache's heads, each of which serves consecutive query heads.  A
-      plain cache has q's type, an 8-bit one takes float32, bfloat16 and
-      float16 queries.
+      plain cache has q's type, an 8-bit one takes float32 (below 2^110: products
+      with the codes are formed in FP32), bfloat16 and float16 queries.
     * ``block_table`` int32 ``[batch, p]``: a sequence's pages in order.
       Entries past its length, or before its window, are not read.
     * ``lengths`` int32 ``[batch]``, up to ``max_length`` (default: what the
@@ -50,6 +50,10 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
     * ``scale`` of the scores, ``head_dim ** -0.5`` by default; ``window`` > 0
       keeps the last ``window`` keys only.
     * ``lse`` float32 ``[batch, q_heads]``: the logarithm of the softmax's sum.
+
+    * ``workspace``: uint8, ``workspace_bytes`` of them, 256-byte aligned and not
+      shared with a call that may overlap this one (by default each call, and
+      each captured graph, takes its own from the caching allocator).
 
     A sequence of length 0 gives zeros (lse -inf).  One whose length is
     negative or above ``max_length``, or whose table names a page outside the

@@ -408,7 +408,8 @@ size_t fpx_paged_attention_workspace_bytes(int cache_dtype, int64_t batch, int q
  * all), in FP32 with one rounding at the end; query head h reads cache head
  * h / (q_heads / heads).  No counterpart in the reference.
  *   dtype       FPX_F32, FPX_BF16 or FPX_F16 of q and out; a plain cache has
- *               the same type, an 8-bit cache takes any
+ *               the same type, an 8-bit cache takes any (FP32 queries below
+ *               2^110: their products with the codes are formed in FP32)
  *   q, out      row (b, h) at q + b*q_sb + h*q_sh, channel stride 1, rows
  *               16-byte aligned; out may be q itself with the same strides
  *   cache       as fpx_cache_write's

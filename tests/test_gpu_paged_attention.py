@@ -215,6 +215,36 @@ def test_shares_of_many_sequences(q_type, cache_type, batch, q_heads, heads, dim
     s.check(again, only={i for i in only if rest[i]})
 
 
+@pytest.mark.parametrize("q_type,cache_type", [(BF16, BF16), (F16, INT8)])
+def test_a_row_of_more_units_than_can_be_joined(q_type, cache_type):
+    """One row of 564 000 keys: more units of a small call's size than the join has
+    places for."""
+    s = Setup(q_type, cache_type, 2, 1, 32, 16, [564_000], seed=18)
+    s.check(s.call())
+
+
+def test_more_sequences_than_a_grid_axis_has_places():
+    g = torch.Generator().manual_seed(19)
+    lengths = torch.randint(0, 40, (66_000,), generator=g)
+    s = Setup(BF16, BF16, 2, 1, 32, 16, lengths.tolist(), seed=19)
+    got = s.call()
+    s.check(got, only=set(range(0, 66_000, 997)) | {65_535, 65_536, 65_999})
+    assert (got[0][lengths == 0] == 0).all() and torch.isfinite(got[0]).all()
+
+
+def test_queries_near_the_limit_over_codes():
+    """Products with 8-bit codes are formed before their scale: a row's largest code
+    is at least 224 (FP8) and 127 (INT8), 448 at most, so queries of 2^118 and more
+    overflow FP32 whatever the keys.  The documented limit is 2^110."""
+    for cache_type in (FP8, INT8):
+        s = Setup(F32, cache_type, 2, 1, 32, 16, [100], seed=20, spread=0.0)
+        s.q[0, 0, 3], s.q[0, 1, 5] = 2.0 ** 110, -(2.0 ** 110)
+        s.check(s.call(scale=2.0 ** -110), 2.0 ** -110)
+        s.q[0, 0, 3] = float("inf")
+        out, _ = s.call()
+        assert torch.isnan(out[0, 0]).all()
+
+
 @pytest.mark.parametrize("q_type,cache_type", [(BF16, BF16), (BF16, FP8), (F32, F32)])
 def test_long_shares(q_type, cache_type):
     """Shares of more keys than one look-up of pages serves."""
