@@ -10,9 +10,10 @@
 // once.  The rows of all sequences, cut into units of 128 keys (FP32: 64), form
 // one line of units, of which each of a fixed number of resident work-groups
 // takes an equal share, whatever the sequences' lengths: cutting every sequence
-// into chunks of one size instead took 62 us at best where this takes @@ (32
+// into chunks of one size instead took 62 us at best where this takes 54 (32
 // sequences of 1 to 4097 BF16 keys, 8 heads of 128), since few large chunks
-// leave CUs idle and many small ones are mostly start and join.  In a row the
+// leave CUs idle and many small ones are mostly start and join.  (Small calls
+// keep to one unit of a row for each work-group: see plan_paged.)  In a row the
 // four waves take its tiles in turn, each with an online softmax of its own, and
 // join at its end.  Rows that two shares meet in leave (max, sum, o) of each to
 // join_shares_kernel.
@@ -31,6 +32,13 @@
 //     row; 4 v_perm per two channels pair the keys up into A operands.
 // K of the next tile is in flight during the softmax and the second product,
 // V of the next during the first.
+//
+// Measured, in one call with its join, against the 6.3 TB/s of a plain read: one
+// sequence of 131071 BF16 keys, 8 heads of 128: 89 us, 6.0 TB/s; 16 of 20001 to
+// 32768 FP8 keys: 235 us, 6.1 TB/s; the ragged 32 above: 5.0 TB/s, of which the
+// start and the join are 8 us.  FP32 rows of 256 channels (7 sequences of up to
+// 8190 keys) stay at 2.8 TB/s: 16 queries' worth of FP32 products for one or two
+// query heads take the matrix cores longer than their memory.
 //
 // Rounding: scores, softmax and accumulators are FP32.  The weights (times the
 // value's scale in an 8-bit cache) enter the second product as two 16-bit
@@ -172,11 +180,13 @@ struct PagedTraits {
   static constexpr int kPartChannels = kPart / kElem;
   static constexpr int kPartWords = (kPart + 3) / 4;
   // Registers of a lane: its queries, the tile of K and V in flight, the
-  // accumulators, and what codes are decoded to.  Where they would spill (256 channels, split queries of two
-  // tiles) the queries stay in LDS, which the four waves share.
+  // accumulators, and what codes are decoded to.  Where they would spill (256
+  // channels, split queries of two tiles) the queries stay in LDS, which the four
+  // waves share.
   static constexpr int kQueryWords = QT * kQuerySteps * kTerms * 4;
   static constexpr int kTileWords = kHalves * (kRow / 16 + 4 * kParts * kPartWords);
-  static constexpr bool kQueryLds = kQueryWords + kTileWords + QT * kChannels * 4 + (kCoded ? 16 : 0) > 160;
+  static constexpr bool kQueryLds =
+      kQueryWords + kTileWords + QT * kChannels * 4 + (kCoded ? 16 : 0) > 160;
   static constexpr float kShift = kF16 ? kWeightShiftF16 : 0.0f;
 };
 
@@ -247,6 +257,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
         upto += lane >= d ? below : 0;
       }
       if (lane == kWave - 1) wave_units[wave] = upto;
+      if (threadIdx.x == 0) found[0] = found[1] = 0;
       __syncthreads();
       total = 0;
       thread_base = upto - thread_sum;
@@ -278,9 +289,10 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
     }
     cur.range = range_of(cur.seq);
     cur.row_units = unit_count(cur.range, a.unit);
-    const int in_seq = share_first - rows * base;
-    cur.head = in_seq / cur.row_units;
-    cur.unit0 = in_seq - cur.head * cur.row_units;
+    // (in bounds also where another stream changes the lengths meanwhile)
+    const int in_seq = max(share_first - rows * base, 0);
+    cur.head = min(in_seq / cur.row_units, rows - 1);
+    cur.unit0 = min(in_seq - cur.head * cur.row_units, cur.row_units - 1);
     cur.unit1 = min(cur.row_units, cur.unit0 + share_end - share_first);
   }
   // (so far the row of the sequence)
@@ -457,354 +469,356 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
     load_v(cur, 0);
   }
   while (true) {
-  // (not known to be the same for every row: what is derived from the lane is
-  // formed again for each, not kept in registers through the loop on its keys)
-  asm volatile("" : "+v"(lane));
-  const int col = lane & 15, g = lane >> 4;
-  const KeyRange range = cur.range;
-  const int start = start_of(cur);
-  const int next_unit = unit + cur.unit1 - cur.unit0;
-  const bool more = next_unit < share_end;
-  Segment next = cur;
-  int next_pages = 0, next_mine = 0;
-  if (more) {
-    next = after(cur);
-    next_mine = tiles_of(next);
-    if (next_mine > 0) next_pages = look_up(next, 0);
-  }
-
-  float m[QT], l[QT];
-  f32x4 o[QT][T::kChannels];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    m[t] = -__builtin_inff();
-    l[t] = 0.0f;
-#pragma unroll
-    for (int c = 0; c < T::kChannels; ++c) o[t][c] = {0.0f, 0.0f, 0.0f, 0.0f};
-  }
-  u32x4_t qw[T::kQueryLds ? 1 : QT * kQuads];
-#pragma unroll
-  for (int i = 0; i < kMySteps; ++i) {
-    const int t = step_of(i) / T::kQuerySteps, st = step_of(i) % T::kQuerySteps;
-    u32x4_t terms[T::kTerms];
-    split_step(raw[i], terms);
-#pragma unroll
-    for (int p = 0; p < T::kTerms; ++p) {
-      if constexpr (!T::kQueryLds)
-        qw[t * kQuads + p * T::kQuerySteps + st] = terms[p];
-      else if (t < QT)
-        query_lds[t * kQuads + p * T::kQuerySteps + st][lane] = terms[p];
+    // (not known to be the same for every row: what is derived from the lane is
+    // formed again for each, not kept in registers through the loop on its keys)
+    asm volatile("" : "+v"(lane));
+    const int col = lane & 15, g = lane >> 4;
+    const KeyRange range = cur.range;
+    const int start = start_of(cur);
+    const int next_unit = unit + cur.unit1 - cur.unit0;
+    const bool more = next_unit < share_end;
+    Segment next = cur;
+    int next_pages = 0, next_mine = 0;
+    if (more) {
+      next = after(cur);
+      next_mine = tiles_of(next);
+      if (next_mine > 0) next_pages = look_up(next, 0);
     }
-  }
-  if constexpr (T::kQueryLds) __syncthreads();
-  int query_lane = lane;
-  auto query = [&](int i) -> u32x4_t {
-    if constexpr (T::kQueryLds)
-      return query_lds[i][query_lane];
-    else
-      return qw[i];
-  };
 
-  for (int n = 0; n < mine; ++n) {
-    const int key0 = start + (wave + kPagedWaves * n) * T::kTile;
-    // (not known to be the same in every tile, so the reads stay in the loop)
-    if constexpr (T::kQueryLds) asm volatile("" : "+v"(query_lane));
-    // ---- S^T = K Q^T.  FP32: four sums of a quarter of the channels, which
-    // halves the rounding of one long sum
-    f32x4 s[QT][kHalves];
+    float m[QT], l[QT];
+    f32x4 o[QT][T::kChannels];
 #pragma unroll
-    for (int t = 0; t < QT; ++t)
+    for (int t = 0; t < QT; ++t) {
+      m[t] = -__builtin_inff();
+      l[t] = 0.0f;
 #pragma unroll
-      for (int u = 0; u < kHalves; ++u) s[t][u] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if constexpr (T::kF32) {
+      for (int c = 0; c < T::kChannels; ++c) o[t][c] = {0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    u32x4_t qw[T::kQueryLds ? 1 : QT * kQuads];
 #pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        f32x4 sum[4] = {};
+    for (int i = 0; i < kMySteps; ++i) {
+      const int t = step_of(i) / T::kQuerySteps, st = step_of(i) % T::kQuerySteps;
+      u32x4_t terms[T::kTerms];
+      split_step(raw[i], terms);
 #pragma unroll
-        for (int c = 0; c < T::kPieces; ++c) {
-          const f32x4 y = __builtin_bit_cast(f32x4, query(t * kQuads + c));
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            sum[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                __builtin_bit_cast(float, kw[0][4 * c + i]), y[i], sum[i], 0, 0, 0);
-        }
-        s[t][0] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      for (int p = 0; p < T::kTerms; ++p) {
+        if constexpr (!T::kQueryLds)
+          qw[t * kQuads + p * T::kQuerySteps + st] = terms[p];
+        else if (t < QT)
+          query_lds[t * kQuads + p * T::kQuerySteps + st][lane] = terms[p];
       }
-    } else {
+    }
+    if constexpr (T::kQueryLds) __syncthreads();
+    int query_lane = lane;
+    auto query = [&](int i) -> u32x4_t {
+      if constexpr (T::kQueryLds)
+        return query_lds[i][query_lane];
+      else
+        return qw[i];
+    };
+
+    for (int n = 0; n < mine; ++n) {
+      const int key0 = start + (wave + kPagedWaves * n) * T::kTile;
+      // (not known to be the same in every tile, so the reads stay in the loop)
+      if constexpr (T::kQueryLds) asm volatile("" : "+v"(query_lane));
+      // ---- S^T = K Q^T.  FP32: four sums of a quarter of the channels, which
+      // halves the rounding of one long sum
+      f32x4 s[QT][kHalves];
 #pragma unroll
-      for (int u = 0; u < kHalves; ++u) {
+      for (int t = 0; t < QT; ++t)
 #pragma unroll
-        for (int st = 0; st < T::kSteps; ++st) {
-          u32x4_t x;
-          if constexpr (T::kCoded) {
-            x[0] = codes_bf16<C, 0>(kw[u][2 * st]);
-            x[1] = codes_bf16<C, 1>(kw[u][2 * st]);
-            x[2] = codes_bf16<C, 0>(kw[u][2 * st + 1]);
-            x[3] = codes_bf16<C, 1>(kw[u][2 * st + 1]);
-          } else {
+        for (int u = 0; u < kHalves; ++u) s[t][u] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (T::kF32) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = kw[u][4 * st + i];
+        for (int t = 0; t < QT; ++t) {
+          f32x4 sum[4] = {};
+#pragma unroll
+          for (int c = 0; c < T::kPieces; ++c) {
+            const f32x4 y = __builtin_bit_cast(f32x4, query(t * kQuads + c));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              sum[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                  __builtin_bit_cast(float, kw[0][4 * c + i]), y[i], sum[i], 0, 0, 0);
           }
+          s[t][0] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        }
+      } else {
 #pragma unroll
-          for (int t = 0; t < QT; ++t) {
+        for (int u = 0; u < kHalves; ++u) {
 #pragma unroll
-            for (int p = T::kTerms - 1; p >= 0; --p) {  // the smallest term first
-              const u32x4_t y = query(t * kQuads + p * T::kQuerySteps + st);
-              if constexpr (T::kF16)
-                s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                    __builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), s[t][u], 0, 0, 0);
-              else
-                s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                    __builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), s[t][u], 0, 0,
-                    0);
+          for (int st = 0; st < T::kSteps; ++st) {
+            u32x4_t x;
+            if constexpr (T::kCoded) {
+              x[0] = codes_bf16<C, 0>(kw[u][2 * st]);
+              x[1] = codes_bf16<C, 1>(kw[u][2 * st]);
+              x[2] = codes_bf16<C, 0>(kw[u][2 * st + 1]);
+              x[3] = codes_bf16<C, 1>(kw[u][2 * st + 1]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x[i] = kw[u][4 * st + i];
+            }
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+#pragma unroll
+              for (int p = T::kTerms - 1; p >= 0; --p) {  // the smallest term first
+                const u32x4_t y = query(t * kQuads + p * T::kQuerySteps + st);
+                if constexpr (T::kF16)
+                  s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                      __builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), s[t][u], 0, 0, 0);
+                else
+                  s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                      __builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), s[t][u], 0, 0,
+                      0);
+              }
             }
           }
         }
       }
-    }
-    // ---- factors of the scores in log2 units; keys outside the range left out
-    const bool edge = key0 < range.first || key0 + T::kTile > range.end;
-    float f[kHalves][T::kCoded ? 4 : 1];
-    uint32_t unseen = 0;  // bit 4u + r
-#pragma unroll
-    for (int u = 0; u < kHalves; ++u)
-#pragma unroll
-      for (int r = 0; r < (T::kCoded ? 4 : 1); ++r)
-        f[u][r] = T::kCoded ? a.scale_log2 * ks[u][r] : a.scale_log2;
-    if (edge) {
+      // ---- factors of the scores in log2 units; keys outside the range left out
+      const bool edge = key0 < range.first || key0 + T::kTile > range.end;
+      float f[kHalves][T::kCoded ? 4 : 1];
+      uint32_t unseen = 0;  // bit 4u + r
 #pragma unroll
       for (int u = 0; u < kHalves; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int key = key0 + 16 * u + 4 * g + r;
-          if (key >= range.first && key < range.end) continue;
-          unseen |= 1u << (4 * u + r);
-          // what the page holds there may be NaN: it must not meet a weight
-          // of zero
-          if constexpr (T::kCoded) vs[u][r] = 0.0f;
+        for (int r = 0; r < (T::kCoded ? 4 : 1); ++r)
+          f[u][r] = T::kCoded ? a.scale_log2 * ks[u][r] : a.scale_log2;
+      if (edge) {
 #pragma unroll
-          for (int i = 0; i < T::kParts * T::kPartWords; ++i) vw[u * 4 + r][i] = 0u;
+        for (int u = 0; u < kHalves; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int key = key0 + 16 * u + 4 * g + r;
+            if (key >= range.first && key < range.end) continue;
+            unseen |= 1u << (4 * u + r);
+            // what the page holds there may be NaN: it must not meet a weight
+            // of zero
+            if constexpr (T::kCoded) vs[u][r] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < T::kParts * T::kPartWords; ++i) vw[u * 4 + r][i] = 0u;
+          }
+      }
+      if (n + 1 < mine) {
+        if ((n + 1) % kAhead == 0) take_pages(look_up(cur, n + 1));
+        load_k(cur, n + 1);
+      }
+      // ---- online softmax; a lane's l covers its own group's keys
+      float p[QT][kHalves * 4];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int u = 0; u < kHalves; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float x = s[t][u][r] * f[u][T::kCoded ? r : 0];
+            top = fmaxf(top, unseen & (1u << (4 * u + r)) ? -__builtin_inff() : x);
+          }
+        const float next = fmaxf(m[t], groups_max(top));
+        const float ref = next == -__builtin_inff() ? 0.0f : next;
+        if (__any(next > m[t])) {
+          const float alpha = exp2_fast(m[t] - ref);
+          l[t] *= alpha;
+#pragma unroll
+          for (int c = 0; c < T::kChannels; ++c) o[t][c] *= alpha;
         }
+        m[t] = next;
+#pragma unroll
+        for (int u = 0; u < kHalves; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            // one rounding from the product to the exponent
+            const float e = __builtin_fmaf(s[t][u][r], f[u][T::kCoded ? r : 0], -ref);
+            float w = exp2_fast(T::kShift == 0.0f ? e : e + T::kShift);
+            w = unseen & (1u << (4 * u + r)) ? 0.0f : w;
+            l[t] += w;
+            if constexpr (T::kCoded)
+              p[t][u * 4 + r] = w * vs[u][r];
+            else
+              p[t][u * 4 + r] = w;
+          }
+      }
+      // ---- O^T += V^T P^T
+      if constexpr (T::kF32) {
+#pragma unroll
+        for (int c = 0; c < T::kChannels; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+              o[t][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                  __builtin_bit_cast(float, vw[r][c]), p[t][r], o[t][c], 0, 0, 0);
+      } else {
+        u32x4_t hi[QT], lo[QT];
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t h, e;
+            split_weights<T::kF16, !T::kCoded>(p[t][2 * i], p[t][2 * i + 1], h, e);
+            hi[t][i] = h;
+            lo[t][i] = e;
+          }
+        uint32_t pair[8];  // two channels of the lane's eight keys
+#pragma unroll
+        for (int c = 0; c < T::kChannels; ++c) {
+          if (c % 2 == 0) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              if constexpr (!T::kCoded)
+                pair[j] = vw[j][c / 2];
+              else
+                pair[j] =
+                    c % 4 == 0 ? codes_bf16<C, 0>(vw[j][c / 4]) : codes_bf16<C, 1>(vw[j][c / 4]);
+            }
+          }
+          u32x4_t x;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            x[i] = __builtin_amdgcn_perm(pair[2 * i + 1], pair[2 * i],
+                                         c % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            if constexpr (T::kF16) {
+              o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                  __builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, lo[t]), o[t][c], 0, 0, 0);
+              o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                  __builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, hi[t]), o[t][c], 0, 0, 0);
+            } else {
+              o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  __builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, lo[t]), o[t][c], 0, 0,
+                  0);
+              o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  __builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, hi[t]), o[t][c], 0, 0,
+                  0);
+            }
+          }
+        }
+      }
+      if (n + 1 < mine) load_v(cur, n + 1);
     }
-    if (n + 1 < mine) {
-      if ((n + 1) % kAhead == 0) take_pages(look_up(cur, n + 1));
-      load_k(cur, n + 1);
+
+    const bool any_bad = __any(bad) || !range.valid;
+    bad = false;
+    if (more) {
+      if constexpr (!T::kQueryLds) load_queries(next);
+      if (next_mine > 0) {
+        take_pages(next_pages);
+        load_k(next, 0);
+        load_v(next, 0);
+      }
     }
-    // ---- online softmax; a lane's l covers its own group's keys
-    float p[QT][kHalves * 4];
+
+    // ---- the four waves joined, in their order
+    if (any_bad) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t) l[t] = __builtin_nanf("");
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      l[t] = groups_sum(l[t]);
+      if (g == 0) {
+        wave_m[wave][t * 16 + col] = m[t];
+        wave_l[wave][t * 16 + col] = l[t];
+      }
+    }
+    __syncthreads();
+    float total_l[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       float top = -__builtin_inff();
 #pragma unroll
-      for (int u = 0; u < kHalves; ++u)
+      for (int w = 0; w < kPagedWaves; ++w) top = fmaxf(top, wave_m[w][t * 16 + col]);
+      const float ref = top == -__builtin_inff() ? 0.0f : top;
+      total_l[t] = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float x = s[t][u][r] * f[u][T::kCoded ? r : 0];
-          top = fmaxf(top, unseen & (1u << (4 * u + r)) ? -__builtin_inff() : x);
-        }
-      const float next = fmaxf(m[t], groups_max(top));
-      const float ref = next == -__builtin_inff() ? 0.0f : next;
-      if (__any(next > m[t])) {
-        const float alpha = exp2_fast(m[t] - ref);
-        l[t] *= alpha;
+      for (int w = 0; w < kPagedWaves; ++w)
+        total_l[t] += wave_l[w][t * 16 + col] * exp2_fast(wave_m[w][t * 16 + col] - ref);
+      const float mine_scale = exp2_fast(m[t] - ref);
 #pragma unroll
-        for (int c = 0; c < T::kChannels; ++c) o[t][c] *= alpha;
-      }
-      m[t] = next;
-#pragma unroll
-      for (int u = 0; u < kHalves; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          // one rounding from the product to the exponent
-          const float e = __builtin_fmaf(s[t][u][r], f[u][T::kCoded ? r : 0], -ref);
-          float w = exp2_fast(T::kShift == 0.0f ? e : e + T::kShift);
-          w = unseen & (1u << (4 * u + r)) ? 0.0f : w;
-          l[t] += w;
-          if constexpr (T::kCoded)
-            p[t][u * 4 + r] = w * vs[u][r];
-          else
-            p[t][u * 4 + r] = w;
-        }
+      for (int c = 0; c < T::kChannels; ++c) o[t][c] *= mine_scale;
+      m[t] = top;
     }
-    // ---- O^T += V^T P^T
-    if constexpr (T::kF32) {
-#pragma unroll
-      for (int c = 0; c < T::kChannels; ++c)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int t = 0; t < QT; ++t)
-            o[t][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                __builtin_bit_cast(float, vw[r][c]), p[t][r], o[t][c], 0, 0, 0);
-    } else {
-      u32x4_t hi[QT], lo[QT];
-#pragma unroll
-      for (int t = 0; t < QT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t h, e;
-          split_weights<T::kF16, !T::kCoded>(p[t][2 * i], p[t][2 * i + 1], h, e);
-          hi[t][i] = h;
-          lo[t][i] = e;
-        }
-      uint32_t pair[8];  // two channels of the lane's eight keys
-#pragma unroll
-      for (int c = 0; c < T::kChannels; ++c) {
-        if (c % 2 == 0) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if constexpr (!T::kCoded)
-              pair[j] = vw[j][c / 2];
-            else
-              pair[j] = c % 4 == 0 ? codes_bf16<C, 0>(vw[j][c / 4]) : codes_bf16<C, 1>(vw[j][c / 4]);
-          }
-        }
-        u32x4_t x;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          x[i] = __builtin_amdgcn_perm(pair[2 * i + 1], pair[2 * i],
-                                       c % 2 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-          if constexpr (T::kF16) {
-            o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                __builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, lo[t]), o[t][c], 0, 0, 0);
-            o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                __builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, hi[t]), o[t][c], 0, 0, 0);
-          } else {
-            o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                __builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, lo[t]), o[t][c], 0, 0,
-                0);
-            o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                __builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, hi[t]), o[t][c], 0, 0,
-                0);
-          }
-        }
-      }
-    }
-    if (n + 1 < mine) load_v(cur, n + 1);
-  }
-
-  const bool any_bad = __any(bad) || !range.valid;
-  bad = false;
-  if (more) {
-    if constexpr (!T::kQueryLds) load_queries(next);
-    if (next_mine > 0) {
-      take_pages(next_pages);
-      load_k(next, 0);
-      load_v(next, 0);
-    }
-  }
-
-  // ---- the four waves joined, in their order
-  if (any_bad) {
-#pragma unroll
-    for (int t = 0; t < QT; ++t) l[t] = __builtin_nanf("");
-  }
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    l[t] = groups_sum(l[t]);
-    if (g == 0) {
-      wave_m[wave][t * 16 + col] = m[t];
-      wave_l[wave][t * 16 + col] = l[t];
-    }
-  }
-  __syncthreads();
-  float total_l[QT];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    float top = -__builtin_inff();
-#pragma unroll
-    for (int w = 0; w < kPagedWaves; ++w) top = fmaxf(top, wave_m[w][t * 16 + col]);
-    const float ref = top == -__builtin_inff() ? 0.0f : top;
-    total_l[t] = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kPagedWaves; ++w)
-      total_l[t] += wave_l[w][t * 16 + col] * exp2_fast(wave_m[w][t * 16 + col] - ref);
-    const float mine_scale = exp2_fast(m[t] - ref);
-#pragma unroll
-    for (int c = 0; c < T::kChannels; ++c) o[t][c] *= mine_scale;
-    m[t] = top;
-  }
-  // two exchanges: waves 2 and 3 into 0 and 1, then 1 into 0 (a loop, as this
-  // code runs once a row and its fetch is not hidden)
+    // two exchanges: waves 2 and 3 into 0 and 1, then 1 into 0 (a loop, as this
+    // code runs once a row and its fetch is not hidden)
 #pragma unroll 1
-  for (int round = 2; round >= 1; round >>= 1) {
-    if (wave >= round && wave < 2 * round) {
+    for (int left = 2; left >= 1; left >>= 1) {
+      if (wave >= left && wave < 2 * left) {
 #pragma unroll
-      for (int t = 0; t < QT; ++t)
+        for (int t = 0; t < QT; ++t)
 #pragma unroll
-        for (int c = 0; c < T::kChannels; ++c)
-          joined[wave - round][t * T::kChannels + c][lane] = o[t][c];
+          for (int c = 0; c < T::kChannels; ++c)
+            joined[wave - left][t * T::kChannels + c][lane] = o[t][c];
+      }
+      __syncthreads();
+      if (wave < left) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+          for (int c = 0; c < T::kChannels; ++c)
+            o[t][c] += joined[wave][t * T::kChannels + c][lane];
+      }
+      __syncthreads();
     }
-    __syncthreads();
-    if (wave < round) {
+    // ---- O^T: lane (query col, group g), register r of channel c of a part:
+    // channel (4g + r) * kPartChannels + c of the part's 16 * kPartChannels
+    if (wave == 0) {
+      const int b = cur.seq, head = cur.head;
+      const int q0 = cur.qtile * 16 * QT;  // the tile's first query head of the cache head's
+      const bool direct = cur.unit0 == 0 && cur.unit1 == cur.row_units;
+      const int place = group * 2 + (unit == share_first ? 0 : 1);
+      if (cur.unit0 == 0 && a.split && lane == 0) {
+        int* info = a.row_info + ((int64_t)b * rows + head * a.qtiles + cur.qtile) * 2;
+        info[0] = place;
+        info[1] = fixed ? cur.row_units
+                        : share_of(shares, unit + cur.row_units - 1) - group + 1;
+      }
 #pragma unroll
-      for (int t = 0; t < QT; ++t)
+      for (int t = 0; t < QT; ++t) {
+        const int qi = q0 + t * 16 + col;
+        if (qi >= a.group) continue;
+        const int hq = head * a.group + qi;
+        const bool empty = range.valid && range.end <= range.first;
+        const float scale = direct ? (empty ? 0.0f : 1.0f / total_l[t]) : 1.0f;
+        const int64_t part_row = (int64_t)place * a.tile_queries + t * 16 + col;
+        // (rows of out are 16-byte aligned)
+        char* to = direct ? reinterpret_cast<char*>(static_cast<Q*>(a.out) + b * a.o_b + hq * a.o_h)
+                          : reinterpret_cast<char*>(a.part + part_row * D);
+        typedef float Piece __attribute__((ext_vector_type(T::kPartChannels)));
+        typedef Q OutPiece __attribute__((ext_vector_type(T::kPartChannels)));
 #pragma unroll
-        for (int c = 0; c < T::kChannels; ++c)
-          o[t][c] += joined[wave][t * T::kChannels + c][lane];
-    }
-    __syncthreads();
-  }
-  // ---- O^T: lane (query col, group g), register r of channel c of a part:
-  // channel (4g + r) * kPartChannels + c of the part's 16 * kPartChannels
-  if (wave == 0) {
-    const int b = cur.seq, head = cur.head;
-    const int q0 = cur.qtile * 16 * QT;  // the tile's first query head of the cache head's
-    const bool direct = cur.unit0 == 0 && cur.unit1 == cur.row_units;
-    const int place = group * 2 + (unit == share_first ? 0 : 1);
-    if (cur.unit0 == 0 && a.split && lane == 0) {
-      int* info = a.row_info + ((int64_t)b * rows + head * a.qtiles + cur.qtile) * 2;
-      info[0] = place;
-      info[1] = fixed ? cur.row_units
-                           : share_of(shares, unit + cur.row_units - 1) - group + 1;
-    }
+        for (int pt = 0; pt < T::kParts; ++pt)
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      const int qi = q0 + t * 16 + col;
-      if (qi >= a.group) continue;
-      const int hq = head * a.group + qi;
-      const bool empty = range.valid && range.end <= range.first;
-      const float scale = direct ? (empty ? 0.0f : 1.0f / total_l[t]) : 1.0f;
-      const int64_t part_row = (int64_t)place * a.tile_queries + t * 16 + col;
-      // (rows of out are 16-byte aligned)
-      char* to = direct ? reinterpret_cast<char*>(static_cast<Q*>(a.out) + b * a.o_b + hq * a.o_h)
-                        : reinterpret_cast<char*>(a.part + part_row * D);
-      typedef float Piece __attribute__((ext_vector_type(T::kPartChannels)));
-      typedef Q OutPiece __attribute__((ext_vector_type(T::kPartChannels)));
+          for (int r = 0; r < 4; ++r) {
+            const int d = (16 * pt + 4 * g + r) * T::kPartChannels;
+            Piece x;
 #pragma unroll
-      for (int pt = 0; pt < T::kParts; ++pt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int d = (16 * pt + 4 * g + r) * T::kPartChannels;
-          Piece x;
-#pragma unroll
-          for (int c = 0; c < T::kPartChannels; ++c)
-            x[c] = o[t][pt * T::kPartChannels + c][r] * scale;
-          if (std::is_same_v<Q, float> || !direct)
-            *reinterpret_cast<Piece*>(to + d * 4) = x;
-          else
-            *reinterpret_cast<OutPiece*>(to + d * sizeof(Q)) = __builtin_convertvector(x, OutPiece);
-        }
-      if (g == 0) {
-        if (!direct) {
-          a.part_ml[part_row * 2] = m[t];
-          a.part_ml[part_row * 2 + 1] = total_l[t];
-        } else if (a.lse) {
-          a.lse[(int64_t)b * a.heads * a.group + hq] =
-              empty ? -__builtin_inff()
-                    : (m[t] + __builtin_amdgcn_logf(total_l[t]) - T::kShift) * kLn2;
+            for (int c = 0; c < T::kPartChannels; ++c)
+              x[c] = o[t][pt * T::kPartChannels + c][r] * scale;
+            if (std::is_same_v<Q, float> || !direct)
+              *reinterpret_cast<Piece*>(to + d * 4) = x;
+            else
+              *reinterpret_cast<OutPiece*>(to + d * sizeof(Q)) =
+                  __builtin_convertvector(x, OutPiece);
+          }
+        if (g == 0) {
+          if (!direct) {
+            a.part_ml[part_row * 2] = m[t];
+            a.part_ml[part_row * 2 + 1] = total_l[t];
+          } else if (a.lse) {
+            a.lse[(int64_t)b * a.heads * a.group + hq] =
+                empty ? -__builtin_inff()
+                      : (m[t] + __builtin_amdgcn_logf(total_l[t]) - T::kShift) * kLn2;
+          }
         }
       }
     }
-  }
 
-  if (!more) break;
-  if constexpr (T::kQueryLds) load_queries(next);  // (no registers for them before)
-  unit = next_unit;
-  cur = next;
-  mine = next_mine;
+    if (!more) break;
+    if constexpr (T::kQueryLds) load_queries(next);  // (no registers for them before)
+    unit = next_unit;
+    cur = next;
+    mine = next_mine;
   }
 }
 

@@ -200,7 +200,8 @@ hipError_t launch_type(RotaryArgs& a, hipStream_t stream) {
     a.tt *= 2;
   // Rows of whole 16-byte vectors that no cache holds anyway are streamed past
   // them (see kStreamBytes); narrower vectors read a line several times over.
-  const bool stream_rows = (int64_t)a.total * heads * a.head_dim * (int64_t)sizeof(T) >= kStreamBytes;
+  const bool stream_rows =
+      (int64_t)a.total * heads * a.head_dim * (int64_t)sizeof(T) >= kStreamBytes;
   hipError_t e = hipSuccess;
   for (int64_t first = 0; first < a.total && e == hipSuccess;
        first += (int64_t)kRotaryMaxGroups * a.tt) {

@@ -44,7 +44,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
       plain cache has q's type, an 8-bit one takes float32 (below 2^110: products
       with the codes are formed in FP32), bfloat16 and float16 queries.
     * ``block_table`` int32 ``[batch, p]``: a sequence's pages in order.
-      Entries past its length, or before its window, are not read.
+      Entries past its length, or before its window, are not used.
     * ``lengths`` int32 ``[batch]``, up to ``max_length`` (default: what the
       table holds; a captured graph keeps the bound it was captured with).
     * ``scale`` of the scores, ``head_dim ** -0.5`` by default; ``window`` > 0
