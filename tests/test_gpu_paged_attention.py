@@ -215,6 +215,15 @@ def test_shares_of_many_sequences(q_type, cache_type, batch, q_heads, heads, dim
     s.check(again, only={i for i in only if rest[i]})
 
 
+@pytest.mark.parametrize("q_type,dim", [(F32, 256), (F32, 128), (BF16, 256)])
+@pytest.mark.parametrize("window", [0, 200])
+def test_short_rows_of_wide_heads_in_parts(q_type, dim, window):
+    """Few rows of 512 keys or fewer, and of more bytes than one work-group reads."""
+    s = Setup(q_type, q_type, 6, 3, dim, 16, [500, 0, 1, 130, 64, 257], seed=21,
+              window=window)
+    s.check(s.call())
+
+
 @pytest.mark.parametrize("q_type,cache_type", [(BF16, BF16), (F16, INT8)])
 def test_a_row_of_more_units_than_can_be_joined(q_type, cache_type):
     """One row of 564 000 keys: more units of a small call's size than the join has
