@@ -160,7 +160,8 @@ def cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor,
     A token with a negative slot (padding) or one past the cache is not
     written; everything else in the cache stays as it is.  The other slots
     must be distinct, as with ``torch.Tensor.index_copy_``: of two tokens with
-    one slot it is not defined what the slot holds.
+    one slot it is not defined what the slot holds.  ``k`` and ``v`` may not be
+    rows of this cache.
     """
     lib = _native.library()
     _, heads, _, head_dim = cache.k.shape
@@ -209,5 +210,7 @@ def cache_read(cache: PagedCache, slots: torch.Tensor, *, dtype: torch.dtype | N
             if torch.is_grad_enabled() and out.requires_grad:
                 raise ValueError("a cache records no gradient: detach the outputs")
         outs.append(out)
+    if outs[0].data_ptr() == outs[1].data_ptr() and outs[0].numel():
+        raise ValueError("k_out and v_out must not share memory")
     _call(lib.fpx_cache_read, "fpx_cache_read", device, dtype, cache, outs[0], outs[1], slots)
     return outs[0], outs[1]

@@ -301,3 +301,17 @@ def test_slots_of_positions_on_the_device():
     positions = torch.tensor([[0, 17, -1], [31, 32, 5]]).cuda()
     top = torch.iinfo(torch.int64).max
     assert kv_cache.cache_slots(table, positions, 16).tolist() == [[32, 1, -1], [63, top, 21]]
+
+
+def test_outputs_of_a_read_share_no_memory():
+    cache = PagedCache(*(torch.zeros(2, 1, 16, 32, device="cuda", dtype=torch.float16)
+                         for _ in range(2)))
+    x = torch.empty(3, 1, 32, device="cuda", dtype=torch.float16)
+    slots = torch.arange(3, device="cuda")
+    with pytest.raises(ValueError):
+        cache_read(cache, slots, k_out=x, v_out=x)
+    with pytest.raises(ValueError):
+        cache_read(cache, slots, k_out=x, v_out=x.view(3, 1, 32))
+    pair = torch.empty(3, 2, 32, device="cuda", dtype=torch.float16)
+    k, v = cache_read(cache, slots, k_out=pair[:, :1], v_out=pair[:, 1:])
+    assert (pair == 0).all() and k.data_ptr() != v.data_ptr()
