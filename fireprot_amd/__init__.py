@@ -10,6 +10,8 @@ Public surface:
 * ``fireprot_amd.registry`` -- ``OperationRegistry`` / ``OperationSignature``;
 * ``fireprot_amd.layer_norm``, ``qkv_projection``, ``attention_gate``,
   ``pair_layout`` -- the per-stage hooks;
+* ``fireprot_amd.rotary``, ``kv_cache``, ``paged_attention`` -- decoding: rotary
+  positions, a paged key-value cache, one new token's attention over it;
 * ``fireprot_amd.workloads`` -- the seeded benchmark configurations.
 
 The native library is ``fireprot_amd/_lib/libfireprot_amd.so`` (built by

@@ -415,7 +415,7 @@ size_t fpx_paged_attention_workspace_bytes(int cache_dtype, int64_t batch, int q
  *   cache       as fpx_cache_write's
  *   block_table int32, sequence b's pages at block_table + b*table_sb, at least
  *               max_length / page_size (rounded up) of them; only the entries
- *               of pages that hold the keys above are read
+ *               of pages that hold the keys above are used
  *   lengths     [batch] int32, the sequences' tokens with the new one
  *   max_length  no length is larger
  *   lse         nullable [batch][q_heads] float: log sum_j exp(scale q . k_j)
