@@ -53,6 +53,8 @@ class PagedCache:
         if head_dim not in HEAD_DIMS or page_size not in PAGE_SIZES or pages < 1 or heads < 1:
             raise ValueError(f"needs head_dim in {HEAD_DIMS}, page_size in {PAGE_SIZES}, and at "
                              "least one page and head")
+        if k.requires_grad or v.requires_grad:
+            raise ValueError("a cache records no gradient: detach k and v")
         scales = (self.k_scale, self.v_scale)
         if k.dtype in CODED_DTYPES:
             if any(s is None or s.shape != k.shape[:3] or s.dtype != torch.float32

@@ -42,6 +42,8 @@ class RotaryFrequencies:
         f = self.inv_freq
         if f.dtype != torch.float64 or f.dim() != 1 or f.numel() < 1 or not f.is_contiguous():
             raise ValueError("inv_freq must be a contiguous float64 vector, not empty")
+        if f.requires_grad:
+            raise ValueError("inv_freq gets no gradient: detach it")
 
     @property
     def rotary_dim(self) -> int:
@@ -105,7 +107,7 @@ def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
 def _output(given: torch.Tensor | None, like: torch.Tensor, rows: torch.Tensor, name: str):
     """(the four-axis output, what the caller gets) for an input and its rows."""
     if given is None:
-        out = rows.new_empty(rows.shape)
+        out = torch.empty_like(rows, memory_format=torch.contiguous_format)
         return out, out if like.dim() == 4 else out[0]
     if (given.shape != like.shape or given.dtype != like.dtype or given.device != like.device
             or given.stride(-1) != 1 or _native.repeats(given)):
@@ -162,7 +164,8 @@ def _launch(q, k, positions, frequencies, layout, inverse, q_out, k_out):
 
 
 def _apply(q, k, positions, frequencies, layout, inverse, q_out, k_out):
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (q, k, q_out, k_out)):
         raise ValueError("no autograd graph is recorded: call without gradients "
                          "(torch.no_grad, detach); rotary_backward gives the gradients")
     outs = _launch(q, k, positions, frequencies, layout, inverse, q_out, k_out)

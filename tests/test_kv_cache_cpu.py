@@ -66,7 +66,8 @@ def test_cache_tensors_are_checked():
             make(**bad)
     k, s = cache.k, coded.k_scale
     for args in ((k, k[:1]), (k, k.float()), (k[0], k[0]), (k, cache.v, s, s), (k, k),
-                 (k, k.view(2, 3, 16, 64)), (coded.k, coded.v),
+                 (k, k.view(2, 3, 16, 64)), (k.clone().requires_grad_(), cache.v),
+                 (k, cache.v.clone().requires_grad_()), (coded.k, coded.v),
                  (coded.k, coded.v, s, None), (coded.k, coded.v, s, s.double()),
                  (coded.k, coded.v, s, s[:1]), (k.transpose(0, 1), k.transpose(0, 1)),
                  (torch.zeros(2 * 3 * 16 * 64 + 1, dtype=torch.float16)[1:].view(2, 3, 16, 64),

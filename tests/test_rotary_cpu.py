@@ -99,7 +99,8 @@ def test_frequencies_refuse(bad):
 
 @pytest.mark.parametrize("inv_freq", [
     torch.ones(4), torch.ones(2, 2, dtype=torch.float64), torch.ones(0, dtype=torch.float64),
-    torch.ones(8, dtype=torch.float64)[::2]])
+    torch.ones(8, dtype=torch.float64)[::2],
+    torch.ones(8, dtype=torch.float64, requires_grad=True)])
 def test_given_frequencies_are_checked(inv_freq):
     with pytest.raises(ValueError, match="inv_freq"):
         rotary.RotaryFrequencies(inv_freq)
