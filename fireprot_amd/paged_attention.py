@@ -93,7 +93,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
     if not lengths.is_contiguous():
         lengths = lengths.contiguous()
     if out is None:
-        out = q.new_empty((batch, q_heads, head_dim))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif (out.shape != q.shape or out.dtype != q.dtype or out.get_device() != device
           or not _aligned_rows(out) or _native.repeats(out)):
         raise ValueError("out must have q's shape, type and device, 16-byte aligned rows and "
