@@ -1001,7 +1001,8 @@ int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb,
     return FPX_ERR_DIMS;
   if (out == q && (o_sb != q_sb || o_sh != q_sh)) return FPX_ERR_DIMS;
   if (table_sb < 0 || table_pages < (max_length + page_size - 1) / page_size) return FPX_ERR_DIMS;
-  if (!(scale - scale == 0.0f)) return FPX_ERR_DIMS;  // infinite or NaN
+  const float scale_log2 = scale * fpx::kLog2e;
+  if (!(scale_log2 - scale_log2 == 0.0f)) return FPX_ERR_DIMS;  // infinite or NaN
   if (batch == 0) return FPX_OK;
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(lengths, 4) ||
       !aligned_or_null(lse, 4) || (max_length > 0 && !aligned(block_table, 4)) ||
@@ -1030,7 +1031,7 @@ int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb,
   a.o_b = o_sb;
   a.o_h = o_sh;
   a.lse = lse;
-  a.scale_log2 = scale * fpx::kLog2e;
+  a.scale_log2 = scale_log2;
   a.weight_shift = cache_dtype == FPX_F16 ? fpx::kWeightShiftF16 : 0.0f;
   a.pages = pages;
   a.batch = (int)batch;

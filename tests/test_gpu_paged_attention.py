@@ -369,6 +369,20 @@ def test_strides_and_given_outputs(q_type, cache_type):
     assert torch.equal(s.call(table=s.table[:, :76], max_length=76 * 16)[0], want)
 
 
+@pytest.mark.parametrize("longest", [150, 3000])
+def test_sequences_that_share_their_pages(longest):
+    """One row of the table, and one query, for every sequence (zero strides)."""
+    s = Setup(BF16, FP8, 8, 2, 64, 16, [longest] * 3, seed=22)
+    s.table[1:], s.q[1:] = s.table[:1], s.q[:1]
+    lengths = torch.tensor([longest, 0, longest - 41], dtype=torch.int32, device="cuda")
+    want, want_lse = s.call(lengths=lengths)
+    got, got_lse = s.call(q=s.q[:1].expand_as(s.q), table=s.table[:1].expand_as(s.table),
+                          lengths=lengths)
+    assert torch.equal(got, want) and torch.equal(got_lse, want_lse)
+    first, _ = s.call(lengths=lengths[:1].expand(3))
+    assert torch.equal(first, want[:1].expand_as(first))
+
+
 def test_poisoned_workspace_and_repeats():
     s = Setup(BF16, BF16, 32, 8, 128, 16, [1, 3000, 12000, 0], seed=15)
     want, want_lse = s.call()

@@ -33,7 +33,7 @@ def _args(**override):
     dict(pages=0), dict(batch=-1), dict(batch=1 << 23), dict(batch=1 << 20), dict(max_length=-1),
     dict(max_length=1 << 30, table_pages=1 << 40), dict(window=-1), dict(q_sb=-8), dict(q_sh=124),
     dict(o_sb=1020), dict(o_sh=-128), dict(table_sb=-1), dict(table_pages=7),
-    dict(scale=float("nan")), dict(scale=float("inf")), dict(out=256, o_sh=256)])
+    dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=3e38), dict(out=256, o_sh=256)])
 def test_sizes_are_refused(lib, bad):
     assert lib.fpx_paged_attention(*_args(**bad)) == _native.FPX_ERR_DIMS
 
