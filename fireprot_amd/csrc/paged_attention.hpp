@@ -241,29 +241,33 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
     if (a.window <= 0 && early_key < a.max_length)
       early_pages = a.table[cur.seq * a.table_b + (early_key >> a.page_shift)];
   } else {
-    int total, thread_first = 0, last = 0, thread_sum = 0, thread_base = 0;
-    if (a.batch == 1) {
-      total = unit_count(range_of(0), a.unit);
-    } else {
-      const int per = (a.batch + kPagedThreads - 1) / kPagedThreads;
-      thread_first = threadIdx.x * per;
-      last = min(a.batch, thread_first + per);
-      for (int i = thread_first; i < last; ++i) thread_sum += units_of(i);
-      const int lane = threadIdx.x & 63;
-      int upto = thread_sum;
+    // The scan over the sequences' units: one to a lane where they fit, in each
+    // wave for itself (0.4 us sooner), a run of them to a thread otherwise.
+    const int lane = threadIdx.x & 63;
+    const bool few = a.batch <= kWave;
+    const int per = few ? 1 : (a.batch + kPagedThreads - 1) / kPagedThreads;
+    const int thread_first = (few ? lane : (int)threadIdx.x) * per;
+    const int last = min(a.batch, thread_first + per);
+    int sum = 0, length = 0;
+    for (int i = thread_first; i < last; ++i) {
+      length = a.lengths[i];
+      sum += unit_count(key_range(length, a.max_length, a.window), a.unit);
+    }
+    int upto = sum;
 #pragma unroll
-      for (int d = 1; d < kWave; d *= 2) {
-        const int below = __shfl_up(upto, d);
-        upto += lane >= d ? below : 0;
-      }
-      if (lane == kWave - 1) wave_units[wave] = upto;
+    for (int d = 1; d < kWave; d *= 2) {
+      const int below = __shfl_up(upto, d);
+      upto += lane >= d ? below : 0;
+    }
+    int total = __builtin_amdgcn_readlane(upto, kWave - 1);
+    if (!few) {
+      if (lane == 0) wave_units[wave] = total;
       if (threadIdx.x == 0) found[0] = found[1] = 0;
       __syncthreads();
       total = 0;
-      thread_base = upto - thread_sum;
 #pragma unroll
       for (int w = 0; w < kPagedWaves; ++w) {
-        thread_base += w < wave ? wave_units[w] : 0;
+        upto += w < wave ? wave_units[w] : 0;
         total += wave_units[w];
       }
       total = __builtin_amdgcn_readfirstlane(total);
@@ -272,12 +276,15 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
     share_first = share_start(shares, group);
     share_end = share_start(shares, group + 1);
     if (share_first >= share_end) return;
-    int base = 0;  // units before the sequence, of one row per sequence
-    cur.seq = 0;
-    if (a.batch > 1) {
-      const int target = share_first / rows;
-      if (target >= thread_base && target < thread_base + thread_sum) {
-        int seq = thread_first, before = thread_base;
+    const int target = share_first / rows;
+    int base;  // units before the sequence, of one row per sequence
+    if (few) {
+      cur.seq = __popcll(__ballot(upto <= target));
+      base = __builtin_amdgcn_readlane(upto - sum, cur.seq);
+      cur.range = key_range(__builtin_amdgcn_readlane(length, cur.seq), a.max_length, a.window);
+    } else {
+      if (target >= upto - sum && target < upto) {
+        int seq = thread_first, before = upto - sum;
         for (int n = units_of(seq); target >= before + n && seq + 1 < last; n = units_of(++seq))
           before += n;
         found[0] = seq;
@@ -286,8 +293,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
       __syncthreads();
       cur.seq = __builtin_amdgcn_readfirstlane(found[0]);
       base = __builtin_amdgcn_readfirstlane(found[1]);
+      cur.range = range_of(cur.seq);
     }
-    cur.range = range_of(cur.seq);
     cur.row_units = unit_count(cur.range, a.unit);
     // (in bounds also where another stream changes the lengths meanwhile)
     const int in_seq = max(share_first - rows * base, 0);
