@@ -36,9 +36,9 @@
 // Measured, in one call with its join, against the 6.3 TB/s of a plain read: one
 // sequence of 131071 BF16 keys, 8 heads of 128: 89 us, 6.0 TB/s; 16 of 20001 to
 // 32768 FP8 keys: 235 us, 6.1 TB/s; the ragged 32 above: 5.0 TB/s, of which the
-// start and the join are 8 us.  FP32 rows of 256 channels (7 sequences of up to
-// 8190 keys) stay at 2.8 TB/s: 16 queries' worth of FP32 products for one or two
-// query heads take the matrix cores longer than their memory.
+// start and the join are 8 us.  FP32 rows of 256 channels: 7 sequences of 513 to 8190
+// keys, 2 heads, 37 us, 3.4 TB/s (four tiles of 128 KB to a work-group, so the start
+// and the join are a third of it); 32 of 16384 keys 331 us, 6.5 TB/s.
 //
 // Rounding: scores, softmax and accumulators are FP32.  The weights (times the
 // value's scale in an 8-bit cache) enter the second product as two 16-bit
@@ -179,6 +179,9 @@ struct PagedTraits {
   static constexpr int kParts = kChannels * kElem / kPart;
   static constexpr int kPartChannels = kPart / kElem;
   static constexpr int kPartWords = (kPart + 3) / 4;
+  static constexpr int kVec = kChannels < 4 ? kChannels : 4;   // for the waves' join
+  static constexpr int kVecs = kChannels / kVec;
+  static constexpr int kPassVecs = kVecs < 2 ? kVecs : 2;      // 32 KB of LDS at most
   // Registers of a lane: its queries, the tile of K and V in flight, the
   // accumulators, and what codes are decoded to.  Where they would spill (256
   // channels, split queries of two tiles) the queries stay in LDS, which the four
@@ -202,7 +205,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
   using T = PagedTraits<Q, C, D, QT>;
   constexpr int kHalves = T::kHalves;
   __shared__ u32x4_t query_lds[T::kQueryLds ? T::kQueryWords / 4 : 1][kWave];
-  __shared__ f32x4 joined[2][QT * T::kChannels][kWave];
+  typedef float Vec __attribute__((ext_vector_type(T::kVec)));
+  __shared__ Vec joined[kPagedWaves][4][T::kPassVecs][kWave];
   __shared__ float wave_m[kPagedWaves][QT * 16], wave_l[kPagedWaves][QT * 16];
   __shared__ int wave_units[kPagedWaves];
   __shared__ int found[2];
@@ -716,107 +720,96 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
       }
     }
 
-    // ---- the four waves joined, in their order
-    if (any_bad) {
-#pragma unroll
-      for (int t = 0; t < QT; ++t) l[t] = __builtin_nanf("");
-    }
+    // ---- the four waves joined, in their order.  Each leaves its maximum, sum and
+    // O^T in LDS, and takes one of the four registers r of all of them: a quarter of
+    // the row's channels, which it scales, sums and stores.  (Two exchanges between
+    // pairs of waves, and one wave's stores, took 0.3 us longer a row of 128
+    // channels, 1 us of 256.)
+    __syncthreads();  // (the last row's are read)
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      l[t] = groups_sum(l[t]);
+      l[t] = any_bad ? __builtin_nanf("") : groups_sum(l[t]);
       if (g == 0) {
         wave_m[wave][t * 16 + col] = m[t];
         wave_l[wave][t * 16 + col] = l[t];
       }
     }
-    __syncthreads();
-    float total_l[QT];
+    const int b = cur.seq, head = cur.head;
+    const bool direct = cur.unit0 == 0 && cur.unit1 == cur.row_units;
+    const bool empty = range.valid && range.end <= range.first;
+    const int place = group * 2 + (unit == share_first ? 0 : 1);
+    if (cur.unit0 == 0 && a.split && threadIdx.x == 0) {
+      int* info = a.row_info + ((int64_t)b * rows + head * a.qtiles + cur.qtile) * 2;
+      info[0] = place;
+      info[1] = fixed ? cur.row_units
+                      : share_of(shares, unit + cur.row_units - 1) - group + 1;
+    }
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      float top = -__builtin_inff();
+      float factor[kPagedWaves], sum[T::kChannels] = {};
+      float top = -__builtin_inff(), total = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kPagedWaves; ++w) top = fmaxf(top, wave_m[w][t * 16 + col]);
-      const float ref = top == -__builtin_inff() ? 0.0f : top;
-      total_l[t] = 0.0f;
+      for (int v0 = 0; v0 < T::kVecs; v0 += T::kPassVecs) {
+        if (t > 0 || v0 > 0) __syncthreads();
 #pragma unroll
-      for (int w = 0; w < kPagedWaves; ++w)
-        total_l[t] += wave_l[w][t * 16 + col] * exp2_fast(wave_m[w][t * 16 + col] - ref);
-      const float mine_scale = exp2_fast(m[t] - ref);
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int c = 0; c < T::kChannels; ++c) o[t][c] *= mine_scale;
-      m[t] = top;
-    }
-    // two exchanges: waves 2 and 3 into 0 and 1, then 1 into 0 (a loop, as this
-    // code runs once a row and its fetch is not hidden)
-#pragma unroll 1
-    for (int left = 2; left >= 1; left >>= 1) {
-      if (wave >= left && wave < 2 * left) {
+          for (int v = 0; v < T::kPassVecs; ++v) {
+            Vec x;
 #pragma unroll
-        for (int t = 0; t < QT; ++t)
-#pragma unroll
-          for (int c = 0; c < T::kChannels; ++c)
-            joined[wave - left][t * T::kChannels + c][lane] = o[t][c];
-      }
-      __syncthreads();
-      if (wave < left) {
-#pragma unroll
-        for (int t = 0; t < QT; ++t)
-#pragma unroll
-          for (int c = 0; c < T::kChannels; ++c)
-            o[t][c] += joined[wave][t * T::kChannels + c][lane];
-      }
-      __syncthreads();
-    }
-    // ---- O^T: lane (query col, group g), register r of channel c of a part:
-    // channel (4g + r) * kPartChannels + c of the part's 16 * kPartChannels
-    if (wave == 0) {
-      const int b = cur.seq, head = cur.head;
-      const int q0 = cur.qtile * 16 * QT;  // the tile's first query head of the cache head's
-      const bool direct = cur.unit0 == 0 && cur.unit1 == cur.row_units;
-      const int place = group * 2 + (unit == share_first ? 0 : 1);
-      if (cur.unit0 == 0 && a.split && lane == 0) {
-        int* info = a.row_info + ((int64_t)b * rows + head * a.qtiles + cur.qtile) * 2;
-        info[0] = place;
-        info[1] = fixed ? cur.row_units
-                        : share_of(shares, unit + cur.row_units - 1) - group + 1;
-      }
-#pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        const int qi = q0 + t * 16 + col;
-        if (qi >= a.group) continue;
-        const int hq = head * a.group + qi;
-        const bool empty = range.valid && range.end <= range.first;
-        const float scale = direct ? (empty ? 0.0f : 1.0f / total_l[t]) : 1.0f;
-        const int64_t part_row = (int64_t)place * a.tile_queries + t * 16 + col;
-        // (rows of out are 16-byte aligned)
-        char* to = direct ? reinterpret_cast<char*>(static_cast<Q*>(a.out) + b * a.o_b + hq * a.o_h)
-                          : reinterpret_cast<char*>(a.part + part_row * D);
-        typedef float Piece __attribute__((ext_vector_type(T::kPartChannels)));
-        typedef Q OutPiece __attribute__((ext_vector_type(T::kPartChannels)));
-#pragma unroll
-        for (int pt = 0; pt < T::kParts; ++pt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int d = (16 * pt + 4 * g + r) * T::kPartChannels;
-            Piece x;
-#pragma unroll
-            for (int c = 0; c < T::kPartChannels; ++c)
-              x[c] = o[t][pt * T::kPartChannels + c][r] * scale;
-            if (std::is_same_v<Q, float> || !direct)
-              *reinterpret_cast<Piece*>(to + d * 4) = x;
-            else
-              *reinterpret_cast<OutPiece*>(to + d * sizeof(Q)) =
-                  __builtin_convertvector(x, OutPiece);
+            for (int c = 0; c < T::kVec; ++c) x[c] = o[t][(v0 + v) * T::kVec + c][r];
+            joined[wave][r][v][lane] = x;
           }
-        if (g == 0) {
-          if (!direct) {
-            a.part_ml[part_row * 2] = m[t];
-            a.part_ml[part_row * 2 + 1] = total_l[t];
-          } else if (a.lse) {
-            a.lse[(int64_t)b * a.heads * a.group + hq] =
-                empty ? -__builtin_inff()
-                      : (m[t] + __builtin_amdgcn_logf(total_l[t]) - T::kShift) * kLn2;
+        __syncthreads();
+        if (v0 == 0) {
+#pragma unroll
+          for (int w = 0; w < kPagedWaves; ++w) top = fmaxf(top, wave_m[w][t * 16 + col]);
+          const float ref = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+          for (int w = 0; w < kPagedWaves; ++w) {
+            factor[w] = exp2_fast(wave_m[w][t * 16 + col] - ref);
+            total += wave_l[w][t * 16 + col] * factor[w];
           }
+        }
+#pragma unroll
+        for (int w = 0; w < kPagedWaves; ++w)
+#pragma unroll
+          for (int v = 0; v < T::kPassVecs; ++v) {
+            const Vec x = joined[w][wave][v][lane];
+#pragma unroll
+            for (int c = 0; c < T::kVec; ++c) sum[(v0 + v) * T::kVec + c] += x[c] * factor[w];
+          }
+      }
+      const int qi = (cur.qtile * QT + t) * 16 + col;  // of the cache head's query heads
+      if (qi >= a.group) continue;
+      // O^T: lane (query col, group g), register r of channel c of a part: channel
+      // (4g + r) * kPartChannels + c of the part's 16 * kPartChannels
+      const int hq = head * a.group + qi;
+      const float scale = direct ? (empty ? 0.0f : 1.0f / total) : 1.0f;
+      const int64_t part_row = (int64_t)place * a.tile_queries + t * 16 + col;
+      // (rows of out are 16-byte aligned)
+      char* to = direct ? reinterpret_cast<char*>(static_cast<Q*>(a.out) + b * a.o_b + hq * a.o_h)
+                        : reinterpret_cast<char*>(a.part + part_row * D);
+      typedef float Piece __attribute__((ext_vector_type(T::kPartChannels)));
+      typedef Q OutPiece __attribute__((ext_vector_type(T::kPartChannels)));
+#pragma unroll
+      for (int pt = 0; pt < T::kParts; ++pt) {
+        const int d = (16 * pt + 4 * g + wave) * T::kPartChannels;
+        Piece x;
+#pragma unroll
+        for (int c = 0; c < T::kPartChannels; ++c) x[c] = sum[pt * T::kPartChannels + c] * scale;
+        if (std::is_same_v<Q, float> || !direct)
+          *reinterpret_cast<Piece*>(to + d * 4) = x;
+        else
+          *reinterpret_cast<OutPiece*>(to + d * sizeof(Q)) = __builtin_convertvector(x, OutPiece);
+      }
+      if (threadIdx.x < 16) {
+        if (!direct) {
+          a.part_ml[part_row * 2] = top;
+          a.part_ml[part_row * 2 + 1] = total;
+        } else if (a.lse) {
+          a.lse[(int64_t)b * a.heads * a.group + hq] =
+              empty ? -__builtin_inff() : (top + __builtin_amdgcn_logf(total) - T::kShift) * kLn2;
         }
       }
     }
