@@ -35,7 +35,7 @@
 //
 // Measured, in one call with its join, against the 6.3 TB/s of a plain read: one
 // sequence of 131071 BF16 keys, 8 heads of 128: 89 us, 6.0 TB/s; 16 of 20001 to
-// 32768 FP8 keys: 235 us, 6.1 TB/s; the ragged 32 above: 5.0 TB/s, of which the
+// 65536 FP8 keys: 235 us, 6.1 TB/s; the ragged 32 above: 5.0 TB/s, of which the
 // start and the join are 8 us.  FP32 rows of 256 channels: 7 sequences of 513 to 8190
 // keys, 2 heads, 37 us, 3.4 TB/s (four tiles of 128 KB to a work-group, so the start
 // and the join are a third of it); 32 of 16384 keys 331 us, 6.5 TB/s.
