@@ -149,6 +149,8 @@ def _launch(q, k, positions, frequencies, layout, inverse, q_out, k_out):
         y = k if k.dim() == 4 and k.stride(3) == 1 else _rows(k, "k")
         k_heads = y.shape[2]
         b, k_ret = _output(k_out, k, y, "k_out")
+        if a.data_ptr() == b.data_ptr() and a.numel() and b.numel():
+            raise ValueError("q_out and k_out must not share memory")
         k_args = (y.data_ptr(), *y.stride()[:3])
         k_out_args = (b.data_ptr(), *b.stride()[:3])
     if q_heads == 0 and k_heads == 0:

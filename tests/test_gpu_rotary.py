@@ -238,6 +238,7 @@ def test_refusals_on_the_device():
                 lambda: rotary.apply_rotary(q, None, p, f, q_out=q[:, :, :1].expand_as(q)),
                 lambda: rotary.apply_rotary(q.clone().requires_grad_(), None, p, f),
                 lambda: rotary.apply_rotary(q, None, p, f, q_out=q.clone().requires_grad_()),
+                lambda: rotary.apply_rotary(q, q, p, f, q_out=q, k_out=q),
                 lambda: rotary.rotary_backward(q, q.clone().requires_grad_(), p, f)):
         with pytest.raises(ValueError):
             bad()
