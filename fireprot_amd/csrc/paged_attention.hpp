@@ -10,7 +10,7 @@
 // once.  The rows of all sequences, cut into units of 128 keys (FP32: 64), form
 // one line of units, of which each of a fixed number of resident work-groups
 // takes an equal share, whatever the sequences' lengths: cutting every sequence
-// into chunks of one size instead took 62 us at best where this takes 54 (32
+// into chunks of one size instead took 62 us at best where this takes 53 (32
 // sequences of 1 to 4097 BF16 keys, 8 heads of 128), since few large chunks
 // leave CUs idle and many small ones are mostly start and join.  (Small calls
 // keep to one unit of a row for each work-group: see plan_paged.)  In a row the
@@ -35,7 +35,7 @@
 //
 // Measured, in one call with its join, against the 6.3 TB/s of a plain read: one
 // sequence of 131071 BF16 keys, 8 heads of 128: 89 us, 6.0 TB/s; 16 of 20001 to
-// 65536 FP8 keys: 235 us, 6.1 TB/s; the ragged 32 above: 5.0 TB/s, of which the
+// 65536 FP8 keys: 235 us, 6.1 TB/s; the ragged 32 above: 5.1 TB/s, of which the
 // start and the join are 8 us.  FP32 rows of 256 channels: 7 sequences of 513 to 8190
 // keys, 2 heads, 37 us, 3.4 TB/s (four tiles of 128 KB to a work-group, so the start
 // and the join are a third of it); 32 of 16384 keys 331 us, 6.5 TB/s.
