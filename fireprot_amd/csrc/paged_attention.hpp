@@ -41,11 +41,13 @@
 // and the join are a third of it); 32 of 16384 keys 331 us, 6.5 TB/s.
 //
 // Rounding: scores, softmax and accumulators are FP32.  The weights (times the
-// value's scale in an 8-bit cache) enter the second product as two 16-bit
-// terms, hi + lo, which keeps 16 (BF16) or 22 (FP16) bits of each; FP16
-// weights are scaled by 2^14 so that small ones keep their bits.  Queries of
-// another type than the operands' are split likewise into two or three terms
-// (exactly).  8-bit codes are exact in BF16.
+// value's scale in an 8-bit cache) enter the second product as 16-bit terms whose
+// sum has 16 bits of each (two BF16 terms, off by at most 2^-16 of the weight:
+// outputs of 8 bits), 22 (two FP16 terms, those weights scaled by 2^14 so that
+// small ones keep their bits) or all 24 (three BF16 terms: FP32 queries, and so
+// outputs, over 8-bit caches).  Queries of another type than the operands' are
+// split likewise into two or three terms (exactly).  8-bit codes are exact in
+// BF16.
 #pragma once
 
 #include "common.hpp"
@@ -145,6 +147,19 @@ __device__ __forceinline__ void split_weights(float x0, float x1, uint32_t& hi, 
   }
 }
 
+// Two weights as three BF16 words whose sum is the weight itself: the first two
+// cut, so what is left of 24 bits fits the third.
+__device__ __forceinline__ void split_weights_exactly(float x0, float x1, uint32_t* terms) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t b0 = __builtin_bit_cast(uint32_t, x0), b1 = __builtin_bit_cast(uint32_t, x1);
+    terms[i] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+    x0 -= __builtin_bit_cast(float, b0 & 0xffff0000u);
+    x1 -= __builtin_bit_cast(float, b1 & 0xffff0000u);
+  }
+  terms[2] = pack_bf16(x0, x1);
+}
+
 // Two 8-bit codes (bytes 2 kHalf and 2 kHalf + 1 of w) as a word of BF16.
 template <typename C, int kHalf>
 __device__ __forceinline__ uint32_t codes_bf16(uint32_t w) {
@@ -167,6 +182,8 @@ struct PagedTraits {
   // terms a query is split into: all of its bits in BF16, 8 to a term
   static constexpr int kTerms = !kCoded ? 1 : std::is_same_v<Q, __bf16> ? 1
                                           : std::is_same_v<Q, _Float16> ? 2 : 3;
+  // terms a weight is split into: what the output's type needs
+  static constexpr int kWeightTerms = kCoded && std::is_same_v<Q, float> ? 3 : 2;
   // K: pieces of kPiece bytes a lane holds of its key's row (16 where a
   // quarter of the row has them)
   static constexpr int kPiece = kRow / 4 < 16 ? kRow / 4 : 16;
@@ -660,15 +677,18 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
               o[t][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(
                   __builtin_bit_cast(float, vw[r][c]), p[t][r], o[t][c], 0, 0, 0);
       } else {
-        u32x4_t hi[QT], lo[QT];
+        u32x4_t weights[QT][T::kWeightTerms];
 #pragma unroll
         for (int t = 0; t < QT; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            uint32_t h, e;
-            split_weights<T::kF16, !T::kCoded>(p[t][2 * i], p[t][2 * i + 1], h, e);
-            hi[t][i] = h;
-            lo[t][i] = e;
+            uint32_t terms[T::kWeightTerms];
+            if constexpr (T::kWeightTerms == 3)
+              split_weights_exactly(p[t][2 * i], p[t][2 * i + 1], terms);
+            else
+              split_weights<T::kF16, !T::kCoded>(p[t][2 * i], p[t][2 * i + 1], terms[0], terms[1]);
+#pragma unroll
+            for (int w = 0; w < T::kWeightTerms; ++w) weights[t][w][i] = terms[w];
           }
         uint32_t pair[8];  // two channels of the lane's eight keys
 #pragma unroll
@@ -690,18 +710,16 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
                                          c % 2 ? 0x07060302u : 0x05040100u);
 #pragma unroll
           for (int t = 0; t < QT; ++t) {
-            if constexpr (T::kF16) {
-              o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                  __builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, lo[t]), o[t][c], 0, 0, 0);
-              o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                  __builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, hi[t]), o[t][c], 0, 0, 0);
-            } else {
-              o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                  __builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, lo[t]), o[t][c], 0, 0,
-                  0);
-              o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                  __builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, hi[t]), o[t][c], 0, 0,
-                  0);
+#pragma unroll
+            for (int w = T::kWeightTerms - 1; w >= 0; --w) {  // the smallest term first
+              if constexpr (T::kF16)
+                o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                    __builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, weights[t][w]),
+                    o[t][c], 0, 0, 0);
+              else
+                o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    __builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, weights[t][w]),
+                    o[t][c], 0, 0, 0);
             }
           }
         }

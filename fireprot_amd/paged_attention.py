@@ -5,7 +5,9 @@ attention: each sequence's query heads attend to the keys its row of the block
 table names, ``lengths[b]`` of them (the new token's own among them), where
 they lie in the ``PagedCache`` (``fpx_paged_attention``).  Query heads share
 cache heads in groups; 8-bit caches are dequantised on the way; scores, softmax
-and sums are FP32.  All sequences' keys are dealt out evenly to the card's
+and sums are FP32, and so are the weights that meet the values of an FP32 output
+(16-bit outputs: cut to 22 bits over an FP16 cache, to 16 over others).  All
+sequences' keys are dealt out evenly to the card's
 work-groups, and a second launch joins what several of them share.  There is no
 counterpart in the reference.
 """

@@ -405,8 +405,11 @@ size_t fpx_paged_attention_workspace_bytes(int cache_dtype, int64_t batch, int q
 /* Attention of one new token per sequence over a paged cache:
  *   out[b][h] = sum_j softmax_j(scale * q[b][h] . k_j) v_j
  * over sequence b's keys j in [max(0, length - window), length) (window = 0:
- * all), in FP32 with one rounding at the end; query head h reads cache head
- * h / (q_heads / heads).  No counterpart in the reference.
+ * all); query head h reads cache head h / (q_heads / heads).  Scores, softmax
+ * and sums are FP32, rounded once at the end.  The weights meet the values as
+ * FP32 numbers where the output is FP32, cut to 22 bits in an FP16 cache and to
+ * 16 otherwise (off by at most 2^-16 of the weight; the output's own rounding is
+ * off by up to 2^-8 in BF16, 2^-11 in FP16).  No counterpart in the reference.
  *   dtype       FPX_F32, FPX_BF16 or FPX_F16 of q and out; a plain cache has
  *               the same type, an 8-bit cache takes any (FP32 queries below
  *               2^110: their products with the codes are formed in FP32)
