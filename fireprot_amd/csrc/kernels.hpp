@@ -438,8 +438,7 @@ constexpr int kPagedMaxGroups = 1024;  // work-groups that share a row
 constexpr int kPagedUnit = 512;        // keys of a small call's unit
 constexpr int kPagedUnitBytes = 256 << 10;  // of K and V that one work-group reads
 constexpr int kPagedEnough = 192;      // work-groups, below which a unit is halved
-constexpr int kPagedFixed = 1152;      // work-groups of a small call
-constexpr int64_t kPagedFixedBytes = 128 << 20;  // that it reads at most
+constexpr int64_t kPagedFixedBytes = 128 << 20;  // that a small call reads at most
 constexpr int kPagedFlight = 128 << 10;  // bytes of K and V in flight aimed at on a CU
 constexpr float kWeightShiftF16 = 14.0f;  // log2 of the FP16 weights' factor
 

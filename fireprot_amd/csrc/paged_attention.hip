@@ -143,12 +143,19 @@ PagedPlan plan_paged(int cache_dtype, int64_t batch, int heads, int group, int h
   while (splits && unit > tile && rows * ((span + unit - 1) / unit) < kPagedEnough) unit /= 2;
   const int64_t each = (span + unit - 1) / unit;
   // This starts sooner than a share, but sequences shorter than the longest leave
-  // work-groups idle: not beyond kPagedFixed of them or kPagedFixedBytes that the
-  // call may read.  (8 sequences of 1 to 2000 BF16 keys, 8 heads of 128, 65 MB:
-  // 15.2 us, 17.1 in shares; of 1 to 8000, 262 MB: 35.9, in shares 30.0.  FP32, 4
-  // heads, 32 sequences of 1 to 2000: 38 and 31.)
-  const bool small = rows * each <= kPagedFixed && each <= kPagedMaxGroups &&
-                     rows * span * 2 * row_bytes <= kPagedFixedBytes;
+  // work-groups idle: not beyond kPagedFixedBytes that the call may read.  How many
+  // work-groups that makes is no matter.  Both cuts were timed on calls of 13 kinds (8
+  // and 16 bits and FP32, heads of 32 to 256, lengths alike or from 1 on, 1 to 16
+  // queries to a cache head) that read up to 134 MB: of 73 with 512 to 1151 work-groups
+  // this took 0.957 of the shares' time in the mean (0.84 to 1.09), of 72 with 1152 and
+  // more 0.916 (0.67 to 1.19, five above 1): INT8, 16 heads of 64, window 1000, 62
+  // sequences, 2976 work-groups, 36.1 us and 38.8; FP8, 8 heads of 64, 16 queries each,
+  // 98 sequences of 1000, 1568: 40.5 and 34.1.  32 queries to a cache head: 0.939 (0.77
+  // to 1.17).  Below 512 it is 1.03 (0.86 to 1.27).  Past the limit a batch of few long
+  // sequences gains most from shares: 8 of 1 to 8000 BF16 keys, 8 heads of 128, 262 MB:
+  // 35.9 us, in shares 30.0.
+  const bool small =
+      each <= kPagedMaxGroups && rows * span * 2 * row_bytes <= kPagedFixedBytes;
   if ((each == 1 || small) && batch <= 65535) {
     p.unit = (int)unit;
     p.each = (int)each;

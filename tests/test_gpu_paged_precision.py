@@ -102,3 +102,44 @@ def test_rows_that_are_not_cut(q_type, cache_type):
     s = Setup(q_type, cache_type, 64, 64, 32, 32, lengths, seed=33)
     assert workspace_bytes(s.q, s.cache, s.max_length) == NO_WORKSPACE
     s.check(s.call(), only={0, 1, 20, 38, 39})
+
+
+@pytest.mark.parametrize("q_type,cache_type", PAIRS)
+@pytest.mark.parametrize("batch,q_heads,heads,dim,longest", [
+    (3, 8, 2, 64, 300), (90, 24, 1, 128, 700), (300, 4, 2, 32, 130), (70, 12, 4, 256, 40)])
+def test_shares_by_a_loose_bound(q_type, cache_type, batch, q_heads, heads, dim, longest):
+    """A bound far above the lengths, as a captured graph is given: by it the call may
+    read so much that it goes by shares, of sequences that are short, and empty."""
+    from fireprot_amd.paged_attention import workspace_bytes
+
+    print(f"loose bound {q_type} {cache_type} {batch, q_heads, heads, dim, longest}", flush=True)
+    g = torch.Generator().manual_seed(batch)
+    lengths = torch.randint(0, longest + 1, (batch,), generator=g)
+    lengths[torch.rand(batch, generator=g) < 0.2] = 0
+    lengths[-1] = longest
+    bound = 1 << 20
+    s = Setup(q_type, cache_type, q_heads, heads, dim, 4096, lengths.tolist(), seed=34,
+              max_length=bound)
+    wide = torch.full((batch, bound // 4096), -9, dtype=torch.int32, device="cuda")
+    wide[:, :s.table.shape[1]] = s.table
+    # (the size goes by the number of shares, not by the bound)
+    assert workspace_bytes(s.q, s.cache, bound) == workspace_bytes(s.q, s.cache, bound // 2) > 256
+    got = s.call(table=wide)
+    s.check(got, only=set(range(0, batch, max(1, batch // 40))) | {batch - 1})
+    assert (got[0][lengths == 0] == 0).all() and torch.isfinite(got[0]).all()
+    again = s.call(table=wide)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
+@pytest.mark.parametrize("batch", [80, 150])
+def test_calls_of_many_units(batch):
+    """More work-groups of one unit each than the card holds at once, and joined: 2560
+    of them for 80 sequences (two units to a row).  150 may read 221 MB and go by
+    shares."""
+    from fireprot_amd.paged_attention import workspace_bytes
+
+    lengths = [(37 * i) % 701 for i in range(batch)]
+    s = Setup(F16, INT8, 16, 16, 64, 16, lengths, seed=35)
+    size, units = workspace_bytes(s.q, s.cache, s.max_length), 2 * 16 * batch
+    assert (size > units * 2 * 64 * 4) == (batch == 80)
+    s.check(s.call(), only=set(range(0, batch, 7)) | {batch - 1})
