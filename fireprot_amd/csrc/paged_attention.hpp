@@ -202,7 +202,11 @@ struct PagedTraits {
   // Registers of a lane: its queries, the tile of K and V in flight, the
   // accumulators, and what codes are decoded to.  Where they would spill (256
   // channels, split queries of two tiles) the queries stay in LDS, which the four
-  // waves share.
+  // waves share.  With that, and one step's queries at a time read for both halves of
+  // a tile, no kernel here spills (253 registers at most at 256 channels, 226 at most
+  // below).  Halves one after the other, which kept all steps' queries from one to the
+  // next, spilled up to 217: 16 sequences of 2001 to 16384 keys, 8 heads of 256, FP32
+  // queries over INT8, 195 us, 125 now; BF16, 8192 keys, 122 and 113.
   static constexpr int kQueryWords = QT * kQuerySteps * kTerms * 4;
   static constexpr int kTileWords = kHalves * (kRow / 16 + 4 * kParts * kPartWords);
   static constexpr bool kQueryLds =
@@ -536,7 +540,15 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
           query_lds[t * kQuads + p * T::kQuerySteps + st][lane] = terms[p];
       }
     }
-    if constexpr (T::kQueryLds) __syncthreads();
+    if constexpr (T::kQueryLds) {
+      // (what was loaded ends here: the compiler keeps it through the loop on the keys
+      // otherwise, and spills)
+#pragma unroll
+      for (int i = 0; i < kMySteps; ++i)
+#pragma unroll
+        for (int j = 0; j < kRaw; ++j) raw[i][j] = u32x4_t{0, 0, 0, 0};
+      __syncthreads();
+    }
     int query_lane = lane;
     auto query = [&](int i) -> u32x4_t {
       if constexpr (T::kQueryLds)
@@ -572,31 +584,35 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
         }
       } else {
 #pragma unroll
-        for (int u = 0; u < kHalves; ++u) {
+        for (int st = 0; st < T::kSteps; ++st) {
+          u32x4_t x[kHalves];
 #pragma unroll
-          for (int st = 0; st < T::kSteps; ++st) {
-            u32x4_t x;
+          for (int u = 0; u < kHalves; ++u) {
             if constexpr (T::kCoded) {
-              x[0] = codes_bf16<C, 0>(kw[u][2 * st]);
-              x[1] = codes_bf16<C, 1>(kw[u][2 * st]);
-              x[2] = codes_bf16<C, 0>(kw[u][2 * st + 1]);
-              x[3] = codes_bf16<C, 1>(kw[u][2 * st + 1]);
+              x[u][0] = codes_bf16<C, 0>(kw[u][2 * st]);
+              x[u][1] = codes_bf16<C, 1>(kw[u][2 * st]);
+              x[u][2] = codes_bf16<C, 0>(kw[u][2 * st + 1]);
+              x[u][3] = codes_bf16<C, 1>(kw[u][2 * st + 1]);
             } else {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) x[i] = kw[u][4 * st + i];
+              for (int i = 0; i < 4; ++i) x[u][i] = kw[u][4 * st + i];
             }
+          }
 #pragma unroll
-            for (int t = 0; t < QT; ++t) {
+          for (int t = 0; t < QT; ++t) {
 #pragma unroll
-              for (int p = T::kTerms - 1; p >= 0; --p) {  // the smallest term first
-                const u32x4_t y = query(t * kQuads + p * T::kQuerySteps + st);
+            for (int p = T::kTerms - 1; p >= 0; --p) {  // the smallest term first
+              const u32x4_t y = query(t * kQuads + p * T::kQuerySteps + st);
+#pragma unroll
+              for (int u = 0; u < kHalves; ++u) {
                 if constexpr (T::kF16)
                   s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                      __builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), s[t][u], 0, 0, 0);
+                      __builtin_bit_cast(f16x8, x[u]), __builtin_bit_cast(f16x8, y), s[t][u], 0, 0,
+                      0);
                 else
                   s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                      __builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), s[t][u], 0, 0,
-                      0);
+                      __builtin_bit_cast(bf16x8, x[u]), __builtin_bit_cast(bf16x8, y), s[t][u], 0,
+                      0, 0);
               }
             }
           }
