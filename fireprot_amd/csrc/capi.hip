@@ -426,8 +426,8 @@ int cache_impl(bool read, int row_dtype, int cache_dtype, const void* k, int64_t
 constexpr int64_t kPagedMaxRows = 1 << 20;  // (sequence, query head): the join's grid
 
 // The cut of a call's work, groups = 0 for unsupported sizes.
-fpx::PagedPlan paged_plan(int cache_dtype, int64_t batch, int q_heads, int heads, int head_dim,
-                          int64_t max_length, int64_t window) {
+fpx::PagedPlan paged_plan(int dtype, int cache_dtype, int64_t batch, int q_heads, int heads,
+                          int head_dim, int64_t max_length, int64_t window) {
   const fpx::PagedPlan none{};
   if (!row_type_ok(cache_dtype) && !is_coded(cache_dtype)) return none;
   if (batch < 0 || batch > kPagedMaxRows || heads < 1 || q_heads < heads || q_heads % heads ||
@@ -435,8 +435,8 @@ fpx::PagedPlan paged_plan(int cache_dtype, int64_t batch, int q_heads, int heads
     return none;
   if (head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256) return none;
   if (max_length < 0 || max_length >= (1 << 30) || window < 0) return none;
-  return fpx::plan_paged(cache_dtype, batch < 1 ? 1 : batch, heads, q_heads / heads, head_dim,
-                         max_length, window < (1 << 30) ? window : 0);
+  return fpx::plan_paged(dtype, cache_dtype, batch < 1 ? 1 : batch, heads, q_heads / heads,
+                         head_dim, max_length, window < (1 << 30) ? window : 0);
 }
 
 // Places of the rows' shares, their (max, sum), and the rows' places.
@@ -974,8 +974,9 @@ int fpx_cache_read(int row_dtype, int cache_dtype, void* k, int64_t k_st, int64_
 
 size_t fpx_paged_attention_workspace_bytes(int cache_dtype, int64_t batch, int q_heads, int heads,
                                            int head_dim, int64_t max_length, int64_t window) {
-  const fpx::PagedPlan p =
-      paged_plan(cache_dtype, batch, q_heads, heads, head_dim, max_length, window);
+  // (of the queries that a cache of this type takes BF16 ones have most shares)
+  const fpx::PagedPlan p = paged_plan(is_coded(cache_dtype) ? FPX_BF16 : cache_dtype, cache_dtype,
+                                      batch, q_heads, heads, head_dim, max_length, window);
   if (p.groups == 0) return 0;
   return p.split ? paged_workspace(p, batch, heads, head_dim).total : 256;
 }
@@ -993,7 +994,7 @@ int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb,
   if (rc != FPX_OK) return rc;
   if (!row_type_ok(dtype) || (!is_coded(cache_dtype) && cache_dtype != dtype)) return FPX_ERR_DIMS;
   const fpx::PagedPlan p =
-      paged_plan(cache_dtype, batch, q_heads, heads, head_dim, max_length, window);
+      paged_plan(dtype, cache_dtype, batch, q_heads, heads, head_dim, max_length, window);
   if (p.groups == 0) return FPX_ERR_DIMS;
   const int64_t row = 16 / (int64_t)type_bytes(dtype);
   if (q_sb < 0 || q_sh < 0 || o_sb < 0 || o_sh < 0 || q_sb % row || q_sh % row || o_sb % row ||

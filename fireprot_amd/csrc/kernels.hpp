@@ -480,7 +480,7 @@ struct PagedPlan {
   int qtiles, query_tiles, tile_queries, split, unit, each;
 };
 
-PagedPlan plan_paged(int cache_dtype, int64_t batch, int heads, int group, int head_dim,
+PagedPlan plan_paged(int dtype, int cache_dtype, int64_t batch, int heads, int group, int head_dim,
                      int64_t max_length, int64_t window);
 hipError_t launch_paged_attention(const PagedArgs& args, hipStream_t stream);
 // one cache type each (paged_attention_*.hip)

@@ -120,7 +120,7 @@ void launch_join(const PagedArgs& a, unsigned rows, hipStream_t stream) {
 
 }  // namespace
 
-PagedPlan plan_paged(int cache_dtype, int64_t batch, int heads, int group, int head_dim,
+PagedPlan plan_paged(int dtype, int cache_dtype, int64_t batch, int heads, int group, int head_dim,
                      int64_t max_length, int64_t window) {
   PagedPlan p{};
   p.query_tiles = group > 16 && head_dim <= 128 ? 2 : 1;
@@ -164,11 +164,15 @@ PagedPlan plan_paged(int cache_dtype, int64_t batch, int heads, int group, int h
     return p;
   }
   // Others: equal shares for as many work-groups to a CU as bring their waves'
-  // tiles in flight to kPagedFlight bytes, all resident
+  // tiles in flight to kPagedFlight bytes and its registers hold at once.  (One more
+  // to a CU than they hold runs by itself when the others are done: 16 sequences of
+  // 2001 to 16384 keys, 8 heads of 128, 32 queries, INT8: FP16 queries 80.1 us in 768
+  // work-groups, 66.0 in 512; FP32 83.5 and 69.6; BF16, of which three fit, 65.0 and
+  // 67.0.)
   p.unit = tile;
   p.split = 1;
   const int64_t each_cu = kPagedFlight / (2 * tile * row_bytes);
-  const int64_t most = head_dim > 128 || p.query_tiles > 1 ? 2 : 3;  // what the registers allow
+  const int64_t most = resident_groups(cache_dtype > 2 && dtype != 1, head_dim, p.query_tiles);
   const int64_t wanted = 256 * (each_cu < 1 ? 1 : each_cu > most ? most : each_cu);
   const int64_t units = rows * ((span + tile - 1) / tile);
   p.groups = (int)(units < wanted ? units : wanted);

@@ -8,7 +8,7 @@
 // A row of the work is one sequence's keys for one cache head and all (up to
 // 16 QT) query heads that share it, so every key and value is read from memory
 // once.  The rows of all sequences, cut into units of 128 keys (FP32: 64), form
-// one line of units, of which each of a fixed number of resident work-groups
+// one line of units, of which each of as many work-groups as fit the card at once
 // takes an equal share, whatever the sequences' lengths: cutting every sequence
 // into chunks of one size instead took 62 us at best where this takes 53 (32
 // sequences of 1 to 4097 BF16 keys, 8 heads of 128), since few large chunks

@@ -77,6 +77,13 @@ FPX_HD int share_of(const Shares& s, int unit) {
   return unit < wide ? unit / (s.size + 1) : s.larger + (unit - wide) / s.size;
 }
 
+// Work-groups of the attention's kernel that a CU's registers hold at once, at least:
+// a work-group has a wave on each SIMD.  `split`: queries that enter the products as
+// several terms (FP32 and FP16 over an 8-bit cache).
+FPX_HD int resident_groups(bool split, int head_dim, int query_tiles) {
+  return head_dim > 128 || query_tiles > 1 || (split && head_dim == 128) ? 2 : 3;
+}
+
 // Entry of the block table that serves a group of keys from `key` on: that of
 // the nearest key of the range, so that a group wholly outside it (its keys
 // are masked) names no page the sequence does not hold.
