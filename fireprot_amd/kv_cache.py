@@ -47,8 +47,6 @@ class PagedCache:
                              f"{[str(t) for t in CACHE_DTYPES]}")
         if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
             raise ValueError("v must have k's shape, type and device")
-        if v is k or (v.data_ptr() == k.data_ptr() and k.numel()):
-            raise ValueError("k and v must not share memory")
         pages, heads, page_size, head_dim = k.shape
         if head_dim not in HEAD_DIMS or page_size not in PAGE_SIZES or pages < 1 or heads < 1:
             raise ValueError(f"needs head_dim in {HEAD_DIMS}, page_size in {PAGE_SIZES}, and at "
@@ -66,6 +64,10 @@ class PagedCache:
         for t in (k, v, *scales):
             if t is not None and (not t.is_contiguous() or t.data_ptr() % 16):
                 raise ValueError("the cache's tensors must be contiguous and 16-byte aligned")
+        ranges = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
+                        for t in (k, v, *scales) if t is not None)
+        if any(end > begin for (_, end), (begin, _) in zip(ranges, ranges[1:])):
+            raise ValueError("k, v and their scales must not share memory")
 
     @classmethod
     def allocate(cls, pages: int, heads: int, page_size: int, head_dim: int, *,
