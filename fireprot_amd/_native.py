@@ -201,7 +201,7 @@ def status() -> dict[str, Any]:
 def check(code: int, what: str) -> None:
     """Raise ``RuntimeError`` for a nonzero status, as ck_attention.py:139-140 does."""
     if code != FPX_OK:
-        names = {FPX_ERR_DIMS: "unsupported sizes or layout",
+        names = {FPX_ERR_DIMS: "unsupported sizes, layout or overlap",
                  FPX_ERR_POINTER: "null or misaligned pointer",
                  FPX_ERR_WORKSPACE: "workspace too small"}
         raise RuntimeError(f"{what} failed with status {code} ({names.get(code, 'HIP error')})")

@@ -8,6 +8,7 @@
 
 #include "common.hpp"
 #include "kernels.hpp"
+#include "overlap.hpp"
 
 #include <cmath>
 #include <mutex>
@@ -387,6 +388,28 @@ bool cache_pointers_ok(int cache_dtype, const void* k, const void* v, const floa
   return !is_coded(cache_dtype) || (aligned(k_scale, 16) && aligned(v_scale, 16));
 }
 
+// A cache's k, v and scales (empty for plain types).
+struct CacheBlocks {
+  fpx::MemoryBlock block[4];
+};
+
+CacheBlocks cache_blocks(int cache_dtype, const void* k, const void* v, const float* k_scale,
+                         const float* v_scale, int64_t pages, int heads, int page_size,
+                         int head_dim) {
+  const int64_t rows = pages * heads * page_size, e = (int64_t)type_bytes(cache_dtype);
+  const bool coded = is_coded(cache_dtype);
+  return {{{k, e, fpx::MemoryAxis{rows * head_dim, 1}},
+           {v, e, fpx::MemoryAxis{rows * head_dim, 1}},
+           {coded ? k_scale : nullptr, 4, fpx::MemoryAxis{rows, 1}},
+           {coded ? v_scale : nullptr, 4, fpx::MemoryAxis{rows, 1}}}};
+}
+
+bool meets_cache(const fpx::MemoryBlock& x, const CacheBlocks& cache) {
+  for (const fpx::MemoryBlock& b : cache.block)
+    if (fpx::blocks_meet(x, b)) return true;
+  return false;
+}
+
 int cache_impl(bool read, int row_dtype, int cache_dtype, const void* k, int64_t k_st,
                int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const int64_t* slots,
                int64_t tokens, const void* cache_k, const void* cache_v, const float* k_scale,
@@ -403,6 +426,27 @@ int cache_impl(bool read, int row_dtype, int cache_dtype, const void* k, int64_t
   if (!aligned(k, elem) || !aligned(v, elem) || !aligned(slots, 8) ||
       !cache_pointers_ok(cache_dtype, cache_k, cache_v, k_scale, v_scale))
     return FPX_ERR_POINTER;
+  {  // what is written meets nothing else
+    using fpx::MemoryAxis;
+    const CacheBlocks cache = cache_blocks(cache_dtype, cache_k, cache_v, k_scale, v_scale, pages,
+                                           heads, page_size, head_dim);
+    const fpx::MemoryBlock rows[2] = {
+        {k, (int64_t)elem, MemoryAxis{tokens, k_st}, MemoryAxis{heads, k_sh}, MemoryAxis{head_dim, 1}},
+        {v, (int64_t)elem, MemoryAxis{tokens, v_st}, MemoryAxis{heads, v_sh},
+         MemoryAxis{head_dim, 1}}};
+    const fpx::MemoryBlock where(slots, 8, MemoryAxis{tokens, 1});
+    if (meets_cache(rows[0], cache) || meets_cache(rows[1], cache)) return FPX_ERR_DIMS;
+    if (read) {
+      if (fpx::blocks_meet(rows[0], rows[1])) return FPX_ERR_DIMS;
+      for (const fpx::MemoryBlock& r : rows)
+        if (fpx::block_meets_itself(r) || fpx::blocks_meet(r, where)) return FPX_ERR_DIMS;
+    } else {
+      for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < i; ++j)
+          if (fpx::blocks_meet(cache.block[i], cache.block[j])) return FPX_ERR_DIMS;
+      if (meets_cache(where, cache)) return FPX_ERR_DIMS;
+    }
+  }
   a.rows[0] = k;
   a.rows[1] = v;
   a.stride_t[0] = k_st;
@@ -936,6 +980,28 @@ int fpx_rotary(int dtype, int layout, const void* q, int64_t q_sb, int64_t q_sn,
       !aligned(inv_freq, 8))
     return FPX_ERR_POINTER;
   if (k_heads > 0 && (!aligned(k, elem) || !aligned(k_out, elem))) return FPX_ERR_POINTER;
+  {  // what is written meets nothing else, but an input in place
+    using fpx::MemoryAxis;
+    auto rows = [&](const void* p, int64_t sb, int64_t sn, int64_t sh, int heads) {
+      return fpx::MemoryBlock(heads > 0 ? p : nullptr, (int64_t)elem, MemoryAxis{batch, sb},
+                              MemoryAxis{tokens, sn}, MemoryAxis{heads, sh},
+                              MemoryAxis{head_dim, 1});
+    };
+    const fpx::MemoryBlock in[2] = {rows(q, q_sb, q_sn, q_sh, q_heads),
+                                    rows(k, k_sb, k_sn, k_sh, k_heads)};
+    const fpx::MemoryBlock out[2] = {rows(q_out, qo_sb, qo_sn, qo_sh, q_heads),
+                                     rows(k_out, ko_sb, ko_sn, ko_sh, k_heads)};
+    const fpx::MemoryBlock place(positions, positions_64 ? 8 : 4, MemoryAxis{batch, p_sb},
+                                 MemoryAxis{tokens, p_sn});
+    const fpx::MemoryBlock freq(inv_freq, 8, MemoryAxis{rotary_dim / 2, 1});
+    const bool in_place[2] = {q_out == q, k_out == k};
+    for (int i = 0; i < 2; ++i)
+      if (fpx::block_meets_itself(out[i]) || (!in_place[i] && fpx::blocks_meet(out[i], in[i])) ||
+          fpx::blocks_meet(out[i], in[1 - i]) || fpx::blocks_meet(out[i], place) ||
+          fpx::blocks_meet(out[i], freq))
+        return FPX_ERR_DIMS;
+    if (fpx::blocks_meet(out[0], out[1])) return FPX_ERR_DIMS;
+  }
   fpx::RotaryArgs a{};
   a.x[0] = {q, q_out, q_sb, q_sn, q_sh, qo_sb, qo_sn, qo_sh, q_heads};
   if (k_heads > 0) a.x[1] = {k, k_out, k_sb, k_sn, k_sh, ko_sb, ko_sn, ko_sh, k_heads};
@@ -1017,6 +1083,30 @@ int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb,
     a.part = as<float>(base);
     a.part_ml = as<float>(base + ws.ml);
     a.row_info = as<int>(base + ws.info);
+  }
+  {  // what is written meets nothing else, but q in place
+    using fpx::MemoryAxis;
+    const int64_t e = (int64_t)type_bytes(dtype);
+    const fpx::MemoryBlock query(q, e, MemoryAxis{batch, q_sb}, MemoryAxis{q_heads, q_sh},
+                                 MemoryAxis{head_dim, 1});
+    const fpx::MemoryBlock written[3] = {
+        {out, e, MemoryAxis{batch, o_sb}, MemoryAxis{q_heads, o_sh}, MemoryAxis{head_dim, 1}},
+        {lse, 4, MemoryAxis{batch * q_heads, 1}},
+        {p.split ? workspace : nullptr, 1, MemoryAxis{(int64_t)ws.total, 1}}};
+    const fpx::MemoryBlock table(block_table, 4, MemoryAxis{batch, table_sb},
+                                 MemoryAxis{(max_length + page_size - 1) / page_size, 1});
+    const fpx::MemoryBlock count(lengths, 4, MemoryAxis{batch, 1});
+    const CacheBlocks cache = cache_blocks(cache_dtype, cache_k, cache_v, k_scale, v_scale, pages,
+                                           heads, page_size, head_dim);
+    if (fpx::block_meets_itself(written[0])) return FPX_ERR_DIMS;
+    for (int i = 0; i < 3; ++i) {
+      if ((!(i == 0 && out == q) && fpx::blocks_meet(written[i], query)) ||
+          fpx::blocks_meet(written[i], table) || fpx::blocks_meet(written[i], count) ||
+          meets_cache(written[i], cache))
+        return FPX_ERR_DIMS;
+      for (int j = 0; j < i; ++j)
+        if (fpx::blocks_meet(written[i], written[j])) return FPX_ERR_DIMS;
+    }
   }
   a.q = q;
   a.q_b = q_sb;

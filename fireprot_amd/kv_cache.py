@@ -165,7 +165,7 @@ def cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor,
     written; everything else in the cache stays as it is.  The other slots
     must be distinct, as with ``torch.Tensor.index_copy_``: of two tokens with
     one slot it is not defined what the slot holds.  ``k`` and ``v`` may not be
-    rows of this cache.
+    rows of this cache (the library refuses them).
     """
     lib = _native.library()
     _, heads, _, head_dim = cache.k.shape
@@ -191,7 +191,9 @@ def cache_read(cache: PagedCache, slots: torch.Tensor, *, dtype: torch.dtype | N
     """``(k, v)``, each ``[tokens, heads, head_dim]`` of ``dtype`` (the outputs'
     where given, the cache's own for a plain cache, float32 for an 8-bit one):
     the rows at ``slots``, dequantised in 32 bits and rounded once.  A negative
-    slot gives zeros, one past the cache NaN.  Slots may repeat."""
+    slot gives zeros, one past the cache NaN.  Slots may repeat.  Outputs that share
+    an element with each other, themselves or the cache are refused, views that only
+    interleave are not."""
     lib = _native.library()
     _, heads, _, head_dim = cache.k.shape
     device = cache.k.get_device()

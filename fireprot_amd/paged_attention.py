@@ -59,7 +59,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
 
     A sequence of length 0 gives zeros (lse -inf).  One whose length is
     negative or above ``max_length``, or whose table names a page outside the
-    cache, gives NaN.  ``out`` may be ``q`` itself.  Records no autograd graph:
+    cache, gives NaN.  ``out`` may be ``q`` itself; it and the workspace may share
+    no other element with the call's tensors.  Records no autograd graph:
     a ``q`` that requires a gradient is refused under grad mode.
     """
     lib = _native.library()

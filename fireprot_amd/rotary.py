@@ -183,8 +183,9 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     k_heads, head_dim]`` (or both without the batch axis) in any non-negative
     strides: views of a fused projection, head-first tensors transposed, a
     channel slice of wider heads.  ``positions`` ``[batch, tokens]`` or
-    ``[tokens]``, int32 or int64.  ``q_out=q, k_out=k`` works in place; any
-    other overlap of inputs and outputs is unsupported.
+    ``[tokens]``, int32 or int64.  ``q_out=q, k_out=k`` works in place; an output
+    that shares an element with anything else is refused, views of one buffer that
+    only interleave are not.
 
     As every operator here it records no autograd graph (tensors that require
     a gradient are refused under grad mode): a training step calls

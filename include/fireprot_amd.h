@@ -342,9 +342,9 @@ int fpx_split_planes(const float* x, int64_t count, uint16_t* planes, void* stre
  *             arithmetic in FP32, the angles in FP64
  *   q         row (b, n, h) at q + b*q_sb + n*q_sn + h*q_sh, channel stride 1;
  *             any alignment of the type (16-byte rows are fastest)
- *   q_out     likewise; may be q itself with the same strides (in place); any
- *             other overlap is unsupported (status 2 when q_out == q with
- *             different strides)
+ *   q_out     likewise; may be q itself with the same strides (in place); an
+ *             output that overlaps anything else, the other output or itself is
+ *             refused (status 2)
  *   k, k_out  the same; k_heads = 0: no keys, pointers and strides ignored
  *   positions int32 (positions_64 = 0) or int64 (1) at b*p_sb + n*p_sn, any sign
  *   inv_freq  [rotary_dim / 2] doubles, radians a position
@@ -373,8 +373,8 @@ int fpx_rotary(int dtype, int layout, const void* q, int64_t q_sb, int64_t q_sn,
  *   both        zeros with scale 0 where top < 2^-100; zeros with scale NaN
  *               where top is infinite or NaN (the row reads back as NaN)
  * A token with a negative slot, or one past the cache, is not written.  The
- * other slots of one call must be distinct, as must be its k and v tensors and
- * the cache's.
+ * other slots of one call must be distinct.  The cache's tensors may not overlap
+ * each other, nor k, v or slots (status 2).
  *   k, v      row (t, h) at k + t*k_st + h*k_sh, channel stride 1, of row_dtype
  *             (FPX_F32, FPX_BF16, FPX_F16); any alignment of the type (16-byte
  *             rows are fastest)
@@ -389,7 +389,8 @@ int fpx_cache_write(int row_dtype, int cache_dtype, const void* k, int64_t k_st,
 
 /* The rows of `slots` read back as row_dtype: code times scale, rounded once.
  * A negative slot gives zeros, one past the cache NaN; slots may repeat.
- * Arguments as fpx_cache_write's, k and v written. */
+ * Arguments as fpx_cache_write's, k and v written: they may not overlap each
+ * other, themselves or an input (status 2). */
 int fpx_cache_read(int row_dtype, int cache_dtype, void* k, int64_t k_st, int64_t k_sh, void* v,
                    int64_t v_st, int64_t v_sh, const int64_t* slots, int64_t tokens,
                    const void* cache_k, const void* cache_v, const float* k_scale,
@@ -414,7 +415,8 @@ size_t fpx_paged_attention_workspace_bytes(int cache_dtype, int64_t batch, int q
  *               the same type, an 8-bit cache takes any (FP32 queries below
  *               2^110: their products with the codes are formed in FP32)
  *   q, out      row (b, h) at q + b*q_sb + h*q_sh, channel stride 1, rows
- *               16-byte aligned; out may be q itself with the same strides
+ *               16-byte aligned; out may be q itself with the same strides; out,
+ *               lse and workspace may not overlap otherwise (status 2)
  *   cache       as fpx_cache_write's
  *   block_table int32, sequence b's pages at block_table + b*table_sb, at least
  *               max_length / page_size (rounded up) of them; only the entries
