@@ -220,6 +220,22 @@ def launch(index: int, entry: Any, *args: Any) -> int:
         return entry(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
+def differentiated(*tensors: Any) -> bool:
+    """Whether one of ``tensors`` (None among them) requires a gradient under grad
+    mode, or carries a forward-mode tangent: an entry that records neither would
+    drop it."""
+    import torch
+    from torch.autograd import forward_ad
+
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    # (outside of any dual level, where no tensor has a tangent, this is one look)
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def repeats(t: Any) -> bool:
     """Whether some of ``t``'s elements share memory through a zero stride (a
     broadcast tensor: no output)."""

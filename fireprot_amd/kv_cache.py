@@ -10,7 +10,7 @@ new tokens at their slots, converted or quantised as they are written
 they are.  There is no counterpart in the reference.
 
 No call records an autograd graph: rows that require a gradient are refused
-under grad mode.
+under grad mode, those with a forward-mode tangent always.
 """
 from __future__ import annotations
 
@@ -176,7 +176,7 @@ def cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor,
     _check_rows(v, "v", shape, device)
     if v.dtype != k.dtype:
         raise ValueError("k and v must have one type")
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+    if _native.differentiated(k, v):
         raise ValueError("a cache records no gradient: detach k and v")
     if k.stride(2) != 1:
         k = k.contiguous()
@@ -213,7 +213,7 @@ def cache_read(cache: PagedCache, slots: torch.Tensor, *, dtype: torch.dtype | N
             if out.dtype != dtype or out.stride(2) != 1 or _native.repeats(out):
                 raise ValueError(f"{name} must be {dtype} with unit channel stride and no "
                                  "repeated elements")
-            if torch.is_grad_enabled() and out.requires_grad:
+            if _native.differentiated(out):
                 raise ValueError("a cache records no gradient: detach the outputs")
         outs.append(out)
     if outs[0].data_ptr() == outs[1].data_ptr() and outs[0].numel():

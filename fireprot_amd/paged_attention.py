@@ -61,7 +61,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
     negative or above ``max_length``, or whose table names a page outside the
     cache, gives NaN.  ``out`` may be ``q`` itself; it and the workspace may share
     no other element with the call's tensors.  Records no autograd graph:
-    a ``q`` that requires a gradient is refused under grad mode.
+    a ``q`` that requires a gradient is refused under grad mode, one with a
+    forward-mode tangent always.
     """
     lib = _native.library()
     k = cache.k
@@ -87,7 +88,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
     if not 0 <= max_length <= held or window < 0:
         raise ValueError(f"needs 0 <= max_length ({max_length}) <= {held}, the block table's "
                          f"slots, and window ({window}) >= 0")
-    if torch.is_grad_enabled() and (q.requires_grad or (out is not None and out.requires_grad)):
+    if _native.differentiated(q, out):
         raise ValueError("no autograd graph is recorded: detach q (and out)")
     if not _aligned_rows(q):
         q = q.clone(memory_format=torch.contiguous_format)

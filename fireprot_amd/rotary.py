@@ -166,8 +166,7 @@ def _launch(q, k, positions, frequencies, layout, inverse, q_out, k_out):
 
 
 def _apply(q, k, positions, frequencies, layout, inverse, q_out, k_out):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (q, k, q_out, k_out)):
+    if _native.differentiated(q, k, q_out, k_out):
         raise ValueError("no autograd graph is recorded: call without gradients "
                          "(torch.no_grad, detach); rotary_backward gives the gradients")
     outs = _launch(q, k, positions, frequencies, layout, inverse, q_out, k_out)
@@ -188,7 +187,8 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     only interleave are not.
 
     As every operator here it records no autograd graph (tensors that require
-    a gradient are refused under grad mode): a training step calls
+    a gradient are refused under grad mode, those with a forward-mode tangent
+    always): a training step calls
     ``rotary_backward`` from its own ``torch.autograd.Function``, or directly.
     """
     return _apply(q, k, positions, frequencies, layout, False, q_out, k_out)
