@@ -115,20 +115,21 @@ def cache_slots(block_table: torch.Tensor, positions: torch.Tensor,
                 page_size: int) -> torch.Tensor:
     """Slots (int64, ``[batch, n]``) of ``positions`` ``[batch, n]`` of
     sequences whose pages are the rows of ``block_table`` ``[batch, p]``.
-    A negative position is no token (slot -1); one past the table gets a slot
-    past every cache."""
+    A negative position is no token (slot -1); one past the table, or whose entry
+    there is negative and so names no page, gets a slot past every cache."""
     if block_table.dim() != 2 or positions.dim() != 2 or len(positions) != len(block_table):
         raise ValueError("block_table must be [batch, p] and positions [batch, n]")
     if page_size not in PAGE_SIZES:
         raise ValueError(f"page_size must be one of {PAGE_SIZES}")
     room = block_table.shape[1] * page_size
     if room == 0:
-        inside = torch.zeros_like(positions, dtype=torch.int64)
+        inside = torch.full_like(positions, torch.iinfo(torch.int64).max, dtype=torch.int64)
     else:
         held = positions.long().clamp(0, room - 1)
-        inside = (block_table.long().gather(1, held // page_size) * page_size
-                  + held % page_size)
-    inside = torch.where(positions >= room, torch.iinfo(torch.int64).max, inside)
+        page = block_table.long().gather(1, held // page_size)
+        outside = (positions >= room) | (page < 0)
+        inside = torch.where(outside, torch.iinfo(torch.int64).max,
+                             page * page_size + held % page_size)
     return torch.where(positions < 0, -1, inside)
 
 
