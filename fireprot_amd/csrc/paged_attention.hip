@@ -134,7 +134,7 @@ PagedPlan plan_paged(int dtype, int cache_dtype, int64_t batch, int heads, int g
   // Small calls: a unit of a row to a work-group, of kPagedUnit keys, or fewer
   // where that leaves CUs without work and the row is long enough to pay for the
   // join: longer than a unit, or of more than kPagedUnitBytes.  (8 sequences of
-  // 500 keys, 4 heads: FP32 rows of 256 channels 36 us in one part, 19 in more;
+  // 500 keys, 4 heads: FP32 rows of 256 channels 33.8 us in one part, 15.8 in more;
   // BF16 rows of 128, 8 heads, 11.2 in one, 12.2 in two.  FP32 rows of 64, 2000
   // keys: 18.4 us in 128 work-groups, 14.0 in 256; BF16 rows of 128, 8 heads of
   // 1500 keys: 16.0 in 192, 17.0 in 384.)

@@ -5,9 +5,11 @@
 //   j over the sequence's keys [first, length), query head h reading cache
 //   head h / group.
 //
-// A row of the work is one sequence's keys for one cache head and all (up to
-// 16 QT) query heads that share it, so every key and value is read from memory
-// once.  The rows of all sequences, cut into units of 128 keys (FP32: 64), form
+// A row of the work is one sequence's keys for one cache head and up to 16 QT of the
+// query heads that share it, so every key and value is read from memory once for 32
+// query heads (16 at 256 channels, whose registers hold one tile of queries): 16
+// sequences of 2001 to 8192 BF16 keys, 4 heads of 128, 43 us with 32 queries to a
+// head, 63 with 40; of 256, 67 with 16, 108 with 24.  The rows of all sequences, cut into units of 128 keys (FP32: 64), form
 // one line of units, of which each of as many work-groups as fit the card at once
 // takes an equal share, whatever the sequences' lengths: cutting every sequence
 // into chunks of one size instead took 62 us at best where this takes 53 (32
@@ -37,8 +39,8 @@
 // sequence of 131071 BF16 keys, 8 heads of 128: 89 us, 6.0 TB/s; 16 of 20001 to
 // 65536 FP8 keys: 235 us, 6.1 TB/s; the ragged 32 above: 5.1 TB/s, of which the
 // start and the join are 8 us.  FP32 rows of 256 channels: 7 sequences of 513 to 8190
-// keys, 2 heads, 37 us, 3.4 TB/s (four tiles of 128 KB to a work-group, so the start
-// and the join are a third of it); 32 of 16384 keys 331 us, 6.5 TB/s.
+// keys, 2 heads, 33 us, 3.8 TB/s (four tiles of 128 KB to a work-group, so the start
+// and the join are a third of it); 32 of 16384 keys 324 to 339 us, 6.3 to 6.6 TB/s.
 //
 // Rounding: scores, softmax and accumulators are FP32.  The weights (times the
 // value's scale in an 8-bit cache) enter the second product as 16-bit terms whose
@@ -419,7 +421,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
 
   // ---- the B operand of S^T = K Q^T: the channels of query `col` in K's order,
   // a step at a time, as they lie in memory and split into terms.  (Lanes past
-  // the tile's last query compute its first one again; their columns are not
+  // the head's last query compute its first one again; their columns are not
   // stored.)
   constexpr int kRaw = T::kF32 ? 1 : (int)sizeof(Q) / 2;  // 16-byte words of a step
   constexpr int kQuads = T::kQuerySteps * T::kTerms;      // of a query tile, term by term
