@@ -396,10 +396,12 @@ struct CacheBlocks {
 CacheBlocks cache_blocks(int cache_dtype, const void* k, const void* v, const float* k_scale,
                          const float* v_scale, int64_t pages, int heads, int page_size,
                          int head_dim) {
+  // (below 2^59; the channels of each row are an axis of their own, as the product of
+  // both could pass 2^63)
   const int64_t rows = pages * heads * page_size, e = (int64_t)type_bytes(cache_dtype);
   const bool coded = is_coded(cache_dtype);
-  return {{{k, e, fpx::MemoryAxis{rows * head_dim, 1}},
-           {v, e, fpx::MemoryAxis{rows * head_dim, 1}},
+  return {{{k, e, fpx::MemoryAxis{rows, head_dim}, fpx::MemoryAxis{head_dim, 1}},
+           {v, e, fpx::MemoryAxis{rows, head_dim}, fpx::MemoryAxis{head_dim, 1}},
            {coded ? k_scale : nullptr, 4, fpx::MemoryAxis{rows, 1}},
            {coded ? v_scale : nullptr, 4, fpx::MemoryAxis{rows, 1}}}};
 }
