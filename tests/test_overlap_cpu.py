@@ -162,8 +162,9 @@ def test_rows_of_the_cache_are_refused(lib, entry, bad):
 
 @pytest.mark.parametrize("entry", ["fpx_cache_write", "fpx_cache_read"])
 def test_rows_inside_a_cache_of_more_bytes_than_63_bits_count(lib, entry):
-    most = dict(pages=2 ** 29, heads=2 ** 15, page_size=4096, head_dim=256, k_st=2 ** 23, k_sh=256,
-                v_st=2 ** 23, v_sh=256, cache_k=1 << 40, cache_v=1 << 41, k=1 << 42, v=1 << 50)
+    most = dict(cache_dtype=1, pages=2 ** 29, heads=2 ** 15, page_size=4096, head_dim=256,
+                k_st=2 ** 23, k_sh=256, v_st=2 ** 23, v_sh=256, cache_k=1 << 40, cache_v=1 << 41,
+                k=1 << 42, v=1 << 50)
     assert getattr(lib, entry)(*cache(**most)) == _native.FPX_ERR_DIMS
 
 
