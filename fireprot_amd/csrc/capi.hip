@@ -433,7 +433,8 @@ int cache_impl(bool read, int row_dtype, int cache_dtype, const void* k, int64_t
     const CacheBlocks cache = cache_blocks(cache_dtype, cache_k, cache_v, k_scale, v_scale, pages,
                                            heads, page_size, head_dim);
     const fpx::MemoryBlock rows[2] = {
-        {k, (int64_t)elem, MemoryAxis{tokens, k_st}, MemoryAxis{heads, k_sh}, MemoryAxis{head_dim, 1}},
+        {k, (int64_t)elem, MemoryAxis{tokens, k_st}, MemoryAxis{heads, k_sh},
+         MemoryAxis{head_dim, 1}},
         {v, (int64_t)elem, MemoryAxis{tokens, v_st}, MemoryAxis{heads, v_sh},
          MemoryAxis{head_dim, 1}}};
     const fpx::MemoryBlock where(slots, 8, MemoryAxis{tokens, 1});

@@ -31,8 +31,8 @@ struct MemoryBlock {
       : base(reinterpret_cast<uintptr_t>(p)), empty(p == nullptr) {
     // (a stride past every memory stays one)
     constexpr int64_t far = int64_t(1) << 58;
-    for (const MemoryAxis x :
-         {MemoryAxis{element, 1}, MemoryAxis{a.count, (a.stride < far ? a.stride : far) * element}...}) {
+    for (const MemoryAxis x : {MemoryAxis{element, 1},
+                               MemoryAxis{a.count, (a.stride < far ? a.stride : far) * element}...}) {
       if (x.count < 1) empty = true;
       if (x.count <= 1) continue;
       span += (__int128)(x.count - 1) * x.stride;

@@ -9,13 +9,13 @@
 // query heads that share it, so every key and value is read from memory once for 32
 // query heads (16 at 256 channels, whose registers hold one tile of queries): 16
 // sequences of 2001 to 8192 BF16 keys, 4 heads of 128, 43 us with 32 queries to a
-// head, 63 with 40; of 256, 67 with 16, 108 with 24.  The rows of all sequences, cut into units of 128 keys (FP32: 64), form
-// one line of units, of which each of as many work-groups as fit the card at once
-// takes an equal share, whatever the sequences' lengths: cutting every sequence
-// into chunks of one size instead took 62 us at best where this takes 53 (32
-// sequences of 1 to 4097 BF16 keys, 8 heads of 128), since few large chunks
-// leave CUs idle and many small ones are mostly start and join.  (Small calls
-// keep to one unit of a row for each work-group: see plan_paged.)  In a row the
+// head, 63 with 40; of 256, 67 with 16, 108 with 24.  The rows of all sequences, cut
+// into units of 128 keys (FP32: 64), form one line of units, of which each of as many
+// work-groups as fit the card at once takes an equal share, whatever the sequences'
+// lengths: cutting every sequence into chunks of one size instead took 62 us at best
+// where this takes 53 (32 sequences of 1 to 4097 BF16 keys, 8 heads of 128), since few
+// large chunks leave CUs idle and many small ones are mostly start and join.  (Small
+// calls keep to one unit of a row for each work-group: see plan_paged.)  In a row the
 // four waves take its tiles in turn, each with an online softmax of its own, and
 // join at its end.  Rows that two shares meet in leave (max, sum, o) of each to
 // join_shares_kernel.
