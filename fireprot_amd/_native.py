@@ -28,6 +28,7 @@ FPX_BF16 = 1
 FPX_F16 = 2
 FPX_F8E4M3 = 3
 FPX_I8 = 4
+FPX_F4E2M1 = 6
 
 _p = ctypes.c_void_p
 _i = ctypes.c_int

@@ -361,7 +361,9 @@ void* device_scratch(hipError_t* err) {
 
 // ---- paged key-value cache: what its entries share
 
-bool is_coded(int dtype) { return dtype == FPX_F8E4M3 || dtype == FPX_I8; }
+bool is_coded(int dtype) {
+  return dtype == FPX_F8E4M3 || dtype == FPX_I8 || dtype == FPX_F4E2M1;
+}
 
 uintptr_t type_bytes(int dtype) {
   return dtype == FPX_F32 ? 4 : dtype == FPX_BF16 || dtype == FPX_F16 ? 2 : 1;
@@ -382,8 +384,8 @@ int cache_dims(int cache_dtype, int64_t pages, int heads, int page_size, int hea
   return FPX_OK;
 }
 
-bool cache_pointers_ok(int cache_dtype, const void* k, const void* v, const float* k_scale,
-                       const float* v_scale) {
+bool cache_pointers_ok(int cache_dtype, const void* k, const void* v, const void* k_scale,
+                       const void* v_scale) {
   if (!aligned(k, 16) || !aligned(v, 16)) return false;
   return !is_coded(cache_dtype) || (aligned(k_scale, 16) && aligned(v_scale, 16));
 }
@@ -393,17 +395,19 @@ struct CacheBlocks {
   fpx::MemoryBlock block[4];
 };
 
-CacheBlocks cache_blocks(int cache_dtype, const void* k, const void* v, const float* k_scale,
-                         const float* v_scale, int64_t pages, int heads, int page_size,
+CacheBlocks cache_blocks(int cache_dtype, const void* k, const void* v, const void* k_scale,
+                         const void* v_scale, int64_t pages, int heads, int page_size,
                          int head_dim) {
   // (below 2^59; the channels of each row are an axis of their own, as the product of
   // both could pass 2^63)
   const int64_t rows = pages * heads * page_size, e = (int64_t)type_bytes(cache_dtype);
-  const bool coded = is_coded(cache_dtype);
-  return {{{k, e, fpx::MemoryAxis{rows, head_dim}, fpx::MemoryAxis{head_dim, 1}},
-           {v, e, fpx::MemoryAxis{rows, head_dim}, fpx::MemoryAxis{head_dim, 1}},
-           {coded ? k_scale : nullptr, 4, fpx::MemoryAxis{rows, 1}},
-           {coded ? v_scale : nullptr, 4, fpx::MemoryAxis{rows, 1}}}};
+  const bool coded = is_coded(cache_dtype), fp4 = cache_dtype == FPX_F4E2M1;
+  const int64_t row = fp4 ? head_dim / 2 : head_dim;  // elements
+  const int64_t scale = fp4 ? head_dim / 32 : 4;      // bytes of a row's scales
+  return {{{k, e, fpx::MemoryAxis{rows, row}, fpx::MemoryAxis{row, 1}},
+           {v, e, fpx::MemoryAxis{rows, row}, fpx::MemoryAxis{row, 1}},
+           {coded ? k_scale : nullptr, scale, fpx::MemoryAxis{rows, 1}},
+           {coded ? v_scale : nullptr, scale, fpx::MemoryAxis{rows, 1}}}};
 }
 
 bool meets_cache(const fpx::MemoryBlock& x, const CacheBlocks& cache) {
@@ -414,8 +418,8 @@ bool meets_cache(const fpx::MemoryBlock& x, const CacheBlocks& cache) {
 
 int cache_impl(bool read, int row_dtype, int cache_dtype, const void* k, int64_t k_st,
                int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const int64_t* slots,
-               int64_t tokens, const void* cache_k, const void* cache_v, const float* k_scale,
-               const float* v_scale, int64_t pages, int heads, int page_size, int head_dim,
+               int64_t tokens, const void* cache_k, const void* cache_v, const void* k_scale,
+               const void* v_scale, int64_t pages, int heads, int page_size, int head_dim,
                void* stream) {
   fpx::CacheArgs a{};
   const int rc = cache_dims(cache_dtype, pages, heads, page_size, head_dim, &a.page_shift);
@@ -459,8 +463,8 @@ int cache_impl(bool read, int row_dtype, int cache_dtype, const void* k, int64_t
   a.slots = slots;
   a.cache[0] = const_cast<void*>(cache_k);
   a.cache[1] = const_cast<void*>(cache_v);
-  a.scale[0] = const_cast<float*>(k_scale);
-  a.scale[1] = const_cast<float*>(v_scale);
+  a.scale[0] = const_cast<void*>(k_scale);
+  a.scale[1] = const_cast<void*>(v_scale);
   a.tokens = tokens;
   a.pages = pages;
   a.heads = heads;
@@ -1026,7 +1030,7 @@ int fpx_rotary(int dtype, int layout, const void* q, int64_t q_sb, int64_t q_sn,
 
 int fpx_cache_write(int row_dtype, int cache_dtype, const void* k, int64_t k_st, int64_t k_sh,
                     const void* v, int64_t v_st, int64_t v_sh, const int64_t* slots,
-                    int64_t tokens, void* cache_k, void* cache_v, float* k_scale, float* v_scale,
+                    int64_t tokens, void* cache_k, void* cache_v, void* k_scale, void* v_scale,
                     int64_t pages, int heads, int page_size, int head_dim, void* stream) {
   return cache_impl(false, row_dtype, cache_dtype, k, k_st, k_sh, v, v_st, v_sh, slots, tokens,
                     cache_k, cache_v, k_scale, v_scale, pages, heads, page_size, head_dim, stream);
@@ -1034,8 +1038,8 @@ int fpx_cache_write(int row_dtype, int cache_dtype, const void* k, int64_t k_st,
 
 int fpx_cache_read(int row_dtype, int cache_dtype, void* k, int64_t k_st, int64_t k_sh, void* v,
                    int64_t v_st, int64_t v_sh, const int64_t* slots, int64_t tokens,
-                   const void* cache_k, const void* cache_v, const float* k_scale,
-                   const float* v_scale, int64_t pages, int heads, int page_size, int head_dim,
+                   const void* cache_k, const void* cache_v, const void* k_scale,
+                   const void* v_scale, int64_t pages, int heads, int page_size, int head_dim,
                    void* stream) {
   return cache_impl(true, row_dtype, cache_dtype, k, k_st, k_sh, v, v_st, v_sh, slots, tokens,
                     cache_k, cache_v, k_scale, v_scale, pages, heads, page_size, head_dim, stream);
@@ -1051,8 +1055,8 @@ size_t fpx_paged_attention_workspace_bytes(int cache_dtype, int64_t batch, int q
 }
 
 int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb, int64_t q_sh,
-                        const void* cache_k, const void* cache_v, const float* k_scale,
-                        const float* v_scale, int64_t pages, int heads, int page_size,
+                        const void* cache_k, const void* cache_v, const void* k_scale,
+                        const void* v_scale, int64_t pages, int heads, int page_size,
                         int head_dim, const int32_t* block_table, int64_t table_sb,
                         int64_t table_pages, const int32_t* lengths, int64_t batch, int q_heads,
                         int64_t max_length, int64_t window, float scale, void* out, int64_t o_sb,

@@ -425,7 +425,7 @@ struct CacheArgs {
   int64_t stride_t[2], stride_h[2];
   const int64_t* slots;  // [tokens]
   void* cache[2];
-  float* scale[2];       // 8-bit caches only
+  void* scale[2];        // coded caches only
   int64_t tokens, pages;
   int heads, head_dim, page_shift;
   int row_dtype, cache_dtype;  // FPX_*
@@ -447,10 +447,10 @@ struct PagedArgs {
   int64_t q_b, q_h;
   const void* k;     // the cache (paged_layout.hpp)
   const void* v;
-  const float* k_scale;
-  const float* v_scale;
-  const int32_t* table;    // pages of a sequence at table + b*table_b
-  int64_t table_b;
+  const void* k_scale;   // coded caches only
+  const void* v_scale;
+  const int32_t* table;    // pages of a sequence at table + b*table_b, of a cache head
+  int64_t table_b, table_h;  // of its own list + h*table_h (0: one list for all)
   const int32_t* lengths;  // [batch]
   void* out;         // as q, strides o_b, o_h
   int64_t o_b, o_h;
@@ -489,6 +489,7 @@ hipError_t launch_paged_bf16(const PagedArgs& args, hipStream_t stream);
 hipError_t launch_paged_f16(const PagedArgs& args, hipStream_t stream);
 hipError_t launch_paged_fp8(const PagedArgs& args, hipStream_t stream);
 hipError_t launch_paged_int8(const PagedArgs& args, hipStream_t stream);
+hipError_t launch_paged_fp4(const PagedArgs& args, hipStream_t stream);
 
 int device_cu_count();
 

@@ -1,15 +1,6 @@
 // The paged key-value cache (fpx_cache_write, fpx_cache_read): rows of keys
 // and values put at their slots, as they are or in 8 bits with a scale per
-// row, and read back.
-//
-// 8-bit rows x of head_dim channels, top = max |x|:
-//   FP8 (E4M3): scale = 2^e, the least e with top <= 448 * 2^e; codes
-//     x / 2^e rounded to nearest even.  A power of two costs a floating format
-//     no precision, makes the division exact, and is what the hardware's own
-//     block scales are.
-//   INT8: scale = top * (1/127), codes x * (1/scale) rounded to nearest even.
-//   top < 2^-100: zeros with scale 0.  top infinite or NaN: zeros with scale
-//     NaN, so the row reads back as NaN.
+// row (in 4 bits: of 32 channels), and read back (cache_rows.hpp has the formats).
 //
 // Both kernels only move rows.  head_dim / 8 threads take a row, 8 channels
 // each (16 bytes of BF16), so the row's maximum is a reduction of at most 32
@@ -18,143 +9,15 @@
 // back from FP8 as BF16, 403 MB, take 64 us, 6.3 TB/s, past the 5.3 of a plain
 // copy, as most of it is writes.  7685 tokens of 16 heads of 64, FP16 and INT8,
 // are written in 13 us and read back in 12, of which 3 to 4 are a launch.
+#include "cache_rows.hpp"
 #include "common.hpp"
 #include "kernels.hpp"
 #include "paged_layout.hpp"
-
-#include <type_traits>
 
 namespace fpx {
 namespace {
 
 constexpr int kCacheThreads = 256;
-constexpr float kTinyRow = 0x1p-100f;
-
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
-struct Fp8 {};
-struct Int8 {};
-
-// ---- eight channels of a row: raw bits in registers, and their values
-template <typename T>
-struct Eight {
-  typedef T Vec __attribute__((ext_vector_type(8)));
-  Vec x;
-  template <bool kStream>
-  __device__ __forceinline__ void load(const T* p) {
-    const Vec* v = reinterpret_cast<const Vec*>(p);
-    x = kStream ? __builtin_nontemporal_load(v) : *v;
-  }
-  // rows of any alignment of T
-  __device__ __forceinline__ void load_each(const T* p) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = p[i];
-  }
-  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Vec*>(p) = x; }
-  __device__ __forceinline__ void store_each(T* p) const {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = x[i];
-  }
-  __device__ __forceinline__ float value(int i) const { return (float)x[i]; }
-  __device__ __forceinline__ void set(int i, float v) { x[i] = (T)v; }
-};
-
-// Eight codes of a row.
-struct Codes {
-  u32x2 x;
-  template <bool kStream>
-  __device__ __forceinline__ void load(const uint8_t* p) {
-    const u32x2* v = reinterpret_cast<const u32x2*>(p);
-    x = kStream ? __builtin_nontemporal_load(v) : *v;
-  }
-  __device__ __forceinline__ void store(uint8_t* p) const { *reinterpret_cast<u32x2*>(p) = x; }
-};
-
-template <typename C>
-constexpr bool kCoded = __is_same(C, Fp8) || __is_same(C, Int8);
-template <typename C>
-using Held = std::conditional_t<kCoded<C>, Codes, Eight<C>>;  // eight channels in the cache
-template <typename C>
-using Elem = std::conditional_t<kCoded<C>, uint8_t, C>;       // one of them
-
-template <int kGroup>
-__device__ __forceinline__ float group_max(float v) {
-  auto mx = [](float x, float y) { return __builtin_elementwise_maximum(x, y); };
-  v = mx(v, dpp<0xB1>(v));                          // lane pairs
-  v = mx(v, dpp<0x4E>(v));                          // quads
-  if constexpr (kGroup >= 8) v = mx(v, dpp<0x141>(v));   // 8 lanes
-  if constexpr (kGroup >= 16) v = mx(v, dpp<0x140>(v));  // 16 lanes
-  if constexpr (kGroup >= 32) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v),
-                                                    __builtin_bit_cast(unsigned, v), false, false);
-    v = mx(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
-  }
-  return v;
-}
-
-// A row's scale and the factor of its codes, from its largest magnitude.
-template <typename C>
-__device__ __forceinline__ void row_scale(float top, float& scale, float& factor) {
-  const uint32_t bits = __builtin_bit_cast(uint32_t, top);
-  if ((bits >> 23) == 255u) {
-    scale = __builtin_nanf("");
-    factor = 0.0f;
-  } else if (top < kTinyRow) {
-    scale = factor = 0.0f;
-  } else if constexpr (__is_same(C, Fp8)) {
-    // 448 = 1.75 * 2^8
-    const uint32_t e = (bits >> 23) - 8u + ((bits & 0x7fffffu) > 0x600000u);
-    scale = __builtin_bit_cast(float, e << 23);
-    factor = __builtin_bit_cast(float, (254u - e) << 23);
-  } else {
-    scale = top * (1.0f / 127.0f);
-    factor = 1.0f / scale;
-  }
-}
-
-// Eight codes of values times the row's factor.  A row without a factor (all
-// but zero, or not finite) holds zeros.
-template <typename C>
-__device__ __forceinline__ u32x2 encode(const float* x, float factor) {
-  float y[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = factor == 0.0f ? 0.0f : x[i] * factor;
-  u32x2 out;
-#pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    if constexpr (__is_same(C, Fp8)) {
-      int r = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * w], y[4 * w + 1], 0, false);
-      out[w] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * w + 2], y[4 * w + 3], r, true);
-    } else {
-      uint32_t r = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        r |= ((uint32_t)(int)__builtin_rintf(y[4 * w + i]) & 0xffu) << (8 * i);
-      out[w] = r;
-    }
-  }
-  return out;
-}
-
-template <typename C>
-__device__ __forceinline__ void decode(u32x2 codes, float scale, float* x) {
-#pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    if constexpr (__is_same(C, Fp8)) {
-      const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes[w], false);
-      const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes[w], true);
-      x[4 * w] = lo[0] * scale;
-      x[4 * w + 1] = lo[1] * scale;
-      x[4 * w + 2] = hi[0] * scale;
-      x[4 * w + 3] = hi[1] * scale;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        x[4 * w + i] = (float)(int)(int8_t)(codes[w] >> (8 * i)) * scale;
-    }
-  }
-}
 
 // tokens x heads rows of S into a cache of C.  kVec: the source rows are
 // 16-byte aligned.
@@ -193,20 +56,13 @@ __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(CacheArgs a)
       if (at[r] < 0) continue;
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        Held<C> y;
         if constexpr (kCoded<C>) {
-          float v[8], top = 0.0f;
+          float v[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            v[i] = x[r][w].value(i);
-            top = __builtin_elementwise_maximum(top, __builtin_fabsf(v[i]));
-          }
-          top = group_max<kGroup>(top);
-          float scale, factor;
-          row_scale<C>(top, scale, factor);
-          y.x = encode<C>(v, factor);
-          if (c == 0) a.scale[w][at[r]] = scale;
+          for (int i = 0; i < 8; ++i) v[i] = x[r][w].value(i);
+          put_codes<C, kDim>(v, a.cache[w], a.scale[w], at[r], c);
         } else {
+          Eight<C> y;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             if constexpr (__is_same(S, C))
@@ -214,8 +70,8 @@ __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(CacheArgs a)
             else
               y.set(i, x[r][w].value(i));
           }
+          y.store(held_at<C, kDim>(a.cache[w], at[r], c));
         }
-        y.store(static_cast<Elem<C>*>(a.cache[w]) + at[r] * kDim + c);
       }
     }
   }
@@ -251,9 +107,9 @@ __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(CacheArgs a) 
       if (at[r] < 0) continue;
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        held[r][w].template load<kStream>(static_cast<const Elem<C>*>(a.cache[w]) + at[r] * kDim +
-                                          c);
-        if constexpr (kCoded<C>) scale[r][w] = a.scale[w][at[r]];
+        held[r][w].template load<kStream>(
+            held_at<C, kDim>(static_cast<const void*>(a.cache[w]), at[r], c));
+        if constexpr (kCoded<C>) scale[r][w] = scale_at<C, kDim>(a.scale[w], at[r], c);
       }
     }
 #pragma unroll
@@ -301,7 +157,7 @@ hipError_t launch_dim(const CacheArgs& a, bool read, hipStream_t stream) {
              (uint64_t)(a.stride_t[w] | a.stride_h[w]) * sizeof(S);
   const bool vec = bytes % 16 == 0;
   // what is read and no cache holds anyway is streamed past them
-  const int64_t row = kDim * (read ? (int64_t)sizeof(Elem<C>) : (int64_t)sizeof(S));
+  const int64_t row = read ? held_bytes<C>(kDim) : kDim * (int64_t)sizeof(S);
   const bool once = 2 * a.tokens * a.heads * row >= kStreamBytes;
   if (read) {
     if (!vec)
@@ -338,7 +194,8 @@ hipError_t launch_source(const CacheArgs& a, bool read, hipStream_t stream) {
     case 1: return launch_cache_type<S, __bf16>(a, read, stream);
     case 2: return launch_cache_type<S, _Float16>(a, read, stream);
     case 3: return launch_cache_type<S, Fp8>(a, read, stream);
-    default: return launch_cache_type<S, Int8>(a, read, stream);
+    case 4: return launch_cache_type<S, Int8>(a, read, stream);
+    default: return launch_cache_type<S, Fp4>(a, read, stream);
   }
 }
 

@@ -126,7 +126,10 @@ PagedPlan plan_paged(int dtype, int cache_dtype, int64_t batch, int heads, int g
   p.query_tiles = group > 16 && head_dim <= 128 ? 2 : 1;
   p.qtiles = (group + 16 * p.query_tiles - 1) / (16 * p.query_tiles);
   p.tile_queries = group < 16 * p.query_tiles ? group : 16 * p.query_tiles;
-  const int row_bytes = head_dim * (cache_dtype == 0 ? 4 : cache_dtype <= 2 ? 2 : 1);
+  const int row_bytes = head_dim / 2 * (cache_dtype == 0   ? 8
+                                        : cache_dtype <= 2 ? 4
+                                        : cache_dtype <= 4 ? 2
+                                                           : 1);
   const int tile = cache_dtype == 0 ? 64 : 128;  // keys: one of PagedTraits::kTile a wave
   const int64_t rows = batch * heads * p.qtiles;
   const int64_t span = unit_limit(max_length, window, 1);
@@ -186,7 +189,8 @@ hipError_t launch_paged_attention(const PagedArgs& a, hipStream_t stream) {
     case 1: e = launch_paged_bf16(a, stream); break;
     case 2: e = launch_paged_f16(a, stream); break;
     case 3: e = launch_paged_fp8(a, stream); break;
-    default: e = launch_paged_int8(a, stream); break;
+    case 4: e = launch_paged_int8(a, stream); break;
+    default: e = launch_paged_fp4(a, stream); break;
   }
   if (e != hipSuccess || !a.split) return e;
   const unsigned rows = (unsigned)((int64_t)a.batch * a.heads * a.group);

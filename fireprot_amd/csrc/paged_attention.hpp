@@ -62,6 +62,7 @@ namespace fpx {
 
 struct Fp8Cache {};
 struct Int8Cache {};
+struct Fp4Cache {};  // codes of 4 bits, a scale to 32 channels
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -92,7 +93,7 @@ __device__ __forceinline__ float groups_max(float v) {
                __builtin_bit_cast(float, (unsigned)s[1]));
 }
 
-// kBytes (2, 4, 8 or 16) bytes into 32-bit words, the first in the low bits.
+// kBytes (1, 2, 4, 8 or 16) bytes into 32-bit words, the first in the low bits.
 // kOnce: non-temporal loads, for whole lines that are read once (V): a plain
 // stream of them reaches 7.1 TB/s on an MI355X where ordinary ones reach 6.3
 // (4 GB in 32 KB work-groups).  K's lines are read in halves, by two loads, and
@@ -100,7 +101,7 @@ __device__ __forceinline__ float groups_max(float v) {
 template <int kBytes, bool kOnce>
 __device__ __forceinline__ void load_words(const char* p, uint32_t* w) {
   using Words = std::conditional_t<
-      kBytes == 2, uint16_t,
+      kBytes <= 2, std::conditional_t<kBytes == 1, uint8_t, uint16_t>,
       std::conditional_t<kBytes == 4, uint32_t,
                          uint32_t __attribute__((ext_vector_type(kBytes < 8 ? 2 : kBytes / 4)))>>;
   const Words* q = reinterpret_cast<const Words*>(p);
@@ -172,13 +173,33 @@ __device__ __forceinline__ uint32_t codes_bf16(uint32_t w) {
     return pack_bf16((float)(int8_t)(w >> (16 * kHalf)), (float)(int8_t)(w >> (16 * kHalf + 8)));
 }
 
+// Two 4-bit codes (byte i of w) times their block's scale (its byte) as a word of BF16:
+// exact, and NaN where the scale is.
+__device__ __forceinline__ uint32_t codes4_bf16(uint32_t w, uint32_t scale, int i) {
+  const float s = __builtin_bit_cast(float, scale << 23);
+  bf16x2 x;
+  switch (i) {
+    case 0: x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0); break;
+    case 1: x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1); break;
+    case 2: x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2); break;
+    default: x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3);
+  }
+  return __builtin_bit_cast(uint32_t, x);
+}
+
 template <typename Q, typename C, int D, int QT>
 struct PagedTraits {
   static constexpr bool kF32 = std::is_same_v<C, float>;
-  static constexpr bool kCoded = std::is_same_v<C, Fp8Cache> || std::is_same_v<C, Int8Cache>;
+  static constexpr bool kFp4 = std::is_same_v<C, Fp4Cache>;
+  // a scale to each row, which its score and its weight are multiplied by
+  static constexpr bool kScaled = std::is_same_v<C, Fp8Cache> || std::is_same_v<C, Int8Cache>;
+  static constexpr bool kCoded = kScaled || kFp4;
   static constexpr bool kF16 = std::is_same_v<C, _Float16>;
-  static constexpr int kElem = kF32 ? 4 : kCoded ? 1 : 2;      // bytes of a cached channel
-  static constexpr int kRow = D * kElem;                       // of a cached row
+  // channels of `bytes` of a cached row, and bytes of the row
+  static constexpr int channels(int bytes) {
+    return kFp4 ? 2 * bytes : bytes / (kF32 ? 4 : kCoded ? 1 : 2);
+  }
+  static constexpr int kRow = D / 2 * (kF32 ? 8 : kFp4 ? 1 : kCoded ? 2 : 4);
   static constexpr int kHalves = kF32 ? 1 : 2;                 // 16-key halves of a tile
   static constexpr int kTile = 16 * kHalves;
   // terms a query is split into: all of its bits in BF16, 8 to a term
@@ -190,13 +211,15 @@ struct PagedTraits {
   // quarter of the row has them)
   static constexpr int kPiece = kRow / 4 < 16 ? kRow / 4 : 16;
   static constexpr int kPieces = kRow / 4 / kPiece;
+  static constexpr int kPieceChannels = channels(kPiece);
+  static constexpr int kPieceSteps = kF32 ? 1 : kPieceChannels / 8;
   static constexpr int kSteps = kF32 ? D / 4 : D / 32;         // of the first product
   static constexpr int kQuerySteps = kF32 ? D / 16 : kSteps;   // 16 bytes of a term each
   // V: channels a lane holds of a row, in pieces
   static constexpr int kChannels = D / 16;
-  static constexpr int kPart = kChannels * kElem < 16 ? kChannels * kElem : 16;  // bytes
-  static constexpr int kParts = kChannels * kElem / kPart;
-  static constexpr int kPartChannels = kPart / kElem;
+  static constexpr int kPart = kRow / 16 < 16 ? kRow / 16 : 16;  // bytes
+  static constexpr int kParts = kRow / 16 / kPart;
+  static constexpr int kPartChannels = channels(kPart);
   static constexpr int kPartWords = (kPart + 3) / 4;
   static constexpr int kVec = kChannels < 4 ? kChannels : 4;   // for the waves' join
   static constexpr int kVecs = kChannels / kVec;
@@ -266,7 +289,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
     early_key = cur.unit0 * a.unit + (wave + kPagedWaves * (lane / kHalves)) * T::kTile +
                 16 * (lane % kHalves);
     if (a.window <= 0 && early_key < a.max_length)
-      early_pages = a.table[cur.seq * a.table_b + (early_key >> a.page_shift)];
+      early_pages = a.table[cur.seq * a.table_b + cur.head / a.qtiles * a.table_h +
+                            (early_key >> a.page_shift)];
   } else {
     // The scan over the sequences' units: one to a lane where they fit, in each
     // wave for itself (0.4 us sooner), a run of them to a thread otherwise.
@@ -345,7 +369,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
 
   uint32_t kw[kHalves][T::kPieces * T::kPiece / 4];
   uint32_t vw[kHalves * 4][T::kParts * T::kPartWords];
-  f32x4 ks[kHalves], vs[kHalves];
+  // scales: a row's, or of a block (K: the lane's of each piece; V: of the lane's
+  // channels in each of its four rows) as bytes
+  f32x4 ks[T::kScaled ? kHalves : 1], vs[T::kScaled ? kHalves : 1];
+  uint32_t kb[T::kFp4 ? kHalves : 1][T::kPieces], vb[T::kFp4 ? kHalves * 4 : 1];
+  constexpr int kBlocks = D / 32;  // of a row
   // The next 64 halves' pages, one to a lane; a page outside the cache is never
   // read: page 0 stands in and the row comes out NaN.
   int pages_ahead = 0;
@@ -361,7 +389,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
   auto look_up = [&](const Segment& x, int n) -> int {
     const int key = start_of(x) + (wave + kPagedWaves * (n + lane / kHalves)) * T::kTile +
                     16 * (lane % kHalves);
-    return a.table[x.seq * a.table_b + table_entry(key, x.range, a.page_shift)];
+    return a.table[x.seq * a.table_b + x.head * a.table_h +
+                   table_entry(key, x.range, a.page_shift)];
   };
   auto take_pages = [&](int pages) {
     const bool ok = page_valid(pages, a.pages);
@@ -382,8 +411,15 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
 #pragma unroll
       for (int c = 0; c < T::kPieces; ++c)
         load_words<T::kPiece, false>(p + c * 64, &kw[u][c * T::kPiece / 4]);
-      if constexpr (T::kCoded)
-        ks[u] = *reinterpret_cast<const f32x4*>(a.k_scale + row + 4 * (lane >> 4));
+      if constexpr (T::kScaled)
+        ks[u] = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.k_scale) + row +
+                                                4 * (lane >> 4));
+      if constexpr (T::kFp4) {
+        const uint8_t* s = static_cast<const uint8_t*>(a.k_scale) + (row + (lane & 15)) * kBlocks +
+                           (lane >> 4) * T::kPieceChannels / 32;
+#pragma unroll
+        for (int c = 0; c < T::kPieces; ++c) kb[u][c] = s[4 * c];
+      }
     }
   };
   auto load_v = [&](const Segment& x, int n) {
@@ -397,8 +433,15 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
 #pragma unroll
         for (int c = 0; c < T::kParts; ++c)
           load_words<T::kPart, true>(p + r * T::kRow + c * 256, &vw[u * 4 + r][c * T::kPartWords]);
-      if constexpr (T::kCoded)
-        vs[u] = *reinterpret_cast<const f32x4*>(a.v_scale + row + 4 * (lane >> 4));
+      if constexpr (T::kScaled)
+        vs[u] = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.v_scale) + row +
+                                                4 * (lane >> 4));
+      if constexpr (T::kFp4) {
+        const uint8_t* s = static_cast<const uint8_t*>(a.v_scale) +
+                           (row + 4 * (lane >> 4)) * kBlocks + (lane & 15) * T::kChannels / 32;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) vb[u * 4 + r] = s[r * kBlocks];
+      }
     }
   };
   // the segment after x, where the share goes on
@@ -430,9 +473,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
     const int qi = (x.qtile * QT + t) * 16 + (lane & 15);
     const Q* q = static_cast<const Q*>(a.q) + x.seq * a.q_b +
                  (int64_t)(x.head * a.group + (qi < a.group ? qi : 0)) * a.q_h;
-    const int d = T::kF32               ? 16 * st + 4 * g
-                  : T::kCoded && D > 32 ? 64 * (st >> 1) + 16 * g + 8 * (st & 1)
-                                        : 32 * st + 8 * g;
+    const int d = T::kPieceChannels * (4 * (st / T::kPieceSteps) + g) + 8 * (st % T::kPieceSteps);
 #pragma unroll
     for (int i = 0; i < kRaw; ++i) raw[i] = *reinterpret_cast<const u32x4_t*>(q + d + 4 * i);
   };
@@ -590,7 +631,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
           u32x4_t x[kHalves];
 #pragma unroll
           for (int u = 0; u < kHalves; ++u) {
-            if constexpr (T::kCoded) {
+            if constexpr (T::kFp4) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                x[u][i] = codes4_bf16(kw[u][st], kb[u][st / T::kPieceSteps], i);
+            } else if constexpr (T::kCoded) {
               x[u][0] = codes_bf16<C, 0>(kw[u][2 * st]);
               x[u][1] = codes_bf16<C, 1>(kw[u][2 * st]);
               x[u][2] = codes_bf16<C, 0>(kw[u][2 * st + 1]);
@@ -622,13 +667,17 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
       }
       // ---- factors of the scores in log2 units; keys outside the range left out
       const bool edge = key0 < range.first || key0 + T::kTile > range.end;
-      float f[kHalves][T::kCoded ? 4 : 1];
+      float f[kHalves][T::kScaled ? 4 : 1];
       uint32_t unseen = 0;  // bit 4u + r
 #pragma unroll
       for (int u = 0; u < kHalves; ++u)
 #pragma unroll
-        for (int r = 0; r < (T::kCoded ? 4 : 1); ++r)
-          f[u][r] = T::kCoded ? a.scale_log2 * ks[u][r] : a.scale_log2;
+        for (int r = 0; r < (T::kScaled ? 4 : 1); ++r) {
+          if constexpr (T::kScaled)
+            f[u][r] = a.scale_log2 * ks[u][r];
+          else
+            f[u][r] = a.scale_log2;
+        }
       if (edge) {
 #pragma unroll
         for (int u = 0; u < kHalves; ++u)
@@ -639,7 +688,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
             unseen |= 1u << (4 * u + r);
             // what the page holds there may be NaN: it must not meet a weight
             // of zero
-            if constexpr (T::kCoded) vs[u][r] = 0.0f;
+            if constexpr (T::kScaled) vs[u][r] = 0.0f;
+            if constexpr (T::kFp4) vb[u * 4 + r] = 0u;
 #pragma unroll
             for (int i = 0; i < T::kParts * T::kPartWords; ++i) vw[u * 4 + r][i] = 0u;
           }
@@ -657,7 +707,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
         for (int u = 0; u < kHalves; ++u)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float x = s[t][u][r] * f[u][T::kCoded ? r : 0];
+            const float x = s[t][u][r] * f[u][T::kScaled ? r : 0];
             top = fmaxf(top, unseen & (1u << (4 * u + r)) ? -__builtin_inff() : x);
           }
         const float next = fmaxf(m[t], groups_max(top));
@@ -674,11 +724,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             // one rounding from the product to the exponent
-            const float e = __builtin_fmaf(s[t][u][r], f[u][T::kCoded ? r : 0], -ref);
+            const float e = __builtin_fmaf(s[t][u][r], f[u][T::kScaled ? r : 0], -ref);
             float w = exp2_fast(T::kShift == 0.0f ? e : e + T::kShift);
             w = unseen & (1u << (4 * u + r)) ? 0.0f : w;
             l[t] += w;
-            if constexpr (T::kCoded)
+            if constexpr (T::kScaled)
               p[t][u * 4 + r] = w * vs[u][r];
             else
               p[t][u * 4 + r] = w;
@@ -716,6 +766,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
             for (int j = 0; j < 8; ++j) {
               if constexpr (!T::kCoded)
                 pair[j] = vw[j][c / 2];
+              else if constexpr (T::kFp4)
+                pair[j] = codes4_bf16(vw[j][c / 8], vb[j], c % 8 / 2);
               else
                 pair[j] =
                     c % 4 == 0 ? codes_bf16<C, 0>(vw[j][c / 4]) : codes_bf16<C, 1>(vw[j][c / 4]);

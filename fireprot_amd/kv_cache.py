@@ -1,11 +1,12 @@
-"""A paged key-value cache on gfx950, plain or in 8 bits.
+"""A paged key-value cache on gfx950, plain, in 8 bits or in 4.
 
 ``PagedCache`` holds keys and values in pages of a power of two of slots, one
 head's rows of a page contiguous: ``[pages, heads, page_size, head_dim]``.  A
 sequence's tokens sit in any pages, in the order of its row of a block table;
 ``cache_slots`` gives the slots of positions.  ``cache_write`` puts the rows of
 new tokens at their slots, converted or quantised as they are written
-(float8_e4m3fn with a power-of-two scale per row, int8 with a scale per row),
+(float8_e4m3fn with a power-of-two scale per row, int8 with a scale per row,
+float4_e2m1fn_x2 with a power-of-two scale per 32 channels: 4.25 bits a channel),
 ``cache_read`` brings rows back, and ``paged_attention`` attends to them where
 they are.  There is no counterpart in the reference.
 
@@ -25,7 +26,10 @@ HEAD_DIMS = (32, 64, 128, 256)
 PAGE_SIZES = tuple(1 << i for i in range(4, 13))
 ROW_DTYPES = {torch.float32: _native.FPX_F32, torch.bfloat16: _native.FPX_BF16,
               torch.float16: _native.FPX_F16}
-CODED_DTYPES = {torch.float8_e4m3fn: _native.FPX_F8E4M3, torch.int8: _native.FPX_I8}
+FP4 = torch.float4_e2m1fn_x2  # two channels to an element, the first in its low half
+BLOCK = 32                    # channels that share a scale in 4 bits
+CODED_DTYPES = {torch.float8_e4m3fn: _native.FPX_F8E4M3, torch.int8: _native.FPX_I8,
+                FP4: _native.FPX_F4E2M1}
 CACHE_DTYPES = {**ROW_DTYPES, **CODED_DTYPES}
 
 
@@ -33,7 +37,9 @@ CACHE_DTYPES = {**ROW_DTYPES, **CODED_DTYPES}
 class PagedCache:
     """``k`` and ``v`` contiguous ``[pages, heads, page_size, head_dim]``;
     ``k_scale`` and ``v_scale`` float32 ``[pages, heads, page_size]`` for the
-    8-bit types, None for the others."""
+    8-bit types, None for the others.  In 4 bits (float4_e2m1fn_x2, two channels to an
+    element) ``k`` and ``v`` are ``[pages, heads, page_size, head_dim / 2]`` and the
+    scales float8_e8m0fnu ``[pages, heads, page_size, head_dim / 32]``."""
 
     k: torch.Tensor
     v: torch.Tensor
@@ -48,19 +54,29 @@ class PagedCache:
         if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
             raise ValueError("v must have k's shape, type and device")
         pages, heads, page_size, head_dim = k.shape
+        if k.dtype == FP4:
+            head_dim *= 2
+        # (looked up by every call)
+        object.__setattr__(self, "sizes", (pages, heads, page_size, head_dim))
         if head_dim not in HEAD_DIMS or page_size not in PAGE_SIZES or pages < 1 or heads < 1:
             raise ValueError(f"needs head_dim in {HEAD_DIMS}, page_size in {PAGE_SIZES}, and at "
                              "least one page and head")
         if k.requires_grad or v.requires_grad:
             raise ValueError("a cache records no gradient: detach k and v")
         scales = (self.k_scale, self.v_scale)
-        if k.dtype in CODED_DTYPES:
+        if k.dtype == FP4:
+            shape = (*k.shape[:3], head_dim // BLOCK)
+            if any(s is None or s.shape != shape or s.dtype != torch.float8_e8m0fnu
+                   or s.device != k.device for s in scales):
+                raise ValueError("a 4-bit cache needs float8_e8m0fnu scales [pages, heads, "
+                                 "page_size, head_dim / 32] on its device")
+        elif k.dtype in CODED_DTYPES:
             if any(s is None or s.shape != k.shape[:3] or s.dtype != torch.float32
                    or s.device != k.device for s in scales):
                 raise ValueError("an 8-bit cache needs float32 scales [pages, heads, page_size] "
                                  "on its device")
         elif any(s is not None for s in scales):
-            raise ValueError("only an 8-bit cache has scales")
+            raise ValueError("only a cache in 8 or 4 bits has scales")
         for t in (k, v, *scales):
             if t is not None and (not t.is_contiguous() or t.data_ptr() % 16):
                 raise ValueError("the cache's tensors must be contiguous and 16-byte aligned")
@@ -77,25 +93,30 @@ class PagedCache:
             return torch.zeros(shape, dtype=kind, device=device)
 
         shape = (pages, heads, page_size, head_dim)
+        if dtype == FP4:
+            rows, blocks = (*shape[:3], head_dim // 2), (*shape[:3], head_dim // BLOCK)
+            k, v, k_scale, v_scale = (zeros(s, torch.uint8) for s in (rows, rows, blocks, blocks))
+            return cls(k.view(FP4), v.view(FP4), k_scale.view(torch.float8_e8m0fnu),
+                       v_scale.view(torch.float8_e8m0fnu))
         coded = dtype in CODED_DTYPES
         scales = [zeros(shape[:3], torch.float32) if coded else None for _ in range(2)]
         return cls(zeros(shape, dtype), zeros(shape, dtype), *scales)
 
     @property
     def pages(self) -> int:
-        return self.k.shape[0]
+        return self.sizes[0]
 
     @property
     def heads(self) -> int:
-        return self.k.shape[1]
+        return self.sizes[1]
 
     @property
     def page_size(self) -> int:
-        return self.k.shape[2]
+        return self.sizes[2]
 
     @property
     def head_dim(self) -> int:
-        return self.k.shape[3]
+        return self.sizes[3]
 
     @property
     def dtype(self) -> torch.dtype:
@@ -152,7 +173,7 @@ def _call(entry, what, device, row_dtype, cache, k, v, slots):
     code = _native.launch(
         device, entry, ROW_DTYPES[row_dtype], CACHE_DTYPES[cache.k.dtype],
         k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2],
-        slots.data_ptr(), slots.shape[0], *cache.pointers(), *cache.k.shape)
+        slots.data_ptr(), slots.shape[0], *cache.pointers(), *cache.sizes)
     if code:
         _native.check(code, what)
 
@@ -169,7 +190,7 @@ def cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor,
     rows of this cache (the library refuses them).
     """
     lib = _native.library()
-    _, heads, _, head_dim = cache.k.shape
+    _, heads, _, head_dim = cache.sizes
     device = cache.k.get_device()
     slots = _check_slots(slots, device)
     shape = (slots.shape[0], heads, head_dim)
@@ -190,13 +211,13 @@ def cache_read(cache: PagedCache, slots: torch.Tensor, *, dtype: torch.dtype | N
                k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None
                ) -> tuple[torch.Tensor, torch.Tensor]:
     """``(k, v)``, each ``[tokens, heads, head_dim]`` of ``dtype`` (the outputs'
-    where given, the cache's own for a plain cache, float32 for an 8-bit one):
+    where given, the cache's own for a plain cache, float32 for a coded one):
     the rows at ``slots``, dequantised in 32 bits and rounded once.  A negative
     slot gives zeros, one past the cache NaN.  Slots may repeat.  Outputs that share
     an element with each other, themselves or the cache are refused, views that only
     interleave are not."""
     lib = _native.library()
-    _, heads, _, head_dim = cache.k.shape
+    _, heads, _, head_dim = cache.sizes
     device = cache.k.get_device()
     slots = _check_slots(slots, device)
     if dtype is None:

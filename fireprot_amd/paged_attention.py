@@ -4,7 +4,7 @@
 attention: each sequence's query heads attend to the keys its row of the block
 table names, ``lengths[b]`` of them (the new token's own among them), where
 they lie in the ``PagedCache`` (``fpx_paged_attention``).  Query heads share
-cache heads in groups; 8-bit caches are dequantised on the way; scores, softmax
+cache heads in groups; 8- and 4-bit caches are dequantised on the way; scores, softmax
 and sums are FP32, and so are the weights that meet the values of an FP32 output
 (16-bit outputs: cut to 22 bits over an FP16 cache, to 16 over others).  All
 sequences' keys are dealt out evenly to the card's
@@ -25,7 +25,7 @@ def workspace_bytes(q: torch.Tensor, cache: PagedCache, max_length: int, window:
     """Device workspace of one call (any contents); 0 for unsupported sizes,
     ``NO_WORKSPACE`` where none is used."""
     return int(_native.library().fpx_paged_attention_workspace_bytes(
-        CACHE_DTYPES[cache.k.dtype], q.shape[0], q.shape[1], cache.k.shape[1], cache.k.shape[3],
+        CACHE_DTYPES[cache.k.dtype], q.shape[0], q.shape[1], cache.heads, cache.head_dim,
         max_length, window))
 
 
@@ -43,8 +43,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
 
     * ``q`` ``[batch, q_heads, head_dim]``, any strides; ``q_heads`` a multiple
       of the cache's heads, each of which serves consecutive query heads.  A
-      plain cache has q's type, an 8-bit one takes float32 (below 2^110: products
-      with the codes are formed in FP32), bfloat16 and float16 queries.
+      plain cache has q's type, an 8- or 4-bit one takes float32 (over 8 bits below
+      2^110: products with the codes are formed in FP32), bfloat16 and float16 queries.
     * ``block_table`` int32 ``[batch, p]``: a sequence's pages in order.
       Entries past its length, or before its window, are not used.
     * ``lengths`` int32 ``[batch]``, up to ``max_length`` (default: what the
@@ -71,7 +71,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
         raise ValueError("q must be float32, bfloat16 or float16 [batch, q_heads, head_dim] on "
                          "the cache's HIP device")
     batch, q_heads, head_dim = q.shape
-    pages, heads, page_size, cache_dim = k.shape
+    pages, heads, page_size, cache_dim = cache.sizes
     if head_dim != cache_dim or q_heads < heads or q_heads % heads:
         raise ValueError(f"q must have head_dim {cache_dim} and a multiple of {heads} heads, "
                          f"got {tuple(q.shape)}")

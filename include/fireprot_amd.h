@@ -42,6 +42,7 @@ extern "C" {
 #define FPX_F16 2
 #define FPX_F8E4M3 3 /* OCP 8-bit float, 4 exponent and 3 mantissa bits */
 #define FPX_I8 4
+#define FPX_F4E2M1 6 /* 4-bit float, 2 exponent and 1 mantissa bit, scale per 32 channels */
 
 /* Layouts of the pairs that fpx_rotary turns. */
 #define FPX_ROTARY_HALF 0        /* channels i and i + rotary_dim / 2 */
@@ -361,17 +362,22 @@ int fpx_rotary(int dtype, int layout, const void* q, int64_t q_sb, int64_t q_sn,
 
 /* A paged key-value cache: `pages` pages of page_size slots; k and v each
  * [pages][heads][page_size][head_dim] of cache_dtype, contiguous; for the 8-bit
- * types scales [pages][heads][page_size] float each, else null.  Slot s is slot
- * s % page_size of page s / page_size.  No counterpart in the reference.
+ * types scales [pages][heads][page_size] float each; for FPX_F4E2M1 rows of head_dim / 2
+ * bytes, channel 2i in the low half of byte i, and scales
+ * [pages][heads][page_size][head_dim / 32] of one byte e each, for 2^(e - 127) (255:
+ * NaN); else null.  Slot s is slot s % page_size of page s / page_size.  No counterpart
+ * in the reference.
  *
  * fpx_cache_write puts token t's rows (every head) at slots[t]: converted to a
- * plain cache_dtype, or as 8-bit codes with a scale per row, top being the
- * row's largest magnitude:
+ * plain cache_dtype, or as 8-bit codes with a scale per row (4-bit codes: per 32
+ * channels), top being the largest magnitude of what shares a scale:
  *   FPX_F8E4M3  scale = 2^e, the least e with top <= 448 * 2^e; the codes are
  *               x / scale rounded to nearest even
  *   FPX_I8      scale = top * (1/127); codes x * (1/scale), to nearest even
- *   both        zeros with scale 0 where top < 2^-100; zeros with scale NaN
- *               where top is infinite or NaN (the row reads back as NaN)
+ *   FPX_F4E2M1  scale = 2^e, the least e <= 125 with top <= 7 * 2^e; codes x / scale,
+ *               to nearest even, at most 6 (0, 0.5, 1, 1.5, 2, 3, 4, 6)
+ *   all         zeros with scale 0 (FPX_F4E2M1: 2^-127) where top < 2^-100; zeros with
+ *               scale NaN where top is infinite or NaN (what shares it reads back as NaN)
  * A token with a negative slot, or one past the cache, is not written.  The
  * other slots of one call must be distinct.  The cache's tensors may not overlap
  * each other, nor k, v or slots (status 2).
@@ -384,7 +390,7 @@ int fpx_rotary(int dtype, int layout, const void* q, int64_t q_sb, int64_t q_sn,
  * when tokens is 0.  The cache's tensors are 16-byte aligned. */
 int fpx_cache_write(int row_dtype, int cache_dtype, const void* k, int64_t k_st, int64_t k_sh,
                     const void* v, int64_t v_st, int64_t v_sh, const int64_t* slots,
-                    int64_t tokens, void* cache_k, void* cache_v, float* k_scale, float* v_scale,
+                    int64_t tokens, void* cache_k, void* cache_v, void* k_scale, void* v_scale,
                     int64_t pages, int heads, int page_size, int head_dim, void* stream);
 
 /* The rows of `slots` read back as row_dtype: code times scale, rounded once.
@@ -393,8 +399,8 @@ int fpx_cache_write(int row_dtype, int cache_dtype, const void* k, int64_t k_st,
  * other, themselves or an input (status 2). */
 int fpx_cache_read(int row_dtype, int cache_dtype, void* k, int64_t k_st, int64_t k_sh, void* v,
                    int64_t v_st, int64_t v_sh, const int64_t* slots, int64_t tokens,
-                   const void* cache_k, const void* cache_v, const float* k_scale,
-                   const float* v_scale, int64_t pages, int heads, int page_size, int head_dim,
+                   const void* cache_k, const void* cache_v, const void* k_scale,
+                   const void* v_scale, int64_t pages, int heads, int page_size, int head_dim,
                    void* stream);
 
 /* Bytes of workspace fpx_paged_attention needs; 0 for unsupported sizes, 256
@@ -412,8 +418,8 @@ size_t fpx_paged_attention_workspace_bytes(int cache_dtype, int64_t batch, int q
  * 16 otherwise (off by at most 2^-16 of the weight; the output's own rounding is
  * off by up to 2^-8 in BF16, 2^-11 in FP16).  No counterpart in the reference.
  *   dtype       FPX_F32, FPX_BF16 or FPX_F16 of q and out; a plain cache has
- *               the same type, an 8-bit cache takes any (FP32 queries below
- *               2^110: their products with the codes are formed in FP32)
+ *               the same type, a coded cache takes any (FP32 queries below
+ *               2^110 over 8 bits: their products with the codes are formed in FP32)
  *   q, out      row (b, h) at q + b*q_sb + h*q_sh, channel stride 1, rows
  *               16-byte aligned; out may be q itself with the same strides; out,
  *               lse and workspace may not overlap otherwise (status 2)
@@ -431,8 +437,8 @@ size_t fpx_paged_attention_workspace_bytes(int cache_dtype, int64_t batch, int q
  * batch * q_heads up to 2^20, and its product with max_length / 64 (a window
  * bounds it as well) below 2^31; nothing is launched when batch is 0. */
 int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb, int64_t q_sh,
-                        const void* cache_k, const void* cache_v, const float* k_scale,
-                        const float* v_scale, int64_t pages, int heads, int page_size,
+                        const void* cache_k, const void* cache_v, const void* k_scale,
+                        const void* v_scale, int64_t pages, int heads, int page_size,
                         int head_dim, const int32_t* block_table, int64_t table_sb,
                         int64_t table_pages, const int32_t* lengths, int64_t batch, int q_heads,
                         int64_t max_length, int64_t window, float scale, void* out, int64_t o_sb,
