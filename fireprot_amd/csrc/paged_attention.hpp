@@ -235,7 +235,7 @@ struct PagedTraits {
   static constexpr int kQueryWords = QT * kQuerySteps * kTerms * 4;
   static constexpr int kTileWords = kHalves * (kRow / 16 + 4 * kParts * kPartWords);
   static constexpr bool kQueryLds =
-      kQueryWords + kTileWords + QT * kChannels * 4 + (kCoded ? 16 : 0) > 160;
+      kQueryWords + kTileWords + QT * kChannels * 4 + (kFp4 ? 32 : kCoded ? 16 : 0) > 160;
   static constexpr float kShift = kF16 ? kWeightShiftF16 : 0.0f;
 };
 
@@ -745,51 +745,55 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
               o[t][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(
                   __builtin_bit_cast(float, vw[r][c]), p[t][r], o[t][c], 0, 0, 0);
       } else {
-        u32x4_t weights[QT][T::kWeightTerms];
 #pragma unroll
-        for (int t = 0; t < QT; ++t)
+        for (int k0 = 0; k0 < kHalves * 4; k0 += 8) {  // the lane's eight of 32 keys
+          u32x4_t weights[QT][T::kWeightTerms];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t terms[T::kWeightTerms];
-            if constexpr (T::kWeightTerms == 3)
-              split_weights_exactly(p[t][2 * i], p[t][2 * i + 1], terms);
-            else
-              split_weights<T::kF16, !T::kCoded>(p[t][2 * i], p[t][2 * i + 1], terms[0], terms[1]);
+          for (int t = 0; t < QT; ++t)
 #pragma unroll
-            for (int w = 0; w < T::kWeightTerms; ++w) weights[t][w][i] = terms[w];
-          }
-        uint32_t pair[8];  // two channels of the lane's eight keys
-#pragma unroll
-        for (int c = 0; c < T::kChannels; ++c) {
-          if (c % 2 == 0) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              if constexpr (!T::kCoded)
-                pair[j] = vw[j][c / 2];
-              else if constexpr (T::kFp4)
-                pair[j] = codes4_bf16(vw[j][c / 8], vb[j], c % 8 / 2);
+            for (int i = 0; i < 4; ++i) {
+              uint32_t terms[T::kWeightTerms];
+              const float p0 = p[t][k0 + 2 * i], p1 = p[t][k0 + 2 * i + 1];
+              if constexpr (T::kWeightTerms == 3)
+                split_weights_exactly(p0, p1, terms);
               else
-                pair[j] =
-                    c % 4 == 0 ? codes_bf16<C, 0>(vw[j][c / 4]) : codes_bf16<C, 1>(vw[j][c / 4]);
+                split_weights<T::kF16, !T::kCoded>(p0, p1, terms[0], terms[1]);
+#pragma unroll
+              for (int w = 0; w < T::kWeightTerms; ++w) weights[t][w][i] = terms[w];
             }
-          }
-          u32x4_t x;
+          uint32_t pair[8];  // two channels of them
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            x[i] = __builtin_amdgcn_perm(pair[2 * i + 1], pair[2 * i],
-                                         c % 2 ? 0x07060302u : 0x05040100u);
+          for (int c = 0; c < T::kChannels; ++c) {
+            if (c % 2 == 0) {
 #pragma unroll
-          for (int t = 0; t < QT; ++t) {
+              for (int j = 0; j < 8; ++j) {
+                if constexpr (!T::kCoded)
+                  pair[j] = vw[k0 + j][c / 2];
+                else if constexpr (T::kFp4)
+                  pair[j] = codes4_bf16(vw[k0 + j][c / 8], vb[k0 + j], c % 8 / 2);
+                else
+                  pair[j] = c % 4 == 0 ? codes_bf16<C, 0>(vw[k0 + j][c / 4])
+                                       : codes_bf16<C, 1>(vw[k0 + j][c / 4]);
+              }
+            }
+            u32x4_t x;
 #pragma unroll
-            for (int w = T::kWeightTerms - 1; w >= 0; --w) {  // the smallest term first
-              if constexpr (T::kF16)
-                o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                    __builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, weights[t][w]),
-                    o[t][c], 0, 0, 0);
-              else
-                o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                    __builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, weights[t][w]),
-                    o[t][c], 0, 0, 0);
+            for (int i = 0; i < 4; ++i)
+              x[i] = __builtin_amdgcn_perm(pair[2 * i + 1], pair[2 * i],
+                                           c % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+#pragma unroll
+              for (int w = T::kWeightTerms - 1; w >= 0; --w) {  // the smallest term first
+                if constexpr (T::kF16)
+                  o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                      __builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, weights[t][w]),
+                      o[t][c], 0, 0, 0);
+                else
+                  o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                      __builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, weights[t][w]),
+                      o[t][c], 0, 0, 0);
+              }
             }
           }
         }
