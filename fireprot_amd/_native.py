@@ -132,6 +132,19 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         _p, _p, _p, _p,              # cache_k, cache_v, k_scale, v_scale
         _i64, _i, _i, _i, _p,        # pages, heads, page_size, head_dim, stream
     ]),
+    "fpx_cache_append": (_i, [
+        _i, _i, _i,                  # dtype, cache_dtype, layout
+        _p, _i64, _i64, _i64,        # q, strides (batch, token, head)
+        _p, _i64, _i64, _i64, _i,    # q_out, strides, q_heads (0: none)
+        _p, _i64, _i64, _i64,        # k
+        _p, _i64, _i64, _i64,        # v
+        _p, _i, _i64, _i64,          # positions, 64-bit, strides (batch, token)
+        _p, _f, _i,                  # inv_freq (double), scale, rotary_dim
+        _p, _p, _i64, _i64,          # slots, or block_table, stride, pages a sequence
+        _i64, _i64,                  # batch, tokens
+        _p, _p, _p, _p,              # cache_k, cache_v, k_scale, v_scale
+        _i64, _i, _i, _i, _p,        # pages, heads, page_size, head_dim, stream
+    ]),
     "fpx_paged_attention_workspace_bytes": (_sz, [_i, _i64, _i, _i, _i, _i64, _i64]),
     "fpx_paged_attention": (_i, [
         _i, _i,                      # dtype, cache_dtype

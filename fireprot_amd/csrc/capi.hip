@@ -1045,6 +1045,108 @@ int fpx_cache_read(int row_dtype, int cache_dtype, void* k, int64_t k_st, int64_
                     cache_k, cache_v, k_scale, v_scale, pages, heads, page_size, head_dim, stream);
 }
 
+int fpx_cache_append(int dtype, int cache_dtype, int layout, const void* q, int64_t q_sb,
+                     int64_t q_sn, int64_t q_sh, void* q_out, int64_t qo_sb, int64_t qo_sn,
+                     int64_t qo_sh, int q_heads, const void* k, int64_t k_sb, int64_t k_sn,
+                     int64_t k_sh, const void* v, int64_t v_sb, int64_t v_sn, int64_t v_sh,
+                     const void* positions, int positions_64, int64_t p_sb, int64_t p_sn,
+                     const double* inv_freq, float scale, int rotary_dim, const int64_t* slots,
+                     const int32_t* block_table, int64_t table_sb, int64_t table_pages,
+                     int64_t batch, int64_t tokens, void* cache_k, void* cache_v, void* k_scale,
+                     void* v_scale, int64_t pages, int heads, int page_size, int head_dim,
+                     void* stream) {
+  fpx::AppendArgs a{};
+  const int rc = cache_dims(cache_dtype, pages, heads, page_size, head_dim, &a.page_shift);
+  if (rc != FPX_OK) return rc;
+  if (!row_type_ok(dtype)) return FPX_ERR_DIMS;
+  if (layout != FPX_ROTARY_HALF && layout != FPX_ROTARY_INTERLEAVED) return FPX_ERR_DIMS;
+  if (positions_64 != 0 && positions_64 != 1) return FPX_ERR_DIMS;
+  if (rotary_dim < 2 || rotary_dim > head_dim || rotary_dim % 2) return FPX_ERR_DIMS;
+  if (q_heads < 0 || q_heads > 8192 || heads > 4096 || q_heads + 2 * heads > 8192)
+    return FPX_ERR_DIMS;
+  if (batch < 0 || tokens < 0 || batch > 0x7fffffff || tokens > 0x7fffffff ||
+      batch * tokens > 0x7fffffff)
+    return FPX_ERR_DIMS;
+  if (k_sb < 0 || k_sn < 0 || k_sh < 0 || v_sb < 0 || v_sn < 0 || v_sh < 0 || p_sb < 0 || p_sn < 0)
+    return FPX_ERR_DIMS;
+  if (q_heads > 0) {
+    if (q_sb < 0 || q_sn < 0 || q_sh < 0 || qo_sb < 0 || qo_sn < 0 || qo_sh < 0)
+      return FPX_ERR_DIMS;
+    if (q == q_out && (q_sb != qo_sb || q_sn != qo_sn || q_sh != qo_sh)) return FPX_ERR_DIMS;
+  }
+  if ((slots == nullptr) == (block_table == nullptr)) return FPX_ERR_DIMS;
+  if (!slots && (table_sb < 0 || table_pages < 0)) return FPX_ERR_DIMS;
+  if (batch == 0 || tokens == 0) return FPX_OK;
+  const uintptr_t elem = type_bytes(dtype);
+  if (!aligned(k, elem) || !aligned(v, elem) || !aligned(positions, positions_64 ? 8 : 4) ||
+      !aligned(inv_freq, 8) || (slots ? !aligned(slots, 8) : !aligned(block_table, 4)) ||
+      !cache_pointers_ok(cache_dtype, cache_k, cache_v, k_scale, v_scale))
+    return FPX_ERR_POINTER;
+  if (q_heads > 0 && (!aligned(q, elem) || !aligned(q_out, elem))) return FPX_ERR_POINTER;
+  {  // what is written meets nothing else, but q in place
+    using fpx::MemoryAxis;
+    auto rows = [&](const void* p, int64_t sb, int64_t sn, int64_t sh, int n) {
+      return fpx::MemoryBlock(n > 0 ? p : nullptr, (int64_t)elem, MemoryAxis{batch, sb},
+                              MemoryAxis{tokens, sn}, MemoryAxis{n, sh}, MemoryAxis{head_dim, 1});
+    };
+    const fpx::MemoryBlock out = rows(q_out, qo_sb, qo_sn, qo_sh, q_heads);
+    const fpx::MemoryBlock in[6] = {
+        rows(q, q_sb, q_sn, q_sh, q_heads), rows(k, k_sb, k_sn, k_sh, heads),
+        rows(v, v_sb, v_sn, v_sh, heads),
+        {positions, positions_64 ? 8 : 4, MemoryAxis{batch, p_sb}, MemoryAxis{tokens, p_sn}},
+        {inv_freq, 8, MemoryAxis{rotary_dim / 2, 1}},
+        slots ? fpx::MemoryBlock(slots, 8, MemoryAxis{batch * tokens, 1})
+              : fpx::MemoryBlock(block_table, 4, MemoryAxis{batch, table_sb},
+                                 MemoryAxis{table_pages, 1})};
+    const CacheBlocks cache = cache_blocks(cache_dtype, cache_k, cache_v, k_scale, v_scale, pages,
+                                           heads, page_size, head_dim);
+    if (fpx::block_meets_itself(out) || meets_cache(out, cache)) return FPX_ERR_DIMS;
+    for (int i = 0; i < 6; ++i)
+      if ((!(i == 0 && q_out == q) && fpx::blocks_meet(out, in[i])) || meets_cache(in[i], cache))
+        return FPX_ERR_DIMS;
+    for (int i = 0; i < 4; ++i)
+      for (int j = 0; j < i; ++j)
+        if (fpx::blocks_meet(cache.block[i], cache.block[j])) return FPX_ERR_DIMS;
+  }
+  const void* in[3] = {q, k, v};
+  const int64_t strides[3][3] = {{q_sb, q_sn, q_sh}, {k_sb, k_sn, k_sh}, {v_sb, v_sn, v_sh}};
+  for (int w = 0; w < 3; ++w) {
+    a.in[w] = in[w];
+    a.in_b[w] = strides[w][0];
+    a.in_n[w] = strides[w][1];
+    a.in_h[w] = strides[w][2];
+  }
+  a.q_out = q_out;
+  a.out_b = qo_sb;
+  a.out_n = qo_sn;
+  a.out_h = qo_sh;
+  a.pos = positions;
+  a.pos_b = p_sb;
+  a.pos_n = p_sn;
+  a.pos64 = positions_64;
+  a.freq = inv_freq;
+  a.scale = scale;
+  a.interleaved = layout == FPX_ROTARY_INTERLEAVED;
+  a.rot = rotary_dim;
+  a.slots = slots;
+  a.table = block_table;
+  a.table_b = table_sb;
+  a.table_pages = table_pages;
+  a.cache[0] = cache_k;
+  a.cache[1] = cache_v;
+  a.cache_scale[0] = k_scale;
+  a.cache_scale[1] = v_scale;
+  a.pages = pages;
+  a.total = batch * tokens;
+  a.tokens = (int)tokens;
+  a.q_heads = q_heads;
+  a.heads = heads;
+  a.head_dim = head_dim;
+  a.row_dtype = dtype;
+  a.cache_dtype = cache_dtype;
+  return status(fpx::launch_cache_append(a, static_cast<hipStream_t>(stream)));
+}
+
 size_t fpx_paged_attention_workspace_bytes(int cache_dtype, int64_t batch, int q_heads, int heads,
                                            int head_dim, int64_t max_length, int64_t window) {
   // (of the queries that a cache of this type takes BF16 ones have most shares)

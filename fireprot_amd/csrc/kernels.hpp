@@ -433,6 +433,38 @@ struct CacheArgs {
 
 hipError_t launch_cache(const CacheArgs& args, bool read, hipStream_t stream);
 
+// ------------------------------------------- new tokens, turned, into the cache
+// Rows (b, n, h) of queries [0], keys [1] and values [2] at in + b*in_b + n*in_n +
+// h*in_h (channel stride 1); q_heads == 0: no queries.
+struct AppendArgs {
+  const void* in[3];
+  int64_t in_b[3], in_n[3], in_h[3];
+  void* q_out;         // turned queries; in[0] itself with the same strides: in place
+  int64_t out_b, out_n, out_h;
+  const void* pos;     // int32 or int64 at b*pos_b + n*pos_n
+  int64_t pos_b, pos_n;
+  int pos64;
+  const double* freq;  // [rot / 2] radians a position
+  float scale;         // of the rotated channels
+  int interleaved, rot;
+  const int64_t* slots;  // [total], or null: by position from
+  const int32_t* table;  // pages of a sequence at table + b*table_b, table_pages of them
+  int64_t table_b, table_pages;
+  void* cache[2];        // as CacheArgs has them
+  void* cache_scale[2];
+  int64_t pages, total;  // total: tokens of all sequences
+  int tokens;            // of a sequence
+  int q_heads, heads, head_dim, page_shift;
+  int row_dtype, cache_dtype;  // FPX_*
+  // launch shape, set by launch_cache_append: first token, tokens of a work-group,
+  // magic number of a token's rows
+  int64_t first;
+  int tt;
+  unsigned rows_magic;
+};
+
+hipError_t launch_cache_append(const AppendArgs& args, hipStream_t stream);
+
 // --------------------------------------- attention of new tokens over the cache
 constexpr int kPagedMaxGroups = 1024;  // work-groups that share a row
 constexpr int kPagedUnit = 512;        // keys of a small call's unit

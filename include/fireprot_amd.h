@@ -403,6 +403,38 @@ int fpx_cache_read(int row_dtype, int cache_dtype, void* k, int64_t k_st, int64_
                    const void* v_scale, int64_t pages, int heads, int page_size, int head_dim,
                    void* stream);
 
+/* New tokens into a paged cache, turned by their positions: q_out = rotate(q), and
+ * token (b, n)'s rotate(k) and v (every head) at its slot, converted as fpx_cache_write
+ * converts them but from the FP32 values of the rotation (one rounding).  rotate and
+ * its arguments are fpx_rotary's, the cache fpx_cache_write's.  No counterpart in the
+ * reference.
+ *   dtype     FPX_F32, FPX_BF16 or FPX_F16 of q, q_out, k and v
+ *   q, q_out  row (b, n, h) at q + b*q_sb + n*q_sn + h*q_sh, channel stride 1; q_out may
+ *             be q itself with the same strides, and overlap nothing else (status 2);
+ *             q_heads = 0: no queries, pointers and strides ignored
+ *   k, v      likewise, `heads` rows a token; any alignment of the type (16-byte rows
+ *             and rotary_dim % 16 == 0, or interleaved pairs, are fastest)
+ *   slots     nullable int64 [batch][tokens], as fpx_cache_write's; null: the slot of
+ *             position p of sequence b is slot p % page_size of page
+ *             block_table[b*table_sb + p / page_size].  A token whose position is
+ *             negative, past table_pages, or on a page outside the cache is not
+ *             written (its query is turned all the same)
+ * The tokens' slots must be distinct; the cache's tensors may not overlap each other or
+ * an input (status 2).
+ * Supported: fpx_rotary's and fpx_cache_write's sizes; exactly one of slots and
+ * block_table; q_heads + 2 * heads <= 8192; nothing is launched when batch or tokens
+ * is 0. */
+int fpx_cache_append(int dtype, int cache_dtype, int layout, const void* q, int64_t q_sb,
+                     int64_t q_sn, int64_t q_sh, void* q_out, int64_t qo_sb, int64_t qo_sn,
+                     int64_t qo_sh, int q_heads, const void* k, int64_t k_sb, int64_t k_sn,
+                     int64_t k_sh, const void* v, int64_t v_sb, int64_t v_sn, int64_t v_sh,
+                     const void* positions, int positions_64, int64_t p_sb, int64_t p_sn,
+                     const double* inv_freq, float scale, int rotary_dim, const int64_t* slots,
+                     const int32_t* block_table, int64_t table_sb, int64_t table_pages,
+                     int64_t batch, int64_t tokens, void* cache_k, void* cache_v, void* k_scale,
+                     void* v_scale, int64_t pages, int heads, int page_size, int head_dim,
+                     void* stream);
+
 /* Bytes of workspace fpx_paged_attention needs; 0 for unsupported sizes, 256
  * where it uses none (sequences too short to be shared by work-groups): its
  * workspace may then be null. */
