@@ -157,6 +157,35 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         _p, _i64, _i64, _p,          # out, strides (batch, head), lse (nullable)
         _p, _sz, _p,                 # workspace, bytes, stream
     ]),
+    "fpx_paged_attention_lists": (_i, [
+        _i, _i,                      # dtype, cache_dtype
+        _p, _i64, _i64,              # q, strides (batch, head)
+        _p, _p, _p, _p,              # cache_k, cache_v, k_scale, v_scale
+        _i64, _i, _i, _i,            # pages, heads, page_size, head_dim
+        _p, _i64, _i64, _i64,        # block_table, strides (batch, head), pages of a list
+        _p, _i64, _i,                # lengths, batch, q_heads
+        _i64, _f,                    # max_length, scale
+        _p, _i64, _i64, _p,          # out, strides (batch, head), lse (nullable)
+        _p, _sz, _p,                 # workspace, bytes, stream
+    ]),
+    "fpx_page_bounds": (_i, [
+        _i, _p, _p,                  # cache_dtype, cache_k, k_scale
+        _i64, _i, _i, _i,            # pages, heads, page_size, head_dim
+        _p, _i64, _i64,              # block_table, stride, pages a sequence
+        _p, _i64, _i64, _i64,        # lengths, batch, max_length, fresh
+        _p, _p,                      # bounds, stream
+    ]),
+    "fpx_select_pages_workspace_bytes": (_sz, [_i64, _i, _i, _i64, _i]),
+    "fpx_select_pages": (_i, [
+        _i, _i,                      # dtype, bounds_dtype
+        _p, _i64, _i64, _i,          # q, strides (batch, head), q_heads
+        _p, _i64, _i, _i, _i,        # bounds, pages, heads, page_size, head_dim
+        _p, _i64, _i64,              # block_table, stride, pages a sequence
+        _p, _i64, _i64,              # lengths, batch, max_length
+        _i, _i, _i,                  # count, sinks, recent
+        _p, _p, _p,                  # index, table_out, lengths_out
+        _p, _sz, _p,                 # workspace, bytes, stream
+    ]),
     "fpx_cache_read": (_i, [
         _i, _i,                      # row_dtype, cache_dtype
         _p, _i64, _i64,              # k (written), strides (token, head)

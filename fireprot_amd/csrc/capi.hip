@@ -504,6 +504,104 @@ PagedWorkspace paged_workspace(const fpx::PagedPlan& p, int64_t batch, int heads
   return w;
 }
 
+int paged_impl(int dtype, int cache_dtype, const void* q, int64_t q_sb, int64_t q_sh,
+               const void* cache_k, const void* cache_v, const void* k_scale, const void* v_scale,
+               int64_t pages, int heads, int page_size, int head_dim, const int32_t* block_table,
+               int64_t table_sb, int64_t table_sh, int64_t table_pages, const int32_t* lengths,
+               int64_t batch, int q_heads, int64_t max_length, int64_t window, float scale,
+               void* out, int64_t o_sb, int64_t o_sh, float* lse, void* workspace,
+               size_t workspace_bytes, void* stream) {
+  fpx::PagedArgs a{};
+  const int rc = cache_dims(cache_dtype, pages, heads, page_size, head_dim, &a.page_shift);
+  if (rc != FPX_OK) return rc;
+  if (!row_type_ok(dtype) || (!is_coded(cache_dtype) && cache_dtype != dtype)) return FPX_ERR_DIMS;
+  const fpx::PagedPlan p =
+      paged_plan(dtype, cache_dtype, batch, q_heads, heads, head_dim, max_length, window);
+  if (p.groups == 0) return FPX_ERR_DIMS;
+  const int64_t row = 16 / (int64_t)type_bytes(dtype);
+  if (q_sb < 0 || q_sh < 0 || o_sb < 0 || o_sh < 0 || q_sb % row || q_sh % row || o_sb % row ||
+      o_sh % row)
+    return FPX_ERR_DIMS;
+  if (out == q && (o_sb != q_sb || o_sh != q_sh)) return FPX_ERR_DIMS;
+  if (table_sb < 0 || table_sh < 0 || table_pages < (max_length + page_size - 1) / page_size)
+    return FPX_ERR_DIMS;
+  const float scale_log2 = scale * fpx::kLog2e;
+  if (!(scale_log2 - scale_log2 == 0.0f)) return FPX_ERR_DIMS;  // infinite or NaN
+  if (batch == 0) return FPX_OK;
+  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(lengths, 4) ||
+      !aligned_or_null(lse, 4) || (max_length > 0 && !aligned(block_table, 4)) ||
+      !cache_pointers_ok(cache_dtype, cache_k, cache_v, k_scale, v_scale))
+    return FPX_ERR_POINTER;
+  const PagedWorkspace ws = paged_workspace(p, batch, heads, head_dim);
+  if (p.split) {
+    if (!aligned(workspace, 256)) return FPX_ERR_POINTER;
+    if (workspace_bytes < ws.total) return FPX_ERR_WORKSPACE;
+    char* base = static_cast<char*>(workspace);
+    a.part = as<float>(base);
+    a.part_ml = as<float>(base + ws.ml);
+    a.row_info = as<int>(base + ws.info);
+  }
+  {  // what is written meets nothing else, but q in place
+    using fpx::MemoryAxis;
+    const int64_t e = (int64_t)type_bytes(dtype);
+    const fpx::MemoryBlock query(q, e, MemoryAxis{batch, q_sb}, MemoryAxis{q_heads, q_sh},
+                                 MemoryAxis{head_dim, 1});
+    const fpx::MemoryBlock written[3] = {
+        {out, e, MemoryAxis{batch, o_sb}, MemoryAxis{q_heads, o_sh}, MemoryAxis{head_dim, 1}},
+        {lse, 4, MemoryAxis{batch * q_heads, 1}},
+        {p.split ? workspace : nullptr, 1, MemoryAxis{(int64_t)ws.total, 1}}};
+    const fpx::MemoryBlock table(block_table, 4, MemoryAxis{batch, table_sb},
+                                 MemoryAxis{table_sh > 0 ? heads : 1, table_sh},
+                                 MemoryAxis{(max_length + page_size - 1) / page_size, 1});
+    const fpx::MemoryBlock count(lengths, 4, MemoryAxis{batch, 1});
+    const CacheBlocks cache = cache_blocks(cache_dtype, cache_k, cache_v, k_scale, v_scale, pages,
+                                           heads, page_size, head_dim);
+    if (fpx::block_meets_itself(written[0])) return FPX_ERR_DIMS;
+    for (int i = 0; i < 3; ++i) {
+      if ((!(i == 0 && out == q) && fpx::blocks_meet(written[i], query)) ||
+          fpx::blocks_meet(written[i], table) || fpx::blocks_meet(written[i], count) ||
+          meets_cache(written[i], cache))
+        return FPX_ERR_DIMS;
+      for (int j = 0; j < i; ++j)
+        if (fpx::blocks_meet(written[i], written[j])) return FPX_ERR_DIMS;
+    }
+  }
+  a.q = q;
+  a.q_b = q_sb;
+  a.q_h = q_sh;
+  a.k = cache_k;
+  a.v = cache_v;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  a.table = block_table;
+  a.table_b = table_sb;
+  a.table_h = table_sh;
+  a.lengths = lengths;
+  a.out = out;
+  a.o_b = o_sb;
+  a.o_h = o_sh;
+  a.lse = lse;
+  a.scale_log2 = scale_log2;
+  a.weight_shift = cache_dtype == FPX_F16 ? fpx::kWeightShiftF16 : 0.0f;
+  a.pages = pages;
+  a.batch = (int)batch;
+  a.heads = heads;
+  a.group = q_heads / heads;
+  a.head_dim = head_dim;
+  a.max_length = (int)max_length;
+  a.window = window < (1 << 30) ? (int)window : 0;
+  a.dtype = dtype;
+  a.cache_dtype = cache_dtype;
+  a.groups = p.groups;
+  a.split = p.split;
+  a.unit = p.unit;
+  a.each = p.each;
+  a.tile_queries = p.tile_queries;
+  a.qtiles = p.qtiles;
+  a.query_tiles = p.query_tiles;
+  return status(fpx::launch_paged_attention(a, static_cast<hipStream_t>(stream)));
+}
+
 }  // namespace
 
 extern "C" {
@@ -1164,55 +1262,133 @@ int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb,
                         int64_t max_length, int64_t window, float scale, void* out, int64_t o_sb,
                         int64_t o_sh, float* lse, void* workspace, size_t workspace_bytes,
                         void* stream) {
-  fpx::PagedArgs a{};
+  return paged_impl(dtype, cache_dtype, q, q_sb, q_sh, cache_k, cache_v, k_scale, v_scale, pages,
+                    heads, page_size, head_dim, block_table, table_sb, 0, table_pages, lengths,
+                    batch, q_heads, max_length, window, scale, out, o_sb, o_sh, lse, workspace,
+                    workspace_bytes, stream);
+}
+
+int fpx_paged_attention_lists(int dtype, int cache_dtype, const void* q, int64_t q_sb, int64_t q_sh,
+                              const void* cache_k, const void* cache_v, const void* k_scale,
+                              const void* v_scale, int64_t pages, int heads, int page_size,
+                              int head_dim, const int32_t* block_table, int64_t table_sb,
+                              int64_t table_sh, int64_t table_pages, const int32_t* lengths,
+                              int64_t batch, int q_heads, int64_t max_length, float scale,
+                              void* out, int64_t o_sb, int64_t o_sh, float* lse, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  return paged_impl(dtype, cache_dtype, q, q_sb, q_sh, cache_k, cache_v, k_scale, v_scale, pages,
+                    heads, page_size, head_dim, block_table, table_sb, table_sh, table_pages,
+                    lengths, batch, q_heads, max_length, 0, scale, out, o_sb, o_sh, lse, workspace,
+                    workspace_bytes, stream);
+}
+
+size_t fpx_select_pages_workspace_bytes(int64_t batch, int heads, int page_size,
+                                        int64_t max_length, int count) {
+  if (batch < 0 || batch > kPagedMaxRows || heads < 1 || heads > kPagedMaxRows || count < 1 ||
+      page_size < 16 || page_size > 4096 || (page_size & (page_size - 1)) || max_length < 0 ||
+      max_length >= (1 << 30))
+    return 0;
+  const int64_t pages = (max_length + page_size - 1) / page_size;
+  if (pages <= count) return 256;
+  // (never the 256 that stand for none)
+  return (size_t)round_up((batch < 1 ? 1 : batch) * heads * pages * 4, 512);
+}
+
+int fpx_page_bounds(int cache_dtype, const void* cache_k, const void* k_scale, int64_t pages,
+                    int heads, int page_size, int head_dim, const int32_t* block_table,
+                    int64_t table_sb, int64_t table_pages, const int32_t* lengths, int64_t batch,
+                    int64_t max_length, int64_t fresh, void* bounds, void* stream) {
+  fpx::BoundsArgs a{};
   const int rc = cache_dims(cache_dtype, pages, heads, page_size, head_dim, &a.page_shift);
   if (rc != FPX_OK) return rc;
-  if (!row_type_ok(dtype) || (!is_coded(cache_dtype) && cache_dtype != dtype)) return FPX_ERR_DIMS;
-  const fpx::PagedPlan p =
-      paged_plan(dtype, cache_dtype, batch, q_heads, heads, head_dim, max_length, window);
-  if (p.groups == 0) return FPX_ERR_DIMS;
-  const int64_t row = 16 / (int64_t)type_bytes(dtype);
-  if (q_sb < 0 || q_sh < 0 || o_sb < 0 || o_sh < 0 || q_sb % row || q_sh % row || o_sb % row ||
-      o_sh % row)
+  if (batch < 0 || batch > kPagedMaxRows || max_length < 0 || max_length >= (1 << 30) || fresh < 1)
     return FPX_ERR_DIMS;
-  if (out == q && (o_sb != q_sb || o_sh != q_sh)) return FPX_ERR_DIMS;
-  if (table_sb < 0 || table_pages < (max_length + page_size - 1) / page_size) return FPX_ERR_DIMS;
-  const float scale_log2 = scale * fpx::kLog2e;
-  if (!(scale_log2 - scale_log2 == 0.0f)) return FPX_ERR_DIMS;  // infinite or NaN
-  if (batch == 0) return FPX_OK;
-  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(lengths, 4) ||
-      !aligned_or_null(lse, 4) || (max_length > 0 && !aligned(block_table, 4)) ||
-      !cache_pointers_ok(cache_dtype, cache_k, cache_v, k_scale, v_scale))
+  const int64_t most = (max_length + page_size - 1) / page_size;
+  if (table_sb < 0 || table_pages < most) return FPX_ERR_DIMS;
+  const int64_t each = fresh >= max_length ? most : (fresh - 1) / page_size + 2;
+  a.each = (int)(each < most ? each : most);
+  if (batch * heads * a.each > 0x7fffffff) return FPX_ERR_DIMS;
+  if (batch == 0 || a.each == 0) return FPX_OK;
+  if (!aligned(bounds, 16) || !aligned(lengths, 4) || !aligned(block_table, 4) ||
+      !cache_pointers_ok(cache_dtype, cache_k, cache_k, k_scale, k_scale))
     return FPX_ERR_POINTER;
-  const PagedWorkspace ws = paged_workspace(p, batch, heads, head_dim);
-  if (p.split) {
-    if (!aligned(workspace, 256)) return FPX_ERR_POINTER;
-    if (workspace_bytes < ws.total) return FPX_ERR_WORKSPACE;
-    char* base = static_cast<char*>(workspace);
-    a.part = as<float>(base);
-    a.part_ml = as<float>(base + ws.ml);
-    a.row_info = as<int>(base + ws.info);
-  }
-  {  // what is written meets nothing else, but q in place
+  {  // the bounds meet nothing else
     using fpx::MemoryAxis;
-    const int64_t e = (int64_t)type_bytes(dtype);
-    const fpx::MemoryBlock query(q, e, MemoryAxis{batch, q_sb}, MemoryAxis{q_heads, q_sh},
-                                 MemoryAxis{head_dim, 1});
-    const fpx::MemoryBlock written[3] = {
-        {out, e, MemoryAxis{batch, o_sb}, MemoryAxis{q_heads, o_sh}, MemoryAxis{head_dim, 1}},
-        {lse, 4, MemoryAxis{batch * q_heads, 1}},
-        {p.split ? workspace : nullptr, 1, MemoryAxis{(int64_t)ws.total, 1}}};
-    const fpx::MemoryBlock table(block_table, 4, MemoryAxis{batch, table_sb},
-                                 MemoryAxis{(max_length + page_size - 1) / page_size, 1});
-    const fpx::MemoryBlock count(lengths, 4, MemoryAxis{batch, 1});
-    const CacheBlocks cache = cache_blocks(cache_dtype, cache_k, cache_v, k_scale, v_scale, pages,
+    const int64_t e = (int64_t)type_bytes(is_coded(cache_dtype) ? FPX_BF16 : cache_dtype);
+    const fpx::MemoryBlock out(bounds, e, MemoryAxis{pages * heads, 2 * head_dim},
+                               MemoryAxis{2 * head_dim, 1});
+    const CacheBlocks cache = cache_blocks(cache_dtype, cache_k, cache_k, k_scale, k_scale, pages,
                                            heads, page_size, head_dim);
-    if (fpx::block_meets_itself(written[0])) return FPX_ERR_DIMS;
-    for (int i = 0; i < 3; ++i) {
-      if ((!(i == 0 && out == q) && fpx::blocks_meet(written[i], query)) ||
-          fpx::blocks_meet(written[i], table) || fpx::blocks_meet(written[i], count) ||
-          meets_cache(written[i], cache))
-        return FPX_ERR_DIMS;
+    const fpx::MemoryBlock table(block_table, 4, MemoryAxis{batch, table_sb}, MemoryAxis{most, 1});
+    const fpx::MemoryBlock count(lengths, 4, MemoryAxis{batch, 1});
+    if (meets_cache(out, cache) || fpx::blocks_meet(out, table) || fpx::blocks_meet(out, count))
+      return FPX_ERR_DIMS;
+  }
+  a.k = cache_k;
+  a.k_scale = k_scale;
+  a.bounds = bounds;
+  a.table = block_table;
+  a.table_b = table_sb;
+  a.lengths = lengths;
+  a.pages = pages;
+  a.batch = (int)batch;
+  a.heads = heads;
+  a.head_dim = head_dim;
+  a.max_length = (int)max_length;
+  a.fresh = (int)(fresh < (1 << 30) ? fresh : (1 << 30));
+  a.cache_dtype = cache_dtype;
+  return status(fpx::launch_page_bounds(a, static_cast<hipStream_t>(stream)));
+}
+
+int fpx_select_pages(int dtype, int bounds_dtype, const void* q, int64_t q_sb, int64_t q_sh,
+                     int q_heads, const void* bounds, int64_t pages, int heads, int page_size,
+                     int head_dim, const int32_t* block_table, int64_t table_sb,
+                     int64_t table_pages, const int32_t* lengths, int64_t batch,
+                     int64_t max_length, int count, int sinks, int recent, int32_t* index,
+                     int32_t* table_out, int32_t* lengths_out, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  fpx::SelectArgs a{};
+  if (!row_type_ok(dtype) || !row_type_ok(bounds_dtype)) return FPX_ERR_DIMS;
+  const int rc = cache_dims(bounds_dtype, pages, heads, page_size, head_dim, &a.page_shift);
+  if (rc != FPX_OK) return rc;
+  const size_t need =
+      fpx_select_pages_workspace_bytes(batch, heads, page_size, max_length, count);
+  if (need == 0 || q_heads < heads || q_heads % heads || q_heads > kPagedMaxRows ||
+      batch * q_heads > kPagedMaxRows)
+    return FPX_ERR_DIMS;
+  if (sinks < 0 || recent < 1 || sinks > count - recent || count > ((1 << 30) - 1) / page_size)
+    return FPX_ERR_DIMS;
+  const int64_t row = 16 / (int64_t)type_bytes(dtype);
+  if (q_sb < 0 || q_sh < 0 || q_sb % row || q_sh % row) return FPX_ERR_DIMS;
+  const int64_t most = (max_length + page_size - 1) / page_size;
+  if (table_sb < 0 || table_pages < most) return FPX_ERR_DIMS;
+  if (batch * heads * ((most + 63) / 64) > 0x7fffffff) return FPX_ERR_DIMS;
+  if (batch == 0) return FPX_OK;
+  if (!aligned(q, 16) || !aligned(bounds, 16) || !aligned(lengths, 4) || !aligned(index, 4) ||
+      !aligned(table_out, 4) || !aligned(lengths_out, 4) ||
+      (max_length > 0 && !aligned(block_table, 4)))
+    return FPX_ERR_POINTER;
+  if (most > count) {
+    if (!aligned(workspace, 256)) return FPX_ERR_POINTER;
+    if (workspace_bytes < need) return FPX_ERR_WORKSPACE;
+  }
+  {  // what is written meets nothing else
+    using fpx::MemoryAxis;
+    const int64_t e = (int64_t)type_bytes(dtype), f = (int64_t)type_bytes(bounds_dtype);
+    const int64_t chosen = batch * heads * (int64_t)count;
+    const fpx::MemoryBlock written[4] = {
+        {index, 4, MemoryAxis{chosen, 1}},
+        {table_out, 4, MemoryAxis{chosen, 1}},
+        {lengths_out, 4, MemoryAxis{batch, 1}},
+        {most > count ? workspace : nullptr, 1, MemoryAxis{(int64_t)need, 1}}};
+    const fpx::MemoryBlock read[4] = {
+        {q, e, MemoryAxis{batch, q_sb}, MemoryAxis{q_heads, q_sh}, MemoryAxis{head_dim, 1}},
+        {bounds, f, MemoryAxis{pages * heads, 2 * head_dim}, MemoryAxis{2 * head_dim, 1}},
+        {block_table, 4, MemoryAxis{batch, table_sb}, MemoryAxis{most, 1}},
+        {lengths, 4, MemoryAxis{batch, 1}}};
+    for (int i = 0; i < 4; ++i) {
+      for (const fpx::MemoryBlock& r : read)
+        if (fpx::blocks_meet(written[i], r)) return FPX_ERR_DIMS;
       for (int j = 0; j < i; ++j)
         if (fpx::blocks_meet(written[i], written[j])) return FPX_ERR_DIMS;
     }
@@ -1220,36 +1396,27 @@ int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb,
   a.q = q;
   a.q_b = q_sb;
   a.q_h = q_sh;
-  a.k = cache_k;
-  a.v = cache_v;
-  a.k_scale = k_scale;
-  a.v_scale = v_scale;
+  a.bounds = bounds;
   a.table = block_table;
   a.table_b = table_sb;
   a.lengths = lengths;
-  a.out = out;
-  a.o_b = o_sb;
-  a.o_h = o_sh;
-  a.lse = lse;
-  a.scale_log2 = scale_log2;
-  a.weight_shift = cache_dtype == FPX_F16 ? fpx::kWeightShiftF16 : 0.0f;
+  a.ranks = static_cast<uint32_t*>(workspace);
+  a.index = index;
+  a.table_out = table_out;
+  a.lengths_out = lengths_out;
   a.pages = pages;
+  a.max_pages = most;
   a.batch = (int)batch;
   a.heads = heads;
   a.group = q_heads / heads;
   a.head_dim = head_dim;
   a.max_length = (int)max_length;
-  a.window = window < (1 << 30) ? (int)window : 0;
+  a.count = count;
+  a.sinks = sinks;
+  a.recent = recent;
   a.dtype = dtype;
-  a.cache_dtype = cache_dtype;
-  a.groups = p.groups;
-  a.split = p.split;
-  a.unit = p.unit;
-  a.each = p.each;
-  a.tile_queries = p.tile_queries;
-  a.qtiles = p.qtiles;
-  a.query_tiles = p.query_tiles;
-  return status(fpx::launch_paged_attention(a, static_cast<hipStream_t>(stream)));
+  a.bounds_dtype = bounds_dtype;
+  return status(fpx::launch_select_pages(a, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -465,6 +465,45 @@ struct AppendArgs {
 
 hipError_t launch_cache_append(const AppendArgs& args, hipStream_t stream);
 
+// ------------------------------------------------------- pages worth attending to
+// Bounds of the keys of pages, [pages][heads][2: lowest, highest][head_dim], of the
+// cache's type, or BF16 where that is coded.
+struct BoundsArgs {
+  const void* k;        // the cache's keys (paged_layout.hpp)
+  const void* k_scale;
+  void* bounds;
+  const int32_t* table;  // pages of a sequence at table + b*table_b
+  int64_t table_b;
+  const int32_t* lengths;  // [batch]
+  int64_t pages;
+  int batch, heads, head_dim, page_shift, max_length;
+  int fresh;       // newest tokens of each sequence, on pages whose bounds are formed
+  int each;        // pages that hold them, at most
+  int cache_dtype;  // FPX_*
+};
+
+hipError_t launch_page_bounds(const BoundsArgs& args, hipStream_t stream);
+
+struct SelectArgs {
+  const void* q;     // [batch][heads * group] rows at q + b*q_b + h*q_h
+  int64_t q_b, q_h;
+  const void* bounds;
+  const int32_t* table;
+  int64_t table_b;
+  const int32_t* lengths;
+  uint32_t* ranks;        // [batch][heads][max_pages]
+  int32_t* index;         // [batch][heads][count]: places in the sequence, ascending
+  int32_t* table_out;     // the same pages' numbers
+  int32_t* lengths_out;   // [batch]: keys on them
+  int64_t pages, max_pages;  // max_pages: that max_length takes
+  int batch, heads, group, head_dim, page_shift, max_length;
+  int count, sinks, recent;
+  int dtype, bounds_dtype;  // FPX_*
+  int tiles;  // of a row's pages, set by launch_select_pages
+};
+
+hipError_t launch_select_pages(const SelectArgs& args, hipStream_t stream);
+
 // --------------------------------------- attention of new tokens over the cache
 constexpr int kPagedMaxGroups = 1024;  // work-groups that share a row
 constexpr int kPagedUnit = 512;        // keys of a small call's unit

@@ -46,7 +46,9 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
       plain cache has q's type, an 8- or 4-bit one takes float32 (over 8 bits below
       2^110: products with the codes are formed in FP32), bfloat16 and float16 queries.
     * ``block_table`` int32 ``[batch, p]``: a sequence's pages in order.
-      Entries past its length, or before its window, are not used.
+      Entries past its length, or before its window, are not used.  ``[batch, heads, p]``:
+      a list for each cache head, of as many keys for all heads of a sequence
+      (``page_selection.select_pages``), without a window.
     * ``lengths`` int32 ``[batch]``, up to ``max_length`` (default: what the
       table holds; a captured graph keeps the bound it was captured with).
     * ``scale`` of the scores, ``head_dim ** -0.5`` by default; ``window`` > 0
@@ -77,12 +79,17 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
                          f"got {tuple(q.shape)}")
     if k.dtype not in CODED_DTYPES and k.dtype != q.dtype:
         raise ValueError(f"a {k.dtype} cache needs {k.dtype} queries")
-    if (block_table.dim() != 2 or block_table.shape[0] != batch or block_table.dtype != torch.int32
-            or block_table.get_device() != device):
-        raise ValueError("block_table must be int32 [batch, pages] on q's device")
+    lists = block_table.dim() == 3
+    if (block_table.shape[:-1] != ((batch, heads) if lists else (batch,))
+            or block_table.dtype != torch.int32 or block_table.get_device() != device):
+        raise ValueError("block_table must be int32 [batch, pages] or [batch, heads, pages] on "
+                         "q's device")
+    if lists and window:
+        raise ValueError("lists of pages for each head take no window")
     if lengths.shape != (batch,) or lengths.dtype != torch.int32 or lengths.get_device() != device:
         raise ValueError("lengths must be int32 [batch] on q's device")
-    held = block_table.shape[1] * page_size
+    columns = block_table.shape[-1]
+    held = columns * page_size
     if max_length is None:
         max_length = held
     if not 0 <= max_length <= held or window < 0:
@@ -92,7 +99,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
         raise ValueError("no autograd graph is recorded: detach q (and out)")
     if not _aligned_rows(q):
         q = q.clone(memory_format=torch.contiguous_format)
-    if block_table.stride(1) != 1 and block_table.shape[1] > 1:
+    if block_table.stride(-1) != 1 and columns > 1:
         block_table = block_table.contiguous()
     if not lengths.is_contiguous():
         lengths = lengths.contiguous()
@@ -117,10 +124,11 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
         # calls that may overlap share it
         workspace = q.new_empty(size, dtype=torch.uint8)
     code = _native.launch(
-        device, lib.fpx_paged_attention, ROW_DTYPES[q.dtype], CACHE_DTYPES[k.dtype],
+        device, lib.fpx_paged_attention_lists if lists else lib.fpx_paged_attention,
+        ROW_DTYPES[q.dtype], CACHE_DTYPES[k.dtype],
         q.data_ptr(), *q.stride()[:2], *cache.pointers(), pages, heads, page_size, head_dim,
-        block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-        lengths.data_ptr(), batch, q_heads, max_length, window,
+        block_table.data_ptr(), *block_table.stride()[:-1], columns, lengths.data_ptr(), batch,
+        q_heads, max_length, *(() if lists else (window,)),
         head_dim ** -0.5 if scale is None else scale, out.data_ptr(), *out.stride()[:2],
         None if lse is None else lse.data_ptr(),
         None if workspace is None else workspace.data_ptr(), size)

@@ -477,6 +477,66 @@ int fpx_paged_attention(int dtype, int cache_dtype, const void* q, int64_t q_sb,
                         int64_t o_sh, float* lse, void* workspace, size_t workspace_bytes,
                         void* stream);
 
+/* fpx_paged_attention with a list of pages for each cache head: sequence b's keys for
+ * cache head h lie, in the list's order, on pages block_table[b*table_sb + h*table_sh +
+ * i], and lengths[b] is how many a head's list holds (the same for all heads; every page
+ * but the last is full).  No window; otherwise as there, with its workspace for window 0.
+ * table_sh = 0: one list for all heads. */
+int fpx_paged_attention_lists(int dtype, int cache_dtype, const void* q, int64_t q_sb,
+                              int64_t q_sh, const void* cache_k, const void* cache_v,
+                              const void* k_scale, const void* v_scale, int64_t pages, int heads,
+                              int page_size, int head_dim, const int32_t* block_table,
+                              int64_t table_sb, int64_t table_sh, int64_t table_pages,
+                              const int32_t* lengths, int64_t batch, int q_heads,
+                              int64_t max_length, float scale, void* out, int64_t o_sb,
+                              int64_t o_sh, float* lse, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/* Bounds of the keys of a paged cache's pages: bounds [pages][heads][2][head_dim], the
+ * least and the greatest value of each channel over a page's keys as fpx_cache_read
+ * gives them in FP32, in the cache's type (exact) or, for a coded cache, BF16 (the
+ * next number not above the least, not below the greatest).  Formed for the pages that
+ * hold the last `fresh` tokens of each sequence, from the keys below its length; other
+ * bounds are left alone, as is a sequence whose length is negative or above max_length
+ * and an entry that names a page outside the cache.  A NaN makes its channel's bounds
+ * NaN.  bounds overlaps nothing else (status 2).  No counterpart in the reference.
+ * Supported: the cache's sizes; max_length < 2^30; fresh >= 1; batch up to 2^20; nothing
+ * is launched when batch or max_length is 0.  bounds is 16-byte aligned; other arguments
+ * as fpx_paged_attention's. */
+int fpx_page_bounds(int cache_dtype, const void* cache_k, const void* k_scale, int64_t pages,
+                    int heads, int page_size, int head_dim, const int32_t* block_table,
+                    int64_t table_sb, int64_t table_pages, const int32_t* lengths, int64_t batch,
+                    int64_t max_length, int64_t fresh, void* bounds, void* stream);
+
+/* Bytes of workspace fpx_select_pages needs; 0 for unsupported sizes, 256 where it uses
+ * none (every page fits the selection): its workspace may then be null. */
+size_t fpx_select_pages_workspace_bytes(int64_t batch, int heads, int page_size,
+                                        int64_t max_length, int count);
+
+/* The `count` pages of each sequence that one new token's queries attend to, for each
+ * cache head: the first `sinks` and the last `recent` pages, then those with the highest
+ *   score = max over the head's queries of sum_c max(q_c lo_c, q_c hi_c),
+ * an upper bound of the page's q . k; it is summed in FP64 and rounded to FP32, the
+ * lower of equal pages comes first, NaN (and a page outside the cache) above all.
+ *   dtype         of q, as fpx_paged_attention's; q_heads a multiple of heads
+ *   bounds_dtype  of bounds (fpx_page_bounds): FPX_F32, FPX_BF16 or FPX_F16
+ *   index         [batch][heads][count]: the pages' places in the sequence, ascending
+ *   table_out     the same pages' numbers: fpx_paged_attention_lists' block_table with
+ *                 table_sb = heads * count, table_sh = count
+ *   lengths_out   [batch]: the keys on them.  A sequence of no more than count pages has
+ *                 all of them; entries past a sequence's pages are -1.  A length that is
+ *                 negative or above max_length gives -1, whose attention is NaN.
+ * Outputs and workspace overlap nothing else (status 2).
+ * Supported: fpx_page_bounds' sizes; 1 <= recent, 0 <= sinks, sinks + recent <= count,
+ * count * page_size < 2^30; batch * q_heads up to 2^20. */
+int fpx_select_pages(int dtype, int bounds_dtype, const void* q, int64_t q_sb, int64_t q_sh,
+                     int q_heads, const void* bounds, int64_t pages, int heads, int page_size,
+                     int head_dim, const int32_t* block_table, int64_t table_sb,
+                     int64_t table_pages, const int32_t* lengths, int64_t batch,
+                     int64_t max_length, int count, int sinks, int recent, int32_t* index,
+                     int32_t* table_out, int32_t* lengths_out, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
