@@ -499,7 +499,7 @@ struct SelectArgs {
   int batch, heads, group, head_dim, page_shift, max_length;
   int count, sinks, recent;
   int dtype, bounds_dtype;  // FPX_*
-  int tiles;  // of a row's pages, set by launch_select_pages
+  int chunks;  // work-groups that share a row's pages, set by launch_select_pages
 };
 
 hipError_t launch_select_pages(const SelectArgs& args, hipStream_t stream);

@@ -20,11 +20,10 @@
 namespace fpx {
 namespace {
 
-typedef double f64x4 __attribute__((ext_vector_type(4)));
-
 constexpr int kBoundsThreads = 256;
 constexpr int kScoreThreads = 256;
-constexpr int kScorePages = 64;  // of a work-group
+constexpr int kScorePages = 64;    // of a work-group at a time
+constexpr int kScoreGroups = 768;  // work-groups, about
 
 __device__ __forceinline__ float lesser(float x, float y) {
   return __builtin_elementwise_minimum(x, y);
@@ -147,74 +146,152 @@ __device__ __forceinline__ uint32_t rank_of(float score) {
   return bits >> 31 ? ~bits : bits | 0x80000000u;
 }
 
-// The ranks of 64 pages of one sequence for one cache head, 16 to a wave: queries are
-// the rows of the products, pages the columns.  A lane holds a quarter of its page's
-// (and of its query's) channels, as they lie in memory: in which order the channels are
-// contracted is no matter as long as both sides have the same.
-template <typename Q, typename T, int kDim>
+// The ranks of a sequence's pages for one cache head, 64 at a time.  In a product the
+// pages are the columns (one to a lane % 16), four queries the rows, and the lane groups
+// (lane / 16) the four channels that are contracted.  Each of the four waves contracts a
+// quarter of the channels for all 64 pages, so that it converts its part of the queries
+// to FP64 once for them (8 VGPRs a channel of eight queries), and the waves' sums meet in
+// LDS.  kTiles: fours of queries at a time; kMany: there are more than those.
+template <typename Q, typename T, int kDim, int kTiles, bool kMany>
 __global__ __launch_bounds__(kScoreThreads) void page_rank_kernel(SelectArgs a) {
-  constexpr int kQuarter = kDim / 4;
-  typedef Q QVec __attribute__((ext_vector_type(8)));
-  typedef T TVec __attribute__((ext_vector_type(8)));
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int kEach = kDim / 16;  // channels of a lane
+  constexpr int kParts = kScorePages / 16;
+  typedef Q QVec __attribute__((ext_vector_type(kEach)));
+  typedef T TVec __attribute__((ext_vector_type(kEach)));
+  __shared__ double sums[2][4][kParts][kTiles][kWave];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
-  const int64_t seq_head = blockIdx.x / (unsigned)a.tiles;
-  const int tile = (int)(blockIdx.x - seq_head * a.tiles);
-  const int64_t b = seq_head / a.heads;
-  const int h = (int)(seq_head - b * a.heads);
+  // heads fastest: their bounds of a page lie next to each other
+  const int h = (int)(blockIdx.x % (unsigned)a.heads);
+  const int seq_chunk = (int)(blockIdx.x / (unsigned)a.heads);
+  const int b = seq_chunk / a.chunks;
+  int tile = seq_chunk - b * a.chunks;
   const KeyRange range = key_range(__builtin_amdgcn_readfirstlane(a.lengths[b]), a.max_length, 0);
   const int total = (range.end + (1 << a.page_shift) - 1) >> a.page_shift;  // pages
-  const int page0 = tile * kScorePages + wave * 16;
-  if (total <= a.count || page0 >= total) return;  // (all pages are taken: no ranks)
-  const int at = min(page0 + col, total - 1);
-  const int page = a.table[b * a.table_b + at];
-  const bool ok = page_valid(page, a.pages);
-  const T* lo = static_cast<const T*>(a.bounds) +
-                ((int64_t)(ok ? page : 0) * a.heads + h) * 2 * kDim + g * kQuarter;
-  float best = -__builtin_inff();
-  for (int q0 = 0; q0 < a.group; q0 += 16) {
-    // (rows past the head's last query have its first one again)
-    const int qi = q0 + col < a.group ? q0 + col : 0;
-    const Q* q = static_cast<const Q*>(a.q) + b * a.q_b + ((int64_t)h * a.group + qi) * a.q_h +
-                 g * kQuarter;
-    f64x4 above = {0.0, 0.0, 0.0, 0.0}, below = {0.0, 0.0, 0.0, 0.0};
+  if (total <= a.count || tile * kScorePages >= total) return;  // (all taken: no ranks)
+  const int channel = (4 * wave + g) * kEach;
+  const int32_t* table = a.table + b * a.table_b;
+  int page[kParts], later[kParts];  // of the tile after this one, and of that after it
+  TVec lo[kParts], hi[kParts];
+  uint32_t inside = 0;  // bit p: the lane's page of part p is one of the cache
+  auto look_up = [&](int at_tile, int* to) {  // (past the last page the last again)
 #pragma unroll
-    for (int s = 0; s < kQuarter; s += 8) {
-      const QVec x = *reinterpret_cast<const QVec*>(q + s);
-      const TVec l = *reinterpret_cast<const TVec*>(lo + s);
-      const TVec u = *reinterpret_cast<const TVec*>(lo + kDim + s);
+    for (int p = 0; p < kParts; ++p)
+      to[p] = table[min(at_tile * kScorePages + 16 * p + col, total - 1)];
+  };
+  auto load = [&](int p) {
+    const bool ok = page_valid(page[p], a.pages);
+    inside = (inside & ~(1u << p)) | (uint32_t)ok << p;
+    const T* edge = static_cast<const T*>(a.bounds) +
+                    ((int64_t)(ok ? page[p] : 0) * a.heads + h) * 2 * kDim + channel;
+    lo[p] = *reinterpret_cast<const TVec*>(edge);
+    hi[p] = *reinterpret_cast<const TVec*>(edge + kDim);
+  };
+  double above[kTiles][kEach], below[kTiles][kEach];  // max(q, 0) and min(q, 0)
+  auto load_queries = [&](int q0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float y = (float)x[j];
-        above = __builtin_amdgcn_mfma_f64_16x16x4f64((double)greater(y, 0.0f), (double)(float)u[j],
-                                                     above, 0, 0, 0);
-        below = __builtin_amdgcn_mfma_f64_16x16x4f64((double)lesser(y, 0.0f), (double)(float)l[j],
-                                                     below, 0, 0, 0);
+    for (int t = 0; t < kTiles; ++t) {
+      // (rows past the head's last query have its first one again)
+      int qi = q0 + 4 * t + (lane & 3);
+      qi = qi < a.group ? qi : 0;
+      const Q* q = static_cast<const Q*>(a.q) + b * a.q_b + ((int64_t)h * a.group + qi) * a.q_h;
+      const QVec x = *reinterpret_cast<const QVec*>(q + channel);
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        above[t][j] = (double)greater((float)x[j], 0.0f);
+        below[t][j] = (double)lesser((float)x[j], 0.0f);
       }
     }
+  };
+  // ---- tile by tile.  A part's bounds for the next tile are asked for as soon as this
+  // tile's are used, and its page numbers a tile before that.  (Past the last tile the
+  // last page is read again: the loads are not branched around, which would make every
+  // wait one for all of them.)
+  look_up(tile, page);
+  look_up(tile + a.chunks, later);
+  if (!kMany) load_queries(0);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) best = greater(best, (float)(above[r] + below[r]));
+  for (int p = 0; p < kParts; ++p) load(p);
+  for (int buffer = 0;; buffer ^= 1) {
+    const uint32_t now_inside = inside;
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) page[p] = later[p];
+    look_up(tile + 2 * a.chunks, later);
+    float best = -__builtin_inff();  // of the page part `wave`
+    for (int q0 = 0;; q0 += 4 * kTiles) {
+      const bool last = !kMany || q0 + 4 * kTiles >= a.group;
+      if (kMany) load_queries(q0);
+#pragma unroll
+      for (int p = 0; p < kParts; ++p) {
+        // (several sums, so that an instruction need not wait for the one before)
+        double up[kTiles] = {}, down[kTiles] = {};
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+          const double u = (double)(float)hi[p][j], l = (double)(float)lo[p][j];
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t)
+            up[t] = __builtin_amdgcn_mfma_f64_4x4x4f64(above[t][j], u, up[t], 0, 0, 0);
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t)
+            down[t] = __builtin_amdgcn_mfma_f64_4x4x4f64(below[t][j], l, down[t], 0, 0, 0);
+        }
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) sums[buffer][wave][p][t][lane] = up[t] + down[t];
+        if (last) load(p);
+      }
+      // (one barrier a turn: what the next one writes is the other buffer)
+      __syncthreads();
+      // (lane group g has query 4t + g)
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        double x = sums[buffer][0][wave][t][lane];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) x += sums[buffer][w][wave][t][lane];
+        best = greater(best, (float)x);
+      }
+      if (last) break;
+      buffer ^= 1;
+    }
+    best = greater(best, __shfl_xor(best, 16));
+    best = greater(best, __shfl_xor(best, 32));
+    const int at = tile * kScorePages + 16 * wave + col;
+    if (g == 0 && at < total) {
+      const bool forced = at < a.sinks || at >= total - a.recent;
+      const bool ok = (now_inside >> wave) & 1;
+      a.ranks[((int64_t)b * a.heads + h) * a.max_pages + at] =
+          forced ? kForced : ok ? rank_of(best) : kNanRank;
+    }
+    tile += a.chunks;
+    if (tile * kScorePages >= total) break;
   }
-  // the queries of the other lane groups
-  best = greater(best, __shfl_xor(best, 16));
-  best = greater(best, __shfl_xor(best, 32));
-  if (g == 0 && page0 + col < total) {
-    const bool forced = at < a.sinks || at >= total - a.recent;
-    a.ranks[seq_head * a.max_pages + at] = forced ? kForced : ok ? rank_of(best) : kNanRank;
-  }
+}
+
+// Sum over the lanes up to and with this one: rows of 16 lanes by shifts, then the rows
+// before by broadcasts of their last lanes.
+__device__ __forceinline__ int wave_prefix(int x) {
+  auto add = [](int v, int shifted) { return v + shifted; };
+  x = add(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true));  // row_shr:1
+  x = add(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true));
+  x = add(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true));
+  x = add(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true));
+  x = add(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));  // row_bcast:15
+  x = add(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));  // row_bcast:31
+  return x;
 }
 
 // The `count` pages of highest rank of one (sequence, cache head), in the order of the
 // sequence: the rank of the last of them is found byte by byte from the counts of each
-// byte's values, then every thread lists its run of pages.
-template <int kThreads>
+// byte's values, then every thread lists its run of pages.  kKeys: pages of a thread,
+// whose ranks (and numbers) it keeps in registers; 0: any number, read again every time.
+template <int kThreads, int kKeys>
 __global__ __launch_bounds__(kThreads) void page_select_kernel(SelectArgs a) {
   constexpr int kWaves = kThreads / kWave;
-  constexpr int kCopies = 8;  // of the counts: neighbouring lanes' ranks begin alike
-  __shared__ uint32_t counts[256][kCopies];
+  constexpr int kCopies = 8;  // of the counts: neighbouring pages' ranks begin alike
+  __shared__ __attribute__((aligned(16))) int counts[2][256][kCopies];
   __shared__ uint32_t found[2];
   __shared__ int wave_sum[2][kWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t seq_head = blockIdx.x;
   const int64_t b = seq_head / a.heads;
   const KeyRange range = key_range(__builtin_amdgcn_readfirstlane(a.lengths[b]), a.max_length, 0);
@@ -224,93 +301,105 @@ __global__ __launch_bounds__(kThreads) void page_select_kernel(SelectArgs a) {
   const int32_t* table = a.table + b * a.table_b;
   int32_t* index = a.index + seq_head * a.count;
   int32_t* out = a.table_out + seq_head * a.count;
-  if (threadIdx.x == 0 && seq_head == b * a.heads)
+  if (tid == 0 && seq_head == b * a.heads)
     a.lengths_out[b] = range.valid ? range.end - ((total - kept) << a.page_shift) : -1;
-  for (int i = kept + threadIdx.x; i < a.count; i += kThreads) index[i] = out[i] = -1;
+  for (int i = kept + tid; i < a.count; i += kThreads) index[i] = out[i] = -1;
   if (total <= a.count) {
-    for (int i = threadIdx.x; i < total; i += kThreads) {
+    for (int i = tid; i < total; i += kThreads) {
       index[i] = i;
       out[i] = table[i];
     }
     return;
   }
   const uint32_t* ranks = a.ranks + seq_head * a.max_pages;
-  uint32_t least = 0, mask = 0;  // the bytes found so far
-  uint32_t wanted = (uint32_t)a.count;  // pages among those that begin with them
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256 * kCopies; i += kThreads)
-      counts[i / kCopies][i % kCopies] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < total; i += kThreads) {
-      const uint32_t r = ranks[i];
-      if (((r ^ least) & mask) == 0) atomicAdd(&counts[(r >> shift) & 255][lane % kCopies], 1u);
+  const int per = kKeys > 0 ? kKeys : (total + kThreads - 1) / kThreads;
+  const int begin = min(total, tid * per), end = min(total, begin + per);
+  uint32_t held[kKeys > 0 ? kKeys : 1];
+  int page[kKeys > 0 ? kKeys : 1];
+#pragma unroll
+  for (int k = 0; k < kKeys; ++k) {
+    held[k] = begin + k < end ? ranks[begin + k] : 0;
+    page[k] = begin + k < end ? table[begin + k] : 0;
+  }
+  // f(place, rank, number of the place among the thread's) for the thread's pages
+  auto each = [&](auto f) {
+    if constexpr (kKeys > 0) {
+#pragma unroll
+      for (int k = 0; k < kKeys; ++k)
+        if (begin + k < end) f(begin + k, held[k], k);
+    } else {
+      for (int i = begin; i < end; ++i) f(i, ranks[i], 0);
     }
+  };
+  for (int i = tid; i < 256 * kCopies; i += kThreads) counts[0][i / kCopies][i % kCopies] = 0;
+  __syncthreads();
+  uint32_t least = 0, mask = 0;  // the bytes found so far
+  int wanted = a.count;          // pages among those that begin with them
+  for (int turn = 0; turn < 4; ++turn) {
+    const int shift = 24 - 8 * turn;
+    int(*now)[kCopies] = counts[turn & 1];
+    each([&](int, uint32_t r, int) {
+      if (((r ^ least) & mask) == 0) atomicAdd(&now[(r >> shift) & 255][lane % kCopies], 1);
+    });
+    if (turn < 3)
+      for (int i = tid; i < 256 * kCopies; i += kThreads)
+        counts[(turn + 1) & 1][i / kCopies][i % kCopies] = 0;
     __syncthreads();
     if (wave == 0) {
-      // lane l has the values 4l to 4l + 3; `upto`: pages of its and all higher ones
-      uint32_t own[4], sum = 0;
+      // lane l has the values 255 - 4l to 252 - 4l
+      int own[4], sum = 0;
 #pragma unroll
-      for (int v = 3; v >= 0; --v) {
+      for (int v = 0; v < 4; ++v) {
         own[v] = 0;
 #pragma unroll
-        for (int k = 0; k < kCopies; ++k) own[v] += counts[4 * lane + v][k];
+        for (int k = 0; k < kCopies; ++k) own[v] += now[255 - 4 * lane - v][k];
         sum += own[v];
       }
-      uint32_t upto = sum;
-#pragma unroll
-      for (int d = 1; d < kWave; d *= 2) {
-        const uint32_t above = __shfl_down(upto, d);
-        upto += lane + d < kWave ? above : 0;
-      }
-      uint32_t above = upto - sum;
+      const int upto = wave_prefix(sum);
+      int above = upto - sum;
       if (above < wanted && wanted <= upto) {
-        int v = 3;
-        while (v > 0 && above + own[v] < wanted) above += own[v--];
-        found[0] = (uint32_t)(4 * lane + v);
-        found[1] = wanted - above;
+        int v = 0;
+#pragma unroll
+        for (int u = 0; u < 3; ++u)
+          if (v == u && above + own[u] < wanted) {
+            above += own[u];
+            v = u + 1;
+          }
+        found[0] = (uint32_t)(255 - 4 * lane - v);
+        found[1] = (uint32_t)(wanted - above);
       }
     }
     __syncthreads();
     least |= found[0] << shift;
-    wanted = found[1];
+    wanted = (int)found[1];
     mask |= 255u << shift;
   }
   // ---- pages of a higher rank, and the first `wanted` of that rank itself
-  const int per = (total + kThreads - 1) / kThreads;
-  const int begin = min(total, (int)threadIdx.x * per), end = min(total, begin + per);
-  int higher = 0, equal = 0;
-  for (int i = begin; i < end; ++i) {
-    higher += ranks[i] > least;
-    equal += ranks[i] == least;
-  }
-  int before[2] = {higher, equal};
+  int own[2] = {0, 0}, before[2];
+  each([&](int, uint32_t r, int) {
+    own[0] += r > least;
+    own[1] += r == least;
+  });
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-      const int x = __shfl_up(before[w], d);
-      before[w] += lane >= d ? x : 0;
-    }
+    before[w] = wave_prefix(own[w]);
     if (lane == kWave - 1) wave_sum[w][wave] = before[w];
+    before[w] -= own[w];
   }
   __syncthreads();
-  before[0] -= higher;
-  before[1] -= equal;
   for (int w = 0; w < wave; ++w) {
     before[0] += wave_sum[0][w];
     before[1] += wave_sum[1][w];
   }
-  for (int i = begin; i < end; ++i) {
-    const uint32_t r = ranks[i];
-    const bool taken = r > least || (r == least && before[1] < (int)wanted);
-    if (taken) {
-      const int to = before[0] + min(before[1], (int)wanted);
+  each([&](int i, uint32_t r, int k) {
+    if (r > least || (r == least && before[1] < wanted)) {
+      const int to = before[0] + min(before[1], wanted);
       index[to] = i;
-      out[to] = table[i];
+      out[to] = kKeys > 0 ? page[k] : table[i];
     }
     before[0] += r > least;
     before[1] += r == least;
-  }
+  });
 }
 
 template <typename C, typename T>
@@ -324,13 +413,23 @@ hipError_t launch_bounds_type(const BoundsArgs& a, unsigned groups, hipStream_t 
   return hipGetLastError();
 }
 
+template <typename Q, typename T, int kDim>
+void launch_rank_dim(const SelectArgs& a, unsigned groups, hipStream_t stream) {
+  if (a.group <= 4)
+    page_rank_kernel<Q, T, kDim, 1, false><<<groups, kScoreThreads, 0, stream>>>(a);
+  else if (a.group <= 8)
+    page_rank_kernel<Q, T, kDim, 2, false><<<groups, kScoreThreads, 0, stream>>>(a);
+  else
+    page_rank_kernel<Q, T, kDim, 2, true><<<groups, kScoreThreads, 0, stream>>>(a);
+}
+
 template <typename Q, typename T>
 void launch_rank_type(const SelectArgs& a, unsigned groups, hipStream_t stream) {
   switch (a.head_dim) {
-    case 32: page_rank_kernel<Q, T, 32><<<groups, kScoreThreads, 0, stream>>>(a); break;
-    case 64: page_rank_kernel<Q, T, 64><<<groups, kScoreThreads, 0, stream>>>(a); break;
-    case 128: page_rank_kernel<Q, T, 128><<<groups, kScoreThreads, 0, stream>>>(a); break;
-    default: page_rank_kernel<Q, T, 256><<<groups, kScoreThreads, 0, stream>>>(a); break;
+    case 32: launch_rank_dim<Q, T, 32>(a, groups, stream); break;
+    case 64: launch_rank_dim<Q, T, 64>(a, groups, stream); break;
+    case 128: launch_rank_dim<Q, T, 128>(a, groups, stream); break;
+    default: launch_rank_dim<Q, T, 256>(a, groups, stream); break;
   }
 }
 
@@ -361,8 +460,12 @@ hipError_t launch_select_pages(const SelectArgs& args, hipStream_t stream) {
   SelectArgs a = args;
   const int64_t rows = (int64_t)a.batch * a.heads;
   if (a.max_pages > a.count) {
-    a.tiles = (int)((a.max_pages + kScorePages - 1) / kScorePages);
-    const unsigned groups = (unsigned)(rows * a.tiles);
+    // work-groups of a row: as many as there are tiles, but not many more in all than
+    // the card holds at once
+    const int64_t tiles = (a.max_pages + kScorePages - 1) / kScorePages;
+    const int64_t most = (kScoreGroups + rows - 1) / rows;
+    a.chunks = (int)(tiles < most ? tiles : most);
+    const unsigned groups = (unsigned)(rows * a.chunks);
     switch (a.dtype) {
       case 0: launch_rank<float>(a, groups, stream); break;
       case 1: launch_rank<__bf16>(a, groups, stream); break;
@@ -371,10 +474,17 @@ hipError_t launch_select_pages(const SelectArgs& args, hipStream_t stream) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  if (a.max_pages > 1024)
-    page_select_kernel<1024><<<(unsigned)rows, 1024, 0, stream>>>(a);
+  const unsigned groups = (unsigned)rows;
+  if (a.max_pages <= 256)
+    page_select_kernel<256, 1><<<groups, 256, 0, stream>>>(a);
+  else if (a.max_pages <= 1024)
+    page_select_kernel<256, 4><<<groups, 256, 0, stream>>>(a);
+  else if (a.max_pages <= 2048)
+    page_select_kernel<1024, 2><<<groups, 1024, 0, stream>>>(a);
+  else if (a.max_pages <= 8192)
+    page_select_kernel<1024, 8><<<groups, 1024, 0, stream>>>(a);
   else
-    page_select_kernel<256><<<(unsigned)rows, 256, 0, stream>>>(a);
+    page_select_kernel<1024, 0><<<groups, 1024, 0, stream>>>(a);
   return hipGetLastError();
 }
 

@@ -214,12 +214,12 @@ def test_selection(q_type, kind, q_heads, heads, dim, page):
         assert torch.equal(got.index, again.index) and torch.equal(got.table, again.table)
 
 
-@pytest.mark.parametrize("total", [1023, 1024, 1025, 4096, 20011])
+@pytest.mark.parametrize("total", [255, 256, 257, 1023, 1024, 1025, 2048, 2049, 8192, 8193, 20011])
 def test_many_pages(total):
     bounds = PageBounds(random_bounds(total, 2, 64, BF16, 5), 16)
     table = torch.randperm(total, generator=torch.Generator().manual_seed(1)).int()[None].cuda()
     q = torch.randn(1, 8, 64, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
-    for n in (total * 16, total * 16 - 15, 600 * 16):
+    for n in (total * 16, total * 16 - 15, min(total, 600) * 16):
         lengths = torch.tensor([n], dtype=torch.int32)
         for count in (1, 100, total // 2, total - 1):
             got = select_pages(q, bounds, table, lengths.cuda(), count)
