@@ -187,8 +187,32 @@ __device__ __forceinline__ uint32_t codes4_bf16(uint32_t w, uint32_t scale, int 
   return __builtin_bit_cast(uint32_t, x);
 }
 
-template <typename Q, typename C, int D, int QT>
+// Lanes 8 to 15 of each row of 16 take x, from 8 lanes below, the others keep own; and the
+// lower eight from 8 lanes above.
+template <typename X>
+__device__ __forceinline__ X upper_from(X own, X x) {
+  return __builtin_bit_cast(X, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, own),
+                                                           __builtin_bit_cast(int, x), 0x118, 0xF,
+                                                           0xC, false));
+}
+template <typename X>
+__device__ __forceinline__ X lower_from(X own, X x) {
+  return __builtin_bit_cast(X, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, own),
+                                                           __builtin_bit_cast(int, x), 0x108, 0xF,
+                                                           0x3, false));
+}
+__device__ __forceinline__ float halves_sum(float v) { return v + dpp<0x128>(v); }  // row_ror:8
+__device__ __forceinline__ float halves_max(float v) { return fmaxf(v, dpp<0x128>(v)); }
+
+// kColumns: of the products, to a query.  Up to eight query heads leave half of the 16
+// columns idle, and half of what the softmax computes unused.  A 4-bit cache, whose codes
+// take as many instructions to decode as 8 bits and half the time to read, gives each
+// query two: in the first product the second column has the query's second term, in the
+// second one the weights' second term, and in between its lanes have the other 16 of a
+// tile's 32 keys.
+template <typename Q, typename C, int D, int QT, int kColumns_>
 struct PagedTraits {
+  static constexpr int kColumns = kColumns_;
   static constexpr bool kF32 = std::is_same_v<C, float>;
   static constexpr bool kFp4 = std::is_same_v<C, Fp4Cache>;
   // a scale to each row, which its score and its weight are multiplied by
@@ -207,6 +231,10 @@ struct PagedTraits {
                                           : std::is_same_v<Q, _Float16> ? 2 : 3;
   // terms a weight is split into: what the output's type needs
   static constexpr int kWeightTerms = kCoded && std::is_same_v<Q, float> ? 3 : 2;
+  // products for them
+  static constexpr int kTermColumns = (kTerms + kColumns - 1) / kColumns;
+  static constexpr int kWeightColumns = (kWeightTerms + kColumns - 1) / kColumns;
+  static constexpr int kSlots = 4 * kHalves / kColumns;  // keys of a lane in the softmax
   // K: pieces of kPiece bytes a lane holds of its key's row (16 where a
   // quarter of the row has them)
   static constexpr int kPiece = kRow / 4 < 16 ? kRow / 4 : 16;
@@ -232,7 +260,7 @@ struct PagedTraits {
   // below).  Halves one after the other, which kept all steps' queries from one to the
   // next, spilled up to 217: 16 sequences of 2001 to 16384 keys, 8 heads of 256, FP32
   // queries over INT8, 195 us, 125 now; BF16, 8192 keys, 122 and 113.
-  static constexpr int kQueryWords = QT * kQuerySteps * kTerms * 4;
+  static constexpr int kQueryWords = QT * kQuerySteps * kTermColumns * 4;
   static constexpr int kTileWords = kHalves * (kRow / 16 + 4 * kParts * kPartWords);
   static constexpr bool kQueryLds =
       kQueryWords + kTileWords + QT * kChannels * 4 + (kFp4 ? 32 : kCoded ? 16 : 0) > 160;
@@ -246,9 +274,10 @@ struct Segment {
   KeyRange range;
 };
 
-template <typename Q, typename C, int D, int QT>
+template <typename Q, typename C, int D, int QT, int kColumns>
 __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(PagedArgs a) {
-  using T = PagedTraits<Q, C, D, QT>;
+  using T = PagedTraits<Q, C, D, QT, kColumns>;
+  static_assert(kColumns == 1 || (T::kFp4 && QT == 1), "two columns: 4-bit caches");
   constexpr int kHalves = T::kHalves;
   __shared__ u32x4_t query_lds[T::kQueryLds ? T::kQueryWords / 4 : 1][kWave];
   typedef float Vec __attribute__((ext_vector_type(T::kVec)));
@@ -467,10 +496,10 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
   // the head's last query compute its first one again; their columns are not
   // stored.)
   constexpr int kRaw = T::kF32 ? 1 : (int)sizeof(Q) / 2;  // 16-byte words of a step
-  constexpr int kQuads = T::kQuerySteps * T::kTerms;      // of a query tile, term by term
+  constexpr int kQuads = T::kQuerySteps * T::kTermColumns;  // of a query tile, term by term
   auto load_step = [&](const Segment& x, int t, int st, u32x4_t* raw) {
     const int g = lane >> 4;
-    const int qi = (x.qtile * QT + t) * 16 + (lane & 15);
+    const int qi = (x.qtile * QT + t) * 16 + (lane & (16 / kColumns - 1));
     const Q* q = static_cast<const Q*>(a.q) + x.seq * a.q_b +
                  (int64_t)(x.head * a.group + (qi < a.group ? qi : 0)) * a.q_h;
     const int d = T::kPieceChannels * (4 * (st / T::kPieceSteps) + g) + 8 * (st % T::kPieceSteps);
@@ -575,8 +604,15 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
       const int t = step_of(i) / T::kQuerySteps, st = step_of(i) % T::kQuerySteps;
       u32x4_t terms[T::kTerms];
       split_step(raw[i], terms);
+      if constexpr (kColumns == 2 && T::kTerms > 1) {
 #pragma unroll
-      for (int p = 0; p < T::kTerms; ++p) {
+        for (int p = 0; p < T::kTermColumns; ++p)
+          terms[p] = col < 8                  ? terms[2 * p]
+                     : 2 * p + 1 < T::kTerms ? terms[2 * p + 1 < T::kTerms ? 2 * p + 1 : 0]
+                                             : u32x4_t{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int p = 0; p < T::kTermColumns; ++p) {
         if constexpr (!T::kQueryLds)
           qw[t * kQuads + p * T::kQuerySteps + st] = terms[p];
         else if (t < QT)
@@ -648,7 +684,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
 #pragma unroll
           for (int t = 0; t < QT; ++t) {
 #pragma unroll
-            for (int p = T::kTerms - 1; p >= 0; --p) {  // the smallest term first
+            for (int p = T::kTermColumns - 1; p >= 0; --p) {  // the smallest term first
               const u32x4_t y = query(t * kQuads + p * T::kQuerySteps + st);
 #pragma unroll
               for (int u = 0; u < kHalves; ++u) {
@@ -668,7 +704,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
       // ---- factors of the scores in log2 units; keys outside the range left out
       const bool edge = key0 < range.first || key0 + T::kTile > range.end;
       float f[kHalves][T::kScaled ? 4 : 1];
-      uint32_t unseen = 0;  // bit 4u + r
+      uint32_t unseen = 0;  // a bit to a slot
 #pragma unroll
       for (int u = 0; u < kHalves; ++u)
 #pragma unroll
@@ -685,7 +721,10 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
           for (int r = 0; r < 4; ++r) {
             const int key = key0 + 16 * u + 4 * g + r;
             if (key >= range.first && key < range.end) continue;
-            unseen |= 1u << (4 * u + r);
+            if constexpr (kColumns == 1)
+              unseen |= 1u << (4 * u + r);
+            else if (u % 2 == (col >> 3))  // (the lane's half of each 32 keys)
+              unseen |= 1u << (4 * (u / 2) + r);
             // what the page holds there may be NaN: it must not meet a weight
             // of zero
             if constexpr (T::kScaled) vs[u][r] = 0.0f;
@@ -698,19 +737,36 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
         if ((n + 1) % kAhead == 0) take_pages(look_up(cur, n + 1));
         load_k(cur, n + 1);
       }
-      // ---- online softmax; a lane's l covers its own group's keys
-      float p[QT][kHalves * 4];
+      // ---- two columns: the terms' scores added up, and of each 32 keys 16 to a column
+      if constexpr (kColumns == 2) {
+#pragma unroll
+        for (int u = 0; u < kHalves; u += 2)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if constexpr (T::kTerms == 1) {
+              s[0][u / 2][r] = upper_from(s[0][u][r], s[0][u + 1][r]);
+            } else {
+              // (both formed by all lanes, whose neighbours read them)
+              const float first = halves_sum(s[0][u][r]), second = halves_sum(s[0][u + 1][r]);
+              s[0][u / 2][r] = col < 8 ? first : second;
+            }
+          }
+      }
+      // ---- online softmax; a lane's l covers its own keys
+      float p[QT][T::kSlots];
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
         float top = -__builtin_inff();
 #pragma unroll
-        for (int u = 0; u < kHalves; ++u)
+        for (int u = 0; u < T::kSlots / 4; ++u)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float x = s[t][u][r] * f[u][T::kScaled ? r : 0];
             top = fmaxf(top, unseen & (1u << (4 * u + r)) ? -__builtin_inff() : x);
           }
-        const float next = fmaxf(m[t], groups_max(top));
+        top = groups_max(top);
+        if constexpr (kColumns == 2) top = halves_max(top);
+        const float next = fmaxf(m[t], top);
         const float ref = next == -__builtin_inff() ? 0.0f : next;
         if (__any(next > m[t])) {
           const float alpha = exp2_fast(m[t] - ref);
@@ -720,7 +776,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
         }
         m[t] = next;
 #pragma unroll
-        for (int u = 0; u < kHalves; ++u)
+        for (int u = 0; u < T::kSlots / 4; ++u)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             // one rounding from the product to the exponent
@@ -747,19 +803,32 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
       } else {
 #pragma unroll
         for (int k0 = 0; k0 < kHalves * 4; k0 += 8) {  // the lane's eight of 32 keys
-          u32x4_t weights[QT][T::kWeightTerms];
+          u32x4_t weights[QT][T::kWeightColumns];
 #pragma unroll
           for (int t = 0; t < QT; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 4 / kColumns; ++i) {
               uint32_t terms[T::kWeightTerms];
-              const float p0 = p[t][k0 + 2 * i], p1 = p[t][k0 + 2 * i + 1];
+              const int slot = k0 / kColumns + 2 * i;
+              const float p0 = p[t][slot], p1 = p[t][slot + 1];
               if constexpr (T::kWeightTerms == 3)
                 split_weights_exactly(p0, p1, terms);
               else
                 split_weights<T::kF16, !T::kCoded>(p0, p1, terms[0], terms[1]);
+              if constexpr (kColumns == 1) {
 #pragma unroll
-              for (int w = 0; w < T::kWeightTerms; ++w) weights[t][w][i] = terms[w];
+                for (int w = 0; w < T::kWeightTerms; ++w) weights[t][w][i] = terms[w];
+              } else {
+                // the lower lanes have the first 16 keys' weights, the upper the others':
+                // the first column gets the first term of both, the second the second
+                weights[t][0][i] = upper_from(terms[0], terms[1]);
+                weights[t][0][2 + i] = lower_from(terms[1], terms[0]);
+                if constexpr (T::kWeightTerms == 3) {
+                  const uint32_t none = 0;
+                  weights[t][1][i] = col < 8 ? terms[2] : none;
+                  weights[t][1][2 + i] = lower_from(none, terms[2]);
+                }
+              }
             }
           uint32_t pair[8];  // two channels of them
 #pragma unroll
@@ -784,7 +853,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
 #pragma unroll
-              for (int w = T::kWeightTerms - 1; w >= 0; --w) {  // the smallest term first
+              for (int w = T::kWeightColumns - 1; w >= 0; --w) {  // the smallest term first
                 if constexpr (T::kF16)
                   o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
                       __builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, weights[t][w]),
@@ -821,6 +890,13 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       l[t] = any_bad ? __builtin_nanf("") : groups_sum(l[t]);
+      if constexpr (kColumns == 2) {
+        l[t] = halves_sum(l[t]);
+#pragma unroll
+        for (int c = 0; c < T::kChannels; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[t][c][r] = halves_sum(o[t][c][r]);
+      }
       if (g == 0) {
         wave_m[wave][t * 16 + col] = m[t];
         wave_l[wave][t * 16 + col] = l[t];
@@ -921,10 +997,16 @@ hipError_t launch_paged_dim(const PagedArgs& a, hipStream_t stream) {
   // all be missing on the same XCDs), or equal shares
   const dim3 groups = a.each > 0 ? dim3(a.heads * a.qtiles, a.batch, a.each) : dim3(a.groups);
   if (a.query_tiles == 1) {
-    paged_attention_kernel<Q, C, D, 1><<<groups, kPagedThreads, 0, stream>>>(a);
+    if constexpr (std::is_same_v<C, Fp4Cache>) {
+      if (a.group <= 8) {
+        paged_attention_kernel<Q, C, D, 1, 2><<<groups, kPagedThreads, 0, stream>>>(a);
+        return hipGetLastError();
+      }
+    }
+    paged_attention_kernel<Q, C, D, 1, 1><<<groups, kPagedThreads, 0, stream>>>(a);
   } else {
     if constexpr (D <= 128)
-      paged_attention_kernel<Q, C, D, 2><<<groups, kPagedThreads, 0, stream>>>(a);
+      paged_attention_kernel<Q, C, D, 2, 1><<<groups, kPagedThreads, 0, stream>>>(a);
     else
       return hipErrorInvalidValue;
   }

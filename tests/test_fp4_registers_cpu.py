@@ -18,8 +18,9 @@ def reports():
 
 
 def test_no_kernel_spills(reports):
-    # three query types; 32, 64 and 128 channels with one and two query tiles, 256 with one
-    assert len(reports[0]) == 21
+    # three query types; four widths with one query tile, of one and two columns a query,
+    # 32, 64 and 128 channels with two
+    assert len(reports[0]) == 3 * (4 * 2 + 3)
     for name, (registers, scratch, spilled) in reports[0].items():
         assert (scratch, spilled) == (0, 0), (name, registers, scratch, spilled)
 
