@@ -11,9 +11,10 @@
 // Memory bounds a prompt (each row is read once and written once), a launch's start a
 // step.  A work-group takes `tt` tokens: their factors (cos, sin) go into LDS once and
 // serve all heads, their slots are looked up meanwhile.  head_dim / 8 neighbouring lanes
-// take a row, 8 channels each, so that a row's maximum needs no LDS; the other half of a
-// pair (half layout) is loaded a second time by the lane that needs it, which costs L1
-// reads only, where an exchange would tie the lanes to the layout and to rotary_dim.
+// take a row, 8 channels each, so that a row's maximum needs no LDS; where the whole head
+// is turned, half as many take two eights half a row apart, which are each other's pairs
+// in the half layout.  Otherwise (a part turned) the other half of a pair is loaded a
+// second time by the lane that needs it.
 #include "cache_rows.hpp"
 #include "common.hpp"
 #include "kernels.hpp"
@@ -24,15 +25,23 @@ namespace fpx {
 namespace {
 
 constexpr int kAppendThreads = 256;
-constexpr int kAppendBatch = 3;            // rows in flight per thread
+constexpr int kAppendBatch = 3;            // vectors in flight per thread, about
 constexpr int kAppendTokens = 16;          // at most, per work-group
 constexpr int kAppendMaxGroups = 1 << 22;  // work-groups of a launch
 constexpr int kAppendAngles = 2048;        // (token, pair) factors held in LDS: 16 KB
 
-// kVec: rows are 16-byte aligned, and so are the halves of a turned part.
-template <typename S, typename C, int kDim, bool kVec>
+// How a thread takes a row's channels: eight one by one from any address; eight as a
+// vector, those of the other halves of their pairs read besides (rows 16-byte aligned, and
+// the halves of the turned part); or two vectors, between which pairs are complete.
+enum AppendMode { kAppendEach, kAppendVector, kAppendPairs };
+
+template <typename S, typename C, int kDim, int kMode, bool kStream>
 __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(AppendArgs a) {
-  constexpr int kGroup = kDim / 8;  // threads of a row
+  constexpr bool kVec = kMode != kAppendEach;
+  constexpr int kSpans = kMode == kAppendPairs ? 2 : 1;
+  constexpr int kApart = kDim / kSpans;
+  constexpr int kGroup = kDim / 8 / kSpans;  // threads of a row
+  constexpr int kBatch = kAppendBatch - kSpans + 1;
   __shared__ float2 factor[kAppendAngles];
   __shared__ const S* row_in[kAppendTokens][3];  // of q, k and v
   __shared__ S* row_out[kAppendTokens];
@@ -89,11 +98,11 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(AppendArgs
   const int rows = a.q_heads + 2 * a.heads;  // of a token
   const int items = tokens * rows * kGroup;
   const int c = (threadIdx.x & (kGroup - 1)) * 8;
-  for (int base = threadIdx.x; base < items; base += kAppendThreads * kAppendBatch) {
-    Eight<S> x[kAppendBatch], y[kAppendBatch];
-    int token[kAppendBatch], head[kAppendBatch], which[kAppendBatch];
+  for (int base = threadIdx.x; base < items; base += kAppendThreads * kBatch) {
+    Eight<S> x[kBatch][kSpans], y[kBatch];
+    int token[kBatch], head[kBatch], which[kBatch];
 #pragma unroll
-    for (int r = 0; r < kAppendBatch; ++r) {
+    for (int r = 0; r < kBatch; ++r) {
       const int item = base + r * kAppendThreads;
       which[r] = -1;
       if (item >= items) continue;
@@ -106,42 +115,60 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(AppendArgs
       head[r] = h;
       which[r] = w;
       const S* src = row_in[tl][w] + h * (w == 0 ? a.in_h[0] : w == 1 ? a.in_h[1] : a.in_h[2]);
-      if constexpr (kVec)
-        x[r].template load<false>(src + c);
-      else
-        x[r].load_each(src + c);
-      if (w < 2 && !a.interleaved && c < a.rot) {  // the pairs' other channels
-        if constexpr (kVec) {
-          y[r].template load<false>(src + (c < half ? c + half : c - half));
-        } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int d = c + i;
-            y[r].x[i] = d < a.rot ? src[d < half ? d + half : d - half] : (S)0.0f;
+      for (int s = 0; s < kSpans; ++s) {
+        if constexpr (kVec)
+          x[r][s].template load<kStream>(src + c + s * kApart);
+        else
+          x[r][s].load_each(src + c + s * kApart);
+      }
+      if constexpr (kMode != kAppendPairs) {
+        if (w < 2 && !a.interleaved && c < a.rot) {  // the pairs' other channels
+          if constexpr (kVec) {
+            y[r].template load<false>(src + (c < half ? c + half : c - half));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int d = c + i;
+              y[r].x[i] = d < a.rot ? src[d < half ? d + half : d - half] : (S)0.0f;
+            }
           }
         }
       }
     }
 #pragma unroll
-    for (int r = 0; r < kAppendBatch; ++r) {
+    for (int r = 0; r < kBatch; ++r) {
       if (which[r] < 0) continue;
       const int64_t row = first_row[token[r]];
       if (which[r] > 0 && row < 0) continue;  // (for all lanes of a row alike)
-      float v[8];
+      float v[kSpans][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = x[r].value(i);
-      if (which[r] < 2 && c < a.rot) {
+      for (int s = 0; s < kSpans; ++s)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[s][i] = x[r][s].value(i);
+      if (which[r] < 2) {
         const float2* f = factor + token[r] * half;
         if (a.interleaved) {
 #pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            if (c + i >= a.rot) break;
-            const float2 cs = f[(c + i) >> 1];
-            const float x1 = v[i], x2 = v[i + 1];
-            v[i] = __builtin_fmaf(x1, cs.x, -(x2 * cs.y));
-            v[i + 1] = __builtin_fmaf(x2, cs.x, x1 * cs.y);
+          for (int s = 0; s < kSpans; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+              const int d = c + s * kApart + i;
+              if (d >= a.rot) break;
+              const float2 cs = f[d >> 1];
+              const float x1 = v[s][i], x2 = v[s][i + 1];
+              v[s][i] = __builtin_fmaf(x1, cs.x, -(x2 * cs.y));
+              v[s][i + 1] = __builtin_fmaf(x2, cs.x, x1 * cs.y);
+            }
+        } else if constexpr (kMode == kAppendPairs) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 cs = f[c + i];
+            const float x1 = v[0][i], x2 = v[1][i];
+            v[0][i] = __builtin_fmaf(x1, cs.x, -(x2 * cs.y));
+            v[1][i] = __builtin_fmaf(x2, cs.x, x1 * cs.y);
           }
-        } else {
+        } else if (c < a.rot) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int d = c + i;
@@ -149,31 +176,37 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(AppendArgs
             const bool lower = d < half;
             const float2 cs = f[lower ? d : d - half];
             const float other = y[r].value(i) * cs.y;
-            v[i] = __builtin_fmaf(v[i], cs.x, lower ? -other : other);
+            v[0][i] = __builtin_fmaf(v[0][i], cs.x, lower ? -other : other);
           }
         }
       }
       if (which[r] == 0) {
-        S* dst = row_out[token[r]] + head[r] * a.out_h + c;
-        Eight<S> out;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) out.set(i, v[i]);
-        if constexpr (kVec)
-          out.store(dst);
-        else
-          out.store_each(dst);
+        for (int s = 0; s < kSpans; ++s) {
+          S* dst = row_out[token[r]] + head[r] * a.out_h + c + s * kApart;
+          Eight<S> out;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) out.set(i, v[s][i]);
+          if constexpr (kVec)
+            out.store(dst);
+          else
+            out.store_each(dst);
+        }
         continue;
       }
       const int64_t at = row + ((int64_t)head[r] << a.page_shift);
       const int w = which[r] - 1;
       void* cache = w ? a.cache[1] : a.cache[0];
       if constexpr (kCoded<C>) {
-        put_codes<C, kDim>(v, cache, w ? a.cache_scale[1] : a.cache_scale[0], at, c);
+        put_codes<C, kDim, kSpans>(v, cache, w ? a.cache_scale[1] : a.cache_scale[0], at, c);
       } else {
-        Eight<C> out;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) out.set(i, v[i]);
-        out.store(held_at<C, kDim>(cache, at, c));
+        for (int s = 0; s < kSpans; ++s) {
+          Eight<C> out;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) out.set(i, v[s][i]);
+          out.store(held_at<C, kDim>(cache, at, c + s * kApart));
+        }
       }
     }
   }
@@ -200,16 +233,25 @@ hipError_t launch_append_dim(AppendArgs& a, hipStream_t stream) {
              (uint64_t)(a.out_b | a.out_n | a.out_h) * sizeof(S);
   // (the vectors of 8 channels lie in one half of a turned part each, too)
   const bool vec = bytes % 16 == 0 && (a.interleaved || half % 8 == 0);
+  const bool pairs = vec && (a.interleaved || a.rot == kDim);
+  // rows that no cache holds anyway are streamed past them
+  const bool once = a.total * rows * kDim * (int64_t)sizeof(S) >= kStreamBytes;
   hipError_t e = hipSuccess;
   for (int64_t first = 0; first < a.total && e == hipSuccess;
        first += (int64_t)kAppendMaxGroups * a.tt) {
     a.first = first;
     const int64_t left = (a.total - first + a.tt - 1) / a.tt;
     const unsigned blocks = (unsigned)(left < kAppendMaxGroups ? left : kAppendMaxGroups);
-    if (vec)
-      cache_append_kernel<S, C, kDim, true><<<blocks, kAppendThreads, 0, stream>>>(a);
+    if (pairs && once)
+      cache_append_kernel<S, C, kDim, kAppendPairs, true><<<blocks, kAppendThreads, 0, stream>>>(a);
+    else if (pairs)
+      cache_append_kernel<S, C, kDim, kAppendPairs, false>
+          <<<blocks, kAppendThreads, 0, stream>>>(a);
+    else if (vec)
+      cache_append_kernel<S, C, kDim, kAppendVector, false>
+          <<<blocks, kAppendThreads, 0, stream>>>(a);
     else
-      cache_append_kernel<S, C, kDim, false><<<blocks, kAppendThreads, 0, stream>>>(a);
+      cache_append_kernel<S, C, kDim, kAppendEach, false><<<blocks, kAppendThreads, 0, stream>>>(a);
     e = hipGetLastError();
   }
   return e;

@@ -110,12 +110,12 @@ __device__ __forceinline__ float scale_at(const void* scale, int64_t row, int c)
   }
 }
 
-// The maximum over kGroup neighbouring lanes (4 to 32, aligned), in each.
+// The maximum over kGroup neighbouring lanes (2 to 32, aligned), in each.
 template <int kGroup>
 __device__ __forceinline__ float group_max(float v) {
   auto mx = [](float x, float y) { return __builtin_elementwise_maximum(x, y); };
   v = mx(v, dpp<0xB1>(v));                          // lane pairs
-  v = mx(v, dpp<0x4E>(v));                          // quads
+  if constexpr (kGroup >= 4) v = mx(v, dpp<0x4E>(v));    // quads
   if constexpr (kGroup >= 8) v = mx(v, dpp<0x141>(v));   // 8 lanes
   if constexpr (kGroup >= 16) v = mx(v, dpp<0x140>(v));  // 16 lanes
   if constexpr (kGroup >= 32) {
@@ -224,28 +224,47 @@ __device__ __forceinline__ void decode(uint32_t codes, float scale, float* x) {
   x[7] = d[1];
 }
 
-// Channels c to c + 7 of a row into a coded cache: v their values, the row's kDim / 8
-// threads neighbouring lanes that all call this.
-template <typename C, int kDim>
-__device__ __forceinline__ void put_codes(const float* v, void* cache, void* scales, int64_t row,
-                                          int c) {
-  float top = 0.0f;
+// Channels c + s * kDim / kSpans to c + 7 + s * kDim / kSpans of a row into a coded
+// cache, v[s] their values; the row's kDim / 8 / kSpans threads are neighbouring lanes that
+// all call this, with c from 0 in steps of 8.
+template <typename C, int kDim, int kSpans>
+__device__ __forceinline__ void put_codes(const float (*v)[8], void* cache, void* scales,
+                                          int64_t row, int c) {
+  constexpr int kLanes = kDim / 8 / kSpans;
+  float top[kSpans];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = __builtin_elementwise_maximum(top, __builtin_fabsf(v[i]));
-  Held<C> y;
-  if constexpr (__is_same(C, Fp4)) {
-    const uint32_t e = block_scale(group_max<kBlock4 / 8>(top));
-    y.x = encode4(v, e);
-    if (c % kBlock4 == 0)
-      static_cast<uint8_t*>(scales)[(row * kDim + c) / kBlock4] = (uint8_t)e;
-  } else {
-    top = group_max<kDim / 8>(top);
-    float scale, factor;
-    row_scale<C>(top, scale, factor);
-    y.x = encode<C>(v, factor);
+  for (int s = 0; s < kSpans; ++s) {
+    top[s] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      top[s] = __builtin_elementwise_maximum(top[s], __builtin_fabsf(v[s][i]));
+  }
+  // (a 4-bit block of 32 channels is that of four lanes, or of all spans of fewer)
+  constexpr bool kTogether = !__is_same(C, Fp4) || kLanes < kBlock4 / 8;
+  if constexpr (kTogether) {
+#pragma unroll
+    for (int s = 1; s < kSpans; ++s) top[0] = __builtin_elementwise_maximum(top[0], top[s]);
+    top[0] = group_max<kLanes>(top[0]);
+  }
+  float scale = 0.0f, factor = 0.0f;
+  if constexpr (!__is_same(C, Fp4)) {
+    row_scale<C>(top[0], scale, factor);
     if (c == 0) static_cast<float*>(scales)[row] = scale;
   }
-  y.store(held_at<C, kDim>(cache, row, c));
+#pragma unroll
+  for (int s = 0; s < kSpans; ++s) {
+    const int at = c + s * (kDim / kSpans);
+    Held<C> y;
+    if constexpr (__is_same(C, Fp4)) {
+      const uint32_t e = block_scale(kTogether ? top[0] : group_max<kBlock4 / 8>(top[s]));
+      y.x = encode4(v[s], e);
+      if (at % kBlock4 == 0)
+        static_cast<uint8_t*>(scales)[(row * kDim + at) / kBlock4] = (uint8_t)e;
+    } else {
+      y.x = encode<C>(v[s], factor);
+    }
+    y.store(held_at<C, kDim>(cache, row, at));
+  }
 }
 
 }  // namespace fpx

@@ -1289,7 +1289,7 @@ size_t fpx_select_pages_workspace_bytes(int64_t batch, int heads, int page_size,
       max_length >= (1 << 30))
     return 0;
   const int64_t pages = (max_length + page_size - 1) / page_size;
-  if (pages <= count) return 256;
+  if (pages <= count || pages <= fpx::kFewPages) return 256;
   // (never the 256 that stand for none)
   return (size_t)round_up((batch < 1 ? 1 : batch) * heads * pages * 4, 512);
 }
@@ -1368,7 +1368,7 @@ int fpx_select_pages(int dtype, int bounds_dtype, const void* q, int64_t q_sb, i
       !aligned(table_out, 4) || !aligned(lengths_out, 4) ||
       (max_length > 0 && !aligned(block_table, 4)))
     return FPX_ERR_POINTER;
-  if (most > count) {
+  if (need > 256) {
     if (!aligned(workspace, 256)) return FPX_ERR_POINTER;
     if (workspace_bytes < need) return FPX_ERR_WORKSPACE;
   }
@@ -1380,7 +1380,7 @@ int fpx_select_pages(int dtype, int bounds_dtype, const void* q, int64_t q_sb, i
         {index, 4, MemoryAxis{chosen, 1}},
         {table_out, 4, MemoryAxis{chosen, 1}},
         {lengths_out, 4, MemoryAxis{batch, 1}},
-        {most > count ? workspace : nullptr, 1, MemoryAxis{(int64_t)need, 1}}};
+        {need > 256 ? workspace : nullptr, 1, MemoryAxis{(int64_t)need, 1}}};
     const fpx::MemoryBlock read[4] = {
         {q, e, MemoryAxis{batch, q_sb}, MemoryAxis{q_heads, q_sh}, MemoryAxis{head_dim, 1}},
         {bounds, f, MemoryAxis{pages * heads, 2 * head_dim}, MemoryAxis{2 * head_dim, 1}},

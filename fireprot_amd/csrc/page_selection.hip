@@ -146,30 +146,33 @@ __device__ __forceinline__ uint32_t rank_of(float score) {
   return bits >> 31 ? ~bits : bits | 0x80000000u;
 }
 
+// Pages of sequence b: 0 where its length does not fit the call.
+__device__ __forceinline__ int pages_of(const SelectArgs& a, int b) {
+  const KeyRange range = key_range(__builtin_amdgcn_readfirstlane(a.lengths[b]), a.max_length, 0);
+  return (int)(((int64_t)range.end + (1 << a.page_shift) - 1) >> a.page_shift);
+}
+
 // The ranks of a sequence's pages for one cache head, 64 at a time.  In a product the
 // pages are the columns (one to a lane % 16), four queries the rows, and the lane groups
 // (lane / 16) the four channels that are contracted.  Each of the four waves contracts a
 // quarter of the channels for all 64 pages, so that it converts its part of the queries
 // to FP64 once for them (8 VGPRs a channel of eight queries), and the waves' sums meet in
 // LDS.  kTiles: fours of queries at a time; kMany: there are more than those.
-template <typename Q, typename T, int kDim, int kTiles, bool kMany>
-__global__ __launch_bounds__(kScoreThreads) void page_rank_kernel(SelectArgs a) {
+template <int kTiles>
+using Sums = double[2][4][kScorePages / 16][kTiles][kWave];
+
+// put(place, rank) for the pages of tiles `tile`, `tile` + step and so on of the `total`
+// pages of sequence b, cache head h.
+template <typename Q, typename T, int kDim, int kTiles, bool kMany, typename Put>
+__device__ __forceinline__ void rank_tiles(const SelectArgs& a, Sums<kTiles>& sums, int b, int h,
+                                           int total, int tile, int step, Put put) {
   constexpr int kEach = kDim / 16;  // channels of a lane
   constexpr int kParts = kScorePages / 16;
   typedef Q QVec __attribute__((ext_vector_type(kEach)));
   typedef T TVec __attribute__((ext_vector_type(kEach)));
-  __shared__ double sums[2][4][kParts][kTiles][kWave];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
-  // heads fastest: their bounds of a page lie next to each other
-  const int h = (int)(blockIdx.x % (unsigned)a.heads);
-  const int seq_chunk = (int)(blockIdx.x / (unsigned)a.heads);
-  const int b = seq_chunk / a.chunks;
-  int tile = seq_chunk - b * a.chunks;
-  const KeyRange range = key_range(__builtin_amdgcn_readfirstlane(a.lengths[b]), a.max_length, 0);
-  const int total = (range.end + (1 << a.page_shift) - 1) >> a.page_shift;  // pages
-  if (total <= a.count || tile * kScorePages >= total) return;  // (all taken: no ranks)
   const int channel = (4 * wave + g) * kEach;
   const int32_t* table = a.table + b * a.table_b;
   int page[kParts], later[kParts];  // of the tile after this one, and of that after it
@@ -209,7 +212,7 @@ __global__ __launch_bounds__(kScoreThreads) void page_rank_kernel(SelectArgs a) 
   // last page is read again: the loads are not branched around, which would make every
   // wait one for all of them.)
   look_up(tile, page);
-  look_up(tile + a.chunks, later);
+  look_up(tile + step, later);
   if (!kMany) load_queries(0);
 #pragma unroll
   for (int p = 0; p < kParts; ++p) load(p);
@@ -217,7 +220,7 @@ __global__ __launch_bounds__(kScoreThreads) void page_rank_kernel(SelectArgs a) 
     const uint32_t now_inside = inside;
 #pragma unroll
     for (int p = 0; p < kParts; ++p) page[p] = later[p];
-    look_up(tile + 2 * a.chunks, later);
+    look_up(tile + 2 * step, later);
     float best = -__builtin_inff();  // of the page part `wave`
     for (int q0 = 0;; q0 += 4 * kTiles) {
       const bool last = !kMany || q0 + 4 * kTiles >= a.group;
@@ -259,12 +262,26 @@ __global__ __launch_bounds__(kScoreThreads) void page_rank_kernel(SelectArgs a) 
     if (g == 0 && at < total) {
       const bool forced = at < a.sinks || at >= total - a.recent;
       const bool ok = (now_inside >> wave) & 1;
-      a.ranks[((int64_t)b * a.heads + h) * a.max_pages + at] =
-          forced ? kForced : ok ? rank_of(best) : kNanRank;
+      put(at, forced ? kForced : ok ? rank_of(best) : kNanRank);
     }
-    tile += a.chunks;
+    tile += step;
     if (tile * kScorePages >= total) break;
   }
+}
+
+template <typename Q, typename T, int kDim, int kTiles, bool kMany>
+__global__ __launch_bounds__(kScoreThreads) void page_rank_kernel(SelectArgs a) {
+  __shared__ Sums<kTiles> sums;
+  // heads fastest: their bounds of a page lie next to each other
+  const int h = (int)(blockIdx.x % (unsigned)a.heads);
+  const int seq_chunk = (int)(blockIdx.x / (unsigned)a.heads);
+  const int b = seq_chunk / a.chunks;
+  const int tile = seq_chunk - b * a.chunks;
+  const int total = pages_of(a, b);
+  if (total <= a.count || tile * kScorePages >= total) return;  // (all taken: no ranks)
+  uint32_t* ranks = a.ranks + ((int64_t)b * a.heads + h) * a.max_pages;
+  rank_tiles<Q, T, kDim, kTiles, kMany>(a, sums, b, h, total, tile, a.chunks,
+                                        [&](int at, uint32_t rank) { ranks[at] = rank; });
 }
 
 // Sum over the lanes up to and with this one: rows of 16 lanes by shifts, then the rows
@@ -280,38 +297,45 @@ __device__ __forceinline__ int wave_prefix(int x) {
   return x;
 }
 
+// The outputs of one (sequence, cache head) that need no ranks: the keys of the chosen
+// pages, entries that name none, and the pages of a sequence that keeps them all.
+__device__ __forceinline__ void select_plain(const SelectArgs& a, int64_t row, int total,
+                                             int threads) {
+  const int64_t b = row / a.heads;
+  const int kept = total < a.count ? total : a.count;
+  int32_t* index = a.index + row * a.count;
+  int32_t* out = a.table_out + row * a.count;
+  if (threadIdx.x == 0 && row == b * a.heads) {
+    const KeyRange range = key_range(a.lengths[b], a.max_length, 0);
+    a.lengths_out[b] = range.valid ? range.end - ((total - kept) << a.page_shift) : -1;
+  }
+  for (int i = threadIdx.x; i < a.count; i += threads) {
+    if (i < kept && total > a.count) break;
+    index[i] = i < kept ? i : -1;
+    out[i] = i < kept ? a.table[b * a.table_b + i] : -1;
+  }
+}
+
 // The `count` pages of highest rank of one (sequence, cache head), in the order of the
 // sequence: the rank of the last of them is found byte by byte from the counts of each
 // byte's values, then every thread lists its run of pages.  kKeys: pages of a thread,
 // whose ranks (and numbers) it keeps in registers; 0: any number, read again every time.
+constexpr int kCopies = 8;  // of the counts: neighbouring pages' ranks begin alike
+
+template <int kThreads>
+struct SelectShared {
+  int counts[2][256][kCopies];
+  uint32_t found[2];
+  int wave_sum[2][kThreads / kWave];
+};
+
 template <int kThreads, int kKeys>
-__global__ __launch_bounds__(kThreads) void page_select_kernel(SelectArgs a) {
-  constexpr int kWaves = kThreads / kWave;
-  constexpr int kCopies = 8;  // of the counts: neighbouring pages' ranks begin alike
-  __shared__ __attribute__((aligned(16))) int counts[2][256][kCopies];
-  __shared__ uint32_t found[2];
-  __shared__ int wave_sum[2][kWaves];
+__device__ __forceinline__ void select_row(const SelectArgs& a, SelectShared<kThreads>& shared,
+                                           int64_t row, int total, const uint32_t* ranks) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t seq_head = blockIdx.x;
-  const int64_t b = seq_head / a.heads;
-  const KeyRange range = key_range(__builtin_amdgcn_readfirstlane(a.lengths[b]), a.max_length, 0);
-  const int size = 1 << a.page_shift;
-  const int total = range.valid ? (range.end + size - 1) >> a.page_shift : 0;
-  const int kept = total < a.count ? total : a.count;
-  const int32_t* table = a.table + b * a.table_b;
-  int32_t* index = a.index + seq_head * a.count;
-  int32_t* out = a.table_out + seq_head * a.count;
-  if (tid == 0 && seq_head == b * a.heads)
-    a.lengths_out[b] = range.valid ? range.end - ((total - kept) << a.page_shift) : -1;
-  for (int i = kept + tid; i < a.count; i += kThreads) index[i] = out[i] = -1;
-  if (total <= a.count) {
-    for (int i = tid; i < total; i += kThreads) {
-      index[i] = i;
-      out[i] = table[i];
-    }
-    return;
-  }
-  const uint32_t* ranks = a.ranks + seq_head * a.max_pages;
+  const int32_t* table = a.table + row / a.heads * a.table_b;
+  int32_t* index = a.index + row * a.count;
+  int32_t* out = a.table_out + row * a.count;
   const int per = kKeys > 0 ? kKeys : (total + kThreads - 1) / kThreads;
   const int begin = min(total, tid * per), end = min(total, begin + per);
   uint32_t held[kKeys > 0 ? kKeys : 1];
@@ -331,19 +355,19 @@ __global__ __launch_bounds__(kThreads) void page_select_kernel(SelectArgs a) {
       for (int i = begin; i < end; ++i) f(i, ranks[i], 0);
     }
   };
-  for (int i = tid; i < 256 * kCopies; i += kThreads) counts[0][i / kCopies][i % kCopies] = 0;
+  for (int i = tid; i < 256 * kCopies; i += kThreads) shared.counts[0][i / kCopies][i % kCopies] = 0;
   __syncthreads();
   uint32_t least = 0, mask = 0;  // the bytes found so far
   int wanted = a.count;          // pages among those that begin with them
   for (int turn = 0; turn < 4; ++turn) {
     const int shift = 24 - 8 * turn;
-    int(*now)[kCopies] = counts[turn & 1];
+    int(*now)[kCopies] = shared.counts[turn & 1];
     each([&](int, uint32_t r, int) {
       if (((r ^ least) & mask) == 0) atomicAdd(&now[(r >> shift) & 255][lane % kCopies], 1);
     });
     if (turn < 3)
       for (int i = tid; i < 256 * kCopies; i += kThreads)
-        counts[(turn + 1) & 1][i / kCopies][i % kCopies] = 0;
+        shared.counts[(turn + 1) & 1][i / kCopies][i % kCopies] = 0;
     __syncthreads();
     if (wave == 0) {
       // lane l has the values 255 - 4l to 252 - 4l
@@ -365,13 +389,13 @@ __global__ __launch_bounds__(kThreads) void page_select_kernel(SelectArgs a) {
             above += own[u];
             v = u + 1;
           }
-        found[0] = (uint32_t)(255 - 4 * lane - v);
-        found[1] = (uint32_t)(wanted - above);
+        shared.found[0] = (uint32_t)(255 - 4 * lane - v);
+        shared.found[1] = (uint32_t)(wanted - above);
       }
     }
     __syncthreads();
-    least |= found[0] << shift;
-    wanted = (int)found[1];
+    least |= shared.found[0] << shift;
+    wanted = (int)shared.found[1];
     mask |= 255u << shift;
   }
   // ---- pages of a higher rank, and the first `wanted` of that rank itself
@@ -383,13 +407,13 @@ __global__ __launch_bounds__(kThreads) void page_select_kernel(SelectArgs a) {
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
     before[w] = wave_prefix(own[w]);
-    if (lane == kWave - 1) wave_sum[w][wave] = before[w];
+    if (lane == kWave - 1) shared.wave_sum[w][wave] = before[w];
     before[w] -= own[w];
   }
   __syncthreads();
   for (int w = 0; w < wave; ++w) {
-    before[0] += wave_sum[0][w];
-    before[1] += wave_sum[1][w];
+    before[0] += shared.wave_sum[0][w];
+    before[1] += shared.wave_sum[1][w];
   }
   each([&](int i, uint32_t r, int k) {
     if (r > least || (r == least && before[1] < wanted)) {
@@ -400,6 +424,36 @@ __global__ __launch_bounds__(kThreads) void page_select_kernel(SelectArgs a) {
     before[0] += r > least;
     before[1] += r == least;
   });
+}
+
+template <int kThreads, int kKeys>
+__global__ __launch_bounds__(kThreads) void page_select_kernel(SelectArgs a) {
+  __shared__ SelectShared<kThreads> shared;
+  const int64_t row = blockIdx.x;
+  const int total = pages_of(a, (int)(row / a.heads));
+  select_plain(a, row, total, kThreads);
+  if (total > a.count)
+    select_row<kThreads, kKeys>(a, shared, row, total, a.ranks + row * a.max_pages);
+}
+
+// Both in one launch, for rows of few pages: a work-group ranks them all, in LDS.
+template <typename Q, typename T, int kDim, int kTiles, bool kMany>
+__global__ __launch_bounds__(kScoreThreads) void page_rank_select_kernel(SelectArgs a) {
+  __shared__ union {
+    Sums<kTiles> sums;
+    SelectShared<kScoreThreads> select;
+  } shared;
+  static_assert(kFewPages <= kScoreThreads, "a page to a thread");
+  __shared__ uint32_t ranks[kFewPages];
+  const int64_t row = blockIdx.x;
+  const int b = (int)(row / a.heads), h = (int)(row - (int64_t)b * a.heads);
+  const int total = pages_of(a, b);
+  select_plain(a, row, total, kScoreThreads);
+  if (total <= a.count) return;
+  rank_tiles<Q, T, kDim, kTiles, kMany>(a, shared.sums, b, h, total, 0, 1,
+                                        [&](int at, uint32_t rank) { ranks[at] = rank; });
+  __syncthreads();
+  select_row<kScoreThreads, 1>(a, shared.select, row, total, ranks);
 }
 
 template <typename C, typename T>
@@ -415,12 +469,22 @@ hipError_t launch_bounds_type(const BoundsArgs& a, unsigned groups, hipStream_t 
 
 template <typename Q, typename T, int kDim>
 void launch_rank_dim(const SelectArgs& a, unsigned groups, hipStream_t stream) {
+  auto run = [&](auto tiles, auto many) {
+    constexpr int kTiles = decltype(tiles)::value;
+    constexpr bool kMany = decltype(many)::value;
+    if (a.max_pages <= kFewPages)
+      page_rank_select_kernel<Q, T, kDim, kTiles, kMany>
+          <<<groups, kScoreThreads, 0, stream>>>(a);
+    else
+      page_rank_kernel<Q, T, kDim, kTiles, kMany><<<groups, kScoreThreads, 0, stream>>>(a);
+  };
+  using std::integral_constant;
   if (a.group <= 4)
-    page_rank_kernel<Q, T, kDim, 1, false><<<groups, kScoreThreads, 0, stream>>>(a);
+    run(integral_constant<int, 1>(), std::false_type());
   else if (a.group <= 8)
-    page_rank_kernel<Q, T, kDim, 2, false><<<groups, kScoreThreads, 0, stream>>>(a);
+    run(integral_constant<int, 2>(), std::false_type());
   else
-    page_rank_kernel<Q, T, kDim, 2, true><<<groups, kScoreThreads, 0, stream>>>(a);
+    run(integral_constant<int, 2>(), std::true_type());
 }
 
 template <typename Q, typename T>
@@ -460,10 +524,10 @@ hipError_t launch_select_pages(const SelectArgs& args, hipStream_t stream) {
   SelectArgs a = args;
   const int64_t rows = (int64_t)a.batch * a.heads;
   if (a.max_pages > a.count) {
-    // work-groups of a row: as many as there are tiles, but not many more in all than
-    // the card holds at once
+    // work-groups of a row: one where it has few pages, otherwise as many as there are
+    // tiles, but not many more in all than the card holds at once
     const int64_t tiles = (a.max_pages + kScorePages - 1) / kScorePages;
-    const int64_t most = (kScoreGroups + rows - 1) / rows;
+    const int64_t most = a.max_pages <= kFewPages ? 1 : (kScoreGroups + rows - 1) / rows;
     a.chunks = (int)(tiles < most ? tiles : most);
     const unsigned groups = (unsigned)(rows * a.chunks);
     switch (a.dtype) {
@@ -472,7 +536,7 @@ hipError_t launch_select_pages(const SelectArgs& args, hipStream_t stream) {
       default: launch_rank<_Float16>(a, groups, stream); break;
     }
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    if (e != hipSuccess || a.max_pages <= kFewPages) return e;
   }
   const unsigned groups = (unsigned)rows;
   if (a.max_pages <= 256)

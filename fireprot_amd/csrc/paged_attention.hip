@@ -130,7 +130,9 @@ PagedPlan plan_paged(int dtype, int cache_dtype, int64_t batch, int heads, int g
                                         : cache_dtype <= 2 ? 4
                                         : cache_dtype <= 4 ? 2
                                                            : 1);
-  const int tile = cache_dtype == 0 ? 64 : 128;  // keys: one of PagedTraits::kTile a wave
+  // keys: one of PagedTraits::kTile a wave
+  const bool fp4 = cache_dtype > 4;
+  const int tile = cache_dtype == 0 ? 64 : fp4 && group <= 8 && wide_tile4(dtype != 1, head_dim) ? 256 : 128;
   const int64_t rows = batch * heads * p.qtiles;
   const int64_t span = unit_limit(max_length, window, 1);
   if (rows < 1 || rows >= (1ll << 31) || (span + tile - 1) / tile >= (1ll << 31) / rows) return p;
@@ -158,7 +160,7 @@ PagedPlan plan_paged(int dtype, int cache_dtype, int64_t batch, int heads, int g
   // sequences gains most from shares: 8 of 1 to 8000 BF16 keys, 8 heads of 128, 262 MB:
   // 35.9 us, in shares 30.0.
   const bool small =
-      each <= kPagedMaxGroups && rows * span * 2 * row_bytes <= kPagedFixedBytes;
+      each <= kPagedMaxGroups && rows * span * 2 * row_bytes <= kPagedFixedBytes / (fp4 ? 2 : 1);
   if ((each == 1 || small) && batch <= 65535) {
     p.unit = (int)unit;
     p.each = (int)each;

@@ -224,7 +224,9 @@ struct PagedTraits {
     return kFp4 ? 2 * bytes : bytes / (kF32 ? 4 : kCoded ? 1 : 2);
   }
   static constexpr int kRow = D / 2 * (kF32 ? 8 : kFp4 ? 1 : kCoded ? 2 : 4);
-  static constexpr int kHalves = kF32 ? 1 : 2;                 // 16-key halves of a tile
+  // 16-key parts of a tile
+  static constexpr int kHalves =
+      kF32 ? 1 : kColumns == 2 && wide_tile4(!std::is_same_v<Q, __bf16>, D) ? 4 : 2;
   static constexpr int kTile = 16 * kHalves;
   // terms a query is split into: all of its bits in BF16, 8 to a term
   static constexpr int kTerms = !kCoded ? 1 : std::is_same_v<Q, __bf16> ? 1
@@ -249,6 +251,10 @@ struct PagedTraits {
   static constexpr int kParts = kRow / 16 / kPart;
   static constexpr int kPartChannels = channels(kPart);
   static constexpr int kPartWords = (kPart + 3) / 4;
+  // 4-bit rows of 32 bytes and less: four and more to a line, read by as many loads (of
+  // 64 bytes non-temporal loads are still ahead: 237 us and 247 where of 32 it is 100
+  // and 93, 16 sequences of 20001 keys and more, 8 heads)
+  static constexpr bool kVOnce = !kFp4 || kRow >= 64;
   static constexpr int kVec = kChannels < 4 ? kChannels : 4;   // for the waves' join
   static constexpr int kVecs = kChannels / kVec;
   static constexpr int kPassVecs = kVecs < 2 ? kVecs : 2;      // 32 KB of LDS at most
@@ -461,7 +467,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int c = 0; c < T::kParts; ++c)
-          load_words<T::kPart, true>(p + r * T::kRow + c * 256, &vw[u * 4 + r][c * T::kPartWords]);
+          load_words<T::kPart, T::kVOnce>(p + r * T::kRow + c * 256,
+                                          &vw[u * 4 + r][c * T::kPartWords]);
       if constexpr (T::kScaled)
         vs[u] = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.v_scale) + row +
                                                 4 * (lane >> 4));

@@ -84,6 +84,15 @@ FPX_HD int resident_groups(bool split, int head_dim, int query_tiles) {
   return head_dim > 128 || query_tiles > 1 || (split && head_dim == 128) ? 2 : 3;
 }
 
+// Whether a wave takes tiles of 64 keys of a 4-bit cache, not 32, two columns to a query
+// (`split`: queries that enter the products as several terms).  16 sequences of 20001 to
+// 65536 keys, 8 heads: of 32 channels 73 us, with 32 keys 84; of 64 100 and 102; of 128,
+// FP16 queries 140 and 152, FP32 154 and 169, but BF16 163 and 151, as two work-groups
+// fit a CU then and not three; of 256 no difference.
+FPX_HD constexpr bool wide_tile4(bool split, int head_dim) {
+  return head_dim <= 64 || (split && head_dim == 128);
+}
+
 // Entry of the block table that serves a group of keys from `key` on: that of
 // the nearest key of the range, so that a group wholly outside it (its keys
 // are masked) names no page the sequence does not hold.

@@ -175,8 +175,7 @@ def select_pages(q: torch.Tensor, bounds: PageBounds, block_table: torch.Tensor,
             raise ValueError(f"workspace must be {size} contiguous bytes on q's device")
     elif size > NO_WORKSPACE:
         workspace = q.new_empty(size, dtype=torch.uint8)
-    both = lengths.new_empty((2, batch, heads, count))
-    table, index = both[0], both[1]
+    table, index = lengths.new_empty((2, batch, heads, count)).unbind(0)
     kept = torch.empty_like(lengths)
     code = _native.launch(
         device, lib.fpx_select_pages, ROW_DTYPES[q.dtype], ROW_DTYPES[values.dtype],

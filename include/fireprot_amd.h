@@ -509,7 +509,7 @@ int fpx_page_bounds(int cache_dtype, const void* cache_k, const void* k_scale, i
                     int64_t max_length, int64_t fresh, void* bounds, void* stream);
 
 /* Bytes of workspace fpx_select_pages needs; 0 for unsupported sizes, 256 where it uses
- * none (every page fits the selection): its workspace may then be null. */
+ * none (few pages, or all of them taken): its workspace may then be null. */
 size_t fpx_select_pages_workspace_bytes(int64_t batch, int heads, int page_size,
                                         int64_t max_length, int count);
 

@@ -214,7 +214,7 @@ def test_selection(q_type, kind, q_heads, heads, dim, page):
         assert torch.equal(got.index, again.index) and torch.equal(got.table, again.table)
 
 
-@pytest.mark.parametrize("total", [255, 256, 257, 1023, 1024, 1025, 2048, 2049, 8192, 8193, 20011])
+@pytest.mark.parametrize("total", [127, 128, 129, 255, 256, 257, 1023, 1024, 1025, 2048, 2049, 8192, 8193, 20011])
 def test_many_pages(total):
     bounds = PageBounds(random_bounds(total, 2, 64, BF16, 5), 16)
     table = torch.randperm(total, generator=torch.Generator().manual_seed(1)).int()[None].cuda()

@@ -24,8 +24,8 @@ def _bounds_args(**override):
 
 def _select_args(**override):
     args = dict(dtype=1, bounds_dtype=1, q=MB, q_sb=1024, q_sh=128, q_heads=8, bounds=2 * MB,
-                pages=40, heads=2, page_size=16, head_dim=128, block_table=3 * MB, table_sb=9,
-                table_pages=9, lengths=4 * MB, batch=3, max_length=144, count=4, sinks=1, recent=1,
+                pages=40, heads=2, page_size=16, head_dim=128, block_table=3 * MB,
+                table_sb=300, table_pages=300, lengths=4 * MB, batch=3, max_length=4800, count=4, sinks=1, recent=1,
                 index=5 * MB, table_out=6 * MB, lengths_out=7 * MB, workspace=8 * MB,
                 workspace_bytes=1 << 16, stream=None)
     assert set(override) <= set(args)
@@ -53,9 +53,9 @@ def test_bounds_pointers_are_refused(lib, bad):  # noqa: F811
 @pytest.mark.parametrize("bad", [
     dict(dtype=3), dict(bounds_dtype=4), dict(bounds_dtype=6), dict(q_heads=7), dict(q_heads=0),
     dict(q_sb=-8), dict(q_sh=132), dict(heads=0), dict(page_size=20), dict(head_dim=96),
-    dict(batch=-1), dict(batch=1 << 18), dict(max_length=145), dict(max_length=1 << 30),
+    dict(batch=-1), dict(batch=1 << 18), dict(max_length=4801), dict(max_length=1 << 30),
     dict(count=0), dict(count=1), dict(sinks=-1), dict(recent=0), dict(sinks=3, recent=2),
-    dict(count=1 << 26), dict(table_sb=-1), dict(table_pages=8),
+    dict(count=1 << 26), dict(table_sb=-1), dict(table_pages=299),
     dict(index=MB), dict(index=2 * MB), dict(table_out=3 * MB), dict(lengths_out=4 * MB),
     dict(table_out=5 * MB + 92), dict(lengths_out=6 * MB), dict(workspace=MB + 1024),
     dict(workspace=7 * MB), dict(index=8 * MB + 212)])
@@ -73,14 +73,14 @@ def test_selection_pointers_are_refused(lib, bad):  # noqa: F811
 
 def test_workspaces(lib):  # noqa: F811
     size = lib.fpx_select_pages_workspace_bytes
-    assert size(3, 2, 16, 144, 4) == 512  # 3 * 2 * 9 ranks, rounded up: not the 256 for none
-    assert size(3, 2, 16, 144, 9) == 256 and size(100, 2, 16, 1600, 100) == 256
-    assert size(100, 2, 16, 1601, 100) == -(-200 * 101 * 4 // 512) * 512
+    assert size(1, 1, 16, 129 * 16, 4) == 1024  # 129 ranks, rounded up
+    assert size(3, 2, 16, 128 * 16, 4) == 256   # few pages: none
+    assert size(100, 2, 16, 4800, 300) == 256 and size(100, 2, 16, 4801, 301) == 256
+    assert size(100, 2, 16, 4801, 300) == -(-200 * 301 * 4 // 512) * 512
     for bad in ((-1, 2, 16, 144, 4), (3, 0, 16, 144, 4), (3, 2, 24, 144, 4), (3, 2, 16, -1, 4),
                 (3, 2, 16, 1 << 30, 4), (3, 2, 16, 144, 0)):
         assert size(*bad) == 0
-    short = dict(batch=100, q_sb=1024, max_length=1600, table_pages=100, table_sb=100,
-                 index=5 * MB, count=4, workspace_bytes=200 * 100 * 4 - 1)
+    short = dict(batch=100, index=5 * MB, count=4, workspace_bytes=200 * 300 * 4 - 1)
     assert lib.fpx_select_pages(*_select_args(**short)) == _native.FPX_ERR_WORKSPACE
 
 
