@@ -78,10 +78,17 @@ __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(CacheArgs a)
 }
 
 // Spans of eight channels of a row that a thread reads, half a row apart: of 4-bit rows
-// two, so that what leads to a row serves as many bytes as in 8 bits (64098 tokens of 8
-// heads of 128 to BF16, 291 MB: 57 us, with one span 78).
+// two, so that what leads to a row serves as many bytes as in 8 bits.  And tokens of one
+// head that are read one after another, before the next head's: 4-bit rows are parts of a
+// line of the cache, and so are their scales, of which the next slot's row has the rest.
+// 64098 tokens of 8 heads of 128 to BF16, 291 MB: 78 us with one span, 84 with two, 70 with
+// tokens in runs of 16, 63 with one row of each tensor in flight in a thread and not four.
 template <typename C>
 constexpr int kReadSpans = __is_same(C, Fp4) ? 2 : 1;
+template <typename C>
+constexpr int kReadTokens = __is_same(C, Fp4) ? 16 : 1;
+template <typename C>
+constexpr int kReadRows = __is_same(C, Fp4) ? 1 : 4;
 
 // The rows of `slots` back as S: zeros where there is no slot, NaN for a slot
 // past the cache's end.
@@ -90,9 +97,10 @@ __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(CacheArgs a) 
   constexpr int kSpans = kReadSpans<C>;
   constexpr int kGroup = kDim / 8 / kSpans;
   constexpr int kPass = kCacheThreads / kGroup;
-  constexpr int kRows = 4;
+  constexpr int kRows = kReadRows<C>;
+  constexpr uint32_t kRun = kReadTokens<C>;
   const int c = (threadIdx.x & (kGroup - 1)) * 8;
-  const int64_t rows = a.tokens * a.heads;
+  const int64_t rows = round_up(a.tokens, kRun) * a.heads;
   for (int64_t base = (int64_t)blockIdx.x * kPass * kRows + threadIdx.x / kGroup; base < rows;
        base += (int64_t)gridDim.x * kPass * kRows) {
     uint32_t t[kRows];
@@ -103,9 +111,11 @@ __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(CacheArgs a) 
       const int64_t row = base + r * kPass;
       at[r] = kSlotNone;
       if (row >= rows) continue;
-      t[r] = (uint32_t)row / (uint32_t)a.heads;
-      h[r] = (int)((uint32_t)row - t[r] * (uint32_t)a.heads);
-      at[r] = cache_row(a.slots[t[r]], h[r], a.pages, a.heads, a.page_shift);
+      const uint32_t run = (uint32_t)row / kRun, first = run / (uint32_t)a.heads;
+      t[r] = first * kRun + (uint32_t)row % kRun;
+      h[r] = (int)(run - first * (uint32_t)a.heads);
+      if (t[r] < a.tokens)
+        at[r] = cache_row(a.slots[t[r]], h[r], a.pages, a.heads, a.page_shift);
     }
     Held<C> held[kRows][2][kSpans];
     float scale[kRows][2][kSpans];
@@ -124,7 +134,7 @@ __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(CacheArgs a) 
     }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      if (base + r * kPass >= rows) continue;
+      if (base + r * kPass >= rows || t[r] >= a.tokens) continue;
 #pragma unroll
       for (int w = 0; w < 2; ++w)
 #pragma unroll
@@ -159,8 +169,9 @@ __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(CacheArgs a) 
 template <typename S, typename C, int kDim>
 hipError_t launch_dim(const CacheArgs& a, bool read, hipStream_t stream) {
   constexpr int kPass = kCacheThreads / (kDim / 8);
-  const int64_t per = kPass * (read ? 4 * kReadSpans<C> : 2);
-  const int64_t blocks = (a.tokens * a.heads + per - 1) / per;
+  const int64_t per = kPass * (read ? kReadRows<C> * kReadSpans<C> : 2);
+  const int64_t rows = (read ? round_up(a.tokens, kReadTokens<C>) : a.tokens) * a.heads;
+  const int64_t blocks = (rows + per - 1) / per;
   // (the kernels walk on in strides of the grid)
   const unsigned grid = (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20));
   uint64_t bytes = 0;

@@ -299,12 +299,12 @@ __device__ __forceinline__ int wave_prefix(int x) {
 
 // The outputs of one (sequence, cache head) that need no ranks: the keys of the chosen
 // pages, entries that name none, and the pages of a sequence that keeps them all.
-__device__ __forceinline__ void select_plain(const SelectArgs& a, int64_t row, int total,
+__device__ __forceinline__ void select_plain(const SelectArgs& a, int row, int total,
                                              int threads) {
-  const int64_t b = row / a.heads;
+  const int b = row / a.heads;
   const int kept = total < a.count ? total : a.count;
-  int32_t* index = a.index + row * a.count;
-  int32_t* out = a.table_out + row * a.count;
+  int32_t* index = a.index + (int64_t)row * a.count;
+  int32_t* out = a.table_out + (int64_t)row * a.count;
   if (threadIdx.x == 0 && row == b * a.heads) {
     const KeyRange range = key_range(a.lengths[b], a.max_length, 0);
     a.lengths_out[b] = range.valid ? range.end - ((total - kept) << a.page_shift) : -1;
@@ -321,21 +321,22 @@ __device__ __forceinline__ void select_plain(const SelectArgs& a, int64_t row, i
 // byte's values, then every thread lists its run of pages.  kKeys: pages of a thread,
 // whose ranks (and numbers) it keeps in registers; 0: any number, read again every time.
 constexpr int kCopies = 8;  // of the counts: neighbouring pages' ranks begin alike
+constexpr int kBins = 256 + 4;  // of a copy, which begins four banks after the one before
 
 template <int kThreads>
 struct SelectShared {
-  int counts[2][256][kCopies];
+  __attribute__((aligned(16))) int counts[2][kCopies][kBins];
   uint32_t found[2];
   int wave_sum[2][kThreads / kWave];
 };
 
 template <int kThreads, int kKeys>
 __device__ __forceinline__ void select_row(const SelectArgs& a, SelectShared<kThreads>& shared,
-                                           int64_t row, int total, const uint32_t* ranks) {
+                                           int row, int total, const uint32_t* ranks) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int32_t* table = a.table + row / a.heads * a.table_b;
-  int32_t* index = a.index + row * a.count;
-  int32_t* out = a.table_out + row * a.count;
+  int32_t* index = a.index + (int64_t)row * a.count;
+  int32_t* out = a.table_out + (int64_t)row * a.count;
   const int per = kKeys > 0 ? kKeys : (total + kThreads - 1) / kThreads;
   const int begin = min(total, tid * per), end = min(total, begin + per);
   uint32_t held[kKeys > 0 ? kKeys : 1];
@@ -355,30 +356,30 @@ __device__ __forceinline__ void select_row(const SelectArgs& a, SelectShared<kTh
       for (int i = begin; i < end; ++i) f(i, ranks[i], 0);
     }
   };
-  for (int i = tid; i < 256 * kCopies; i += kThreads) shared.counts[0][i / kCopies][i % kCopies] = 0;
+  auto clear = [&](int(*counts)[kBins]) {
+    for (int i = tid; i < kCopies * kBins; i += kThreads) counts[0][i] = 0;
+  };
+  clear(shared.counts[0]);
   __syncthreads();
   uint32_t least = 0, mask = 0;  // the bytes found so far
   int wanted = a.count;          // pages among those that begin with them
   for (int turn = 0; turn < 4; ++turn) {
     const int shift = 24 - 8 * turn;
-    int(*now)[kCopies] = shared.counts[turn & 1];
+    int(*now)[kBins] = shared.counts[turn & 1];
     each([&](int, uint32_t r, int) {
-      if (((r ^ least) & mask) == 0) atomicAdd(&now[(r >> shift) & 255][lane % kCopies], 1);
+      if (((r ^ least) & mask) == 0) atomicAdd(&now[lane % kCopies][(r >> shift) & 255], 1);
     });
-    if (turn < 3)
-      for (int i = tid; i < 256 * kCopies; i += kThreads)
-        shared.counts[(turn + 1) & 1][i / kCopies][i % kCopies] = 0;
+    if (turn < 3) clear(shared.counts[(turn + 1) & 1]);
     __syncthreads();
     if (wave == 0) {
       // lane l has the values 255 - 4l to 252 - 4l
-      int own[4], sum = 0;
+      typedef int Four __attribute__((ext_vector_type(4)));
+      Four bins = {0, 0, 0, 0};
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        own[v] = 0;
-#pragma unroll
-        for (int k = 0; k < kCopies; ++k) own[v] += now[255 - 4 * lane - v][k];
-        sum += own[v];
-      }
+      for (int k = 0; k < kCopies; ++k)
+        bins += *reinterpret_cast<const Four*>(&now[k][252 - 4 * lane]);
+      const int own[4] = {bins[3], bins[2], bins[1], bins[0]};
+      const int sum = bins[0] + bins[1] + bins[2] + bins[3];
       const int upto = wave_prefix(sum);
       int above = upto - sum;
       if (above < wanted && wanted <= upto) {
@@ -429,8 +430,8 @@ __device__ __forceinline__ void select_row(const SelectArgs& a, SelectShared<kTh
 template <int kThreads, int kKeys>
 __global__ __launch_bounds__(kThreads) void page_select_kernel(SelectArgs a) {
   __shared__ SelectShared<kThreads> shared;
-  const int64_t row = blockIdx.x;
-  const int total = pages_of(a, (int)(row / a.heads));
+  const int row = blockIdx.x;
+  const int total = pages_of(a, row / a.heads);
   select_plain(a, row, total, kThreads);
   if (total > a.count)
     select_row<kThreads, kKeys>(a, shared, row, total, a.ranks + row * a.max_pages);
@@ -445,8 +446,8 @@ __global__ __launch_bounds__(kScoreThreads) void page_rank_select_kernel(SelectA
   } shared;
   static_assert(kFewPages <= kScoreThreads, "a page to a thread");
   __shared__ uint32_t ranks[kFewPages];
-  const int64_t row = blockIdx.x;
-  const int b = (int)(row / a.heads), h = (int)(row - (int64_t)b * a.heads);
+  const int row = blockIdx.x;
+  const int b = row / a.heads, h = row - b * a.heads;
   const int total = pages_of(a, b);
   select_plain(a, row, total, kScoreThreads);
   if (total <= a.count) return;
