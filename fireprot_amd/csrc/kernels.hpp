@@ -480,6 +480,7 @@ struct BoundsArgs {
   int fresh;       // newest tokens of each sequence, on pages whose bounds are formed
   int each;        // pages that hold them, at most
   int cache_dtype;  // FPX_*
+  uint32_t first;  // (sequence, head, page) of a launch, set by launch_page_bounds
 };
 
 hipError_t launch_page_bounds(const BoundsArgs& args, hipStream_t stream);

@@ -21,6 +21,7 @@ namespace fpx {
 namespace {
 
 constexpr int kBoundsThreads = 256;
+constexpr int64_t kBoundsMaxGroups = 1 << 22;  // work-groups of a launch
 constexpr int kScoreThreads = 256;
 constexpr int kScorePages = 64;    // of a work-group at a time
 constexpr int kScoreGroups = 768;  // work-groups, about
@@ -58,11 +59,11 @@ __global__ __launch_bounds__(kBoundsThreads) void page_bounds_kernel(BoundsArgs 
   __shared__ float part[2][kWaves][kDim];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = (threadIdx.x & (kGroup - 1)) * 8;
-  const int64_t item = blockIdx.x;
-  const int64_t seq_head = item / a.each;
-  const int i = (int)(item - seq_head * a.each);
-  const int64_t b = seq_head / a.heads;
-  const int h = (int)(seq_head - b * a.heads);
+  const uint32_t item = a.first + blockIdx.x;
+  const uint32_t seq_head = item / (uint32_t)a.each;
+  const int i = (int)(item - seq_head * (uint32_t)a.each);
+  const int64_t b = seq_head / (uint32_t)a.heads;
+  const int h = (int)(seq_head - (uint32_t)b * (uint32_t)a.heads);
   const KeyRange range = key_range(a.lengths[b], a.max_length, 0);
   if (!range.valid) return;
   const int from = range.end > a.fresh ? range.end - a.fresh : 0;
@@ -509,16 +510,24 @@ void launch_rank(const SelectArgs& a, unsigned groups, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_page_bounds(const BoundsArgs& a, hipStream_t stream) {
-  const unsigned groups = (unsigned)((int64_t)a.batch * a.heads * a.each);
-  switch (a.cache_dtype) {
-    case 0: return launch_bounds_type<float, float>(a, groups, stream);
-    case 1: return launch_bounds_type<__bf16, __bf16>(a, groups, stream);
-    case 2: return launch_bounds_type<_Float16, _Float16>(a, groups, stream);
-    case 3: return launch_bounds_type<Fp8, __bf16>(a, groups, stream);
-    case 4: return launch_bounds_type<Int8, __bf16>(a, groups, stream);
-    default: return launch_bounds_type<Fp4, __bf16>(a, groups, stream);
+hipError_t launch_page_bounds(const BoundsArgs& args, hipStream_t stream) {
+  BoundsArgs a = args;
+  const int64_t items = (int64_t)a.batch * a.heads * a.each;
+  hipError_t e = hipSuccess;
+  for (int64_t first = 0; first < items && e == hipSuccess; first += kBoundsMaxGroups) {
+    a.first = (uint32_t)first;
+    const int64_t left = items - first;
+    const unsigned groups = (unsigned)(left < kBoundsMaxGroups ? left : kBoundsMaxGroups);
+    switch (a.cache_dtype) {
+      case 0: e = launch_bounds_type<float, float>(a, groups, stream); break;
+      case 1: e = launch_bounds_type<__bf16, __bf16>(a, groups, stream); break;
+      case 2: e = launch_bounds_type<_Float16, _Float16>(a, groups, stream); break;
+      case 3: e = launch_bounds_type<Fp8, __bf16>(a, groups, stream); break;
+      case 4: e = launch_bounds_type<Int8, __bf16>(a, groups, stream); break;
+      default: e = launch_bounds_type<Fp4, __bf16>(a, groups, stream);
+    }
   }
+  return e;
 }
 
 hipError_t launch_select_pages(const SelectArgs& args, hipStream_t stream) {

@@ -132,7 +132,8 @@ PagedPlan plan_paged(int dtype, int cache_dtype, int64_t batch, int heads, int g
                                                            : 1);
   // keys: one of PagedTraits::kTile a wave
   const bool fp4 = cache_dtype > 4;
-  const int tile = cache_dtype == 0 ? 64 : fp4 && group <= 8 && wide_tile4(dtype != 1, head_dim) ? 256 : 128;
+  const bool wide = fp4 && group <= 8 && wide_tile4(dtype != 1, head_dim);
+  const int tile = cache_dtype == 0 ? 64 : wide ? 256 : 128;
   const int64_t rows = batch * heads * p.qtiles;
   const int64_t span = unit_limit(max_length, window, 1);
   if (rows < 1 || rows >= (1ll << 31) || (span + tile - 1) / tile >= (1ll << 31) / rows) return p;
@@ -177,7 +178,10 @@ PagedPlan plan_paged(int dtype, int cache_dtype, int64_t batch, int heads, int g
   p.unit = tile;
   p.split = 1;
   const int64_t each_cu = kPagedFlight / (2 * tile * row_bytes);
-  const int64_t most = resident_groups(cache_dtype > 2 && dtype != 1, head_dim, p.query_tiles);
+  const bool split = cache_dtype > 2 && dtype != 1;
+  const int64_t most =
+      fp4 ? resident_groups4(dtype == 0, split, head_dim, p.query_tiles, group <= 8)
+          : resident_groups(split, head_dim, p.query_tiles);
   const int64_t wanted = 256 * (each_cu < 1 ? 1 : each_cu > most ? most : each_cu);
   const int64_t units = rows * ((span + tile - 1) / tile);
   p.groups = (int)(units < wanted ? units : wanted);

@@ -93,6 +93,12 @@ FPX_HD constexpr bool wide_tile4(bool split, int head_dim) {
   return head_dim <= 64 || (split && head_dim == 128);
 }
 
+// Those of the kernel over a 4-bit cache: its tiles of 64 keys leave room for one less
+// where 64 channels meet FP32 queries.
+FPX_HD int resident_groups4(bool f32, bool split, int head_dim, int query_tiles, bool columns) {
+  return f32 && columns && head_dim == 64 ? 2 : resident_groups(split, head_dim, query_tiles);
+}
+
 // Entry of the block table that serves a group of keys from `key` on: that of
 // the nearest key of the range, so that a group wholly outside it (its keys
 // are masked) names no page the sequence does not hold.

@@ -94,7 +94,8 @@ def update_page_bounds(bounds: PageBounds, cache: PagedCache, block_table: torch
                        max_length: int | None = None) -> None:
     """Form the bounds of the pages that hold the last ``new`` tokens of each sequence
     (a step: 1; a prompt: its length, or the longest of a batch), from the keys below
-    its length.  Pages of earlier tokens keep theirs.
+    its length.  Pages of earlier tokens keep theirs.  (A page that several sequences
+    hold must be full in all of them: its bounds are those of its keys in one.)
 
     ``block_table``, ``lengths`` and ``max_length`` as ``paged_attention``'s.  A
     sequence whose length is negative or above ``max_length``, and an entry that names
@@ -162,6 +163,8 @@ def select_pages(q: torch.Tensor, bounds: PageBounds, block_table: torch.Tensor,
     if sinks < 0 or recent < 1 or count < sinks + recent:
         raise ValueError(f"needs sinks ({sinks}) >= 0, recent ({recent}) >= 1 and count ({count}) "
                          ">= their sum")
+    if count * page_size >= 1 << 30:
+        raise ValueError(f"count ({count}) pages of {page_size} slots are 2^30 keys or more")
     if _native.differentiated(q):
         raise ValueError("no autograd graph is recorded: detach q")
     if not _aligned_rows(q):

@@ -137,6 +137,23 @@ def test_what_gets_no_bounds():
     assert same(bounds.values, want)
 
 
+def test_bounds_of_more_pages_than_a_launch_has_work_groups():
+    """2048 sequences, 64 heads, up to 33 pages each: 4.3 million (sequence, head, page)."""
+    cache = PagedCache.allocate(40, 64, 16, 32, dtype=F16)
+    cache.k.normal_(generator=torch.Generator("cuda").manual_seed(2))
+    lengths = torch.zeros(2048, dtype=torch.int32)
+    table = torch.full((2048, 33), -1, dtype=torch.int32)
+    lengths[0], lengths[1023], lengths[2047] = 5, 300, 17
+    table[0, 0] = 7
+    table[1023, :19] = torch.arange(10, 29)
+    table[2047, :2] = torch.tensor([31, 3])
+    table, lengths = table.cuda(), lengths.cuda()
+    bounds = PageBounds.allocate(cache)
+    want = expected_bounds(cache, table, lengths, 1 << 20, bounds.values)
+    update_page_bounds(bounds, cache, table, lengths, new=528)
+    assert same(bounds.values, want)
+
+
 # ---------------------------------------------------------------- selection
 
 def expected_index(q, values, table, lengths, page, count, sinks, recent, max_length):
@@ -376,7 +393,8 @@ def test_refusals():
             update_page_bounds(**{**good, **change})
     good = dict(q=q, bounds=bounds, block_table=table, lengths=lengths, count=2)
     for change in (dict(q=q[0]), dict(q=q.double()), dict(q=q.cpu()), dict(q=q[:, :3]),
-                   dict(q=q[..., :16]), dict(q=q[:1]), dict(count=0), dict(count=1, sinks=1),
+                   dict(q=q[..., :16]), dict(q=q[:1]), dict(count=0), dict(count=1 << 26),
+                   dict(count=(1 << 32) + 2), dict(count=1, sinks=1),
                    dict(recent=0), dict(sinks=-1), dict(max_length=-1),
                    dict(max_length=table.shape[1] * 16 + 1), dict(block_table=table.long()),
                    dict(lengths=lengths.long()), dict(lengths=lengths.cpu()),
