@@ -121,7 +121,7 @@ def update_page_bounds(bounds: PageBounds, cache: PagedCache, block_table: torch
         device, lib.fpx_page_bounds, CACHE_DTYPES[cache.k.dtype], cache.k.data_ptr(),
         None if k_scale is None else k_scale.data_ptr(), pages, heads, page_size, head_dim,
         block_table.data_ptr(), block_table.stride(0), block_table.shape[1], lengths.data_ptr(),
-        batch, max_length, new, values.data_ptr())
+        batch, max_length, min(new, max_length + 1), values.data_ptr())
     if code:
         _native.check(code, "fpx_page_bounds")
 
