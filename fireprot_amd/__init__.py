@@ -11,7 +11,11 @@ Public surface:
 * ``fireprot_amd.layer_norm``, ``qkv_projection``, ``attention_gate``,
   ``pair_layout`` -- the per-stage hooks;
 * ``fireprot_amd.rotary``, ``kv_cache``, ``paged_attention`` -- decoding: rotary
-  positions, a paged key-value cache, one new token's attention over it;
+  positions, a paged key-value cache (in up to 32 and down to 4 bits), one new token's
+  attention over it;
+* ``fireprot_amd.cache_append``, ``page_selection`` -- a step's rows turned and put into
+  the cache in one launch; bounds of the cache's pages, and attention over those chosen
+  by them;
 * ``fireprot_amd.workloads`` -- the seeded benchmark configurations.
 
 The native library is ``fireprot_amd/_lib/libfireprot_amd.so`` (built by

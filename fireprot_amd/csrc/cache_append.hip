@@ -15,6 +15,11 @@
 // is turned, half as many take two eights half a row apart, which are each other's pairs
 // in the half layout.  Otherwise (a part turned) the other half of a pair is loaded a
 // second time by the lane that needs it.
+//
+// 16384 tokens of 32 query and 8 cache heads of 128 BF16 channels into 4 bits, 354 MB:
+// 67 to 70 us, 5.2 TB/s, a plain copy's rate (one eight to a lane, not streamed: 83).
+// 1665 tokens of 16 and 16 heads of 64 FP16 channels into INT8: 8.6 us.  64 tokens of 32
+// and 8 heads into BF16: 4.6 us, of which a launch is 3 to 4.
 #include "cache_rows.hpp"
 #include "common.hpp"
 #include "kernels.hpp"

@@ -486,8 +486,8 @@ struct BoundsArgs {
 hipError_t launch_page_bounds(const BoundsArgs& args, hipStream_t stream);
 
 // Rows of up to so many pages are ranked and chosen from in one launch, which needs no
-// workspace: one sequence of 64 pages, 4 heads, 7.1 us where two launches take 7.3 and
-// their call 3.5 us longer; 384 rows of 1 to 251 pages 14.4 us where two take 13.3.
+// workspace: one sequence of 64 pages, 4 heads, 6.4 us where two launches took 7.3 and
+// their call 3.5 us longer; 384 rows of 1 to 251 pages 14.4 us where two took 13.3.
 constexpr int kFewPages = 128;
 
 struct SelectArgs {
