@@ -114,7 +114,8 @@ __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(CacheArgs a) 
       const uint32_t run = (uint32_t)row / kRun, first = run / (uint32_t)a.heads;
       t[r] = first * kRun + (uint32_t)row % kRun;
       h[r] = (int)(run - first * (uint32_t)a.heads);
-      if (t[r] < a.tokens)
+      // (a look at t where no run passes the end would part the loads of the slots)
+      if (kRun == 1 || t[r] < a.tokens)
         at[r] = cache_row(a.slots[t[r]], h[r], a.pages, a.heads, a.page_shift);
     }
     Held<C> held[kRows][2][kSpans];
@@ -134,7 +135,7 @@ __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(CacheArgs a) 
     }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      if (base + r * kPass >= rows || t[r] >= a.tokens) continue;
+      if (base + r * kPass >= rows || (kRun > 1 && t[r] >= a.tokens)) continue;
 #pragma unroll
       for (int w = 0; w < 2; ++w)
 #pragma unroll
