@@ -199,11 +199,26 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
 _lock = threading.RLock()
 _library: ctypes.CDLL | None = None
 _error: str | None = None
+# torch and its forward_ad from the first call on that needs them: an import statement
+# in every call takes as long as a few of its checks
+_torch: Any = None
+_forward_ad: Any = None
+
+
+def _import_torch() -> None:
+    global _torch, _forward_ad
+    import torch
+    from torch.autograd import forward_ad
+
+    _forward_ad, _torch = forward_ad, torch  # (_torch last: it stands for both)
 
 
 def library() -> ctypes.CDLL:
     """Return the loaded library, or raise ``RuntimeError`` saying why not."""
     global _library, _error
+    lib = _library  # (set once, when all of it is checked)
+    if lib is not None:
+        return lib
     with _lock:
         if _library is not None:
             return _library
@@ -255,28 +270,27 @@ def launch(index: int, entry: Any, *args: Any) -> int:
     of its current stream; returns the status.  Where the device is current
     already, the ordinary call, nothing is switched: a call of a few microseconds
     would otherwise pay as much for the switch as for its launch."""
-    import torch
-
-    if torch._C._cuda_getDevice() == index:
-        return entry(*args, torch._C._cuda_getCurrentRawStream(index))
-    with torch.cuda.device(index):
-        return entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    if _torch is None:
+        _import_torch()
+    if _torch._C._cuda_getDevice() == index:
+        return entry(*args, _torch._C._cuda_getCurrentRawStream(index))
+    with _torch.cuda.device(index):
+        return entry(*args, _torch._C._cuda_getCurrentRawStream(index))
 
 
 def differentiated(*tensors: Any) -> bool:
     """Whether one of ``tensors`` (None among them) requires a gradient under grad
     mode, or carries a forward-mode tangent: an entry that records neither would
     drop it."""
-    import torch
-    from torch.autograd import forward_ad
-
-    if torch.is_grad_enabled():
+    if _torch is None:
+        _import_torch()
+    if _torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
     # (outside of any dual level, where no tensor has a tangent, this is one look)
-    return forward_ad._current_level >= 0 and any(
-        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    return _forward_ad._current_level >= 0 and any(
+        t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def repeats(t: Any) -> bool:
