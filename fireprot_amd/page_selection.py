@@ -71,22 +71,27 @@ class PageSelection:
 
 
 def _sequences(block_table, lengths, device, batch, page_size, max_length):
-    """(block_table, lengths, max_length), checked, rows of unit stride."""
-    if (block_table.dim() != 2 or block_table.shape[0] != batch or block_table.dtype != torch.int32
+    """(table, its stride, its pages a sequence, lengths, max_length), checked, rows of
+    unit stride."""
+    shape = block_table.shape
+    if (len(shape) != 2 or shape[0] != batch or block_table.dtype != torch.int32
             or block_table.get_device() != device):
         raise ValueError("block_table must be int32 [batch, pages] on the cache's device")
     if lengths.shape != (batch,) or lengths.dtype != torch.int32 or lengths.get_device() != device:
         raise ValueError("lengths must be int32 [batch] on the cache's device")
-    held = block_table.shape[1] * page_size
+    columns = shape[1]
+    held = columns * page_size
     if max_length is None:
         max_length = held
     if not 0 <= max_length <= held:
         raise ValueError(f"needs 0 <= max_length ({max_length}) <= {held}, the block table's slots")
-    if block_table.stride(1) != 1 and block_table.shape[1] > 1:
+    row, one = block_table.stride()
+    if one != 1 and columns > 1:
         block_table = block_table.contiguous()
+        row = columns
     if not lengths.is_contiguous():
         lengths = lengths.contiguous()
-    return block_table, lengths, max_length
+    return block_table, row, columns, lengths, max_length
 
 
 def update_page_bounds(bounds: PageBounds, cache: PagedCache, block_table: torch.Tensor,
@@ -112,16 +117,15 @@ def update_page_bounds(bounds: PageBounds, cache: PagedCache, block_table: torch
             or values.dtype != bounds_dtype(cache.k.dtype)):
         raise ValueError("the bounds are not of this cache: PageBounds.allocate(cache)")
     batch = lengths.shape[0] if lengths.dim() == 1 else -1
-    block_table, lengths, max_length = _sequences(block_table, lengths, device, batch, page_size,
-                                                  max_length)
+    block_table, row, columns, lengths, max_length = _sequences(
+        block_table, lengths, device, batch, page_size, max_length)
     if new < 1:
         raise ValueError(f"needs new ({new}) >= 1")
     k_scale = cache.k_scale
     code = _native.launch(
         device, lib.fpx_page_bounds, CACHE_DTYPES[cache.k.dtype], cache.k.data_ptr(),
         None if k_scale is None else k_scale.data_ptr(), pages, heads, page_size, head_dim,
-        block_table.data_ptr(), block_table.stride(0), block_table.shape[1], lengths.data_ptr(),
-        batch, max_length, min(new, max_length + 1), values.data_ptr())
+        block_table.data_ptr(), row, columns, lengths.data_ptr(), batch, max_length, min(new, max_length + 1), values.data_ptr())
     if code:
         _native.check(code, "fpx_page_bounds")
 
@@ -151,15 +155,16 @@ def select_pages(q: torch.Tensor, bounds: PageBounds, block_table: torch.Tensor,
     values, page_size = bounds.values, bounds.page_size
     pages, heads, _, head_dim = values.shape
     device = values.get_device()
-    if q.dim() != 3 or q.dtype not in ROW_DTYPES or device < 0 or q.get_device() != device:
+    kind = ROW_DTYPES.get(q.dtype)
+    if q.dim() != 3 or kind is None or device < 0 or q.get_device() != device:
         raise ValueError("q must be float32, bfloat16 or float16 [batch, q_heads, head_dim] on "
                          "the bounds' HIP device")
     batch, q_heads, q_dim = q.shape
     if q_dim != head_dim or q_heads < heads or q_heads % heads:
         raise ValueError(f"q must have head_dim {head_dim} and a multiple of {heads} heads, got "
                          f"{tuple(q.shape)}")
-    block_table, lengths, max_length = _sequences(block_table, lengths, device, batch, page_size,
-                                                  max_length)
+    block_table, row, columns, lengths, max_length = _sequences(
+        block_table, lengths, device, batch, page_size, max_length)
     if sinks < 0 or recent < 1 or count < sinks + recent:
         raise ValueError(f"needs sinks ({sinks}) >= 0, recent ({recent}) >= 1 and count ({count}) "
                          ">= their sum")
@@ -178,13 +183,12 @@ def select_pages(q: torch.Tensor, bounds: PageBounds, block_table: torch.Tensor,
             raise ValueError(f"workspace must be {size} contiguous bytes on q's device")
     elif size > NO_WORKSPACE:
         workspace = q.new_empty(size, dtype=torch.uint8)
-    table, index = lengths.new_empty((2, batch, heads, count)).unbind(0)
-    kept = torch.empty_like(lengths)
+    table = lengths.new_empty((batch, heads, count))
+    index, kept = torch.empty_like(table), torch.empty_like(lengths)
     code = _native.launch(
-        device, lib.fpx_select_pages, ROW_DTYPES[q.dtype], ROW_DTYPES[values.dtype],
-        q.data_ptr(), *q.stride()[:2], q_heads, values.data_ptr(), pages, heads, page_size,
-        head_dim, block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-        lengths.data_ptr(), batch, max_length, count, sinks, recent, index.data_ptr(),
+        device, lib.fpx_select_pages, kind, ROW_DTYPES[values.dtype], q.data_ptr(),
+        *q.stride()[:2], q_heads, values.data_ptr(), pages, heads, page_size, head_dim,
+        block_table.data_ptr(), row, columns, lengths.data_ptr(), batch, max_length, count, sinks, recent, index.data_ptr(),
         table.data_ptr(), kept.data_ptr(), None if workspace is None else workspace.data_ptr(),
         size)
     if code:

@@ -68,8 +68,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
     """
     lib = _native.library()
     k = cache.k
-    device = k.get_device()
-    if q.dim() != 3 or q.dtype not in ROW_DTYPES or device < 0 or q.get_device() != device:
+    device, held_dtype, dtype = k.get_device(), k.dtype, q.dtype
+    if q.dim() != 3 or dtype not in ROW_DTYPES or device < 0 or q.get_device() != device:
         raise ValueError("q must be float32, bfloat16 or float16 [batch, q_heads, head_dim] on "
                          "the cache's HIP device")
     batch, q_heads, head_dim = q.shape
@@ -77,10 +77,11 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
     if head_dim != cache_dim or q_heads < heads or q_heads % heads:
         raise ValueError(f"q must have head_dim {cache_dim} and a multiple of {heads} heads, "
                          f"got {tuple(q.shape)}")
-    if k.dtype not in CODED_DTYPES and k.dtype != q.dtype:
-        raise ValueError(f"a {k.dtype} cache needs {k.dtype} queries")
-    lists = block_table.dim() == 3
-    if (block_table.shape[:-1] != ((batch, heads) if lists else (batch,))
+    if held_dtype not in CODED_DTYPES and held_dtype != dtype:
+        raise ValueError(f"a {held_dtype} cache needs {held_dtype} queries")
+    shape = block_table.shape
+    lists = len(shape) == 3
+    if (len(shape) not in (2, 3) or shape[0] != batch or (lists and shape[1] != heads)
             or block_table.dtype != torch.int32 or block_table.get_device() != device):
         raise ValueError("block_table must be int32 [batch, pages] or [batch, heads, pages] on "
                          "q's device")
@@ -88,7 +89,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
         raise ValueError("lists of pages for each head take no window")
     if lengths.shape != (batch,) or lengths.dtype != torch.int32 or lengths.get_device() != device:
         raise ValueError("lengths must be int32 [batch] on q's device")
-    columns = block_table.shape[-1]
+    columns = shape[-1]
     held = columns * page_size
     if max_length is None:
         max_length = held
@@ -99,8 +100,10 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
         raise ValueError("no autograd graph is recorded: detach q (and out)")
     if not _aligned_rows(q):
         q = q.clone(memory_format=torch.contiguous_format)
-    if block_table.stride(-1) != 1 and columns > 1:
+    *rows, one = block_table.stride()
+    if one != 1 and columns > 1:
         block_table = block_table.contiguous()
+        rows = block_table.stride()[:-1]
     if not lengths.is_contiguous():
         lengths = lengths.contiguous()
     if out is None:
@@ -110,7 +113,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
         raise ValueError("out must have q's shape, type and device, 16-byte aligned rows and "
                          "no repeated elements")
     lse = q.new_empty((batch, q_heads), dtype=torch.float32) if return_lse else None
-    size = lib.fpx_paged_attention_workspace_bytes(CACHE_DTYPES[k.dtype], batch, q_heads, heads,
+    size = lib.fpx_paged_attention_workspace_bytes(CACHE_DTYPES[held_dtype], batch, q_heads, heads,
                                                    head_dim, max_length, window)
     if size == 0:
         raise ValueError(f"unsupported sizes: batch {batch}, {q_heads} query heads, "
@@ -125,9 +128,9 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
         workspace = q.new_empty(size, dtype=torch.uint8)
     code = _native.launch(
         device, lib.fpx_paged_attention_lists if lists else lib.fpx_paged_attention,
-        ROW_DTYPES[q.dtype], CACHE_DTYPES[k.dtype],
+        ROW_DTYPES[dtype], CACHE_DTYPES[held_dtype],
         q.data_ptr(), *q.stride()[:2], *cache.pointers(), pages, heads, page_size, head_dim,
-        block_table.data_ptr(), *block_table.stride()[:-1], columns, lengths.data_ptr(), batch,
+        block_table.data_ptr(), *rows, columns, lengths.data_ptr(), batch,
         q_heads, max_length, *(() if lists else (window,)),
         head_dim ** -0.5 if scale is None else scale, out.data_ptr(), *out.stride()[:2],
         None if lse is None else lse.data_ptr(),
