@@ -1305,7 +1305,8 @@ int fpx_page_bounds(int cache_dtype, const void* cache_k, const void* k_scale, i
     return FPX_ERR_DIMS;
   const int64_t most = (max_length + page_size - 1) / page_size;
   if (table_sb < 0 || table_pages < most) return FPX_ERR_DIMS;
-  const int64_t each = fresh >= max_length ? most : (fresh - 1) / page_size + 2;
+  // (so many consecutive tokens touch at most)
+  const int64_t each = fresh >= max_length ? most : (fresh + page_size - 2) / page_size + 1;
   a.each = (int)(each < most ? each : most);
   if (batch * heads * a.each > 0x7fffffff) return FPX_ERR_DIMS;
   if (batch == 0 || a.each == 0) return FPX_OK;
