@@ -1284,11 +1284,14 @@ int fpx_paged_attention_lists(int dtype, int cache_dtype, const void* q, int64_t
 
 size_t fpx_select_pages_workspace_bytes(int64_t batch, int heads, int page_size,
                                         int64_t max_length, int count) {
-  if (batch < 0 || batch > kPagedMaxRows || heads < 1 || heads > kPagedMaxRows || count < 1 ||
-      page_size < 16 || page_size > 4096 || (page_size & (page_size - 1)) || max_length < 0 ||
-      max_length >= (1 << 30))
+  // (each factor is bounded before the next product is formed)
+  if (batch < 0 || batch > kPagedMaxRows || heads < 1 || heads > 65535 ||
+      batch * heads > kPagedMaxRows || page_size < 16 || page_size > 4096 ||
+      (page_size & (page_size - 1)) || max_length < 0 || max_length >= (1 << 30) || count < 1 ||
+      count > ((1 << 30) - 1) / page_size)
     return 0;
   const int64_t pages = (max_length + page_size - 1) / page_size;
+  if (batch * heads * ((pages + 63) / 64) > 0x7fffffff) return 0;
   if (pages <= count || pages <= fpx::kFewPages) return 256;
   // (never the 256 that stand for none)
   return (size_t)round_up((batch < 1 ? 1 : batch) * heads * pages * 4, 512);
@@ -1357,13 +1360,11 @@ int fpx_select_pages(int dtype, int bounds_dtype, const void* q, int64_t q_sb, i
   if (need == 0 || q_heads < heads || q_heads % heads || q_heads > kPagedMaxRows ||
       batch * q_heads > kPagedMaxRows)
     return FPX_ERR_DIMS;
-  if (sinks < 0 || recent < 1 || sinks > count - recent || count > ((1 << 30) - 1) / page_size)
-    return FPX_ERR_DIMS;
+  if (sinks < 0 || recent < 1 || sinks > count - recent) return FPX_ERR_DIMS;
   const int64_t row = 16 / (int64_t)type_bytes(dtype);
   if (q_sb < 0 || q_sh < 0 || q_sb % row || q_sh % row) return FPX_ERR_DIMS;
   const int64_t most = (max_length + page_size - 1) / page_size;
   if (table_sb < 0 || table_pages < most) return FPX_ERR_DIMS;
-  if (batch * heads * ((most + 63) / 64) > 0x7fffffff) return FPX_ERR_DIMS;
   if (batch == 0) return FPX_OK;
   if (!aligned(q, 16) || !aligned(bounds, 16) || !aligned(lengths, 4) || !aligned(index, 4) ||
       !aligned(table_out, 4) || !aligned(lengths_out, 4) ||
