@@ -4,12 +4,12 @@
 //   bounds[page][head] = (lo, hi), channel by channel over the page's keys
 //   score(b, h, page)  = max over head h's queries of sum_c max(q_c lo_c, q_c hi_c),
 //
-// no less than any q . k of the page.  With q+ = max(q, 0) and q- = min(q, 0) it is a
-// product, q+ . hi + q- . lo, which runs on the FP64 matrix cores: two pages next to
-// each other in rank must come out in the same order whatever order the sum is taken
-// in, and an FP32 sum of 128 terms is off by more than the step between scores where
-// thousands of pages compete for the last place.  The sum is rounded to FP32 once; of
-// pages alike the lower is preferred.
+// no less than any q . k of the page.  With q+ = max(q, 0) and q- = min(q, 0) it is, for
+// finite bounds, a product, q+ . hi + q- . lo, which runs on the FP64 matrix cores: two
+// pages next to each other in rank must come out in the same order whatever order the sum
+// is taken in, and an FP32 sum of 128 terms is off by more than the step between scores
+// where thousands of pages compete for the last place.  The sum is rounded to FP32 once;
+// of pages alike the lower is preferred.
 //
 // What bounds the ranks is the larger of the bounds' way from memory and the FP64
 // products, which are about as long: 16 sequences of up to 2048 pages, 8 cache heads of
@@ -158,6 +158,33 @@ __device__ __forceinline__ int pages_of(const SelectArgs& a, int b) {
   return (int)(((int64_t)range.end + (1 << a.page_shift) - 1) >> a.page_shift);
 }
 
+__device__ __forceinline__ int lane_of() {
+  return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+}
+
+// A query's sum_c max(q_c lo_c, q_c hi_c) term by term.  In the product form a bound on
+// the side that the query does not ask for meets a zero, which makes NaN of an infinite
+// one; here only a zero of the query's own does, and a sum of both infinities.
+template <typename Q, typename T, int kDim>
+__device__ __forceinline__ double score_by_terms(const Q* q, const T* edge) {
+  typedef Q QVec __attribute__((ext_vector_type(4)));
+  typedef T TVec __attribute__((ext_vector_type(4)));
+  double sum = 0.0;
+#pragma unroll 1
+  for (int c = 0; c < kDim; c += 4) {
+    const QVec x = *reinterpret_cast<const QVec*>(q + c);
+    const TVec lo = *reinterpret_cast<const TVec*>(edge + c);
+    const TVec hi = *reinterpret_cast<const TVec*>(edge + kDim + c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const double l = (double)(float)x[i] * (double)(float)lo[i];
+      const double u = (double)(float)x[i] * (double)(float)hi[i];
+      sum += l > u || !(l == l) ? l : u;  // (NaN where either is)
+    }
+  }
+  return sum;
+}
+
 // The ranks of a sequence's pages for one cache head, 64 at a time.  In a product the
 // pages are the columns (one to a lane % 16), four queries the rows, and the lane groups
 // (lane / 16) the four channels that are contracted.  Each of the four waves contracts a
@@ -167,11 +194,11 @@ __device__ __forceinline__ int pages_of(const SelectArgs& a, int b) {
 template <int kTiles>
 using Sums = double[2][4][kScorePages / 16][kTiles][kWave];
 
-// put(place, rank) for the pages of tiles `tile`, `tile` + step and so on of the `total`
-// pages of sequence b, cache head h.
-template <typename Q, typename T, int kDim, int kTiles, bool kMany, typename Put>
+// rank(place), a reference, for the pages of tiles `tile`, `tile` + step and so on of the
+// `total` pages of sequence b, cache head h.
+template <typename Q, typename T, int kDim, int kTiles, bool kMany, typename Rank>
 __device__ __forceinline__ void rank_tiles(const SelectArgs& a, Sums<kTiles>& sums, int b, int h,
-                                           int total, int tile, int step, Put put) {
+                                           int total, int tile, int step, Rank rank) {
   constexpr int kEach = kDim / 16;  // channels of a lane
   constexpr int kParts = kScorePages / 16;
   typedef Q QVec __attribute__((ext_vector_type(kEach)));
@@ -189,11 +216,17 @@ __device__ __forceinline__ void rank_tiles(const SelectArgs& a, Sums<kTiles>& su
     for (int p = 0; p < kParts; ++p)
       to[p] = table[min(at_tile * kScorePages + 16 * p + col, total - 1)];
   };
+  auto edge_of = [&](int number) {  // (of a page outside the cache the first's)
+    return static_cast<const T*>(a.bounds) +
+           ((int64_t)(page_valid(number, a.pages) ? number : 0) * a.heads + h) * 2 * kDim;
+  };
+  auto query_of = [&](int qi) {  // (rows past the head's last query have its first one again)
+    return static_cast<const Q*>(a.q) + b * a.q_b +
+           ((int64_t)h * a.group + (qi < a.group ? qi : 0)) * a.q_h;
+  };
   auto load = [&](int p) {
-    const bool ok = page_valid(page[p], a.pages);
-    inside = (inside & ~(1u << p)) | (uint32_t)ok << p;
-    const T* edge = static_cast<const T*>(a.bounds) +
-                    ((int64_t)(ok ? page[p] : 0) * a.heads + h) * 2 * kDim + channel;
+    inside = (inside & ~(1u << p)) | (uint32_t)page_valid(page[p], a.pages) << p;
+    const T* edge = edge_of(page[p]) + channel;
     lo[p] = *reinterpret_cast<const TVec*>(edge);
     hi[p] = *reinterpret_cast<const TVec*>(edge + kDim);
   };
@@ -201,11 +234,8 @@ __device__ __forceinline__ void rank_tiles(const SelectArgs& a, Sums<kTiles>& su
   auto load_queries = [&](int q0) {
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
-      // (rows past the head's last query have its first one again)
-      int qi = q0 + 4 * t + (lane & 3);
-      qi = qi < a.group ? qi : 0;
-      const Q* q = static_cast<const Q*>(a.q) + b * a.q_b + ((int64_t)h * a.group + qi) * a.q_h;
-      const QVec x = *reinterpret_cast<const QVec*>(q + channel);
+      const QVec x =
+          *reinterpret_cast<const QVec*>(query_of(q0 + 4 * t + (lane & 3)) + channel);
 #pragma unroll
       for (int j = 0; j < kEach; ++j) {
         above[t][j] = (double)greater((float)x[j], 0.0f);
@@ -217,6 +247,8 @@ __device__ __forceinline__ void rank_tiles(const SelectArgs& a, Sums<kTiles>& su
   // tile's are used, and its page numbers a tile before that.  (Past the last tile the
   // last page is read again: the loads are not branched around, which would make every
   // wait one for all of them.)
+  const int first_tile = tile;
+  uint64_t unsure = 0;  // lanes with a score that is NaN
   look_up(tile, page);
   look_up(tile + step, later);
   if (!kMany) load_queries(0);
@@ -268,10 +300,32 @@ __device__ __forceinline__ void rank_tiles(const SelectArgs& a, Sums<kTiles>& su
     if (g == 0 && at < total) {
       const bool forced = at < a.sinks || at >= total - a.recent;
       const bool ok = (now_inside >> wave) & 1;
-      put(at, forced ? kForced : ok ? rank_of(best) : kNanRank);
+      rank(at) = forced ? kForced : ok ? rank_of(best) : kNanRank;
     }
+    unsure |= __ballot(!(best == best));
     tile += step;
     if (tile * kScorePages >= total) break;
+  }
+  // ---- pages that a NaN has ranked, by the terms of their scores: after all tiles, and
+  // with the lane's number formed anew, so that it takes no registers in their loop (30
+  // more there, and at 128 FP32 channels a work-group less to a CU)
+  if (unsure == 0) return;
+  const int me = lane_of(), my_group = me >> 4;
+  for (tile = first_tile; tile * kScorePages < total; tile += step) {
+    const int at = tile * kScorePages + 16 * wave + (me & 15);
+    // (each lane reads what it has put itself)
+    const uint32_t put = my_group == 0 && at < total ? rank(at) : 0u;
+    const int number = table[min(at, total - 1)];
+    const bool again =
+        (uint32_t)__shfl((int)put, me & 15) == kNanRank && page_valid(number, a.pages);
+    float best = -__builtin_inff();
+    if (again)
+      for (int qi = my_group; qi < a.group; qi += 4)
+        best = greater(best,
+                       (float)score_by_terms<Q, T, kDim>(query_of(qi), edge_of(number)));
+    best = greater(best, __shfl_xor(best, 16));
+    best = greater(best, __shfl_xor(best, 32));
+    if (my_group == 0 && again) rank(at) = rank_of(best);
   }
 }
 
@@ -287,7 +341,7 @@ __global__ __launch_bounds__(kScoreThreads) void page_rank_kernel(SelectArgs a) 
   if (total <= a.count || tile * kScorePages >= total) return;  // (all taken: no ranks)
   uint32_t* ranks = a.ranks + ((int64_t)b * a.heads + h) * a.max_pages;
   rank_tiles<Q, T, kDim, kTiles, kMany>(a, sums, b, h, total, tile, a.chunks,
-                                        [&](int at, uint32_t rank) { ranks[at] = rank; });
+                                        [&](int at) -> uint32_t& { return ranks[at]; });
 }
 
 // Sum over the lanes up to and with this one: rows of 16 lanes by shifts, then the rows
@@ -461,7 +515,7 @@ __global__ __launch_bounds__(kScoreThreads) void page_rank_select_kernel(SelectA
   select_plain(a, row, total, kScoreThreads);
   if (total <= a.count) return;
   rank_tiles<Q, T, kDim, kTiles, kMany>(a, shared.sums, b, h, total, 0, 1,
-                                        [&](int at, uint32_t rank) { ranks[at] = rank; });
+                                        [&](int at) -> uint32_t& { return ranks[at]; });
   __syncthreads();
   select_row<kScoreThreads, 1>(a, shared.select, row, total, ranks);
 }

@@ -140,8 +140,9 @@ def select_pages(q: torch.Tensor, bounds: PageBounds, block_table: torch.Tensor,
     of a sequence are always among them; the others are those with the highest ``max
     over the head's queries of sum_c max(q_c lo_c, q_c hi_c)``, which no key of the page
     exceeds.  The sum is taken in FP64 and rounded to FP32; of equal pages the lower
-    comes first, NaN and pages outside the cache above all (a page with an infinite key
-    scores infinity or NaN).  A sequence of no more than ``count`` pages keeps them all.
+    comes first, NaN and pages outside the cache above all (NaN are zero times an infinite
+    bound and a sum of both infinities).  A sequence of no more than ``count`` pages keeps
+    them all.
 
     * ``q`` ``[batch, q_heads, head_dim]`` as ``paged_attention``'s, ``q_heads`` a
       multiple of the bounds' heads; for a negative ``scale`` of the scores pass ``-q``.

@@ -517,9 +517,8 @@ size_t fpx_select_pages_workspace_bytes(int64_t batch, int heads, int page_size,
  * cache head: the first `sinks` and the last `recent` pages, then those with the highest
  *   score = max over the head's queries of sum_c max(q_c lo_c, q_c hi_c),
  * an upper bound of the page's q . k; it is summed in FP64 and rounded to FP32, the
- * lower of equal pages comes first, NaN (and a page outside the cache) above all.  An
- * infinite bound makes the score of finite queries infinite or NaN (the sum is taken as
- * max(q, 0) . hi + min(q, 0) . lo).
+ * lower of equal pages comes first, NaN (and a page outside the cache) above all: zero
+ * times an infinite bound, and a sum of both infinities, are NaN.
  *   dtype         of q, as fpx_paged_attention's; q_heads a multiple of heads
  *   bounds_dtype  of bounds (fpx_page_bounds): FPX_F32, FPX_BF16 or FPX_F16
  *   index         [batch][heads][count]: the pages' places in the sequence, ascending
