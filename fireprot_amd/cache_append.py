@@ -44,9 +44,11 @@ def cache_append(cache: PagedCache, q: torch.Tensor | None, k: torch.Tensor, v: 
       turned by, and with ``block_table`` also their places in the sequences.
     * ``block_table`` int32 ``[batch, p]``, the sequences' pages in order, or ``slots``
       int64 ``[batch, tokens]`` (``[tokens]`` without the batch axis): one of the two.
-      A token with a negative slot or position (padding), past the table, or on a page
-      outside the cache is not written; its query is turned all the same.  The other
-      tokens' slots must be distinct.
+      By ``block_table`` a token with a negative position (padding), past the table, or on
+      a page outside the cache is not written; by ``slots`` one with a negative slot, or
+      past the cache (its position, negative or not, only turns it, so padding has to show
+      in ``slots``).  Its query is turned all the same.  The other tokens' slots must be
+      distinct.
     * ``q_out=q`` works in place; an output that shares an element with anything else is
       refused, as are inputs that are rows of this cache.
 
