@@ -486,8 +486,12 @@ struct BoundsArgs {
 hipError_t launch_page_bounds(const BoundsArgs& args, hipStream_t stream);
 
 // Rows of up to so many pages are ranked and chosen from in one launch, which needs no
-// workspace: one sequence of 64 pages, 4 heads, 6.4 us where two launches took 7.3 and
-// their call 3.5 us longer; 384 rows of 1 to 251 pages 14.4 us where two took 13.3.
+// workspace and 4 us less of the host.  Times on the GPU in one launch and in two: rows
+// of 64 pages, 4 of them, 6.6 and 8.1 us; of 128 pages, 4 rows 7.5 and 8.3, 64 rows 8.6
+// and 8.8, 384 rows 13.2 and 13.5, 1024 rows 19.3 and 21.7.  Past the border few rows are
+// longer in one, as a row is then one work-group's: of 192 pages, 64 rows 10.0 and 8.8; of
+// 256, 4 rows 9.6 and 8.3, 64 rows 11.4 and 8.9, 384 rows 21.1 and 20.4 (1024 rows 30.0
+// and 33.6, which a rule on pages alone gives away).
 constexpr int kFewPages = 128;
 
 struct SelectArgs {

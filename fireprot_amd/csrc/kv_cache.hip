@@ -81,7 +81,7 @@ __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(CacheArgs a)
 // two, so that what leads to a row serves as many bytes as in 8 bits.  And tokens of one
 // head that are read one after another, before the next head's: 4-bit rows are parts of a
 // line of the cache, and so are their scales, of which the next slot's row has the rest.
-// 64098 tokens of 8 heads of 128 to BF16, 291 MB: 78 us with one span, 84 with two, 70 with
+// 64098 tokens of 8 heads of 128 to BF16, 332 MB: 78 us with one span, 84 with two, 70 with
 // tokens in runs of 16, 63 with one row of each tensor in flight in a thread and not four.
 template <typename C>
 constexpr int kReadSpans = __is_same(C, Fp4) ? 2 : 1;

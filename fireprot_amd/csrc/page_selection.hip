@@ -11,12 +11,15 @@
 // where thousands of pages compete for the last place.  The sum is rounded to FP32 once;
 // of pages alike the lower is preferred.
 //
-// What bounds the ranks is the larger of the bounds' way from memory and the FP64
-// products, which are about as long: 16 sequences of up to 2048 pages, 8 cache heads of
-// 128 BF16 channels with 8 queries each, 88 MB of bounds: 28 us, the products alone
-// 24.6 (17 clocks each for 16 pages, 4 queries and 4 channels; the form with 16 queries
-// takes 78 and the whole 49), the loads alone 21.  4 queries to a head, 8 heads of one
-// sequence of 2048 pages, 8.5 MB: 5.6 us, of which a launch is 3 to 4.
+// What bounds the ranks is the bounds' way from memory.  16 sequences of equal length, 8
+// cache heads of 128 BF16 channels with 8 queries each: 11.4 us with 384 pages a sequence,
+// and 5.4 for each further 384 (25 MB, 4.7 TB/s).  The FP64 products are 3.0 of those 5.4
+// (16 to 17 clocks each for 16 pages, 4 queries and 4 channels; the form with 16 queries
+// takes 78: ranks in 49 us), the waves' exchange 0.4, and the conversions to FP64 go on
+// beside them.  6 us are fixed: a launch, and three looks at memory of which each needs the
+// one before (length, page, bounds).  626 to 2048 pages, 88 MB: 26.7 us by itself, of which
+// uneven rows are 2, and 29 to 31 between the other kernels of a step.  4 queries to a head,
+// 8 heads of one sequence of 2048 pages, 8.5 MB: 5.7 us, a launch being 3 to 4.
 #include "cache_rows.hpp"
 #include "common.hpp"
 #include "kernels.hpp"
@@ -382,7 +385,9 @@ __device__ __forceinline__ void select_plain(const SelectArgs& a, int row, int t
 // whose ranks (and numbers) it keeps in registers; 0: any number, read again every time.
 // 128 rows of 626 to 2048 pages, 128 of them chosen, take 4.9 us, 8 rows of 2048 5.2: a
 // launch, and eight barriers with a look into LDS between them (with one copy of the
-// counts, and ranks read again in each turn, 9.1 and 8.9).
+// counts, and ranks read again in each turn, 9.1 and 8.9).  Rows too long for registers
+// read them again: ranks and choice of 8 rows of 8192 pages are 22 us, of 8193 27, of
+// 16384 65.
 constexpr int kCopies = 8;  // of the counts: neighbouring pages' ranks begin alike
 constexpr int kBins = 256 + 4;  // of a copy, which begins four banks after the one before
 

@@ -43,7 +43,9 @@
 // and the join are a third of it); 32 of 16384 keys 324 to 339 us, 6.3 to 6.6 TB/s.
 // In 4 bits, 8 heads of 128: 16 of 20001 to 131071 keys, 64 queries, 235 us, 5.6 TB/s;
 // 32 of 4096, 32 queries, 36.6 us, 3.9, where each further 4096 keys take 25 (5.7): the
-// start, the join and the launches between are 11 us.
+// start, the join and the launches between are 11 us.  4 heads of 256, FP16, 24 sequences
+// of 4096 keys 34.8 us, of 16384 84.7, 5.1 TB/s: 18 us are fixed, with two work-groups to
+// a CU, and the rest runs at 6.1 to 6.6.
 //
 // Rounding: scores, softmax and accumulators are FP32.  The weights (times the
 // value's scale in an 8-bit cache) enter the second product as 16-bit terms whose

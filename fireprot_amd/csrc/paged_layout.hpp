@@ -4,7 +4,8 @@
 //
 // A cache holds `pages` pages of 2^page_shift slots.  k and v each are
 // [pages][heads][slots of a page][head_dim], the scales of an 8-bit cache
-// [pages][heads][slots of a page]: one head's keys of a page are contiguous,
+// [pages][heads][slots of a page], a float each; rows of a 4-bit cache are head_dim / 2
+// bytes with head_dim / 32 scale bytes: one head's keys of a page are contiguous,
 // which is what an attention work-group reads.
 #pragma once
 

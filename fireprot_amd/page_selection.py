@@ -125,7 +125,8 @@ def update_page_bounds(bounds: PageBounds, cache: PagedCache, block_table: torch
     code = _native.launch(
         device, lib.fpx_page_bounds, CACHE_DTYPES[cache.k.dtype], cache.k.data_ptr(),
         None if k_scale is None else k_scale.data_ptr(), pages, heads, page_size, head_dim,
-        block_table.data_ptr(), row, columns, lengths.data_ptr(), batch, max_length, min(new, max_length + 1), values.data_ptr())
+        block_table.data_ptr(), row, columns, lengths.data_ptr(), batch, max_length,
+        min(new, max_length + 1), values.data_ptr())
     if code:
         _native.check(code, "fpx_page_bounds")
 
@@ -142,7 +143,8 @@ def select_pages(q: torch.Tensor, bounds: PageBounds, block_table: torch.Tensor,
     exceeds.  The sum is taken in FP64 and rounded to FP32; of equal pages the lower
     comes first, NaN and pages outside the cache above all (NaN are zero times an infinite
     bound and a sum of both infinities).  A sequence of no more than ``count`` pages keeps
-    them all.
+    them all; the outputs have ``count`` places whatever the table holds, and an attention
+    over them plans for as many unless its ``max_length`` says less.
 
     * ``q`` ``[batch, q_heads, head_dim]`` as ``paged_attention``'s, ``q_heads`` a
       multiple of the bounds' heads; for a negative ``scale`` of the scores pass ``-q``.
@@ -189,9 +191,9 @@ def select_pages(q: torch.Tensor, bounds: PageBounds, block_table: torch.Tensor,
     code = _native.launch(
         device, lib.fpx_select_pages, kind, ROW_DTYPES[values.dtype], q.data_ptr(),
         *q.stride()[:2], q_heads, values.data_ptr(), pages, heads, page_size, head_dim,
-        block_table.data_ptr(), row, columns, lengths.data_ptr(), batch, max_length, count, sinks, recent, index.data_ptr(),
-        table.data_ptr(), kept.data_ptr(), None if workspace is None else workspace.data_ptr(),
-        size)
+        block_table.data_ptr(), row, columns, lengths.data_ptr(), batch, max_length, count,
+        sinks, recent, index.data_ptr(), table.data_ptr(), kept.data_ptr(),
+        None if workspace is None else workspace.data_ptr(), size)
     if code:
         _native.check(code, "fpx_select_pages")
     return PageSelection(table, kept, index)
